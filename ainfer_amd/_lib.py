@@ -17,6 +17,9 @@ SCALE_BF16, SCALE_FP16 = 0, 1
 PRECISION_W4A16, PRECISION_W4A8 = 0, 1
 NORM_PLAIN, NORM_ONE_PLUS = 0, 1
 ACT_F32, ACT_BF16 = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
+LORA_MAX_PROJ = 4
 FILL_BYTES, FILL_BF16_NORMAL, FILL_FP16_ABSNORMAL, FILL_BF16_ABSNORMAL = 0, 1, 2, 3
 MAX_TOKENS = 65536
 STACK_MAX_TOKENS = 4
@@ -31,6 +34,8 @@ EXPORTS = (
     "ainfer_moe_route",
     "ainfer_moe_dispatch", "ainfer_moe_experts", "ainfer_moe_combine", "ainfer_moe_rmsnorm", "ainfer_moe_fill",
     "ainfer_moe_act_quant_i8", "ainfer_moe_int4_gemv_i8",
+    "ainfer_moe_route_scored", "ainfer_moe_lora_workspace_bytes", "ainfer_moe_lora_apply",
+    "ainfer_moe_silu_mul",
     "ainfer_moe_profile_enable", "ainfer_moe_profile_read", "ainfer_moe_profile_kernel", "ainfer_moe_debug_spin_limit",
     "ainfer_moe_set_strict",
     "ainfer_moe_mfma_probe", "ainfer_moe_read_probe",
@@ -51,6 +56,22 @@ class Weights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in (
         "router_w", "router_bias", "shared_gate_w", "w_gate", "s_gate", "w_up", "s_up",
         "w_down", "s_down", "ws_gate", "ss_gate", "ws_up", "ss_up", "ws_down", "ss_down")]
+
+
+class Routing(C.Structure):
+    """Scored routing (ainfer_moe_routing): how experts are scored, grouped,
+    selected and weighted."""
+    _fields_ = [("n_experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32),
+                ("n_groups", C.c_int32), ("top_groups", C.c_int32), ("group_score", C.c_int32),
+                ("renormalize", C.c_int32), ("scale", C.c_float)]
+
+
+class Lora(C.Structure):
+    _fields_ = [("n_adapters", C.c_int32), ("rank", C.c_int32), ("in_", C.c_int32),
+                ("n_proj", C.c_int32), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32),
+                ("out", C.c_int32 * LORA_MAX_PROJ), ("a", C.c_void_p * LORA_MAX_PROJ),
+                ("b", C.c_void_p * LORA_MAX_PROJ), ("ranks", C.c_void_p),
+                ("scales", C.c_void_p)]
 
 
 class MoeError(RuntimeError):
@@ -95,6 +116,13 @@ def lib():
         L.ainfer_moe_fill.argtypes = [I32, C.c_uint64, F, SZ, P, P]
         L.ainfer_moe_act_quant_i8.argtypes = [P, I32, I32, I32, P, P, P]
         L.ainfer_moe_int4_gemv_i8.argtypes = [P, P, I32, P, P, I32, I32, I32, P, P]
+        I64 = C.c_int64
+        L.ainfer_moe_route_scored.argtypes = [C.POINTER(Routing), P, I32, I64, P, I32, P, P, P]
+        L.ainfer_moe_lora_workspace_bytes.restype = SZ
+        L.ainfer_moe_lora_workspace_bytes.argtypes = [C.POINTER(Lora), I32]
+        L.ainfer_moe_lora_apply.argtypes = [C.POINTER(Lora), P, I64, P, I32, C.POINTER(P),
+                                            C.POINTER(I64), P, SZ, P]
+        L.ainfer_moe_silu_mul.argtypes = [P, I64, P, I64, I32, I32, I32, P, I64, I32, P]
         L.ainfer_moe_profile_enable.argtypes = [I32]
         L.ainfer_moe_profile_kernel.argtypes = [C.POINTER(C.c_float), C.POINTER(I32)]
         L.ainfer_moe_mfma_probe.argtypes = [I32, I32, I32, P, C.POINTER(C.c_float)]

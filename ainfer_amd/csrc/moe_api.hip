@@ -696,6 +696,25 @@ int do_route(const ainfer_moe_shape *s, const ainfer_moe_weights *w, const void 
                           at<float>(ws, L.sg_logit), nullptr, T, s->hidden, s->n_experts, st));
   return AINFER_OK;
 }
+
+// ---- the operators around the expert stage ----------------------------------
+bool mis(const void *p, uintptr_t align) { return ((uintptr_t)p & (align - 1)) != 0; }
+bool is_act(int32_t dtype) { return dtype == AINFER_ACT_F32 || dtype == AINFER_ACT_BF16; }
+int act_size(int32_t dtype) { return dtype == AINFER_ACT_F32 ? 4 : 2; }
+// row pitches (in elements) whose products with a token count stay far from 2^63
+constexpr int64_t MAX_LD = (int64_t)1 << 40;
+
+int check_lora(const ainfer_moe_lora *l) {
+  if (!l) return AINFER_ERR_NULL;
+  if (l->n_adapters < 1 || l->n_adapters > 4096 || l->rank < 8 || l->rank > 128 || l->rank % 8 ||
+      l->in < 8 || l->in > 65536 || l->in % 8 || l->n_proj < 1 ||
+      l->n_proj > AINFER_LORA_MAX_PROJ)
+    return AINFER_ERR_SHAPE;
+  for (int p = 0; p < l->n_proj; ++p)
+    if (l->out[p] < 1 || l->out[p] > (1 << 20)) return AINFER_ERR_SHAPE;
+  if (!is_act(l->x_dtype) || !is_act(l->y_dtype)) return AINFER_ERR_ARG;
+  return AINFER_OK;
+}
 }  // namespace
 
 extern "C" {
@@ -1129,6 +1148,76 @@ int ainfer_moe_int4_gemv_i8(const uint8_t *packed, const void *scales, int32_t s
       (uintptr_t)sq % 4 || (uintptr_t)y % 4)
     return AINFER_ERR_ARG;
   HIP_TRY(launch_int4_gemv_i8(packed, scales, scale_dtype, q, sq, M, K, T, y, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_route_scored(const ainfer_moe_routing *r, const void *logits, int32_t logits_dtype,
+                            int64_t ld, const float *bias, int32_t T, int32_t *topk_idx,
+                            float *topk_w, void *stream) {
+  if (!r) return AINFER_ERR_NULL;
+  if (r->n_experts < 1 || r->n_experts > 1024 || r->n_groups < 1 || r->n_groups > 64 ||
+      r->n_experts % r->n_groups || r->top_groups < 1 || r->top_groups > r->n_groups)
+    return AINFER_ERR_SHAPE;
+  if (r->top_k < 1 || r->top_k > 32 ||
+      r->top_k > r->top_groups * (r->n_experts / r->n_groups))
+    return AINFER_ERR_SHAPE;
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS) return AINFER_ERR_TOKENS;
+  if ((r->score != AINFER_SCORE_SOFTMAX && r->score != AINFER_SCORE_SIGMOID) ||
+      (r->group_score != AINFER_GROUP_MAX && r->group_score != AINFER_GROUP_TOP2) ||
+      (r->renormalize != 0 && r->renormalize != 1) || !std::isfinite(r->scale) || !is_act(logits_dtype))
+    return AINFER_ERR_ARG;
+  if (T == 0) return AINFER_OK;
+  if (!logits || !topk_idx || !topk_w) return AINFER_ERR_NULL;
+  if (ld < r->n_experts || ld > MAX_LD || mis(logits, act_size(logits_dtype)) || mis(bias, 4) ||
+      mis(topk_idx, 4) || mis(topk_w, 4))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_route_scored(*r, logits, logits_dtype, ld, bias, T, topk_idx, topk_w,
+                              (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+size_t ainfer_moe_lora_workspace_bytes(const ainfer_moe_lora *l, int32_t max_tokens) {
+  if (check_lora(l) != AINFER_OK || max_tokens < 0 || max_tokens > AINFER_MOE_MAX_TOKENS) return 0;
+  return lora_workspace_bytes(*l, max_tokens > 0 ? max_tokens : 1);
+}
+
+int ainfer_moe_lora_apply(const ainfer_moe_lora *l, const void *x, int64_t x_ld,
+                          const int32_t *token_adapter, int32_t T, void *const *y,
+                          const int64_t *y_ld, void *ws, size_t ws_bytes, void *stream) {
+  int rc = check_lora(l);
+  if (rc) return rc;
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS) return AINFER_ERR_TOKENS;
+  if (T == 0) return AINFER_OK;
+  if (!x || !token_adapter || !y || !y_ld || !ws) return AINFER_ERR_NULL;
+  for (int p = 0; p < l->n_proj; ++p)
+    if (!l->a[p] || !l->b[p] || !y[p]) return AINFER_ERR_NULL;
+  const int xsz = act_size(l->x_dtype), ysz = act_size(l->y_dtype);
+  if (x_ld < l->in || x_ld > MAX_LD || mis(x, 16) || (x_ld * xsz) % 16 || mis(token_adapter, 4) ||
+      mis(l->ranks, 4) || mis(l->scales, 4))
+    return AINFER_ERR_ARG;
+  for (int p = 0; p < l->n_proj; ++p)
+    if (mis(l->a[p], 16) || mis(l->b[p], 16) || mis(y[p], ysz) || y_ld[p] < l->out[p] ||
+        y_ld[p] > MAX_LD)
+      return AINFER_ERR_ARG;
+  if (mis(ws, 256) || ws_bytes < lora_workspace_bytes(*l, T)) return AINFER_ERR_WORKSPACE;
+  HIP_TRY(launch_lora(*l, x, x_ld, token_adapter, T, y, y_ld, ws, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,
+                        int32_t in_dtype, int32_t T, int32_t I, void *act, int64_t act_ld,
+                        int32_t act_dtype, void *stream) {
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS) return AINFER_ERR_TOKENS;
+  if (I <= 0) return AINFER_ERR_SHAPE;
+  if (!is_act(in_dtype) || !is_act(act_dtype)) return AINFER_ERR_ARG;
+  if (T == 0) return AINFER_OK;
+  if (!gate || !up || !act) return AINFER_ERR_NULL;
+  const int isz = act_size(in_dtype);
+  if (gate_ld < I || up_ld < I || act_ld < I || gate_ld > MAX_LD || up_ld > MAX_LD ||
+      act_ld > MAX_LD || mis(gate, isz) || mis(up, isz) || mis(act, act_size(act_dtype)))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_silu_rows(gate, gate_ld, up, up_ld, in_dtype, T, I, act, act_ld, act_dtype,
+                           (hipStream_t)stream));
   return AINFER_OK;
 }
 

@@ -380,3 +380,31 @@ int stack_flag_words(const ainfer_moe_shape &s, int cap);
 hipError_t launch_decode_stack(int scale_dtype, const ainfer_moe_shape &s, const StackGeom &g,
                                const StackLayer *layers, int L, const void *x0, void *r, int T,
                                int norm_mode, float eps, const StackWs &w, hipStream_t st);
+
+// ---- scored routing (moe_scored.hip) ---------------------------------------
+struct ScoredArgs {
+  const void *logits;
+  const float *bias;
+  int32_t *idx;
+  float *w;
+  int64_t ld;
+  int dtype, T, k;
+  int G, top, per;  // groups, groups kept, experts per group
+  int gl;           // log2 of the lanes that hold a group
+  int group_score, renorm;
+  float scale;
+  bool vec;         // rows readable in 16-byte pieces
+};
+constexpr int SR_MAX_GRID = 2048;
+hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, int dtype,
+                               int64_t ld, const float *bias, int T, int32_t *idx, float *w,
+                               hipStream_t s);
+
+// ---- adapters (moe_lora.hip) ------------------------------------------------
+size_t lora_workspace_bytes(const ainfer_moe_lora &l, int max_tokens);
+hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, const int32_t *ids,
+                       int T, void *const *y, const int64_t *y_ld, void *ws, hipStream_t s);
+
+// ---- gated activation (moe_silu.hip) ----------------------------------------
+hipError_t launch_silu_rows(const void *g, int64_t gld, const void *u, int64_t uld, int in_dtype,
+                            int T, int I, void *y, int64_t yld, int out_dtype, hipStream_t s);

@@ -248,3 +248,135 @@ def rmsnorm(x, y, w=None, mode=L.NORM_PLAIN, eps=1e-6, stream=None):
     T, H = x.shape
     return L.check(L.lib().ainfer_moe_rmsnorm(_ptr(x), _ptr(w), mode, eps, _ptr(y), T, H,
                                               _stream(stream)))
+
+
+# ---- the operators around the expert stage -----------------------------------
+_ACT = {torch.float32: L.ACT_F32, torch.bfloat16: L.ACT_BF16}
+
+
+def _require(ok, what):
+    if not ok:
+        raise L.MoeError(what)
+
+
+def _rows(t, name, cols=None):
+    """A device matrix of fp32 or bf16 rows, each contiguous: (dtype, pitch)."""
+    _require(t.dim() == 2 and t.dtype in _ACT, f"{name}: rows of fp32 or bf16")
+    _require(t.is_cuda, f"{name}: a device tensor")
+    _require(cols is None or t.shape[1] == cols, f"{name}: {cols} columns")
+    _require(t.shape[1] == 1 or t.stride(1) == 1, f"{name}: contiguous rows")
+    # a single row has no pitch
+    return _ACT[t.dtype], max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t, name, dtype, n, device):
+    _require(t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == device,
+             f"{name}: {n} contiguous {dtype} values on the inputs' device")
+
+
+def _call(fn, device, stream, *args):
+    """fn(*args, stream) on the device the tensors are on."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return L.check(fn(*args, _stream(stream)))
+    return L.check(fn(*args, _stream(stream)))
+
+
+def route_scored(routing, logits, bias=None, out=None, stream=None):
+    """Scored routing of logits [T][E] (ainfer_moe_route_scored; routing: an
+    L.Routing): (topk_idx [T][k] int32, topk_w [T][k] fp32), as MoeLayer.dispatch,
+    experts and combine take them.  out: the two tensors to write."""
+    dt, ld = _rows(logits, "logits", routing.n_experts)
+    T, k = logits.shape[0], routing.top_k
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, routing.n_experts, logits.device)
+    if out is None:
+        out = (torch.empty(T, k, dtype=torch.int32, device=logits.device),
+               torch.empty(T, k, dtype=torch.float32, device=logits.device))
+    idx, w = out
+    for t, d in ((idx, torch.int32), (w, torch.float32)):
+        _require(t.shape == (T, k) and t.dtype == d and t.is_contiguous()
+                 and t.device == logits.device, "out: (idx int32, w fp32), [T][k] contiguous")
+    _call(L.lib().ainfer_moe_route_scored, logits.device, stream, C.byref(routing), _ptr(logits),
+          dt, ld, _ptr(bias), T, _ptr(idx), _ptr(w))
+    return idx, w
+
+
+def silu_mul(gate, up, act, stream=None):
+    """act = gate / (1 + exp(-gate)) * up over rows of any pitch
+    (ainfer_moe_silu_mul)."""
+    dt, gld = _rows(gate, "gate")
+    udt, uld = _rows(up, "up", gate.shape[1])
+    adt, ald = _rows(act, "act", gate.shape[1])
+    _require(udt == dt and up.shape == gate.shape and act.shape == gate.shape
+             and up.device == gate.device and act.device == gate.device,
+             "gate, up and act: one shape and device, gate and up one type")
+    T, n = gate.shape
+    _call(L.lib().ainfer_moe_silu_mul, gate.device, stream, _ptr(gate), gld, _ptr(up), uld, dt, T,
+          n, _ptr(act), ald, adt)
+    return act
+
+
+class LoraAdapters:
+    """The adapters of up to LORA_MAX_PROJ projections of one input, resident
+    on one device: a[p] [N][R][K] and b[p] [N][M_p][R] bf16, optional ranks
+    ([N] int32, the rows of each adapter in use) and scales ([N] fp32)."""
+
+    def __init__(self, a, b, ranks=None, scales=None, x_dtype=torch.bfloat16,
+                 y_dtype=torch.bfloat16):
+        a, b = list(a), list(b)
+        _require(1 <= len(a) == len(b) <= L.LORA_MAX_PROJ, "one a and one b per projection")
+        _require(x_dtype in _ACT and y_dtype in _ACT, "x and y: fp32 or bf16")
+        _require(a[0].dim() == 3, "a: [adapters][rank][columns]")
+        N, R, K = a[0].shape
+        dev = a[0].device
+        for t in a + b:
+            _require(t.dtype == torch.bfloat16 and t.is_cuda and t.device == dev
+                     and t.is_contiguous() and t.dim() == 3,
+                     "a and b: contiguous bf16 on one device")
+        for ta, tb in zip(a, b):
+            _require(ta.shape == (N, R, K) and tb.shape[0] == N and tb.shape[2] == R,
+                     "a [N][R][K] and b [N][M][R] of one N, R and K")
+        if ranks is not None:
+            _vector(ranks, "ranks", torch.int32, N, dev)
+        if scales is not None:
+            _vector(scales, "scales", torch.float32, N, dev)
+        self.keep = (a, b, ranks, scales)
+        self.device, self.x_dtype, self.y_dtype = dev, x_dtype, y_dtype
+        n = len(a)
+        s = L.Lora(N, R, K, n, _ACT[x_dtype], _ACT[y_dtype])
+        for p in range(n):
+            s.out[p], s.a[p], s.b[p] = b[p].shape[1], a[p].data_ptr(), b[p].data_ptr()
+        s.ranks = ranks.data_ptr() if ranks is not None else None
+        s.scales = scales.data_ptr() if scales is not None else None
+        self.s = s
+        _require(L.lib().ainfer_moe_lora_workspace_bytes(C.byref(s), 1) > 0,
+                 "adapter sizes outside the supported range")
+
+    def workspace(self, max_tokens):
+        n = L.lib().ainfer_moe_lora_workspace_bytes(C.byref(self.s), max_tokens)
+        if n == 0:
+            raise L.MoeError("invalid token count for an adapter workspace")
+        ws = torch.empty(n + 256, dtype=torch.uint8, device=self.device)
+        off = (-ws.data_ptr()) % 256
+        return ws[off:off + n]
+
+    def apply(self, x, token_adapter, ys, ws, stream=None):
+        """ys[p] += scale * (x a^T) b^T of each token's adapter, in place
+        (ainfer_moe_lora_apply); tokens without one keep their rows."""
+        s = self.s
+        _, ld = _rows(x, "x", s.in_)
+        _require(x.dtype == self.x_dtype and x.device == self.device, "x: the adapters' x type")
+        T = x.shape[0]
+        _vector(token_adapter, "token_adapter", torch.int32, T, self.device)
+        _require(len(ys) == s.n_proj, "one y per projection")
+        n = L.LORA_MAX_PROJ
+        yp, yl = (C.c_void_p * n)(), (C.c_int64 * n)()
+        for p, y in enumerate(ys):
+            _, yl[p] = _rows(y, "y", s.out[p])
+            _require(y.shape[0] == T and y.dtype == self.y_dtype and y.device == self.device,
+                     "y: T rows of the adapters' y type")
+            yp[p] = y.data_ptr()
+        _call(L.lib().ainfer_moe_lora_apply, self.device, stream, C.byref(s), _ptr(x), ld,
+              _ptr(token_adapter), T, yp, yl, _ptr(ws), ws.numel())
+        return ys

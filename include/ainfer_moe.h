@@ -410,6 +410,103 @@ int ainfer_moe_debug_spin_limit(int32_t polls);
  * graph capture the check is skipped (nothing can be waited for there). */
 int ainfer_moe_set_strict(int32_t on);
 
+/* ---- scored routing: the router forms the layer's own softmax lacks ------
+ * For models that score experts with a sigmoid, add a bias for selection
+ * only (load balance), or pick groups of experts first.  From given logits
+ * (ainfer_moe_route's, or a router of the caller's):
+ *   masked e    logit_e <= the lowest finite value of its type, or NaN, or
+ *               bias_e NaN or -inf
+ *   s_e         SIGMOID 1 / (1 + exp(-logit_e)); SOFTMAX exp(logit_e) / sum
+ *               of exp over the unmasked experts; a logit of +inf counts as
+ *               the largest finite one
+ *   key_e       logit_e without a bias (both scores rise with it), s_e +
+ *               bias_e with one (bias clamped to +-1e38), in the order of the
+ *               64-bit values
+ *   groups      n_groups runs of E / n_groups consecutive experts; a group's
+ *               value is its largest key (GROUP_MAX) or the sum of its two
+ *               largest s_e + bias_e (GROUP_TOP2; one or none where fewer are
+ *               unmasked); the top_groups groups of largest value are kept, of
+ *               equal ones the lower first
+ *   topk_idx[t] the top_k experts of the kept groups with the largest keys, equal
+ *               keys lower index first; masked experts come after all others,
+ *               lower index first, and only where fewer than top_k are left
+ *   topk_w[t][j] scale * s, or scale * s / (sum of the selected s) with
+ *               renormalize; 0 for a masked expert, also where all are masked
+ * Scores and sums are fp32; where two keys or group values are too near for
+ * fp32 the comparison is redone in fp64.  The rows are what
+ * ainfer_moe_dispatch, _experts and _combine take.  No reference counterpart
+ * (the reference is dense). */
+enum { AINFER_SCORE_SOFTMAX = 0, AINFER_SCORE_SIGMOID = 1 };
+enum { AINFER_GROUP_MAX = 0, AINFER_GROUP_TOP2 = 1 };
+typedef struct ainfer_moe_routing {
+  int32_t n_experts;   /* E, 1..1024                                         */
+  int32_t top_k;       /* 1..32, at most top_groups * E / n_groups           */
+  int32_t score;       /* AINFER_SCORE_*                                     */
+  int32_t n_groups;    /* 1..64, divides E; 1 = no groups                    */
+  int32_t top_groups;  /* 1..n_groups                                        */
+  int32_t group_score; /* AINFER_GROUP_* (unused when n_groups is 1)         */
+  int32_t renormalize; /* 0 or 1                                             */
+  float scale;         /* finite; multiplies every weight                    */
+} ainfer_moe_routing;
+/* logits [T] rows of E values (AINFER_ACT_F32 or AINFER_ACT_BF16), row t at
+ * t * ld elements (ld >= E); bias [E] fp32 or NULL; topk_idx, topk_w
+ * [T][top_k].  No workspace. */
+int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logits,
+                            int32_t logits_dtype, int64_t ld, const float *bias, int32_t T,
+                            int32_t *topk_idx, float *topk_w, void *stream);
+
+/* ---- low-rank adapters of many requests beside shared projections --------
+ * y_p[t][m] += scale_a * sum_{r < rank_a} v_p[t][r] * b_p[a][m][r],
+ * v_p[t][r] = sum_k x[t][k] * a_p[a][r][k],      a = token_adapter[t],
+ * for up to AINFER_LORA_MAX_PROJ projections p of one input (gate and up; q,
+ * k and v), in place beside the shared projection that wrote y_p
+ * (ainfer_moe_int4_gemv_i8, decode_l0.cpp:494-504's gemvE).  A token whose
+ * adapter is outside [0, n_adapters) keeps its rows of y untouched (they are
+ * not read either), as does one whose adapter has rank 0.  Tokens of a batch
+ * may name adapters in any order.  Rows r >= rank_a of a and columns
+ * r >= rank_a of b may hold anything.  x, a and b enter exactly; v and the
+ * products are fp32 sums, v is scaled in fp32 and enters the second product as
+ * the sum of three bf16 values (its 24 bits) where y is fp32, of two (2^-16 of
+ * it) where y is bf16; y is rounded once.  No reference counterpart (the
+ * reference serves one model to one request). */
+#define AINFER_LORA_MAX_PROJ 4
+typedef struct ainfer_moe_lora {
+  int32_t n_adapters;  /* N, 1..4096                                         */
+  int32_t rank;        /* R, rows stored per adapter, multiple of 8, 8..128  */
+  int32_t in;          /* K, multiple of 8, 8..65536                         */
+  int32_t n_proj;      /* P, 1..AINFER_LORA_MAX_PROJ                         */
+  int32_t x_dtype;     /* AINFER_ACT_F32 or AINFER_ACT_BF16                  */
+  int32_t y_dtype;     /* AINFER_ACT_F32 or AINFER_ACT_BF16                  */
+  int32_t out[AINFER_LORA_MAX_PROJ];   /* M_p, 1..1048576                    */
+  const void *a[AINFER_LORA_MAX_PROJ]; /* [N][R][K] bf16, 16-byte aligned    */
+  const void *b[AINFER_LORA_MAX_PROJ]; /* [N][M_p][R] bf16, 16-byte aligned  */
+  const int32_t *ranks; /* device [N] (values are clamped to 0..R), or NULL:
+                           every adapter has rank R                          */
+  const float *scales;  /* device [N], or NULL: 1                            */
+} ainfer_moe_lora;
+/* Workspace bytes of calls with up to max_tokens tokens (0 on an invalid
+ * description); 256-byte aligned, no initialisation, scratch between calls:
+ * calls that share it must be stream-ordered. */
+size_t ainfer_moe_lora_workspace_bytes(const ainfer_moe_lora *lora, int32_t max_tokens);
+/* x: T rows of K values, row t at t * x_ld elements, 16-byte aligned rows;
+ * token_adapter [T] int32; y[p]: T rows of M_p values at t * y_ld[p] elements
+ * (aligned to their type; rows must not overlap x, a, b or each other). */
+int ainfer_moe_lora_apply(const ainfer_moe_lora *lora, const void *x, int64_t x_ld,
+                          const int32_t *token_adapter, int32_t T, void *const *y,
+                          const int64_t *y_ld, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* Gated activation: act[t][i] = g / (1 + exp(-g)) * u with g = gate[t][i],
+ * u = up[t][i], computed in fp32.  Row t of gate, up and act starts at t * its
+ * ld elements (so gate and up may be the halves of one [T][2 * I] buffer);
+ * in_dtype of gate and up, act_dtype of act: AINFER_ACT_F32 or
+ * AINFER_ACT_BF16.  act may be gate or up itself (same pointer, type and ld).
+ * Replaces SiluMul, tools/cmdlist/kernels.cpp:29-37, where the projections
+ * around it are calls of their own (an adapted MLP). */
+int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,
+                        int32_t in_dtype, int32_t T, int32_t I, void *act, int64_t act_ld,
+                        int32_t act_dtype, void *stream);
+
 /* ---- synthetic data (counter-based, bit-identical to the CPU oracle) --- */
 enum {
   AINFER_FILL_BYTES = 0,      /* uniform random bytes (packed int4 weights)  */

@@ -1,0 +1,227 @@
+"""Adapters of many requests (ainfer_moe_lora_apply) against the formula in 64 bits.
+
+Bound per element, from the arithmetic: x and A enter exactly and v is a sum of K
+products in fp32, so |v - v64| <= (K + 32) 2^-23 sum|x||A| (2^-23: the matrix
+instructions may round either way); v * scale rounds once; as two bf16 parts (y in
+bf16) it is off by 2^-16, as three not at all; the second sum has at most 3 R terms;
+y rounds once (2^-24, or 2^-8 in bf16)."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch
+
+
+class Case:
+    def __init__(self, torch, T, N, R, K, Ms, x="bf16", y="fp32", ids=None, ranks=None,
+                 scales=True, seed=0, x_pad=0, y_pad=0):
+        dt = {"bf16": torch.bfloat16, "fp32": torch.float32}
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed + T * 31 + K)
+
+        def normal(*s, std=1.0, dtype=torch.float32):
+            return (torch.randn(*s, generator=g, device="cuda") * std).to(dtype)
+
+        self.torch, self.T, self.N, self.R, self.K, self.Ms = torch, T, N, R, K, Ms
+        self.a = [normal(N, R, K, std=K ** -0.5, dtype=torch.bfloat16) for _ in Ms]
+        self.b = [normal(N, M, R, std=0.2, dtype=torch.bfloat16) for M in Ms]
+        self.x = normal(T, K + x_pad, dtype=dt[x])[:, :K]
+        self.y = [normal(T, M + y_pad, dtype=dt[y])[:, :M] for M in Ms]
+        self.scales = torch.rand(N, generator=g, device="cuda") + 0.5 if scales else None
+        if ranks is None:
+            self.ranks = None
+        else:
+            self.ranks = torch.tensor(ranks, dtype=torch.int32, device="cuda")
+        if ids is None:
+            ids = torch.randint(-1, N, (T,), generator=g, device="cuda").tolist()
+        self.ids = torch.tensor(ids, dtype=torch.int32, device="cuda")
+        from ainfer_amd.moe import LoraAdapters
+        self.lora = LoraAdapters(self.a, self.b, ranks=self.ranks, scales=self.scales,
+                                 x_dtype=dt[x], y_dtype=dt[y])
+        print(f"[case] T={T} N={N} R={R} K={K} M={Ms} x={x} y={y}", flush=True)
+
+    def apply(self, ys, ws=None, stream=None):
+        ws = self.lora.workspace(self.T) if ws is None else ws
+        self.lora.apply(self.x, self.ids, ys, ws, stream=stream)
+
+    def check(self):
+        torch = self.torch
+        ys = [y.clone() if y.is_contiguous() else y for y in self.y]
+        before = [y.clone() for y in ys]
+        self.apply(ys)
+        torch.cuda.synchronize()
+        self.compare(before, ys)
+
+    def compare(self, before, after):
+        torch = self.torch
+        step = 2.0 ** -24 if before[0].dtype == torch.float32 else 2.0 ** -8
+        split = 0.0 if before[0].dtype == torch.float32 else 2.0 ** -16
+        ids = self.ids.cpu()
+        for p in range(len(self.Ms)):
+            y0, y1 = before[p].double().cpu(), after[p].double().cpu()
+            want, bound = y0.clone(), torch.zeros_like(y0)
+            same = torch.ones(self.T, dtype=torch.bool)
+            x = self.x.double().cpu()
+            for n in sorted(set(ids.tolist())):
+                if not 0 <= n < self.N:
+                    continue
+                r = self.R
+                if self.ranks is not None:
+                    r = min(max(int(self.ranks[n]), 0), self.R)
+                rows = (ids == n).nonzero()[:, 0]
+                if r == 0:
+                    continue
+                same[rows] = False
+                s = 1.0 if self.scales is None else float(self.scales[n])
+                A = self.a[p][n, :r].double().cpu()
+                B = self.b[p][n, :, :r].double().cpu()
+                v = x[rows] @ A.t()
+                mag = x[rows].abs() @ A.abs().t()
+                want[rows] += s * (v @ B.t())
+                bound[rows] = s * (((self.K + 3 * self.R + 40) * 2.0 ** -23 * mag
+                                    + split * v.abs()) @ B.abs().t())
+            assert torch.equal(y1[same], y0[same])       # rows without an adapter: untouched
+            assert torch.isfinite(y1).all()
+            assert ((y1 - want).abs() <= bound * (1 + step) + step * want.abs()).all(), (
+                p, float(((y1 - want).abs() - bound - step * want.abs()).max()))
+
+
+# T, N, R, K, Ms: one token, odd token counts around the tile sizes, ranks of every
+# block count, K of one chunk to many with tails, M of one to many with tails
+SHAPES = [(1, 1, 8, 8, [1]), (1, 4, 16, 4096, [4096]), (2, 3, 8, 72, [33, 7]),
+          (5, 2, 24, 520, [100]), (16, 16, 64, 1024, [257]), (17, 5, 32, 200, [64, 64, 31]),
+          (63, 40, 16, 640, [96]), (64, 64, 128, 264, [40]), (65, 3, 40, 136, [129]),
+          (255, 9, 16, 264, [48, 80]), (257, 7, 8, 128, [65]), (300, 2, 104, 328, [72]),
+          (1003, 12, 8, 1024, [136, 1, 2, 3]), (40, 2, 96, 2056, [33])]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("x,y", (("bf16", "fp32"), ("fp32", "bf16"), ("fp32", "fp32"),
+                                 ("bf16", "bf16")))
+def test_matches_formula(torch, shape, x, y):
+    Case(torch, *shape, x=x, y=y).check()
+
+
+@pytest.mark.parametrize("R", (8, 16, 32, 64, 128))
+def test_ragged_ranks_and_garbage_beyond_them(torch, R):
+    """Ranks 0, 1, odd ones, R, and values outside 0..R; NaN and inf in the rows
+    of A and columns of B beyond them."""
+    ranks = [0, 1, 3, R - 1, R, -4, R + 9, R // 2]
+    c = Case(torch, 50, 8, R, 136, [70, 9], ranks=ranks)
+    for n, r in enumerate(ranks):
+        r = min(max(r, 0), R)
+        for a, b in zip(c.a, c.b):
+            a[n, r:] = math.nan
+            b[n, :, r:] = math.inf
+    c.check()
+
+
+@pytest.mark.parametrize("T", (1, 20, 100, 700))
+def test_prompts_and_tokens_without_adapter(torch, T):
+    """Requests one after the other, ids outside the adapters, all without one."""
+    ids = [(t * 5 // T) - 1 for t in range(T)]
+    Case(torch, T, 4, 16, 264, [100], ids=ids).check()
+    Case(torch, T, 4, 16, 264, [100], ids=[4] * T, y="bf16").check()
+    Case(torch, T, 4, 16, 264, [100], ids=[(-7, 4, 1 << 30)[t % 3] for t in range(T)]).check()
+    Case(torch, T, 4, 16, 264, [100], ids=[t % 4 for t in range(T)], scales=False).check()
+
+
+def test_pitches_and_alignment(torch):
+    """Rows of x and y inside wider ones: 16-byte pieces of y, and not."""
+    for y in ("fp32", "bf16"):
+        for pad in (8, 3, 1):
+            Case(torch, 33, 5, 16, 200, [64, 50], x_pad=8, y_pad=pad, y=y).check()
+
+
+def test_other_tokens_do_not_leak(torch):
+    """A token's NaN and an adapter's inf stay in that token's rows and that
+    adapter's tokens."""
+    c = Case(torch, 32, 4, 16, 264, [80], ids=[t % 4 for t in range(32)])
+    c.x[5] = math.nan
+    c.b[0][3] = math.inf
+    ys = [y.clone() for y in c.y]
+    c.apply(ys)
+    torch.cuda.synchronize()
+    bad = torch.tensor([t == 5 or t % 4 == 3 for t in range(32)], device="cuda")
+    assert not torch.isfinite(ys[0][bad]).any()
+    assert torch.isfinite(ys[0][~bad]).all()
+    d = Case(torch, 32, 4, 16, 264, [80], ids=[t % 4 for t in range(32)])
+    clean = [y.clone() for y in d.y]
+    d.apply(clean)
+    assert torch.equal(clean[0][~bad], ys[0][~bad])
+
+
+def test_infinite_and_large_fp32_inputs(torch):
+    """fp32 x of inf gives inf or NaN, the largest finite x what the formula gives."""
+    c = Case(torch, 4, 1, 8, 64, [16], x="fp32", ids=[0, 0, 0, 0], ranks=[1],
+             scales=False)
+    c.a[0].zero_()
+    c.a[0][:, 0, 0] = 1.0
+    c.b[0].zero_()
+    c.b[0][:, :, 0] = 2.0 ** -10
+    c.x.zero_()
+    c.x[0, 0] = math.inf
+    c.x[1, 0] = torch.finfo(torch.float32).max
+    c.x[2, 0] = 1 + 2.0 ** -23
+    ys = [torch.zeros_like(c.y[0])]
+    c.apply(ys)
+    torch.cuda.synchronize()
+    assert (ys[0][0] == math.inf).all()
+    assert (ys[0][1] == torch.finfo(torch.float32).max * 2.0 ** -10).all()
+    assert (ys[0][2] == (1 + 2.0 ** -23) * 2.0 ** -10).all()
+    assert (ys[0][3] == 0).all()
+
+
+def test_shared_workspace_streams_and_graph(torch):
+    """One workspace for calls of several sizes in turn; another stream; a captured
+    call replayed between eager ones."""
+    big = Case(torch, 300, 6, 16, 520, [200])
+    ws = big.lora.workspace(300)
+    for T in (300, 1, 17, 300):
+        c = Case(torch, T, 6, 16, 520, [200], seed=T)
+        ys = [y.clone() for y in c.y]
+        c.apply(ys, ws)
+        torch.cuda.synchronize()
+        c.compare(c.y, ys)
+    side = torch.cuda.Stream()
+    ys = [y.clone() for y in big.y]
+    side.wait_stream(torch.cuda.current_stream())
+    big.apply(ys, ws, stream=side)
+    side.synchronize()
+    big.compare(big.y, ys)
+    ref = [y.clone() for y in ys]
+    buf = [y.clone() for y in big.y]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        big.apply(buf, ws)
+    for _ in range(3):
+        for b, y in zip(buf, big.y):
+            b.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(b, r) for b, r in zip(buf, ref))
+        Case(torch, 17, 6, 16, 520, [200]).check()
+
+
+def test_offsets_past_32_bits(torch):
+    """x and y pitches whose products with the token pass 2^31 elements."""
+    T, K, M = 33, 64, 48
+    c = Case(torch, T, 3, 8, K, [M])
+    pitch = (1 << 27) + 8
+    xs = torch.empty((T - 1) * pitch + K, dtype=torch.bfloat16, device="cuda")
+    ys = torch.empty((T - 1) * pitch + M, dtype=torch.float32, device="cuda")
+    x = xs.as_strided((T, K), (pitch, 1))
+    y = ys.as_strided((T, M), (pitch, 1))
+    x.copy_(c.x)
+    y.copy_(c.y[0])
+    c.lora.apply(x, c.ids, [y], c.lora.workspace(T))
+    torch.cuda.synchronize()
+    c.compare(c.y, [y.contiguous()])
