@@ -1,23 +1,29 @@
 // moe_lora.hip - low-rank adapters of many requests beside shared projections
 // (ainfer_moe_lora_apply): y_p += scale_a (x A_a^T) B_a^T, a = the token's adapter.
 //
-// Tokens are taken in tiles of up to 16 neighbours, a column each of a
-// v_mfma_f32_16x16x32_bf16; a tile runs once per distinct adapter in it, with the
-// other tokens' columns ignored, so batches need no sorting: a batch of
-// requests has one adapter per token (bound by reading A and B, where an empty
-// column costs nothing), a prompt one adapter per tile.
-//   k_lora_down  partial sums of v = x A^T over a part of K, to the workspace
-//   k_lora_up    v = the sum of the parts, scaled; y += v B^T
-// All products are exact: bf16 values enter the MFMA as they are, fp32 values as
-// the sum of two or three bf16 (split_bf16).
+// Batches of requests (an adapter per token: bound by reading A and B once for
+// every token, by launches and by latency) take dot products in fp32:
+//   k_lora_dec    a workgroup owns rows of one token's y: a wave per row of A, v to
+//                 LDS, then the rows of B; A is read by every workgroup of the
+//                 token, which costs less than a second launch while it is small
+//   k_lora_rows   v = x A^T, a wave per row of A, and k_lora_dec without its first
+//                 half, where A is large
+// Prompts (neighbouring tokens share an adapter) take 32 tokens a wave on
+// v_mfma_f32_16x16x32_bf16, once per distinct adapter among them, other tokens'
+// columns ignored: no sorting, tokens may name adapters in any order:
+//   k_lora_down   partial sums of v over a part of K, to the workspace
+//   k_lora_up     v = the sum of the parts, scaled; y += v B^T
+// Their products are exact too: bf16 values enter the MFMA as they are, fp32 values
+// as the sum of two or three bf16 (split_bf16).
 #include "moe_common.h"
 #include "moe_internal.h"
 
 namespace {
 
-constexpr int LT = 16;      // columns of a tile
-constexpr int KB = 64;      // k of two MFMAs: 128 bytes of every bf16 row
-constexpr int L_WAVES = 4;
+constexpr int TT = 16;       // tokens of an MFMA tile
+constexpr int R_WAVES = 4;   // waves of a workgroup: k_lora_rows
+constexpr int D_WAVES = 8;   // k_lora_dec
+constexpr int T_WAVES = 8;   // k_lora_tile
 
 struct LoraArgs {
   const void *x;
@@ -27,14 +33,259 @@ struct LoraArgs {
   void *y[AINFER_LORA_MAX_PROJ];
   int64_t y_ld[AINFER_LORA_MAX_PROJ], x_ld;
   int m[AINFER_LORA_MAX_PROJ];
-  bool y_vec[AINFER_LORA_MAX_PROJ];  // y rows readable in 16-byte pieces
-  float *part;    // [splits][P][T][R]
+  bool y_vec[AINFER_LORA_MAX_PROJ];  // y rows readable in pieces of 4 values
+  float *v;       // [P][T][R], of k_lora_rows
   int N, R, K, P, T;
-  int tt;         // tokens per tile
-  int splits;     // parts of K over workgroups
-  int kw;         // blocks of KB per wave
-  int units;      // 32-row units per wave of k_lora_up
+  int units;      // groups of 64 rows of y per wave
 };
+
+__device__ __forceinline__ int rank_of(const LoraArgs &a, int ad) {
+  return a.ranks ? min(max(a.ranks[ad], 0), a.R) : a.R;
+}
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// ---- batches of requests ------------------------------------------------------
+
+__device__ __forceinline__ float wave_sum_f32(float v) {
+  auto dpp = [](float x, auto ctrl, auto rows) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value,
+                                                      decltype(rows)::value, 0xF, false));
+  };
+  using std::integral_constant;
+  v += dpp(v, integral_constant<int, 0xB1>(), integral_constant<int, 0xF>());
+  v += dpp(v, integral_constant<int, 0x4E>(), integral_constant<int, 0xF>());
+  v += dpp(v, integral_constant<int, 0x141>(), integral_constant<int, 0xF>());
+  v += dpp(v, integral_constant<int, 0x140>(), integral_constant<int, 0xF>());
+  v += dpp(v, integral_constant<int, 0x142>(), integral_constant<int, 0xA>());
+  v += dpp(v, integral_constant<int, 0x143>(), integral_constant<int, 0xC>());
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// 8 values of x from k
+template <bool XF32>
+struct X8 {
+  u32x4 v[XF32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char *row, int k) {
+#pragma unroll
+    for (int i = 0; i < (XF32 ? 2 : 1); ++i)
+      v[i] = *(const u32x4 *)(row + (size_t)k * (XF32 ? 4 : 2) + 16 * i);
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (XF32) return __uint_as_float(v[i / 4][i & 3]);
+    return i & 1 ? bf16_hi(v[0][i / 2]) : bf16_lo(v[0][i / 2]);
+  }
+};
+template <bool XF32>
+__device__ __forceinline__ void dot8(const X8<XF32> &x, const u32x4 &w, float &acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc = fmaf(x.at(2 * i), bf16_lo(w[i]), acc);
+    acc = fmaf(x.at(2 * i + 1), bf16_hi(w[i]), acc);
+  }
+}
+
+// x . A's rows row and row + step (NR = 2), or the first alone: a wave, 512 k a
+// step, four steps' loads in flight; every lane gets the sums
+template <bool XF32, int NR>
+__device__ __forceinline__ void row_dots(const char *xr, const uint16_t *ar, size_t step, int K,
+                                         int lane, float (&sum)[NR]) {
+  float acc[NR][2];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) acc[r][0] = acc[r][1] = 0.0f;
+  int k = lane * 8;
+  constexpr int U = 4;
+  for (; k - lane * 8 + 512 * U <= K; k += 512 * U) {
+    X8<XF32> x[U];
+    u32x4 w[U][NR];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u].load(xr, k + 512 * u);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) w[u][r] = *(const u32x4 *)(ar + r * step + k + 512 * u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) dot8(x[u], w[u][r], acc[r][u & 1]);
+  }
+  if (k - lane * 8 < K) {
+    X8<XF32> x[U];
+    u32x4 w[U][NR];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int ku = k + 512 * u;
+#pragma unroll
+      for (auto &p : x[u].v) p = (u32x4){0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < NR; ++r) w[u][r] = (u32x4){0, 0, 0, 0};
+      if (ku < K) {  // K is a multiple of 8
+        x[u].load(xr, ku);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) w[u][r] = *(const u32x4 *)(ar + r * step + ku);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) dot8(x[u], w[u][r], acc[r][u & 1]);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) sum[r] = wave_sum_f32(acc[r][0] + acc[r][1]);
+}
+
+// v of one token: rows first, first + step, ... below rank, two at a time
+template <bool XF32, typename Put>
+__device__ __forceinline__ void token_rows(const LoraArgs &a, int p, int t, int ad, int first,
+                                           int step, int rank, int lane, Put put) {
+  const char *xr = (const char *)a.x + (size_t)t * a.x_ld * (XF32 ? 4 : 2);
+  const uint16_t *A = a.a[p] + (size_t)ad * a.R * a.K;
+  int r = first;
+  for (; r + step < rank; r += 2 * step) {
+    float s[2];
+    row_dots<XF32, 2>(xr, A + (size_t)r * a.K, (size_t)step * a.K, a.K, lane, s);
+    put(r, s[0]);
+    put(r + step, s[1]);
+  }
+  if (r < rank) {
+    float s[1];
+    row_dots<XF32, 1>(xr, A + (size_t)r * a.K, 0, a.K, lane, s);
+    put(r, s[0]);
+  }
+}
+
+template <bool XF32>
+__global__ __launch_bounds__(64 * R_WAVES) void k_lora_rows(LoraArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x, p = blockIdx.z;
+  const int ad = a.ids[t];
+  if (ad < 0 || ad >= a.N) return;
+  float *v = a.v + ((size_t)p * a.T + t) * a.R;
+  const int step = gridDim.y * R_WAVES;
+  token_rows<XF32>(a, p, t, ad, blockIdx.y * R_WAVES + wave, step, rank_of(a, ad), lane,
+                   [&](int r, float s) {
+                     if (lane == 0) v[r] = s;
+                   });
+}
+
+template <int M>
+__device__ __forceinline__ float xor_lane(float v) {
+  if constexpr (M == 1)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
+  else if constexpr (M == 2)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false));
+  else
+    return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), (M << 10) | 0x1F));
+}
+// Lane s of a run of LR lanes gets the run's sum of d[s]: at each step a lane
+// keeps one half of its values and receives its partner's of the same half.
+template <int LR, int M = LR / 2>
+__device__ __forceinline__ void sum_transpose(float (&d)[LR], int s) {
+  if constexpr (M >= 1) {
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const bool up = s & M;
+      const float keep = up ? d[j + M] : d[j], send = up ? d[j] : d[j + M];
+      d[j] = keep + xor_lane<M>(send);
+    }
+    sum_transpose<LR, M / 2>(d, s);
+  }
+}
+
+// One token's rows of y.  LR lanes share a row of B, 8 of its columns each, so a
+// wave reads 1 KB of consecutive rows per load; LR loads cover 64 rows, whose
+// sums end one per lane, in order.  FUSED: v is computed here, in LDS, with the
+// first rows of B and y already in flight.
+template <int LR, bool FUSED, bool XF32, bool YF32>
+__global__ __launch_bounds__(64 * D_WAVES) void k_lora_dec(LoraArgs a) {
+  constexpr int G = LR >= 8 ? 1 : 8 / LR;  // groups of 64 rows in flight
+  constexpr int RW = 64 / LR;              // rows of a load
+  __shared__ float s_v[FUSED ? 128 : 1];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x, p = blockIdx.z, M = a.m[p];
+  const int ad = a.ids[t];
+  if (ad < 0 || ad >= a.N) return;
+  const int rank = rank_of(a, ad);
+  if (rank == 0) return;
+  const int g0 = (blockIdx.y * D_WAVES + wave) * a.units;  // this wave's groups of 64 rows
+  const int g1 = min(g0 + a.units, (M + 63) / 64);
+  if (blockIdx.y * D_WAVES * a.units * 64 >= M) return;
+  const float scale = a.scales ? a.scales[ad] : 1.0f;
+  const int s = lane & (LR - 1), rs = lane / LR, r0 = s * 8;
+  const uint16_t *B = a.b[p] + (size_t)ad * M * a.R;
+  const size_t yrow = (size_t)t * a.y_ld[p];
+
+  u32x4 w[G][LR];
+  float y[G];
+  auto load = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      if (g + i >= g1) continue;
+#pragma unroll
+      for (int j = 0; j < LR; ++j) {
+        w[i][j] = (u32x4){0, 0, 0, 0};
+        const int m = min((g + i) * 64 + j * RW + rs, M - 1);
+        if (r0 < rank) w[i][j] = *(const u32x4 *)(B + (size_t)m * a.R + r0);
+      }
+      const int m = (g + i) * 64 + s * RW + rs;
+      if (m < M)
+        y[i] = YF32 ? ((const float *)a.y[p])[yrow + m]
+                    : bf16_to_f32(((const uint16_t *)a.y[p])[yrow + m]);
+    }
+  };
+  load(g0);
+  __builtin_amdgcn_sched_barrier(0);
+  float v[8];
+  if constexpr (FUSED) {
+    token_rows<XF32>(a, p, t, ad, wave, D_WAVES, rank, lane, [&](int r, float d) {
+      if (lane == 0) s_v[r] = d;
+    });
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r0 + i < rank ? s_v[r0 + i] * scale : 0.0f;
+  } else {
+    const float *src = a.v + ((size_t)p * a.T + t) * a.R;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r0 + i < rank ? src[r0 + i] * scale : 0.0f;
+  }
+  u32x4 keep;  // clears B's columns from rank on (they may hold anything)
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    keep[i] = (r0 + 2 * i < rank ? 0xFFFFu : 0u) | (r0 + 2 * i + 1 < rank ? 0xFFFF0000u : 0u);
+  for (int g = g0; g < g1; g += G) {
+    if (g != g0) load(g);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      if (g + i >= g1) continue;
+      float d[LR];
+#pragma unroll
+      for (int j = 0; j < LR; ++j) {
+        const u32x4 b = w[i][j] & keep;
+        float acc = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc = fmaf(v[2 * e], bf16_lo(b[e]), acc);
+          acc = fmaf(v[2 * e + 1], bf16_hi(b[e]), acc);
+        }
+        d[j] = acc;
+      }
+      sum_transpose<LR>(d, s);
+      const int m = (g + i) * 64 + s * RW + rs;
+      if (m < M) {
+        if constexpr (YF32)
+          ((float *)a.y[p])[yrow + m] = y[i] + d[0];
+        else
+          ((uint16_t *)a.y[p])[yrow + m] = f32_to_bf16(y[i] + d[0]);
+      }
+    }
+  }
+}
+
+// ---- prompts ------------------------------------------------------------------
 
 // N values that sum to x, each exact in bf16 (x's bits from the top, 8 at a
 // time: N = 3 holds all 24, N = 2 x to 2^-16), as fp32 with the low half clear.
@@ -52,225 +303,361 @@ __device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
-// ids of a tile's tokens, one per lane below tt; -1 = none
+template <bool YF32>
+struct alignas(YF32 ? 16 : 8) YRun {  // 4 values of y
+  uint32_t v[YF32 ? 4 : 2];
+};
+
+// ids of a tile's tokens, one per lane below 16; -1 = none
 __device__ __forceinline__ int tile_ids(const LoraArgs &a, int t0, int lane) {
   int id = -1;
-  if (lane < a.tt && t0 + lane < a.T) id = a.ids[t0 + lane];
+  if (lane < TT && t0 + lane < a.T) id = a.ids[t0 + lane];
   return id >= 0 && id < a.N ? id : -1;
 }
 
-// NRB: blocks of 16 rows of A.  A wave sums kw blocks of KB columns, the
-// workgroup's four waves meet in LDS.
-template <int NRB, bool XF32>
-__global__ __launch_bounds__(64 * L_WAVES) void k_lora_down(LoraArgs a) {
-  __shared__ f32x4 red[L_WAVES][NRB][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * a.tt, p = blockIdx.z;
-  const int id = tile_ids(a, t0, lane);
-  uint64_t rem = __ballot(id >= 0);
-  const int col = lane & 15, q = lane >> 4;
-  const int row = min(t0 + min(col, a.tt - 1), a.T - 1);
-  const int nb = (a.K + KB - 1) / KB;
-  const int b0 = (blockIdx.y * L_WAVES + wave) * a.kw, b1 = min(b0 + a.kw, nb);
-  const char *xr = (const char *)a.x + (size_t)row * a.x_ld * (XF32 ? 4 : 2);
-  while (rem) {
-    const int ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(rem));
-    const uint64_t mask = __ballot(id == ad) & rem;
-    rem &= ~mask;
-    const uint16_t *A = a.a[p] + (size_t)ad * a.R * a.K;
-    f32x4 acc[NRB];
-#pragma unroll
-    for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const uint16_t *ar[NRB];
-#pragma unroll
-    for (int r = 0; r < NRB; ++r) ar[r] = A + (size_t)min(r * 16 + col, a.R - 1) * a.K;
-    for (int b = b0; b < b1; ++b) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = b * KB + q * 16 + h * 8;
-        const bool in = k < a.K;  // K is a multiple of 8
-        u32x4 af[NRB];
-#pragma unroll
-        for (int r = 0; r < NRB; ++r) af[r] = in ? *(const u32x4 *)(ar[r] + k) : (u32x4){0, 0, 0, 0};
-        if constexpr (!XF32) {
-          const u32x4 xf = in ? *(const u32x4 *)((const uint16_t *)xr + k) : (u32x4){0, 0, 0, 0};
-#pragma unroll
-          for (int r = 0; r < NRB; ++r) acc[r] = mfma_bf16_16x16x32(af[r], xf, acc[r]);
-        } else {
-          f32x4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
-          if (in) {
-            v0 = *(const f32x4 *)((const float *)xr + k);
-            v1 = *(const f32x4 *)((const float *)xr + k + 4);
-          }
-          u32x4 xf[3];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float lo[3], hi[3];
-            split_bf16(i < 2 ? v0[2 * i] : v1[2 * i - 4], lo);
-            split_bf16(i < 2 ? v0[2 * i + 1] : v1[2 * i - 3], hi);
-#pragma unroll
-            for (int s = 0; s < 3; ++s) xf[s][i] = pack_hi(lo[s], hi[s]);
-          }
-#pragma unroll
-          for (int s = 0; s < 3; ++s)
-#pragma unroll
-            for (int r = 0; r < NRB; ++r) acc[r] = mfma_bf16_16x16x32(af[r], xf[s], acc[r]);
-        }
-      }
-    }
-    __syncthreads();  // the previous adapter's sums are read
-#pragma unroll
-    for (int r = 0; r < NRB; ++r) red[wave][r][lane] = acc[r];
-    __syncthreads();
-    for (int r = wave; r < NRB; r += L_WAVES) {
-      f32x4 v = red[0][r][lane];
-#pragma unroll
-      for (int w = 1; w < L_WAVES; ++w) v += red[w][r][lane];
-      const int r0 = r * 16 + q * 4;
-      if (((mask >> col) & 1) && r0 < a.R)
-        *(f32x4 *)(a.part + (((size_t)blockIdx.y * a.P + p) * a.T + t0 + col) * a.R + r0) = v;
-    }
-  }
+__device__ __forceinline__ void lds_order() {  // a wave's own LDS writes before its reads
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// NRK: blocks of 32 columns of B; NS: bf16 values that v enters as
-template <int NRK, int NS, bool YF32>
-__global__ __launch_bounds__(64 * L_WAVES) void k_lora_up(LoraArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * a.tt, p = blockIdx.z;
-  const int M = a.m[p];
-  const int u0 = (blockIdx.y * L_WAVES + wave) * a.units;
-  if (u0 * 32 >= M) return;
-  const int u1 = min(u0 + a.units, (M + 31) / 32);
-  const int id = tile_ids(a, t0, lane);
-  uint64_t rem = __ballot(id >= 0);
-  const int col = lane & 15, q = lane >> 4;
-  const int row = min(t0 + col, a.T - 1);
-  while (rem) {
-    const int ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(rem));
-    const uint64_t mask = __ballot(id == ad) & rem;
-    rem &= ~mask;
-    int rank = a.R;
-    if (a.ranks) rank = min(max(a.ranks[ad], 0), a.R);
-    if (rank == 0) continue;
-    const float scale = a.scales ? a.scales[ad] : 1.0f;
-    const bool mine = (mask >> col) & 1;
-    u32x4 vf[NRK][NS], keep[NRK];
+// 16 rows of CK columns, read by one wave as whole rows (LPR lanes a row, 16
+// bytes each) and handed to the MFMA's layout (lane (q, col): row col, columns
+// 32 s + 8 q) through 16 x CK x 2 bytes of its LDS.  A load straight into that
+// layout touches a line per lane, four times what whole rows do.  Piece c of
+// row r lies at place c ^ swz(r) of its row, so that neither side meets a bank
+// twice.
+template <int CK>
+struct Panel {
+  static constexpr int LPR = CK / 8, LOADS = LPR / 4, RPL = 64 / LPR;
+  static __device__ __forceinline__ int swz(int row) { return CK == 128 ? row & 15 : (row >> 1) & 7; }
+  u32x4 v[LOADS];
+  // row i * RPL + lane / LPR at base + row * pitch, columns k0 + (lane % LPR) * 8
+  __device__ __forceinline__ void load(const uint16_t *base, int pitch, int rows, int k0, int K,
+                                       int lane) {
+    const int k = k0 + (lane & (LPR - 1)) * 8;
 #pragma unroll
-    for (int rb = 0; rb < NRK; ++rb) {
-      const int r0 = rb * 32 + q * 8;
-      f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-      if (mine && r0 < a.R)
-        for (int ks = 0; ks < a.splits; ++ks) {
-          const float *v = a.part + (((size_t)ks * a.P + p) * a.T + row) * a.R + r0;
-          s0 += *(const f32x4 *)v;
-          s1 += *(const f32x4 *)(v + 4);
-        }
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = i * RPL + lane / LPR;
+      v[i] = (u32x4){0, 0, 0, 0};
+      if (r < rows && k < K) v[i] = *(const u32x4 *)(base + (size_t)r * pitch + k);
+    }
+  }
+  __device__ __forceinline__ void to_lds(u32x4 *buf, int lane) const {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 2 * i;
-        float lo[NS], hi[NS];
-        split_bf16(r < rank ? (i < 2 ? s0[2 * i] : s1[2 * i - 4]) * scale : 0.0f, lo);
-        split_bf16(r + 1 < rank ? (i < 2 ? s0[2 * i + 1] : s1[2 * i - 3]) * scale : 0.0f, hi);
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = i * RPL + lane / LPR;
+      buf[r * LPR + ((lane & (LPR - 1)) ^ swz(r))] = v[i];
+    }
+  }
+  static __device__ __forceinline__ void frags(const u32x4 *buf, int lane, u32x4 (&f)[CK / 32]) {
+    const int col = lane & 15, q = lane >> 4;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) vf[rb][s][i] = pack_hi(lo[s], hi[s]);
-        keep[rb][i] = (r < rank ? 0xFFFFu : 0u) | (r + 1 < rank ? 0xFFFF0000u : 0u);
+    for (int s = 0; s < CK / 32; ++s) f[s] = buf[col * LPR + ((s * 4 + q) ^ swz(col))];
+  }
+};
+
+// the same of fp32 rows: the wave splits what it read, one plane of bf16 each
+struct PanelF32 {
+  static constexpr int CK = 64, LPR = 16;
+  u32x4 v[4];  // row i * 4 + lane / 16, columns k0 + (lane % 16) * 4
+  __device__ __forceinline__ void to_lds(u32x4 *buf, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 4 + lane / 16, piece = (lane & 15) >> 1;
+      float e[4][3];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_bf16(__uint_as_float(v[i][j]), e[j]);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        u32x2 w = {pack_hi(e[0][s], e[1][s]), pack_hi(e[2][s], e[3][s])};
+        u32x4 *row = buf + s * 128 + r * 8;
+        ((u32x2 *)(row + (piece ^ Panel<CK>::swz(r))))[lane & 1] = w;
       }
     }
-    const uint16_t *B = a.b[p] + (size_t)ad * M * a.R;
-    for (int u = u0; u < u1; ++u) {
-      // rows of B so that a lane ends with 8 consecutive ones of its token
-      const int m0 = u * 32, mr = m0 + (col >> 2) * 8 + (col & 3);
-      f32x4 acc[2];
+  }
+};
+
+// One adapter's tokens of a tile of 16, all of K, then all of this workgroup's
+// rows of y.  blockIdx.x: tile (fastest, so that the first adapters of all tiles
+// start first; a workgroup of an adapter that a tile lacks ends after one load),
+// blockIdx.y: which distinct adapter of the tile, blockIdx.z: projection and
+// part of its rows.
+//   1. v = A x^T: a wave takes every T_WAVES-th chunk of CK columns; A's next rows
+//      are read while the last ones are multiplied.  The sums meet in LDS.
+//   2. v scaled, split and laid out for the MFMA.
+//   3. units of 64 rows of B: column c of MFMA j is row 4 c + j, so that a lane
+//      ends with 4 consecutive values of y of each of its 4 tokens.  B's rows
+//      are read whole and turned in LDS as A's; what the next unit reads of B
+//      and y is in flight meanwhile.
+template <int NRB, bool XF32, bool YF32>
+__global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
+  constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
+  constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
+  constexpr int RING = NRB < 4 ? NRB : 4;  // panels of A in flight
+  constexpr int STAGE = 512;               // 16-byte pieces of a wave's LDS: 8 KB
+  constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it
+  __shared__ u32x4 s_stage[T_WAVES][STAGE];
+  __shared__ u32x2 s_v[NRK][NS][64][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = blockIdx.x * TT, p = blockIdx.z % a.P, part = blockIdx.z / a.P;
+  const int M = a.m[p];
+  const int id = tile_ids(a, t0, lane);
+  uint64_t rem = __ballot(id >= 0), mask = 0;
+  int ad = -1;
+  for (int i = 0; i <= (int)blockIdx.y && rem; ++i) {
+    ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(rem));
+    mask = __ballot(id == ad) & rem;
+    rem &= ~mask;
+    if (i < (int)blockIdx.y) ad = -1;
+  }
+  if (ad < 0) return;
+  const int rank = rank_of(a, ad);
+  const int u0 = part * a.units * T_WAVES, u_end = min(u0 + a.units * T_WAVES, (M + 63) / 64);
+  if (rank == 0 || u0 * 64 >= M) return;
+  const float scale = a.scales ? a.scales[ad] : 1.0f;
+  const int col = lane & 15, q = lane >> 4;
+  u32x4 *stage = s_stage[wave];
+
+  // 1.
+  f32x4 acc[NRB];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint16_t *br = B + (size_t)min(mr + j * 4, M - 1) * a.R;
-        acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  {
+    const uint16_t *A = a.a[p] + (size_t)ad * a.R * a.K;
+    const int nc = (a.K + CK - 1) / CK;
+    Panel<CK> pa[RING];
+    typename std::conditional<XF32, PanelF32, Panel<CK>>::type px;
+    auto load_a = [&](int r, int c) {
+      pa[r % RING].load(A + (size_t)r * 16 * a.K, a.K, a.R - r * 16, c * CK, a.K, lane);
+    };
+    auto load_x = [&](int c) {
+      constexpr int EPL = XF32 ? 4 : 8;  // elements a lane, 16 lanes a row
+      const int k = c * CK + (lane & 15) * EPL;
 #pragma unroll
-        for (int rb = 0; rb < NRK; ++rb) {
-          const int r0 = rb * 32 + q * 8;
-          u32x4 bf = {0, 0, 0, 0};
-          if (r0 < rank) bf = *(const u32x4 *)(br + r0) & keep[rb];
-#pragma unroll
-          for (int s = 0; s < NS; ++s) acc[j] = mfma_bf16_16x16x32(bf, vf[rb][s], acc[j]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const size_t row = min(t0 + i * 4 + lane / 16, a.T - 1);
+        px.v[i] = (u32x4){0, 0, 0, 0};
+        if (k < a.K)
+          px.v[i] = *(const u32x4 *)((const char *)a.x + (row * a.x_ld + k) * (XF32 ? 4 : 2));
       }
-      const int m = m0 + q * 8;
-      if (!mine || m >= M) continue;
-      const size_t at = (size_t)row * a.y_ld[p] + m;
-      if (a.y_vec[p] && m + 8 <= M) {
-        if constexpr (YF32) {
-          f32x4 *y = (f32x4 *)((float *)a.y[p] + at);
-          y[0] += acc[0];
-          y[1] += acc[1];
-        } else {
-          u32x4 *y = (u32x4 *)((uint16_t *)a.y[p] + at);
-          u32x4 v = *y;
+    };
+    if (wave < nc) {
+      load_x(wave);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float lo = __uint_as_float(v[i] << 16) + acc[i / 2][2 * (i & 1)];
-            const float hi = __uint_as_float(v[i] & 0xFFFF0000u) + acc[i / 2][2 * (i & 1) + 1];
-            v[i] = (uint32_t)f32_to_bf16(lo) | ((uint32_t)f32_to_bf16(hi) << 16);
-          }
-          *y = v;
+      for (int r = 0; r < RING; ++r) load_a(r, wave);
+    }
+    for (int c = wave; c < nc; c += T_WAVES) {
+      const int next = c + T_WAVES;
+      u32x4 xf[NX][KS];
+      px.to_lds(stage, lane);
+      if (next < nc) load_x(next);
+      lds_order();
+#pragma unroll
+      for (int s = 0; s < NX; ++s) Panel<CK>::frags(stage + s * 128, lane, xf[s]);
+#pragma unroll
+      for (int r = 0; r < NRB; ++r) {
+        u32x4 *buf = stage + XPART;
+        pa[r % RING].to_lds(buf, lane);
+        if (r + RING < NRB) load_a(r + RING, c);
+        else if (next < nc) load_a((r + RING) % NRB, next);
+        lds_order();
+        u32x4 af[KS];
+        Panel<CK>::frags(buf, lane, af);
+#pragma unroll
+        for (int s = 0; s < NX; ++s)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) acc[r] = mfma_bf16_16x16x32(af[k], xf[s][k], acc[r]);
+        lds_order();
+      }
+    }
+  }
+  __syncthreads();  // every wave is done with its stage
+  {
+    f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
+#pragma unroll
+    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane] = acc[r];
+  }
+  __syncthreads();
+  // 2. ranks rb * 16 + q * 4 .. + 3 of token col
+  for (int rb = wave; rb < 2 * NRK; rb += T_WAVES) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (rb < NRB) {
+      const f32x4 *red = (const f32x4 *)s_stage;
+#pragma unroll
+      for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane];
+    }
+    float e[4][NS];
+    const int r0 = rb * 16 + q * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_bf16(r0 + i < rank ? v[i] * scale : 0.0f, e[i]);
+    const int slot = ((r0 & 31) >> 3) * 16 + col;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      s_v[rb >> 1][s][slot][(r0 >> 2) & 1] =
+          (u32x2){pack_hi(e[0][s], e[1][s]), pack_hi(e[2][s], e[3][s])};
+  }
+  __syncthreads();
+
+  // 3.
+  constexpr int CP = NRK * 4;              // pieces of a row of B, padded
+  constexpr int HALF = NRK == 4 ? 2 : 1;   // a unit's pieces pass the stage in halves
+  constexpr int HC = CP / HALF, HB = NRK / HALF;
+  const int cpr = a.R / 8;
+  const uint16_t *B = a.b[p] + (size_t)ad * M * a.R;
+  // piece i * 64 + lane of a unit: its place in the stage (0xFFFF: not in this half)
+  int place[CP];
+#pragma unroll
+  for (int i = 0; i < CP; ++i) {
+    const int l = i * 64 + lane, row = l / cpr, ch = l - row * cpr;
+    const int s = row >> 2;
+    place[i] = s * 4 * HC + (((row & 3) * HC + ch % HC) ^ (s & 15)) + (ch / HC) * 0x10000;
+    if (i >= cpr) place[i] = -1;
+  }
+  u32x4 keep[NRK];  // clears B's columns from rank on (they may hold anything)
+#pragma unroll
+  for (int rb = 0; rb < NRK; ++rb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = rb * 32 + q * 8 + 2 * i;
+      keep[rb][i] = (r < rank ? 0xFFFFu : 0u) | (r + 1 < rank ? 0xFFFF0000u : 0u);
+    }
+  u32x4 vf[NRK][NS];
+#pragma unroll
+  for (int rb = 0; rb < NRK; ++rb)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) vf[rb][s] = *(const u32x4 *)s_v[rb][s][lane];
+
+  u32x4 w[CP];
+  YRun<YF32> y[4];
+  auto y_at = [&](int u, int i) {
+    return (char *)a.y[p] +
+           ((size_t)(t0 + q * 4 + i) * a.y_ld[p] + u * 64 + 4 * col) * (YF32 ? 4 : 2);
+  };
+  auto load_b = [&](int u) {
+    const int left = (M - u * 64) * cpr;  // pieces of B from this unit on
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int l = i * 64 + lane;
+      w[i] = (u32x4){0, 0, 0, 0};
+      if (i < cpr && l < left) w[i] = *(const u32x4 *)(B + ((size_t)u * 64 * cpr + l) * 8);
+    }
+  };
+  auto whole = [&](int u) { return a.y_vec[p] && u * 64 + 4 * col + 4 <= M; };
+  auto load_y = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (whole(u) && ((mask >> (q * 4 + i)) & 1)) y[i] = *(const YRun<YF32> *)y_at(u, i);
+  };
+  int u = u0 + wave;
+  if (u < u_end) {
+    load_b(u);
+    load_y(u);
+  }
+  for (; u < u_end; u += T_WAVES) {
+    f32x4 d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < HALF; ++h) {
+#pragma unroll
+      for (int i = 0; i < CP; ++i)
+        if (place[i] >= 0 && (HALF == 1 || place[i] >> 16 == h)) stage[place[i] & 0xFFFF] = w[i];
+      if (h == HALF - 1 && u + T_WAVES < u_end) load_b(u + T_WAVES);
+      lds_order();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int rb = 0; rb < HB; ++rb) {
+          const u32x4 b = stage[col * 4 * HC + ((j * HC + rb * 4 + q) ^ col)] & keep[h * HB + rb];
+#pragma unroll
+          for (int s = 0; s < NS; ++s) d[j] = mfma_bf16_16x16x32(vf[h * HB + rb][s], b, d[j]);
         }
+      lds_order();
+    }
+    const bool vec = whole(u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!((mask >> (q * 4 + i)) & 1)) continue;
+      if (vec) {
+        YRun<YF32> o;
+        if constexpr (YF32) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o.v[j] = __float_as_uint(__uint_as_float(y[i].v[j]) + d[j][i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            o.v[j] = bf16x2_bits(bf16_lo(y[i].v[j]) + d[2 * j][i], bf16_hi(y[i].v[j]) + d[2 * j + 1][i]);
+        }
+        *(YRun<YF32> *)y_at(u, i) = o;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (m + i < M) {
+        for (int j = 0; j < 4; ++j)
+          if (u * 64 + 4 * col + j < M) {
             if constexpr (YF32) {
-              ((float *)a.y[p])[at + i] += acc[i / 4][i & 3];
+              ((float *)y_at(u, i))[j] += d[j][i];
             } else {
-              uint16_t *y = (uint16_t *)a.y[p] + at + i;
-              *y = f32_to_bf16(bf16_to_f32(*y) + acc[i / 4][i & 3]);
+              uint16_t *e = (uint16_t *)y_at(u, i) + j;
+              *e = f32_to_bf16(bf16_to_f32(*e) + d[j][i]);
             }
           }
       }
     }
+    if (u + T_WAVES < u_end) load_y(u + T_WAVES);
   }
 }
 
+// ---- launches -----------------------------------------------------------------
+
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Tokens per tile: one while a batch of requests (an adapter per token) fills
-// the device with a workgroup each, 16 for prompts.
-int tile_tokens(int T) { return T <= 64 ? 1 : T <= 256 ? 4 : LT; }
+#ifndef LORA_DEC_MAX_T
+#define LORA_DEC_MAX_T 128
+#endif
+#ifndef LORA_FUSED_BYTES
+#define LORA_FUSED_BYTES (256 << 10)
+#endif
 
-// Parts of K over workgroups: about LORA_WGS workgroups, a wave no less than one
-// block of KB columns.
-constexpr int LORA_WGS = 512, MAX_SPLITS = 16;
-int k_splits(const ainfer_moe_lora &l, int T) {
-  const int tiles = div_up(T, tile_tokens(T)) * l.n_proj;
-  const int most = div_up(div_up(l.in, KB), L_WAVES);
-  const int want = LORA_WGS / (tiles < LORA_WGS ? tiles : LORA_WGS);
-  const int n = want < most ? want : most;
-  return n < MAX_SPLITS ? n : MAX_SPLITS;
+template <int LR, bool FUSED>
+void launch_dec(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
+  const dim3 b(64 * D_WAVES);
+  if constexpr (FUSED) {
+    if (xf32) {
+      if (yf32) k_lora_dec<LR, true, true, true><<<grid, b, 0, s>>>(a);
+      else k_lora_dec<LR, true, true, false><<<grid, b, 0, s>>>(a);
+      return;
+    }
+  }
+  if (yf32) k_lora_dec<LR, FUSED, false, true><<<grid, b, 0, s>>>(a);
+  else k_lora_dec<LR, FUSED, false, false><<<grid, b, 0, s>>>(a);
 }
-
-template <int NRK>
-void launch_up(const LoraArgs &a, dim3 grid, bool yf32, hipStream_t s) {
-  if (yf32)
-    k_lora_up<NRK, 3, true><<<grid, 64 * L_WAVES, 0, s>>>(a);
-  else
-    k_lora_up<NRK, 2, false><<<grid, 64 * L_WAVES, 0, s>>>(a);
+template <bool FUSED>
+void launch_dec_lr(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
+  if (a.R <= 8) launch_dec<1, FUSED>(a, grid, xf32, yf32, s);
+  else if (a.R <= 16) launch_dec<2, FUSED>(a, grid, xf32, yf32, s);
+  else if (a.R <= 32) launch_dec<4, FUSED>(a, grid, xf32, yf32, s);
+  else if (a.R <= 64) launch_dec<8, FUSED>(a, grid, xf32, yf32, s);
+  else launch_dec<16, FUSED>(a, grid, xf32, yf32, s);
 }
 template <int NRB>
-void launch_down(const LoraArgs &a, dim3 grid, bool xf32, hipStream_t s) {
-  if (xf32)
-    k_lora_down<NRB, true><<<grid, 64 * L_WAVES, 0, s>>>(a);
-  else
-    k_lora_down<NRB, false><<<grid, 64 * L_WAVES, 0, s>>>(a);
+void launch_tile(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
+  const dim3 b(64 * T_WAVES);
+  if (xf32) {
+    if (yf32) k_lora_tile<NRB, true, true><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<NRB, true, false><<<grid, b, 0, s>>>(a);
+  } else {
+    if (yf32) k_lora_tile<NRB, false, true><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<NRB, false, false><<<grid, b, 0, s>>>(a);
+  }
 }
 
 }  // namespace
 
-// The parts of every call with up to max_tokens tokens: k_splits(T) * T is T
-// itself, or at most LORA_WGS tiles' tokens, or MAX_SPLITS * T.
+// v of k_lora_rows
 size_t lora_workspace_bytes(const ainfer_moe_lora &l, int max_tokens) {
-  const size_t T = max_tokens, wide = (size_t)LORA_WGS * tile_tokens(max_tokens);
-  const size_t split = T * MAX_SPLITS < wide ? T * MAX_SPLITS : wide;
-  const size_t n = (T > split ? T : split) * l.n_proj * l.rank * sizeof(float);
-  return (n + 255) & ~(size_t)255;
+  const size_t T = max_tokens < LORA_DEC_MAX_T ? max_tokens : LORA_DEC_MAX_T;
+  const size_t n = T * l.n_proj * l.rank * sizeof(float);
+  return n > 256 ? (n + 255) & ~(size_t)255 : 256;
 }
 
 hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, const int32_t *ids,
@@ -281,17 +668,12 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   a.ranks = l.ranks;
   a.scales = l.scales;
   a.x_ld = x_ld;
-  a.part = (float *)ws;
+  a.v = (float *)ws;
   a.N = l.n_adapters;
   a.R = l.rank;
   a.K = l.in;
   a.P = l.n_proj;
   a.T = T;
-  a.tt = tile_tokens(T);
-  a.splits = k_splits(l, T);
-  const int nb = div_up(l.in, KB);
-  a.kw = div_up(nb, a.splits * L_WAVES);
-  a.splits = div_up(nb, a.kw * L_WAVES);  // none empty
   const bool yf32 = l.y_dtype == AINFER_ACT_F32, xf32 = l.x_dtype == AINFER_ACT_F32;
   const int ysz = yf32 ? 4 : 2;
   int m_most = 1;
@@ -302,24 +684,38 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     a.y[p] = on ? y[p] : nullptr;
     a.y_ld[p] = on ? y_ld[p] : 0;
     a.m[p] = on ? l.out[p] : 0;
-    a.y_vec[p] = on && (uintptr_t)y[p] % 16 == 0 && (y_ld[p] * ysz) % 16 == 0;
+    a.y_vec[p] = on && (uintptr_t)y[p] % (4 * ysz) == 0 && y_ld[p] % 4 == 0;
     if (on && l.out[p] > m_most) m_most = l.out[p];
   }
-  const int tiles = div_up(T, a.tt);
-  const int nrb = div_up(l.rank, 16), nrk = div_up(l.rank, 32);
-  const dim3 gd(tiles, a.splits, l.n_proj);
-  if (nrb <= 1) launch_down<1>(a, gd, xf32, s);
-  else if (nrb <= 2) launch_down<2>(a, gd, xf32, s);
-  else if (nrb <= 4) launch_down<4>(a, gd, xf32, s);
-  else launch_down<8>(a, gd, xf32, s);
-  // rows of y over the workgroups
-  const int units = div_up(m_most, 32);
-  int per = div_up(units * tiles * l.n_proj, 4096);
-  per = per < 1 ? 1 : per > 8 ? 8 : per;
-  a.units = per;
-  const dim3 gu(tiles, div_up(units, per * L_WAVES), l.n_proj);
-  if (nrk <= 1) launch_up<1>(a, gu, yf32, s);
-  else if (nrk <= 2) launch_up<2>(a, gu, yf32, s);
-  else launch_up<4>(a, gu, yf32, s);
+  if (T <= LORA_DEC_MAX_T) {
+    const int groups = div_up(m_most, 64);
+    // about DEC_WGS workgroups
+    int per = div_up(groups * T * l.n_proj, 1024 * D_WAVES);
+    const bool fused = (size_t)l.rank * l.in * 2 <= LORA_FUSED_BYTES;
+    a.units = per;
+    const dim3 grid(T, div_up(groups, per * D_WAVES), l.n_proj);
+    if (fused) {
+      launch_dec_lr<true>(a, grid, xf32, yf32, s);
+    } else {
+      const dim3 gr(T, div_up(l.rank, 2 * R_WAVES), l.n_proj);
+      if (xf32) k_lora_rows<true><<<gr, 64 * R_WAVES, 0, s>>>(a);
+      else k_lora_rows<false><<<gr, 64 * R_WAVES, 0, s>>>(a);
+      launch_dec_lr<false>(a, grid, xf32, yf32, s);
+    }
+    return hipGetLastError();
+  }
+  const int tiles = div_up(T, TT), units = div_up(m_most, 64);
+  // parts of y's rows, each of which computes v again, while tiles leave CUs idle
+  int parts = 256 / (tiles * l.n_proj);
+  parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
+  a.units = div_up(units, parts * T_WAVES);
+  parts = div_up(units, a.units * T_WAVES);
+  const int slots = l.n_adapters < TT ? l.n_adapters : TT;
+  const dim3 grid(tiles, slots, l.n_proj * parts);
+  const int nrb = div_up(l.rank, 16);
+  if (nrb <= 1) launch_tile<1>(a, grid, xf32, yf32, s);
+  else if (nrb <= 2) launch_tile<2>(a, grid, xf32, yf32, s);
+  else if (nrb <= 4) launch_tile<4>(a, grid, xf32, yf32, s);
+  else launch_tile<8>(a, grid, xf32, yf32, s);
   return hipGetLastError();
 }

@@ -251,69 +251,78 @@ def rmsnorm(x, y, w=None, mode=L.NORM_PLAIN, eps=1e-6, stream=None):
 
 
 # ---- the operators around the expert stage -----------------------------------
+# These calls are short (a kernel takes a few microseconds), so the checks below
+# read each tensor attribute once and pass plain integers to the library.
 _ACT = {torch.float32: L.ACT_F32, torch.bfloat16: L.ACT_BF16}
 
 
-def _require(ok, what):
-    if not ok:
-        raise L.MoeError(what)
-
-
 def _rows(t, name, cols=None):
-    """A device matrix of fp32 or bf16 rows, each contiguous: (dtype, pitch)."""
-    _require(t.dim() == 2 and t.dtype in _ACT, f"{name}: rows of fp32 or bf16")
-    _require(t.is_cuda, f"{name}: a device tensor")
-    _require(cols is None or t.shape[1] == cols, f"{name}: {cols} columns")
-    _require(t.shape[1] == 1 or t.stride(1) == 1, f"{name}: contiguous rows")
-    # a single row has no pitch
-    return _ACT[t.dtype], max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    """A device matrix of fp32 or bf16 rows, each contiguous: (dtype, rows,
+    columns, pitch)."""
+    dt = _ACT.get(t.dtype)
+    if dt is None or not t.is_cuda or t.dim() != 2:
+        raise L.MoeError(f"{name}: a device matrix of fp32 or bf16 rows")
+    (n, m), (ld, one) = t.shape, t.stride()
+    if (cols is not None and m != cols) or (one != 1 and m != 1):
+        raise L.MoeError(f"{name}: contiguous rows" + (f" of {cols} columns" if cols else ""))
+    return dt, n, m, (ld if n > 1 else m)  # a single row has no pitch
 
 
 def _vector(t, name, dtype, n, device):
-    _require(t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == device,
-             f"{name}: {n} contiguous {dtype} values on the inputs' device")
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+        raise L.MoeError(f"{name}: {n} contiguous {dtype} values on the inputs' device")
 
 
 def _call(fn, device, stream, *args):
-    """fn(*args, stream) on the device the tensors are on."""
-    if device.index is not None and device.index != torch.cuda.current_device():
+    """fn(*args, stream) on the device the tensors are on; its current stream
+    when none is given."""
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return L.check(fn(*args, _stream(stream)))
-    return L.check(fn(*args, _stream(stream)))
+            return _enqueue(fn, device, stream, args)
+    return _enqueue(fn, device, stream, args)
+
+
+def _enqueue(fn, device, stream, args):
+    raw = (torch._C._cuda_getCurrentRawStream(device.index) if stream is None
+           else stream.cuda_stream)
+    rc = fn(*args, raw)
+    if rc:
+        L.check(rc)
 
 
 def route_scored(routing, logits, bias=None, out=None, stream=None):
     """Scored routing of logits [T][E] (ainfer_moe_route_scored; routing: an
     L.Routing): (topk_idx [T][k] int32, topk_w [T][k] fp32), as MoeLayer.dispatch,
     experts and combine take them.  out: the two tensors to write."""
-    dt, ld = _rows(logits, "logits", routing.n_experts)
-    T, k = logits.shape[0], routing.top_k
+    dt, T, E, ld = _rows(logits, "logits", routing.n_experts)
+    dev, k = logits.device, routing.top_k
     if bias is not None:
-        _vector(bias, "bias", torch.float32, routing.n_experts, logits.device)
+        _vector(bias, "bias", torch.float32, E, dev)
     if out is None:
-        out = (torch.empty(T, k, dtype=torch.int32, device=logits.device),
-               torch.empty(T, k, dtype=torch.float32, device=logits.device))
-    idx, w = out
-    for t, d in ((idx, torch.int32), (w, torch.float32)):
-        _require(t.shape == (T, k) and t.dtype == d and t.is_contiguous()
-                 and t.device == logits.device, "out: (idx int32, w fp32), [T][k] contiguous")
-    _call(L.lib().ainfer_moe_route_scored, logits.device, stream, C.byref(routing), _ptr(logits),
-          dt, ld, _ptr(bias), T, _ptr(idx), _ptr(w))
+        idx = torch.empty(T, k, dtype=torch.int32, device=dev)
+        w = torch.empty(T, k, dtype=torch.float32, device=dev)
+    else:
+        idx, w = out
+        if not (idx.dtype == torch.int32 and w.dtype == torch.float32
+                and idx.shape == w.shape == (T, k) and idx.device == dev == w.device
+                and idx.is_contiguous() and w.is_contiguous()):
+            raise L.MoeError("out: (idx int32, w fp32), [T][k] contiguous on the logits' device")
+    _call(L.lib().ainfer_moe_route_scored, dev, stream, C.byref(routing), logits.data_ptr(), dt,
+          ld, bias.data_ptr() if bias is not None else None, T, idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
 def silu_mul(gate, up, act, stream=None):
     """act = gate / (1 + exp(-gate)) * up over rows of any pitch
     (ainfer_moe_silu_mul)."""
-    dt, gld = _rows(gate, "gate")
-    udt, uld = _rows(up, "up", gate.shape[1])
-    adt, ald = _rows(act, "act", gate.shape[1])
-    _require(udt == dt and up.shape == gate.shape and act.shape == gate.shape
-             and up.device == gate.device and act.device == gate.device,
-             "gate, up and act: one shape and device, gate and up one type")
-    T, n = gate.shape
-    _call(L.lib().ainfer_moe_silu_mul, gate.device, stream, _ptr(gate), gld, _ptr(up), uld, dt, T,
-          n, _ptr(act), ald, adt)
+    dt, T, n, gld = _rows(gate, "gate")
+    udt, uT, _, uld = _rows(up, "up", n)
+    adt, aT, _, ald = _rows(act, "act", n)
+    dev = gate.device
+    if not (udt == dt and uT == T == aT and up.device == dev == act.device):
+        raise L.MoeError("gate, up and act: one shape and device, gate and up one type")
+    _call(L.lib().ainfer_moe_silu_mul, dev, stream, gate.data_ptr(), gld, up.data_ptr(), uld, dt,
+          T, n, act.data_ptr(), ald, adt)
     return act
 
 
@@ -325,36 +334,39 @@ class LoraAdapters:
     def __init__(self, a, b, ranks=None, scales=None, x_dtype=torch.bfloat16,
                  y_dtype=torch.bfloat16):
         a, b = list(a), list(b)
-        _require(1 <= len(a) == len(b) <= L.LORA_MAX_PROJ, "one a and one b per projection")
-        _require(x_dtype in _ACT and y_dtype in _ACT, "x and y: fp32 or bf16")
-        _require(a[0].dim() == 3, "a: [adapters][rank][columns]")
-        N, R, K = a[0].shape
+        if not 1 <= len(a) == len(b) <= L.LORA_MAX_PROJ:
+            raise L.MoeError("one a and one b for each of up to "
+                             f"{L.LORA_MAX_PROJ} projections")
+        if x_dtype not in _ACT or y_dtype not in _ACT:
+            raise L.MoeError("x and y: fp32 or bf16")
         dev = a[0].device
         for t in a + b:
-            _require(t.dtype == torch.bfloat16 and t.is_cuda and t.device == dev
-                     and t.is_contiguous() and t.dim() == 3,
-                     "a and b: contiguous bf16 on one device")
+            if not (t.dtype == torch.bfloat16 and t.is_cuda and t.device == dev
+                    and t.is_contiguous() and t.dim() == 3):
+                raise L.MoeError("a and b: contiguous [N][R][K] and [N][M][R] bf16 on one device")
+        N, R, K = a[0].shape
         for ta, tb in zip(a, b):
-            _require(ta.shape == (N, R, K) and tb.shape[0] == N and tb.shape[2] == R,
-                     "a [N][R][K] and b [N][M][R] of one N, R and K")
+            if ta.shape != (N, R, K) or tb.shape[0] != N or tb.shape[2] != R:
+                raise L.MoeError("a [N][R][K] and b [N][M][R] of one N, R and K")
         if ranks is not None:
             _vector(ranks, "ranks", torch.int32, N, dev)
         if scales is not None:
             _vector(scales, "scales", torch.float32, N, dev)
-        self.keep = (a, b, ranks, scales)
+        self.tensors = (a, b, ranks, scales)
         self.device, self.x_dtype, self.y_dtype = dev, x_dtype, y_dtype
-        n = len(a)
-        s = L.Lora(N, R, K, n, _ACT[x_dtype], _ACT[y_dtype])
-        for p in range(n):
-            s.out[p], s.a[p], s.b[p] = b[p].shape[1], a[p].data_ptr(), b[p].data_ptr()
+        self.cols, self.rows = K, [t.shape[1] for t in b]
+        s = L.Lora(N, R, K, len(a), _ACT[x_dtype], _ACT[y_dtype])
+        for p, (ta, tb) in enumerate(zip(a, b)):
+            s.out[p], s.a[p], s.b[p] = tb.shape[1], ta.data_ptr(), tb.data_ptr()
         s.ranks = ranks.data_ptr() if ranks is not None else None
         s.scales = scales.data_ptr() if scales is not None else None
-        self.s = s
-        _require(L.lib().ainfer_moe_lora_workspace_bytes(C.byref(s), 1) > 0,
-                 "adapter sizes outside the supported range")
+        self.struct = s
+        if L.lib().ainfer_moe_lora_workspace_bytes(C.byref(s), 1) == 0:
+            raise L.MoeError("adapter sizes outside the supported range")
 
     def workspace(self, max_tokens):
-        n = L.lib().ainfer_moe_lora_workspace_bytes(C.byref(self.s), max_tokens)
+        """Scratch for calls with up to max_tokens tokens (no initialisation)."""
+        n = L.lib().ainfer_moe_lora_workspace_bytes(C.byref(self.struct), max_tokens)
         if n == 0:
             raise L.MoeError("invalid token count for an adapter workspace")
         ws = torch.empty(n + 256, dtype=torch.uint8, device=self.device)
@@ -364,19 +376,19 @@ class LoraAdapters:
     def apply(self, x, token_adapter, ys, ws, stream=None):
         """ys[p] += scale * (x a^T) b^T of each token's adapter, in place
         (ainfer_moe_lora_apply); tokens without one keep their rows."""
-        s = self.s
-        _, ld = _rows(x, "x", s.in_)
-        _require(x.dtype == self.x_dtype and x.device == self.device, "x: the adapters' x type")
-        T = x.shape[0]
-        _vector(token_adapter, "token_adapter", torch.int32, T, self.device)
-        _require(len(ys) == s.n_proj, "one y per projection")
-        n = L.LORA_MAX_PROJ
-        yp, yl = (C.c_void_p * n)(), (C.c_int64 * n)()
+        dt, T, _, ld = _rows(x, "x", self.cols)
+        dev = self.device
+        if x.dtype != self.x_dtype or x.device != dev or ws.device != dev:
+            raise L.MoeError("x: the adapters' x type; x and the workspace on their device")
+        _vector(token_adapter, "token_adapter", torch.int32, T, dev)
+        if len(ys) != len(self.rows):
+            raise L.MoeError("one y per projection")
+        yp, yl = (C.c_void_p * len(ys))(), (C.c_int64 * len(ys))()
         for p, y in enumerate(ys):
-            _, yl[p] = _rows(y, "y", s.out[p])
-            _require(y.shape[0] == T and y.dtype == self.y_dtype and y.device == self.device,
-                     "y: T rows of the adapters' y type")
+            _, n, _, yl[p] = _rows(y, "y", self.rows[p])
+            if n != T or y.dtype != self.y_dtype or y.device != dev:
+                raise L.MoeError("y: a row per token, of the adapters' y type and device")
             yp[p] = y.data_ptr()
-        _call(L.lib().ainfer_moe_lora_apply, self.device, stream, C.byref(s), _ptr(x), ld,
-              _ptr(token_adapter), T, yp, yl, _ptr(ws), ws.numel())
+        _call(L.lib().ainfer_moe_lora_apply, dev, stream, C.byref(self.struct), x.data_ptr(), ld,
+              token_adapter.data_ptr(), T, yp, yl, ws.data_ptr(), ws.numel())
         return ys
