@@ -33,7 +33,6 @@ struct LoraArgs {
   void *y[AINFER_LORA_MAX_PROJ];
   int64_t y_ld[AINFER_LORA_MAX_PROJ], x_ld;
   int m[AINFER_LORA_MAX_PROJ];
-  bool y_vec[AINFER_LORA_MAX_PROJ];  // y rows readable in pieces of 4 values
   float *v;       // [P][T][R], of k_lora_rows
   int N, R, K, P, T;
   int units;      // groups of 64 rows of y per wave
@@ -304,8 +303,25 @@ __device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
 }
 
 template <bool YF32>
-struct alignas(YF32 ? 16 : 8) YRun {  // 4 values of y
+struct YRun {  // 4 values of y
   uint32_t v[YF32 ? 4 : 2];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    if constexpr (YF32) {
+      const u32x4 t = buf_load16(r, at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = t[j];
+    } else {
+      const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+      v[0] = t[0];
+      v[1] = t[1];
+    }
+  }
+  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t at) const {
+    if constexpr (YF32)
+      __builtin_amdgcn_raw_buffer_store_b128((u32x4){v[0], v[1], v[2], v[3]}, r, at, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b64((u32x2){v[0], v[1]}, r, at, 0, 0);
+  }
 };
 
 // ids of a tile's tokens, one per lane below 16; -1 = none
@@ -331,16 +347,14 @@ struct Panel {
   static constexpr int LPR = CK / 8, LOADS = LPR / 4, RPL = 64 / LPR;
   static __device__ __forceinline__ int swz(int row) { return CK == 128 ? row & 15 : (row >> 1) & 7; }
   u32x4 v[LOADS];
-  // row i * RPL + lane / LPR at base + row * pitch, columns k0 + (lane % LPR) * 8
-  __device__ __forceinline__ void load(const uint16_t *base, int pitch, int rows, int k0, int K,
-                                       int lane) {
+  // rows row0 + i * RPL + lane / LPR, columns k0 + (lane % LPR) * 8 of a matrix of
+  // rows of K columns (at most 16 MB); 0 past its last row and column
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t m, int row0, int k0, int K, int lane) {
     const int k = k0 + (lane & (LPR - 1)) * 8;
+    const uint32_t at = k < K ? (uint32_t)(lane / LPR * K + k) * 2 : BUF_OOB;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int r = i * RPL + lane / LPR;
-      v[i] = (u32x4){0, 0, 0, 0};
-      if (r < rows && k < K) v[i] = *(const u32x4 *)(base + (size_t)r * pitch + k);
-    }
+    for (int i = 0; i < LOADS; ++i)
+      v[i] = buf_load16(m, at + (uint32_t)((row0 + i * RPL) * K) * 2);
   }
   __device__ __forceinline__ void to_lds(u32x4 *buf, int lane) const {
 #pragma unroll
@@ -358,7 +372,7 @@ struct Panel {
 
 // the same of fp32 rows: the wave splits what it read, one plane of bf16 each
 struct PanelF32 {
-  static constexpr int CK = 64, LPR = 16;
+  static constexpr int CK = 64;
   u32x4 v[4];  // row i * 4 + lane / 16, columns k0 + (lane % 16) * 4
   __device__ __forceinline__ void to_lds(u32x4 *buf, int lane) const {
 #pragma unroll
@@ -389,34 +403,37 @@ struct PanelF32 {
 //      ends with 4 consecutive values of y of each of its 4 tokens.  B's rows
 //      are read whole and turned in LDS as A's; what the next unit reads of B
 //      and y is in flight meanwhile.
-template <int NRB, bool XF32, bool YF32>
-__global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
+template <int LP, bool XF32, bool YF32, bool VEC>
+__global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(LoraArgs a) {
+  constexpr int NRB = LP <= 2 ? 1 : LP / 2;  // blocks of 16 rows of A
   constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
   constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
   constexpr int RING = NRB < 4 ? NRB : 4;  // panels of A in flight
-  constexpr int STAGE = 512;               // 16-byte pieces of a wave's LDS: 8 KB
+  constexpr int STAGE = NRK == 4 ? 1024 : 512;  // 16-byte pieces of a wave's LDS
   constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it
-  __shared__ u32x4 s_stage[T_WAVES][STAGE];
+  __shared__ u32x4 s_stage[T_WAVES][STAGE + 64];
   __shared__ u32x2 s_v[NRK][NS][64][2];
-  const int lane = threadIdx.x & 63;
+  const int lane0 = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t0 = blockIdx.x * TT, p = blockIdx.z % a.P, part = blockIdx.z / a.P;
+  // neighbouring tiles on one XCD, whose L2 then holds their adapters
+  const int t0 = xcd_remap(blockIdx.x, gridDim.x) * TT;
+  const int p = blockIdx.z % a.P, part = blockIdx.z / a.P;
   const int M = a.m[p];
-  const int id = tile_ids(a, t0, lane);
-  uint64_t rem = __ballot(id >= 0), mask = 0;
-  int ad = -1;
-  for (int i = 0; i <= (int)blockIdx.y && rem; ++i) {
-    ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(rem));
-    mask = __ballot(id == ad) & rem;
-    rem &= ~mask;
-    if (i < (int)blockIdx.y) ad = -1;
-  }
-  if (ad < 0) return;
-  const int rank = rank_of(a, ad);
+  const int id = tile_ids(a, t0, lane0);
   const int u0 = part * a.units * T_WAVES, u_end = min(u0 + a.units * T_WAVES, (M + 63) / 64);
-  if (rank == 0 || u0 * 64 >= M) return;
+  if (u0 * 64 >= M) return;
+  uint32_t rem = (uint32_t)__ballot(id >= 0);  // 16 tokens
+  for (int nth = 0; rem; ++nth) {
+  const int ad = __builtin_amdgcn_readlane(id, __builtin_ctz(rem));
+  const uint32_t mask = (uint32_t)__ballot(id == ad) & rem;
+  rem &= ~mask;
+  if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
+  const int rank = rank_of(a, ad);
+  if (rank == 0) continue;
   const float scale = a.scales ? a.scales[ad] : 1.0f;
-  const int col = lane & 15, q = lane >> 4;
+  // opaque, so that what depends on the lane is computed again for each adapter
+  // and not held in registers across this loop
+  const int lane = tid_opaque() & 63;
   u32x4 *stage = s_stage[wave];
 
   // 1.
@@ -424,34 +441,40 @@ __global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
 #pragma unroll
   for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
   {
-    const uint16_t *A = a.a[p] + (size_t)ad * a.R * a.K;
+    const __amdgpu_buffer_rsrc_t A =
+        make_rsrc(a.a[p] + (size_t)ad * a.R * a.K, (uint32_t)(a.R * a.K) * 2);
     const int nc = (a.K + CK - 1) / CK;
     Panel<CK> pa[RING];
-    typename std::conditional<XF32, PanelF32, Panel<CK>>::type px;
-    auto load_a = [&](int r, int c) {
-      pa[r % RING].load(A + (size_t)r * 16 * a.K, a.K, a.R - r * 16, c * CK, a.K, lane);
-    };
-    auto load_x = [&](int c) {
-      constexpr int EPL = XF32 ? 4 : 8;  // elements a lane, 16 lanes a row
-      const int k = c * CK + (lane & 15) * EPL;
+    using XPanel = typename std::conditional<XF32, PanelF32, Panel<CK>>::type;
+    XPanel px;
+    auto load_a = [&](int r, int c) { pa[r % RING].load(A, r * 16, c * CK, a.K, lane); };
+    // the tile's rows of x; rows past the last token are never multiplied into a
+    // token's column, and read as 0
+    const int xsz = XF32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t X =
+        make_rsrc((const char *)a.x + (size_t)t0 * a.x_ld * xsz, 0x7FFFFFFFu);
+    const uint32_t xpitch = (uint32_t)a.x_ld * xsz;
+    uint32_t x_row[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const size_t row = min(t0 + i * 4 + lane / 16, a.T - 1);
-        px.v[i] = (u32x4){0, 0, 0, 0};
-        if (k < a.K)
-          px.v[i] = *(const u32x4 *)((const char *)a.x + (row * a.x_ld + k) * (XF32 ? 4 : 2));
-      }
-    };
-    if (wave < nc) {
-      load_x(wave);
-#pragma unroll
-      for (int r = 0; r < RING; ++r) load_a(r, wave);
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 4 + lane / 16;
+      x_row[i] = t0 + r < a.T ? r * xpitch : BUF_OOB;
     }
+    auto load_x = [&](int c) {
+      const int k = c * CK + (lane & 15) * (16 / xsz);  // 16 lanes a row
+#pragma unroll
+      for (int i = 0; i < 4; ++i) px.v[i] = buf_load16(X, k < a.K ? x_row[i] + k * xsz : BUF_OOB);
+    };
+    // chunks from nc on read as 0, without a branch: a branch around a load or a
+    // store makes every later wait a wait for all of them
+    load_x(wave);
+#pragma unroll
+    for (int r = 0; r < RING; ++r) load_a(r, wave);
     for (int c = wave; c < nc; c += T_WAVES) {
       const int next = c + T_WAVES;
       u32x4 xf[NX][KS];
       px.to_lds(stage, lane);
-      if (next < nc) load_x(next);
+      load_x(next);
       lds_order();
 #pragma unroll
       for (int s = 0; s < NX; ++s) Panel<CK>::frags(stage + s * 128, lane, xf[s]);
@@ -460,7 +483,7 @@ __global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
         u32x4 *buf = stage + XPART;
         pa[r % RING].to_lds(buf, lane);
         if (r + RING < NRB) load_a(r + RING, c);
-        else if (next < nc) load_a((r + RING) % NRB, next);
+        else load_a((r + RING) % NRB, next);
         lds_order();
         u32x4 af[KS];
         Panel<CK>::frags(buf, lane, af);
@@ -472,26 +495,57 @@ __global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
       }
     }
   }
+  const int lane_y = tid_opaque() & 63, col_y = lane_y & 15, q_y = lane_y >> 4;
+  const uint32_t own = mask >> (q_y * 4);  // bit i: this lane's token q * 4 + i
+  constexpr int CP = NRK * 4;              // pieces of a row of B, padded
+  const int cpr = a.R / 8;
+  const __amdgpu_buffer_rsrc_t B =
+      make_rsrc(a.b[p] + (size_t)ad * M * a.R, (uint32_t)M * a.R * 2);
+  u32x4 w[LP];
+  YRun<YF32> y[4];
+  const int ysz = YF32 ? 4 : 2;
+  const __amdgpu_buffer_rsrc_t Y =
+      make_rsrc((const char *)a.y[p] + (size_t)t0 * a.y_ld[p] * ysz, 0x7FFFFFFFu);
+  const uint32_t ypitch = (uint32_t)a.y_ld[p] * ysz;
+  uint32_t y_tok[4];  // this lane's tokens q * 4 + i, or past the buffer
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y_tok[i] = (own >> i) & 1 ? (q_y * 4 + i) * ypitch : BUF_OOB;
+  auto y_at = [&](int u, int i, int j) {
+    const int m = u * 64 + 4 * col_y + j;
+    return m < M ? y_tok[i] + m * ysz : BUF_OOB;
+  };
+  auto load_b = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < LP; ++i)  // piece i * 64 + lane of the unit
+      w[i] = buf_load16(B, (uint32_t)(u * cpr + i) * 1024 + lane_y * 16);
+  };
+  auto load_y = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i].load(Y, y_at(u, i, 0));
+  };
+  int u = u0 + wave;
+  load_b(u);
+  if (VEC) load_y(u);
   __syncthreads();  // every wave is done with its stage
   {
     f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
 #pragma unroll
-    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane] = acc[r];
+    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane_y] = acc[r];
   }
   __syncthreads();
-  // 2. ranks rb * 16 + q * 4 .. + 3 of token col
+  // 2. ranks rb * 16 + q_y * 4 .. + 3 of token col
   for (int rb = wave; rb < 2 * NRK; rb += T_WAVES) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (rb < NRB) {
       const f32x4 *red = (const f32x4 *)s_stage;
 #pragma unroll
-      for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane];
+      for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane_y];
     }
     float e[4][NS];
-    const int r0 = rb * 16 + q * 4;
+    const int r0 = rb * 16 + q_y * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_bf16(r0 + i < rank ? v[i] * scale : 0.0f, e[i]);
-    const int slot = ((r0 & 31) >> 3) * 16 + col;
+    const int slot = ((r0 & 31) >> 3) * 16 + col_y;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
       s_v[rb >> 1][s][slot][(r0 >> 2) & 1] =
@@ -500,110 +554,93 @@ __global__ __launch_bounds__(64 * T_WAVES) void k_lora_tile(LoraArgs a) {
   __syncthreads();
 
   // 3.
-  constexpr int CP = NRK * 4;              // pieces of a row of B, padded
-  constexpr int HALF = NRK == 4 ? 2 : 1;   // a unit's pieces pass the stage in halves
-  constexpr int HC = CP / HALF, HB = NRK / HALF;
-  const int cpr = a.R / 8;
-  const uint16_t *B = a.b[p] + (size_t)ad * M * a.R;
-  // piece i * 64 + lane of a unit: its place in the stage (0xFFFF: not in this half)
-  int place[CP];
+  // piece i * 64 + lane of a unit: its place in the stage.  4 rows (a column of
+  // the MFMAs) are 4 CP pieces, turned by the column so that neither side meets a
+  // bank twice.
+  int place[LP];
 #pragma unroll
-  for (int i = 0; i < CP; ++i) {
-    const int l = i * 64 + lane, row = l / cpr, ch = l - row * cpr;
-    const int s = row >> 2;
-    place[i] = s * 4 * HC + (((row & 3) * HC + ch % HC) ^ (s & 15)) + (ch / HC) * 0x10000;
-    if (i >= cpr) place[i] = -1;
+  for (int i = 0; i < LP; ++i) {
+    const int l = i * 64 + lane_y, row = l / cpr, ch = l - row * cpr, s = row >> 2;
+    place[i] = row < 64 ? s * 4 * CP + (((row & 3) * CP + ch) ^ (s & 15)) : STAGE + lane_y;
   }
-  u32x4 keep[NRK];  // clears B's columns from rank on (they may hold anything)
+  u32x4 keep;  // clears B's columns from rank on (they may hold anything) in rank's block of 32
 #pragma unroll
-  for (int rb = 0; rb < NRK; ++rb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = rb * 32 + q * 8 + 2 * i;
-      keep[rb][i] = (r < rank ? 0xFFFFu : 0u) | (r + 1 < rank ? 0xFFFF0000u : 0u);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int r = q_y * 8 + 2 * i, n = rank & 31;
+    keep[i] = (r < n ? 0xFFFFu : 0u) | (r + 1 < n ? 0xFFFF0000u : 0u);
+  }
   u32x4 vf[NRK][NS];
 #pragma unroll
   for (int rb = 0; rb < NRK; ++rb)
 #pragma unroll
-    for (int s = 0; s < NS; ++s) vf[rb][s] = *(const u32x4 *)s_v[rb][s][lane];
+    for (int s = 0; s < NS; ++s) vf[rb][s] = *(const u32x4 *)s_v[rb][s][lane_y];
 
-  u32x4 w[CP];
-  YRun<YF32> y[4];
-  auto y_at = [&](int u, int i) {
-    return (char *)a.y[p] +
-           ((size_t)(t0 + q * 4 + i) * a.y_ld[p] + u * 64 + 4 * col) * (YF32 ? 4 : 2);
-  };
-  auto load_b = [&](int u) {
-    const int left = (M - u * 64) * cpr;  // pieces of B from this unit on
-#pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      const int l = i * 64 + lane;
-      w[i] = (u32x4){0, 0, 0, 0};
-      if (i < cpr && l < left) w[i] = *(const u32x4 *)(B + ((size_t)u * 64 * cpr + l) * 8);
-    }
-  };
-  auto whole = [&](int u) { return a.y_vec[p] && u * 64 + 4 * col + 4 <= M; };
-  auto load_y = [&](int u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (whole(u) && ((mask >> (q * 4 + i)) & 1)) y[i] = *(const YRun<YF32> *)y_at(u, i);
-  };
-  int u = u0 + wave;
-  if (u < u_end) {
-    load_b(u);
-    load_y(u);
-  }
-  for (; u < u_end; u += T_WAVES) {
-    f32x4 d[4];
+  // d = v B^T of unit u, and the next unit's rows on their way
+  auto product = [&](int u, f32x4 (&d)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < HALF; ++h) {
+    for (int i = 0; i < LP; ++i) stage[place[i]] = w[i];
+    load_b(u + T_WAVES);
+    lds_order();
 #pragma unroll
-      for (int i = 0; i < CP; ++i)
-        if (place[i] >= 0 && (HALF == 1 || place[i] >> 16 == h)) stage[place[i] & 0xFFFF] = w[i];
-      if (h == HALF - 1 && u + T_WAVES < u_end) load_b(u + T_WAVES);
-      lds_order();
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int rb = 0; rb < NRK; ++rb) {
+        u32x4 b = stage[col_y * 4 * CP + ((j * CP + rb * 4 + q_y) ^ col_y)];
+        // from rank on B may hold anything: its block of 32 is masked, later ones are left out
+        if (rb * 32 + 32 > rank) b = rb * 32 < rank ? b & keep : (u32x4){0, 0, 0, 0};
 #pragma unroll
-        for (int rb = 0; rb < HB; ++rb) {
-          const u32x4 b = stage[col * 4 * HC + ((j * HC + rb * 4 + q) ^ col)] & keep[h * HB + rb];
+        for (int s = 0; s < NS; ++s) d[j] = mfma_bf16_16x16x32(vf[rb][s], b, d[j]);
+      }
+    lds_order();
+  };
+  if constexpr (VEC) {
+    for (; u < u_end; u += T_WAVES) {
+      f32x4 d[4];
+      product(u, d);
+      YRun<YF32> o[4];
 #pragma unroll
-          for (int s = 0; s < NS; ++s) d[j] = mfma_bf16_16x16x32(vf[h * HB + rb][s], b, d[j]);
-        }
-      lds_order();
-    }
-    const bool vec = whole(u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!((mask >> (q * 4 + i)) & 1)) continue;
-      if (vec) {
-        YRun<YF32> o;
+      for (int i = 0; i < 4; ++i) {
         if constexpr (YF32) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o.v[j] = __float_as_uint(__uint_as_float(y[i].v[j]) + d[j][i]);
+          for (int j = 0; j < 4; ++j)
+            o[i].v[j] = __float_as_uint(__uint_as_float(y[i].v[j]) + d[j][i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            o.v[j] = bf16x2_bits(bf16_lo(y[i].v[j]) + d[2 * j][i], bf16_hi(y[i].v[j]) + d[2 * j + 1][i]);
+            o[i].v[j] = bf16x2_bits(bf16_lo(y[i].v[j]) + d[2 * j][i],
+                                    bf16_hi(y[i].v[j]) + d[2 * j + 1][i]);
         }
-        *(YRun<YF32> *)y_at(u, i) = o;
-      } else {
+      }
+      load_y(u + T_WAVES);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i].store(Y, y_at(u, i, 0));
+    }
+  } else {
+    for (; u < u_end; u += T_WAVES) {
+      f32x4 d[4];
+      product(u, d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (u * 64 + 4 * col + j < M) {
-            if constexpr (YF32) {
-              ((float *)y_at(u, i))[j] += d[j][i];
-            } else {
-              uint16_t *e = (uint16_t *)y_at(u, i) + j;
-              *e = f32_to_bf16(bf16_to_f32(*e) + d[j][i]);
-            }
-          }
+          v[j] = YF32 ? __builtin_amdgcn_raw_buffer_load_b32(Y, y_at(u, i, j), 0, 0)
+                      : __builtin_amdgcn_raw_buffer_load_b16(Y, y_at(u, i, j), 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (YF32)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(__uint_as_float(v[j]) + d[j][i]), Y,
+                                                  y_at(u, i, j), 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(bf16_to_f32((uint16_t)v[j]) + d[j][i]),
+                                                  Y, y_at(u, i, j), 0, 0);
+        }
       }
     }
-    if (u + T_WAVES < u_end) load_y(u + T_WAVES);
+  }
+  if (rem) __syncthreads();  // the stage is the next adapter's
   }
 }
 
@@ -613,6 +650,9 @@ int div_up(int a, int b) { return (a + b - 1) / b; }
 
 #ifndef LORA_DEC_MAX_T
 #define LORA_DEC_MAX_T 128
+#endif
+#ifndef LORA_SLOTS
+#define LORA_SLOTS 4
 #endif
 #ifndef LORA_FUSED_BYTES
 #define LORA_FUSED_BYTES (256 << 10)
@@ -639,16 +679,21 @@ void launch_dec_lr(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream
   else if (a.R <= 64) launch_dec<8, FUSED>(a, grid, xf32, yf32, s);
   else launch_dec<16, FUSED>(a, grid, xf32, yf32, s);
 }
-template <int NRB>
-void launch_tile(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
+template <int LP, bool VEC>
+void launch_tile_y(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
   const dim3 b(64 * T_WAVES);
   if (xf32) {
-    if (yf32) k_lora_tile<NRB, true, true><<<grid, b, 0, s>>>(a);
-    else k_lora_tile<NRB, true, false><<<grid, b, 0, s>>>(a);
+    if (yf32) k_lora_tile<LP, true, true, VEC><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<LP, true, false, VEC><<<grid, b, 0, s>>>(a);
   } else {
-    if (yf32) k_lora_tile<NRB, false, true><<<grid, b, 0, s>>>(a);
-    else k_lora_tile<NRB, false, false><<<grid, b, 0, s>>>(a);
+    if (yf32) k_lora_tile<LP, false, true, VEC><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<LP, false, false, VEC><<<grid, b, 0, s>>>(a);
   }
+}
+template <int LP>
+void launch_tile(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, bool vec, hipStream_t s) {
+  if (vec) launch_tile_y<LP, true>(a, grid, xf32, yf32, s);
+  else launch_tile_y<LP, false>(a, grid, xf32, yf32, s);
 }
 
 }  // namespace
@@ -677,6 +722,8 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   const bool yf32 = l.y_dtype == AINFER_ACT_F32, xf32 = l.x_dtype == AINFER_ACT_F32;
   const int ysz = yf32 ? 4 : 2;
   int m_most = 1;
+  bool tiled = T > LORA_DEC_MAX_T && (15 * x_ld + l.in) * (xf32 ? 4 : 2) < INT32_MAX;
+  bool vec = true;  // every y in whole pieces of 4 values
   for (int p = 0; p < AINFER_LORA_MAX_PROJ; ++p) {
     const bool on = p < l.n_proj;
     a.a[p] = on ? (const uint16_t *)l.a[p] : nullptr;
@@ -684,10 +731,12 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     a.y[p] = on ? y[p] : nullptr;
     a.y_ld[p] = on ? y_ld[p] : 0;
     a.m[p] = on ? l.out[p] : 0;
-    a.y_vec[p] = on && (uintptr_t)y[p] % (4 * ysz) == 0 && y_ld[p] % 4 == 0;
+    if (on && ((uintptr_t)y[p] % (4 * ysz) || y_ld[p] % 4 || l.out[p] % 4)) vec = false;
+    // k_lora_tile's offsets within a tile are 32-bit
+    if (on && (15 * y_ld[p] + l.out[p]) * ysz >= INT32_MAX) tiled = false;
     if (on && l.out[p] > m_most) m_most = l.out[p];
   }
-  if (T <= LORA_DEC_MAX_T) {
+  if (!tiled) {
     const int groups = div_up(m_most, 64);
     // about DEC_WGS workgroups
     int per = div_up(groups * T * l.n_proj, 1024 * D_WAVES);
@@ -710,12 +759,16 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
   a.units = div_up(units, parts * T_WAVES);
   parts = div_up(units, a.units * T_WAVES);
-  const int slots = l.n_adapters < TT ? l.n_adapters : TT;
-  const dim3 grid(tiles, slots, l.n_proj * parts);
-  const int nrb = div_up(l.rank, 16);
-  if (nrb <= 1) launch_tile<1>(a, grid, xf32, yf32, s);
-  else if (nrb <= 2) launch_tile<2>(a, grid, xf32, yf32, s);
-  else if (nrb <= 4) launch_tile<4>(a, grid, xf32, yf32, s);
-  else launch_tile<8>(a, grid, xf32, yf32, s);
+  int slots = 512 / (tiles * l.n_proj * parts);
+  slots = slots < LORA_SLOTS ? LORA_SLOTS : slots > TT ? TT : slots;
+  if (slots > l.n_adapters) slots = l.n_adapters;
+  // a multiple of the XCDs, so that blockIdx.x alone tells the XCD
+  const dim3 grid(div_up(tiles, N_XCD) * N_XCD, slots, l.n_proj * parts);
+  const int cpr = l.rank / 8;
+  if (cpr <= 1) launch_tile<1>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 2) launch_tile<2>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 4) launch_tile<4>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 8) launch_tile<8>(a, grid, xf32, yf32, vec, s);
+  else launch_tile<16>(a, grid, xf32, yf32, vec, s);
   return hipGetLastError();
 }

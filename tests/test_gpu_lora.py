@@ -100,7 +100,9 @@ SHAPES = [(1, 1, 8, 8, [1]), (1, 4, 16, 4096, [4096]), (2, 3, 8, 72, [33, 7]),
           (5, 2, 24, 520, [100]), (16, 16, 64, 1024, [257]), (17, 5, 32, 200, [64, 64, 31]),
           (63, 40, 16, 640, [96]), (64, 64, 128, 264, [40]), (65, 3, 40, 136, [129]),
           (255, 9, 16, 264, [48, 80]), (257, 7, 8, 128, [65]), (300, 2, 104, 328, [72]),
-          (1003, 12, 8, 1024, [136, 1, 2, 3]), (40, 2, 96, 2056, [33])]
+          (1003, 12, 8, 1024, [136, 1, 2, 3]), (40, 2, 96, 2056, [33]),
+          (129, 3, 32, 2184, [1100, 260]), (700, 5, 64, 1096, [64]), (150, 20, 40, 72, [131]),
+          (1030, 2, 128, 520, [516]), (513, 1, 24, 8, [4])]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -110,12 +112,13 @@ def test_matches_formula(torch, shape, x, y):
     Case(torch, *shape, x=x, y=y).check()
 
 
-@pytest.mark.parametrize("R", (8, 16, 32, 64, 128))
-def test_ragged_ranks_and_garbage_beyond_them(torch, R):
+@pytest.mark.parametrize("R", (8, 16, 24, 32, 64, 72, 128))
+@pytest.mark.parametrize("T", (50, 200))
+def test_ragged_ranks_and_garbage_beyond_them(torch, R, T):
     """Ranks 0, 1, odd ones, R, and values outside 0..R; NaN and inf in the rows
     of A and columns of B beyond them."""
     ranks = [0, 1, 3, R - 1, R, -4, R + 9, R // 2]
-    c = Case(torch, 50, 8, R, 136, [70, 9], ranks=ranks)
+    c = Case(torch, T, 8, R, 136, [72, 9], ranks=ranks)
     for n, r in enumerate(ranks):
         r = min(max(r, 0), R)
         for a, b in zip(c.a, c.b):
@@ -138,31 +141,34 @@ def test_pitches_and_alignment(torch):
     """Rows of x and y inside wider ones: 16-byte pieces of y, and not."""
     for y in ("fp32", "bf16"):
         for pad in (8, 3, 1):
-            Case(torch, 33, 5, 16, 200, [64, 50], x_pad=8, y_pad=pad, y=y).check()
+            for T, R in ((33, 16), (150, 8), (150, 32), (140, 128)):
+                Case(torch, T, 5, R, 200, [64, 50], x_pad=8, y_pad=pad, y=y).check()
+                Case(torch, T, 5, R, 200, [68], x_pad=8, y_pad=pad, y=y, x="fp32").check()
 
 
-def test_other_tokens_do_not_leak(torch):
+@pytest.mark.parametrize("T", (32, 160))
+def test_other_tokens_do_not_leak(torch, T):
     """A token's NaN and an adapter's inf stay in that token's rows and that
     adapter's tokens."""
-    c = Case(torch, 32, 4, 16, 264, [80], ids=[t % 4 for t in range(32)])
+    c = Case(torch, T, 4, 16, 264, [80], ids=[t % 4 for t in range(T)])
     c.x[5] = math.nan
     c.b[0][3] = math.inf
     ys = [y.clone() for y in c.y]
     c.apply(ys)
     torch.cuda.synchronize()
-    bad = torch.tensor([t == 5 or t % 4 == 3 for t in range(32)], device="cuda")
+    bad = torch.tensor([t == 5 or t % 4 == 3 for t in range(T)], device="cuda")
     assert not torch.isfinite(ys[0][bad]).any()
     assert torch.isfinite(ys[0][~bad]).all()
-    d = Case(torch, 32, 4, 16, 264, [80], ids=[t % 4 for t in range(32)])
+    d = Case(torch, T, 4, 16, 264, [80], ids=[t % 4 for t in range(T)])
     clean = [y.clone() for y in d.y]
     d.apply(clean)
     assert torch.equal(clean[0][~bad], ys[0][~bad])
 
 
-def test_infinite_and_large_fp32_inputs(torch):
-    """fp32 x of inf gives inf or NaN, the largest finite x what the formula gives."""
-    c = Case(torch, 4, 1, 8, 64, [16], x="fp32", ids=[0, 0, 0, 0], ranks=[1],
-             scales=False)
+@pytest.mark.parametrize("T", (4, 140))
+def test_infinite_and_large_fp32_inputs(torch, T):
+    """fp32 x of inf gives inf, the largest finite x what the formula gives."""
+    c = Case(torch, T, 1, 8, 64, [16], x="fp32", ids=[0] * T, ranks=[1], scales=False)
     c.a[0].zero_()
     c.a[0][:, 0, 0] = 1.0
     c.b[0].zero_()
@@ -211,11 +217,13 @@ def test_shared_workspace_streams_and_graph(torch):
         Case(torch, 17, 6, 16, 520, [200]).check()
 
 
-def test_offsets_past_32_bits(torch):
-    """x and y pitches whose products with the token pass 2^31 elements."""
-    T, K, M = 33, 64, 48
+@pytest.mark.parametrize("T,pitch", ((33, (1 << 27) + 8), (130, (1 << 26) + (1 << 23)),
+                                     (200, (1 << 24) + 8)))
+def test_offsets_past_32_bits(torch, T, pitch):
+    """x and y pitches whose products with the token pass 2^31 elements, or
+    2^31 bytes within 16 tokens."""
+    K, M = 64, 48
     c = Case(torch, T, 3, 8, K, [M])
-    pitch = (1 << 27) + 8
     xs = torch.empty((T - 1) * pitch + K, dtype=torch.bfloat16, device="cuda")
     ys = torch.empty((T - 1) * pitch + M, dtype=torch.float32, device="cuda")
     x = xs.as_strided((T, K), (pitch, 1))
