@@ -1,28 +1,35 @@
 // moe_lora.hip - low-rank adapters of many requests beside shared projections
 // (ainfer_moe_lora_apply): y_p += scale_a (x A_a^T) B_a^T, a = the token's adapter.
 //
-// Batches of requests (an adapter per token: bound by reading A and B once for
-// every token, by launches and by latency) take dot products in fp32:
+// Batches of requests (an adapter per token: A and B are read for every token, and
+// launches and latency count) take dot products in fp32, one token a workgroup:
 //   k_lora_dec    a workgroup owns rows of one token's y: a wave per row of A, v to
-//                 LDS, then the rows of B; A is read by every workgroup of the
-//                 token, which costs less than a second launch while it is small
-//   k_lora_rows   v = x A^T, a wave per row of A, and k_lora_dec without its first
-//                 half, where A is large
-// Prompts (neighbouring tokens share an adapter) take 32 tokens a wave on
-// v_mfma_f32_16x16x32_bf16, once per distinct adapter among them, other tokens'
-// columns ignored: no sorting, tokens may name adapters in any order:
-//   k_lora_down   partial sums of v over a part of K, to the workspace
-//   k_lora_up     v = the sum of the parts, scaled; y += v B^T
-// Their products are exact too: bf16 values enter the MFMA as they are, fp32 values
-// as the sum of two or three bf16 (split_bf16).
+//                 LDS, then the rows of B, whose loads are in flight before A's.
+//                 A is read by every workgroup of the token, which costs less than
+//                 a second launch while it is small
+//   k_lora_rows   else v = x A^T first, a workgroup per 2 or 4 rows of A
+// Prompts (neighbouring tokens share an adapter):
+//   k_lora_tile   16 neighbouring tokens are the columns of
+//                 v_mfma_f32_16x16x32_bf16, once per distinct adapter among them,
+//                 other tokens' columns ignored: no sorting, tokens may name
+//                 adapters in any order.  Its products are exact too: bf16 values
+//                 enter the MFMA as they are, fp32 values as the sum of two or three
+//                 bf16 (split_bf16).  v never leaves the CU.
+// GPU us a call (inside a graph) of the benchmark's larger shapes, and the time the
+// bytes of x, y, and each A and B used once take at 5.1 TB/s: one token 4096 x
+// 4096 rank 16 4.8 (0.1; a launch alone is 2.5), 64 tokens 4096 x (1024 + 1024) rank
+// 16 6.2 (2.2), 16 tokens 5120 x 17408 rank 64 14.8 (8.3), 1003 tokens of 7 requests
+// 1024 x 4096 rank 8 in fp32 14.6 (7.3), 4096 tokens 4096 x 4096 rank 32 of 24
+// requests 28 (19.3), of one request 22 (19.7).
 #include "moe_common.h"
 #include "moe_internal.h"
 
 namespace {
 
+constexpr int N_CU = 256;
 constexpr int TT = 16;       // tokens of an MFMA tile
 constexpr int R_WAVES = 4;   // waves of a workgroup: k_lora_rows
-constexpr int D_WAVES = 8;   // k_lora_dec
+constexpr int dec_waves(bool fused) { return fused ? 8 : 4; }  // k_lora_dec
 constexpr int T_WAVES = 8;   // k_lora_tile
 
 struct LoraArgs {
@@ -84,53 +91,42 @@ __device__ __forceinline__ void dot8(const X8<XF32> &x, const u32x4 &w, float &a
   }
 }
 
-// x . A's rows row and row + step (NR = 2), or the first alone: a wave, 512 k a
-// step, four steps' loads in flight; every lane gets the sums
-template <bool XF32, int NR>
+// x . A's NR rows, step apart, over the k of wave `wave` of W (runs of 512 in
+// turn), four runs' loads in flight; every lane gets the sums
+template <bool XF32, int NR, int W>
 __device__ __forceinline__ void row_dots(const char *xr, const uint16_t *ar, size_t step, int K,
-                                         int lane, float (&sum)[NR]) {
+                                         int wave, int lane, float (&sum)[NR]) {
+  constexpr int U = 4, RUN = 512 * W;
   float acc[NR][2];
 #pragma unroll
   for (int r = 0; r < NR; ++r) acc[r][0] = acc[r][1] = 0.0f;
-  int k = lane * 8;
-  constexpr int U = 4;
-  for (; k - lane * 8 + 512 * U <= K; k += 512 * U) {
+  const int k1 = wave * 512 + lane * 8;
+  auto runs = [&](int k0, auto whole) {  // runs k0, k0 + RUN, ...
     X8<XF32> x[U];
     u32x4 w[U][NR];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      x[u].load(xr, k + 512 * u);
+      const int k = k0 + k1 + RUN * u;
+      if constexpr (!decltype(whole)::value) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) w[u][r] = *(const u32x4 *)(ar + r * step + k + 512 * u);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+        for (auto &v : x[u].v) v = (u32x4){0, 0, 0, 0};
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < NR; ++r) dot8(x[u], w[u][r], acc[r][u & 1]);
-  }
-  if (k - lane * 8 < K) {
-    X8<XF32> x[U];
-    u32x4 w[U][NR];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int ku = k + 512 * u;
-#pragma unroll
-      for (auto &p : x[u].v) p = (u32x4){0, 0, 0, 0};
-#pragma unroll
-      for (int r = 0; r < NR; ++r) w[u][r] = (u32x4){0, 0, 0, 0};
-      if (ku < K) {  // K is a multiple of 8
-        x[u].load(xr, ku);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) w[u][r] = *(const u32x4 *)(ar + r * step + ku);
+        for (int r = 0; r < NR; ++r) w[u][r] = (u32x4){0, 0, 0, 0};
+        if (k >= K) continue;  // K is a multiple of 8
       }
+      x[u].load(xr, k);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) w[u][r] = *(const u32x4 *)(ar + r * step + k);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < NR; ++r) dot8(x[u], w[u][r], acc[r][u & 1]);
-  }
+  };
+  int k0 = 0;
+  for (; k0 + U * RUN <= K; k0 += U * RUN) runs(k0, std::true_type());
+  if (k0 < K) runs(k0, std::false_type());
 #pragma unroll
   for (int r = 0; r < NR; ++r) sum[r] = wave_sum_f32(acc[r][0] + acc[r][1]);
 }
@@ -144,30 +140,44 @@ __device__ __forceinline__ void token_rows(const LoraArgs &a, int p, int t, int 
   int r = first;
   for (; r + step < rank; r += 2 * step) {
     float s[2];
-    row_dots<XF32, 2>(xr, A + (size_t)r * a.K, (size_t)step * a.K, a.K, lane, s);
+    row_dots<XF32, 2, 1>(xr, A + (size_t)r * a.K, (size_t)step * a.K, a.K, 0, lane, s);
     put(r, s[0]);
     put(r + step, s[1]);
   }
   if (r < rank) {
     float s[1];
-    row_dots<XF32, 1>(xr, A + (size_t)r * a.K, 0, a.K, lane, s);
+    row_dots<XF32, 1, 1>(xr, A + (size_t)r * a.K, 0, a.K, 0, lane, s);
     put(r, s[0]);
   }
 }
 
-template <bool XF32>
+// NR rows of A a workgroup, its waves 512 k after each other: all of a row's loads
+// are in flight up to K = 8192
+template <int NR, bool XF32>
 __global__ __launch_bounds__(64 * R_WAVES) void k_lora_rows(LoraArgs a) {
+  __shared__ float s_sum[R_WAVES][NR];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x, p = blockIdx.z;
+  const int t = blockIdx.x, p = blockIdx.z, r0 = blockIdx.y * NR;
   const int ad = a.ids[t];
   if (ad < 0 || ad >= a.N) return;
-  float *v = a.v + ((size_t)p * a.T + t) * a.R;
-  const int step = gridDim.y * R_WAVES;
-  token_rows<XF32>(a, p, t, ad, blockIdx.y * R_WAVES + wave, step, rank_of(a, ad), lane,
-                   [&](int r, float s) {
-                     if (lane == 0) v[r] = s;
-                   });
+  const int rank = rank_of(a, ad);
+  if (r0 >= rank) return;
+  const char *xr = (const char *)a.x + (size_t)t * a.x_ld * (XF32 ? 4 : 2);
+  const uint16_t *A = a.a[p] + ((size_t)ad * a.R + r0) * a.K;  // R is a multiple of NR
+  float sum[NR];
+  row_dots<XF32, NR, R_WAVES>(xr, A, a.K, a.K, wave, lane, sum);
+  if (lane == 0) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) s_sum[wave][r] = sum[r];
+  }
+  __syncthreads();
+  if (wave == 0 && lane < NR) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < R_WAVES; ++w) v += s_sum[w][lane];
+    a.v[((size_t)p * a.T + t) * a.R + r0 + lane] = v;
+  }
 }
 
 template <int M>
@@ -199,7 +209,8 @@ __device__ __forceinline__ void sum_transpose(float (&d)[LR], int s) {
 // sums end one per lane, in order.  FUSED: v is computed here, in LDS, with the
 // first rows of B and y already in flight.
 template <int LR, bool FUSED, bool XF32, bool YF32>
-__global__ __launch_bounds__(64 * D_WAVES) void k_lora_dec(LoraArgs a) {
+__global__ __launch_bounds__(64 * dec_waves(FUSED)) void k_lora_dec(LoraArgs a) {
+  constexpr int D_WAVES = dec_waves(FUSED);
   constexpr int G = LR >= 8 ? 1 : 8 / LR;  // groups of 64 rows in flight
   constexpr int RW = 64 / LR;              // rows of a load
   __shared__ float s_v[FUSED ? 128 : 1];
@@ -648,19 +659,35 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
 
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
-#ifndef LORA_DEC_MAX_T
-#define LORA_DEC_MAX_T 128
-#endif
-#ifndef LORA_SLOTS
-#define LORA_SLOTS 4
-#endif
-#ifndef LORA_FUSED_BYTES
-#define LORA_FUSED_BYTES (256 << 10)
-#endif
+// Up to this many tokens a call is taken as a batch of requests.  GPU us of one
+// projection, 4096 x 4096, rank 16: every token another of 64 adapters, 256 tokens
+// 14.7 by tokens and 37 by tiles, 1024 tokens 34 and 85; 4 requests' prompts, 128
+// tokens 12.8 and 10.5, 256 15.0 and 10.8, 512 18.6 and 14.4, 1024 25 and 15; at
+// rank 64 256 tokens of 4 requests 23 and 16, 512 35 and 27.
+constexpr int DEC_MAX_T = 256;
+
+// v in every workgroup of a token, or by k_lora_rows first.  us, K 4096, M 4096
+// (8 workgroups a token up to 64 tokens, 4 and 2 at 128 and 256), fused and not:
+// rank 16, T 1 4.8 and 6.3, 64 8.5 and 9.1, 128 10.3 and 13.4, 256 14.7 and 17.4;
+// rank 32, T 1 6.5 and 6.5, 16 6.8 and 6.2, 64 13.3 and 11.3; rank 64, T 1 9.9 and
+// 6.3.  K 5120, M 17408, rank 16, T 16 (17 workgroups a token): 9.7 and 8.3.
+constexpr size_t FUSED_BYTES = 256 << 10;  // of an adapter's A
+constexpr size_t FUSED_AGAIN = 64 << 20;   // of A read again by a token's further workgroups
+bool fuse(size_t bytes_a, int tokens, int workgroups) {
+  const size_t again = (size_t)(workgroups - 1) * tokens * bytes_a;
+  return bytes_a <= FUSED_BYTES && again * (workgroups > 8 ? 2 : 1) <= FUSED_AGAIN;
+}
+// about this many waves of k_lora_dec: fused, more workgroups read A more often
+// (rank 16, T 128 13.6 us at 8192, 10.3 at 4096); alone, more loads are in flight
+// (rank 32, T 256 27.3 at 4096, 23.8 at 8192, 25.5 at 16384)
+constexpr int dec_waves_wanted(bool fused) { return fused ? 4096 : 8192; }
+// k_lora_rows: two rows a workgroup, four from this many rows in the call (fewer
+// workgroups for equal time: rank 128, T 256 76.9 and 77.3 us)
+constexpr int ROWS_TWO = 4096;
 
 template <int LR, bool FUSED>
 void launch_dec(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
-  const dim3 b(64 * D_WAVES);
+  const dim3 b(64 * dec_waves(FUSED));
   if constexpr (FUSED) {
     if (xf32) {
       if (yf32) k_lora_dec<LR, true, true, true><<<grid, b, 0, s>>>(a);
@@ -700,7 +727,7 @@ void launch_tile(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, bool vec, h
 
 // v of k_lora_rows
 size_t lora_workspace_bytes(const ainfer_moe_lora &l, int max_tokens) {
-  const size_t T = max_tokens < LORA_DEC_MAX_T ? max_tokens : LORA_DEC_MAX_T;
+  const size_t T = max_tokens < DEC_MAX_T ? max_tokens : DEC_MAX_T;
   const size_t n = T * l.n_proj * l.rank * sizeof(float);
   return n > 256 ? (n + 255) & ~(size_t)255 : 256;
 }
@@ -722,7 +749,7 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   const bool yf32 = l.y_dtype == AINFER_ACT_F32, xf32 = l.x_dtype == AINFER_ACT_F32;
   const int ysz = yf32 ? 4 : 2;
   int m_most = 1;
-  bool tiled = T > LORA_DEC_MAX_T && (15 * x_ld + l.in) * (xf32 ? 4 : 2) < INT32_MAX;
+  bool tiled = T > DEC_MAX_T && (15 * x_ld + l.in) * (xf32 ? 4 : 2) < INT32_MAX;
   bool vec = true;  // every y in whole pieces of 4 values
   for (int p = 0; p < AINFER_LORA_MAX_PROJ; ++p) {
     const bool on = p < l.n_proj;
@@ -738,29 +765,39 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   }
   if (!tiled) {
     const int groups = div_up(m_most, 64);
-    // about DEC_WGS workgroups
-    int per = div_up(groups * T * l.n_proj, 1024 * D_WAVES);
-    const bool fused = (size_t)l.rank * l.in * 2 <= LORA_FUSED_BYTES;
-    a.units = per;
-    const dim3 grid(T, div_up(groups, per * D_WAVES), l.n_proj);
-    if (fused) {
-      launch_dec_lr<true>(a, grid, xf32, yf32, s);
+    auto grid = [&](bool fused) {
+      const int waves = dec_waves(fused);
+      a.units = div_up(groups * T * l.n_proj, dec_waves_wanted(fused));
+      return dim3(T, div_up(groups, a.units * waves), l.n_proj);
+    };
+    const size_t bytes_a = (size_t)l.rank * l.in * 2;
+    dim3 g = grid(true);
+    if (fuse(bytes_a, T * l.n_proj, g.y)) {
+      launch_dec_lr<true>(a, g, xf32, yf32, s);
     } else {
-      const dim3 gr(T, div_up(l.rank, 2 * R_WAVES), l.n_proj);
-      if (xf32) k_lora_rows<true><<<gr, 64 * R_WAVES, 0, s>>>(a);
-      else k_lora_rows<false><<<gr, 64 * R_WAVES, 0, s>>>(a);
-      launch_dec_lr<false>(a, grid, xf32, yf32, s);
+      g = grid(false);
+      const bool four = l.rank * T * l.n_proj > ROWS_TWO;
+      const dim3 gr(T, l.rank / (four ? 4 : 2), l.n_proj);
+      const dim3 b(64 * R_WAVES);
+      if (xf32 && four) k_lora_rows<4, true><<<gr, b, 0, s>>>(a);
+      else if (xf32) k_lora_rows<2, true><<<gr, b, 0, s>>>(a);
+      else if (four) k_lora_rows<4, false><<<gr, b, 0, s>>>(a);
+      else k_lora_rows<2, false><<<gr, b, 0, s>>>(a);
+      launch_dec_lr<false>(a, g, xf32, yf32, s);
     }
     return hipGetLastError();
   }
   const int tiles = div_up(T, TT), units = div_up(m_most, 64);
   // parts of y's rows, each of which computes v again, while tiles leave CUs idle
-  int parts = 256 / (tiles * l.n_proj);
+  int parts = N_CU / (tiles * l.n_proj);
   parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
   a.units = div_up(units, parts * T_WAVES);
   parts = div_up(units, a.units * T_WAVES);
-  int slots = 512 / (tiles * l.n_proj * parts);
-  slots = slots < LORA_SLOTS ? LORA_SLOTS : slots > TT ? TT : slots;
+  // workgroups of a tile, which share its adapters: as many as two on each CU, and
+  // 4 (T 4096, 16 requests: 33.3 us with 2, 27.8 with 4; 512 tokens, 4 requests
+  // 12.1 and 14.4)
+  int slots = 2 * N_CU / (tiles * l.n_proj * parts);
+  slots = slots < 4 ? 4 : slots > TT ? TT : slots;
   if (slots > l.n_adapters) slots = l.n_adapters;
   // a multiple of the XCDs, so that blockIdx.x alone tells the XCD
   const dim3 grid(div_up(tiles, N_XCD) * N_XCD, slots, l.n_proj * parts);
