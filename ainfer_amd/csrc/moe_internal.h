@@ -391,11 +391,14 @@ struct ScoredArgs {
   int dtype, T, k;
   int G, top, per;  // groups, groups kept, experts per group
   int gl;           // log2 of the lanes that hold a group
+  int more;         // lanes above top_k that the candidates' threshold may let in
   int group_score, renorm;
   float scale;
   bool vec;         // rows readable in 16-byte pieces
 };
-constexpr int SR_MAX_GRID = 2048;
+#ifndef SR_MAX_GRID
+#define SR_MAX_GRID 2048
+#endif
 hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, int dtype,
                                int64_t ld, const float *bias, int T, int32_t *idx, float *w,
                                hipStream_t s);

@@ -26,6 +26,14 @@
 #include "moe_internal.h"
 #include "moe_topk.h"
 
+// 1 / i.  A symbol that the compiler may not fold: the coefficients of exp64 then
+// stay in scalar registers.  As literals (and as the library's exp has its own)
+// they are held in vector registers throughout the token loop: 124 VGPRs against
+// 92 at 8 experts a lane, which costs the common path its waves.
+__constant__ double ainfer_scored_inv[14] = {
+    0, 1.0, 1.0 / 2, 1.0 / 3, 1.0 / 4, 1.0 / 5, 1.0 / 6, 1.0 / 7,
+    1.0 / 8, 1.0 / 9, 1.0 / 10, 1.0 / 11, 1.0 / 12, 1.0 / 13};
+
 namespace {
 
 constexpr int SR_WAVES = 4;  // tokens in flight per workgroup
@@ -37,14 +45,24 @@ __device__ __forceinline__ float dpp_f(float old, float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL,
                                                     RMASK, 0xF, false));
 }
+// as unsigned keys: one instruction a step, 0 being the identity of the lanes that
+// a step leaves out
+__device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
+  auto step = [&](auto ctrl, auto rows) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value,
+                                                     decltype(rows)::value, 0xF, false));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0xB1>(), integral_constant<int, 0xF>());
+  step(integral_constant<int, 0x4E>(), integral_constant<int, 0xF>());
+  step(integral_constant<int, 0x141>(), integral_constant<int, 0xF>());
+  step(integral_constant<int, 0x140>(), integral_constant<int, 0xF>());
+  step(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());
+  step(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ float wave_max_f(float v) {
-  v = fmaxf(v, dpp_f<0xB1, 0xF>(v, v));
-  v = fmaxf(v, dpp_f<0x4E, 0xF>(v, v));
-  v = fmaxf(v, dpp_f<0x141, 0xF>(v, v));
-  v = fmaxf(v, dpp_f<0x140, 0xF>(v, v));
-  v = fmaxf(v, dpp_f<0x142, 0xA>(v, v));
-  v = fmaxf(v, dpp_f<0x143, 0xC>(v, v));
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  return key_to_float(wave_max_key(ordered_key(v)));
 }
 __device__ __forceinline__ float wave_sum_f(float v) {
   v += dpp_f<0xB1, 0xF>(0.f, v);
@@ -75,6 +93,19 @@ __device__ __forceinline__ float step_f(float v, int d) {
   }
 }
 
+// exp(x) in fp64 for the rare comparisons below fp32: x = n ln 2 + r, Horner's form
+// of the Taylor sum to r^13 / 13! (|r| <= 0.35: 4e-18).
+__device__ __forceinline__ double exp64(double x) {
+  x = fmin(fmax(x, -800.0), 800.0);  // beyond: 0 and inf all the same
+  const double n = rint(x * 1.4426950408889634);
+  // ln 2 as its upper 32 bits and the rest
+  const double r = fma(n, -0x1.a39ef35793c76p-33, fma(n, -0x1.62e42feep-1, x));
+  double p = 1.0;
+#pragma unroll
+  for (int i = 13; i >= 1; --i) p = fma(p * r, ainfer_scored_inv[i], 1.0);
+  return ldexp(p, (int)n);
+}
+
 // fp64 -> uint64 whose unsigned order is the order of the numbers
 __device__ __forceinline__ uint64_t ordered_key_d(double d) {
   uint64_t u = __builtin_bit_cast(uint64_t, d);
@@ -94,12 +125,14 @@ __device__ __forceinline__ float exp_fast(float d) {
   return __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
 }
 // Bounds on a biased key's error.  Sigmoid: 2^-22, and half an ulp of the sum.
-// Softmax: p = e / Z, e = exp(l - max) off by 2^-23 |l - max| 1.5 + 2^-23, and
-// e |l - max| <= 0.37; Z is a sum of at most 1024 such terms, relative error below
-// 2^-23 1.5 (mean |l - max| by weight, below 10) + 38 2^-24 (32 in a lane, 6
-// across): below 2^-18 p in all, with p <= 1 / Z.
+// Softmax: p = e / Z with e = exp(-d), d = max - l, off by (1.125 d + 1) 2^-23
+// relative (the difference, the product with log2 e, the constant, the exp2), so
+// e by 1.01 2^-23; Z by the mean of that, weighted by e (the mean d is at most
+// ln 1024 = 6.9: 8.8 2^-23), and by 11 levels of additions (5.5 2^-23) and the
+// reciprocal: below 17.4 2^-23 p in all, with p <= 1 / Z.
 constexpr float KEY_REL = 0x1p-23f;
-constexpr float SIG_ABS = 0x1p-22f, SOFT_REL = 0x1p-18f;
+constexpr float SIG_ABS = 0x1p-22f, SOFT_REL = 0x1.2p-19f;
+constexpr float Z_REL = 0x1.1p-19f;  // of Z and p = e / Z in fp64: (8.8 + 5.5 + 1) 2^-23
 constexpr float BIAS_MOST = 1e38f;
 
 // a logit as the definition takes it: -inf where masked, +inf the largest
@@ -111,15 +144,18 @@ __device__ __forceinline__ float clean_bias(float b) {
 }
 
 struct Row {  // one token's logits and what its keys need
-  const void *p;
+  const void *base;
+  int64_t ld;
+  int t;
   const float *bias;
   int dtype;
   float lowest;
   float m;    // softmax: largest logit
   double z;   // softmax: sum of exp(l - m)
   __device__ __forceinline__ float logit(int e) const {
-    const float x = dtype == AINFER_ACT_F32 ? ((const float *)p)[e]
-                                            : bf16_to_f32(((const uint16_t *)p)[e]);
+    const size_t at = (size_t)t * ld + e;
+    const float x = dtype == AINFER_ACT_F32 ? ((const float *)base)[at]
+                                            : bf16_to_f32(((const uint16_t *)base)[at]);
     return clean_logit(x, lowest);
   }
 };
@@ -130,7 +166,8 @@ __device__ double key64(const Row &r, int e, float l) {
   if constexpr (!BIAS) return (double)l;
   const float b = clean_bias(r.bias[e]);
   if (l == neg_inf() || b == neg_inf()) return -INFINITY;
-  const double s = SOFT ? exp((double)l - (double)r.m) / r.z : 1.0 / (1.0 + exp(-(double)l));
+  const double s =
+      SOFT ? exp64((double)l - (double)r.m) / r.z : 1.0 / (1.0 + exp64(-(double)l));
   return s + (double)b;
 }
 // score + bias in 64 bits, also without a bias (the sum of two of a group);
@@ -139,20 +176,36 @@ template <bool BIAS, bool SOFT>
 __device__ double score64(const Row &r, int e, float l) {
   if constexpr (BIAS) return key64<BIAS, SOFT>(r, e, l);
   if (l == neg_inf()) return -INFINITY;
-  return SOFT ? exp((double)l - (double)r.m) : 1.0 / (1.0 + exp(-(double)l));
+  return SOFT ? exp64((double)l - (double)r.m) : 1.0 / (1.0 + exp64(-(double)l));
+}
+
+// rank of this lane's candidate by 64-bit key, equal ones lower expert first
+__device__ __forceinline__ int rank64(double d, int e, int nc) {
+  int rank = 0;
+  for (int j = 0; j < nc; ++j) {
+    const double o = readlane_d(d, j);
+    rank += (o > d || (o == d && __builtin_amdgcn_readlane(e, j) < e)) ? 1 : 0;
+  }
+  return rank;
 }
 
 struct Slot {  // the experts of this lane: base .. base + n - 1 of its group
   int base, n;
 };
 
-// softmax's sum in 64 bits
+// softmax's sum in 64 bits, four terms at a time
 __device__ double soft_sum64(const Row &r, const Slot &s) {
   double z = 0.0;
 #pragma unroll 1
-  for (int i = 0; i < s.n; ++i) {
-    const float l = r.logit(s.base + i);
-    if (l != neg_inf()) z += exp((double)l - (double)r.m);
+  for (int i = 0; i < s.n; i += 4) {
+    float l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l[j] = i + j < s.n ? r.logit(s.base + i + j) : neg_inf();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double e = exp64((double)fmaxf(l[j], -3.402823466e38f) - (double)r.m);
+      z += l[j] != neg_inf() ? e : 0.0;
+    }
   }
   return wave_sum_f64(z);
 }
@@ -229,80 +282,120 @@ __device__ int pick_rounds(const Row &r, const Slot &s, bool kept, int k, int la
   return mine;
 }
 
-struct Cand {  // one candidate in LDS: ordered key and ~expert (one 64-bit
-  uint64_t c;  // order: key up, then lower expert), and its logit
-  float l;
-  uint32_t e;
+// a lane's NV logits of one row, as loaded: whole 16- or 8-byte pieces where
+// VEC allows, else one by one; what lies past the lane's experts reads as 0
+template <int NV>
+struct Raw {
+  uint32_t v[NV];  // fp32 bits
+  __device__ __forceinline__ void load(const ScoredArgs &a, int t, const Slot &s) {
+    const int esz = a.dtype == AINFER_ACT_F32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t r =
+        make_rsrc((const char *)a.logits + (size_t)t * a.ld * esz, a.G * a.per * esz);
+    auto at = [&](int i) { return i < s.n ? (uint32_t)(s.base + i) * esz : BUF_OOB; };
+    if (esz == 4) {
+      if constexpr (NV >= 4) {
+        if (a.vec) {
+#pragma unroll
+          for (int i = 0; i < NV; i += 4) {
+            const u32x4 q = buf_load16(r, at(i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] = q[j];
+          }
+          return;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at(i), 0, 0);
+    } else {
+      if constexpr (NV >= 4) {
+        if (a.vec) {
+          constexpr int P = NV >= 8 ? 8 : 4;
+#pragma unroll
+          for (int i = 0; i < NV; i += P) {
+            u32x4 q;
+            if constexpr (P == 8) {
+              q = buf_load16(r, at(i));
+            } else {
+              const u32x2 h = __builtin_bit_cast(
+                  u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at(i), 0, 0));
+              q = (u32x4){h[0], h[1], 0, 0};
+            }
+#pragma unroll
+            for (int j = 0; j < P; ++j) v[i + j] = j & 1 ? q[j / 2] & 0xFFFF0000u : q[j / 2] << 16;
+          }
+          return;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        v[i] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at(i), 0, 0) << 16;
+    }
+  }
 };
 
-template <int NV, bool BIAS, bool SOFT>
+// The candidates of one token in a wave's LDS: key, logit, expert.
+struct Cands {
+  float key[64], l[64], b[64];
+  int e[64];
+};
+
+template <int NV, bool BIAS, bool SOFT, bool GRP>
 __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
-  __shared__ Cand s_cand[SR_WAVES][64];
+  __shared__ __align__(16) Cands s_cand[SR_WAVES];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Cand *cand = s_cand[wave];
-  const int lanes = 1 << a.gl;  // lanes of a group's slot
-  const int g = lane >> a.gl, sub = lane & (lanes - 1);
+  Cands &cand = s_cand[wave];
+  const int gl = GRP ? a.gl : 6;  // log2 of a group's lanes
+  const int lanes = 1 << gl;
+  const int g = lane >> gl, sub = lane & (lanes - 1);
   Slot sl;
   sl.base = g * a.per + sub * NV;
   sl.n = g < a.G ? min(max(a.per - sub * NV, 0), NV) : 0;
-  const bool f32 = a.dtype == AINFER_ACT_F32;
-  const size_t esz = f32 ? 4 : 2;
+  const bool full = __ballot(sl.n == NV) == ~0ull;  // every lane has NV experts
+  const int step = gridDim.x * SR_WAVES;
+  int t = blockIdx.x * SR_WAVES + wave;
+  if (t >= a.T) return;
+  Raw<NV> raw;
+  raw.load(a, t, sl);
   float b[BIAS ? NV : 1];
   if constexpr (BIAS) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) b[i] = i < sl.n ? clean_bias(a.bias[sl.base + i]) : neg_inf();
+    for (int i = 0; i < NV; ++i) {  // all in flight, without a branch
+      const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(
+          make_rsrc(a.bias, a.G * a.per * 4), i < sl.n ? (sl.base + i) * 4 : BUF_OOB, 0, 0);
+      b[i] = __uint_as_float(v);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) b[i] = i < sl.n ? clean_bias(b[i]) : neg_inf();
   }
   Row r;
+  r.base = a.logits;
+  r.ld = a.ld;
   r.bias = a.bias;
   r.dtype = a.dtype;
-  r.lowest = f32 ? -3.402823466e38f : -3.3895313892515355e38f;
+  r.lowest = a.dtype == AINFER_ACT_F32 ? -3.402823466e38f : -3.3895313892515355e38f;
   const bool need_z = SOFT && (BIAS || !a.renorm);
-  const bool need_m = SOFT && (need_z || a.G > 1);
+  const bool need_m = SOFT && (need_z || GRP);
 
-  for (int t = blockIdx.x * SR_WAVES + wave; t < a.T; t += gridDim.x * SR_WAVES) {
-    r.p = (const char *)a.logits + (size_t)t * a.ld * esz;
+  for (; t < a.T; t += step) {
+    r.t = t;
     float l[NV];
-    {
+    bool odd = false;  // a mask, an infinity or NaN
 #pragma unroll
-      for (int i = 0; i < NV; ++i) l[i] = neg_inf();
-      bool done = false;
-      if constexpr (NV >= 4) {
-        if (f32 && a.vec) {  // whole 16-byte pieces: per is a multiple of 4
-          const float *p = (const float *)r.p + sl.base;
-#pragma unroll
-          for (int i = 0; i < NV; i += 4)
-            if (i < sl.n) {
-              const f32x4 v = *(const f32x4 *)(p + i);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) l[i + q] = v[q];
-            }
-          done = true;
-        }
-      }
-      if constexpr (NV >= 8) {
-        if (!f32 && a.vec) {  // per is a multiple of 8
-          const uint16_t *p = (const uint16_t *)r.p + sl.base;
-#pragma unroll
-          for (int i = 0; i < NV; i += 8)
-            if (i < sl.n) {
-              const u32x4 v = *(const u32x4 *)(p + i);
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                l[i + q] = __uint_as_float(q & 1 ? v[q / 2] & 0xFFFF0000u : v[q / 2] << 16);
-            }
-          done = true;
-        }
-      }
-      if (!done) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i < sl.n)
-            l[i] = f32 ? ((const float *)r.p)[sl.base + i]
-                       : bf16_to_f32(((const uint16_t *)r.p)[sl.base + i]);
-      }
+    for (int i = 0; i < NV; ++i) {
+      l[i] = __uint_as_float(raw.v[i]);
+      odd |= !(fabsf(l[i]) < -r.lowest);
+    }
+    if (t + step < a.T) raw.load(a, t + step, sl);  // the next token's, in flight meanwhile
+    const bool masks = __ballot(odd) != 0;
+    if (__builtin_expect(masks, 0)) {
+      asm volatile("");  // a branch, not selects that every row pays for
 #pragma unroll
       for (int i = 0; i < NV; ++i) l[i] = clean_logit(l[i], r.lowest);
+    }
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) l[i] = i < sl.n ? l[i] : neg_inf();
     }
 
     // scores where the selection or the weights need them
@@ -315,32 +408,36 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
       m = wave_max_f(m);
       r.m = m == neg_inf() ? 0.0f : m;
     }
-    float v[NV];  // selection keys
+    float v[NV];  // selection keys; -inf: masked, or not there (its bias is -inf too)
     if constexpr (SOFT) {
       if (need_z) {
         float e[NV];
-        float sum = 0.0f;
+        float sum[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          e[i] = exp_fast(l[i] - r.m);  // masked: exp2(-inf) = 0
-          sum += e[i];
-        }
-        z = wave_sum_f(sum);
+        for (int i = 0; i < NV; ++i) sum[i] = e[i] = exp_fast(l[i] - r.m);  // masked: exp2(-inf) = 0
+#pragma unroll
+        for (int d = NV / 2; d >= 1; d /= 2)
+#pragma unroll
+          for (int i = 0; i < d; ++i) sum[i] += sum[i + d];
+        z = wave_sum_f(sum[0]);
         if (z == 0.0f) z = 1.0f;
         if constexpr (BIAS) {
           const float rz = 1.0f / z;
           eps_abs = SOFT_REL * rz;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) v[i] = l[i] == neg_inf() ? neg_inf() : fmaf(e[i], rz, b[i]);
+          for (int i = 0; i < NV; ++i) v[i] = fmaf(e[i], rz, b[i]);
         }
       }
     } else if constexpr (BIAS) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] = l[i] == neg_inf() ? neg_inf() : sigmoid_fast(l[i]) + b[i];
+      for (int i = 0; i < NV; ++i) v[i] = sigmoid_fast(l[i]) + b[i];
     }
     if constexpr (!BIAS) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) v[i] = l[i];
+    } else if (masks) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = l[i] == neg_inf() ? neg_inf() : v[i];
     }
 
     bool have_z64 = false;
@@ -352,8 +449,8 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
     };
 
     // groups: the kept ones' lanes go on
-    bool kept = g < a.G;
-    if (a.G > 1) {
+    bool kept = GRP ? g < a.G : true;
+    if constexpr (GRP) {
       const bool top2 = a.group_score == AINFER_GROUP_TOP2;
       float m1 = v[0], m2 = neg_inf();
 #pragma unroll
@@ -366,98 +463,161 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
         m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
         m1 = fmaxf(m1, o1);
       }
-      float gv = m1, eps = 0.0f;
+      float gv = m1;
       if (top2) {
         if constexpr (!BIAS) {  // the logits order the scores: the two largest give the sum
           m1 = m1 == neg_inf() ? m1 : SOFT ? exp_fast(m1 - r.m) : sigmoid_fast(m1);
           m2 = m2 == neg_inf() ? m2 : SOFT ? exp_fast(m2 - r.m) : sigmoid_fast(m2);
         }
         gv = m2 == neg_inf() ? m1 : m1 + m2;
-        // exp alone is off by 2^-22.4 (0.37 1.5 2^-23 + 2^-23)
-        eps = 2.0f * (BIAS ? eps_abs : SIG_ABS) + KEY_REL * (fabsf(m1) + fabsf(m2));
-      } else if constexpr (BIAS) {
-        eps = eps_abs + KEY_REL * fabsf(m1);
-      }
-      if (gv == neg_inf()) eps = 0.0f;
-      int rank = 0, above = 0, near = 0;
-      for (int h = 0; h < a.G; ++h) {
-        const float o = readlane_f(gv, h << a.gl), oe = readlane_f(eps, h << a.gl);
-        const float d = o - gv, e = oe + eps;  // both -inf: d is NaN, equal
-        rank += (o > gv || (o == gv && h < g)) ? 1 : 0;
-        above += d > e ? 1 : 0;
-        near += d < -e ? 0 : 1;  // itself among them
       }
       const bool exact = !BIAS && !top2;
-      if (!exact && __ballot(g < a.G && above < a.top && near > a.top)) {
-        z64();
-        rank = group_rank64(group64<BIAS, SOFT>(r, sl, lanes, top2), a.G, a.gl, g);
+      // the errors of two values: each of up to two keys (exp alone is off by
+      // 1.01 2^-23) and the rounding of their sum
+      float tol = 0.0f;
+      if (!exact)
+        tol = 4.0f * (BIAS ? eps_abs : SIG_ABS) +
+              4.0f * KEY_REL * (m2 == neg_inf() ? fabsf(gv) : fabsf(m1) + fabsf(m2));
+      if (gv == neg_inf()) tol = 0.0f;
+      const float hi_g = gv + tol, lo_g = gv - tol;
+      int above = 0, near = 0;
+      for (int h = 0; h < a.G; ++h) {
+        const float o = readlane_f(gv, h << gl);
+        above += o > hi_g ? 1 : 0;
+        near += o >= lo_g ? 1 : 0;  // itself among them
       }
-      kept = g < a.G && rank < a.top;
+      kept = g < a.G && near <= a.top;
+      if (__builtin_expect(__ballot(g < a.G && above < a.top && near > a.top) != 0, 0)) {
+        z64();
+        const double v64 = exact ? (double)gv : group64<BIAS, SOFT>(r, sl, lanes, top2);
+        kept = g < a.G && group_rank64(v64, a.G, gl, g) < a.top;
+      }
     }
 
-    // a value that k lanes' maxima reach
+    // a value that at least k lanes' maxima reach, and few more: down from the
+    // largest in growing steps, then by halves
     float lm = v[0];
 #pragma unroll
     for (int i = 1; i < NV; ++i) lm = fmaxf(lm, v[i]);
     const uint32_t ok = kept && lm != neg_inf() ? ordered_key(lm) : 0u;
     float tf = -3.402823466e38f;
     if (__popcll(__ballot(ok != 0)) >= a.k) {
-      uint32_t tk = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = tk | (1u << bit);
+      const uint32_t most = wave_max_key(ok);
+      uint32_t lo = 1, hi = most + 1;  // at least k lanes reach lo, fewer reach hi
+      uint32_t down = 1u << 20;
+      while (hi - lo > 1) {
+        uint32_t c = lo + (hi - lo) / 2;
+        if (down && most - down < hi && most - down > lo && most > down) c = most - down;
         const int n = __popcll(__ballot(ok >= c));
-        if (n >= a.k) tk = c;
-        if (n == a.k) break;
+        if (n >= a.k) {
+          lo = c;
+          down = 0;
+          if (n <= a.k + a.more) break;
+        } else {
+          hi = c;
+          down *= 4;
+        }
       }
-      tf = key_to_float(tk);
+      tf = key_to_float(lo);
       if constexpr (BIAS) tf -= 4.0f * eps_abs + 4.0f * KEY_REL * fabsf(tf);
     }
     if (!kept) tf = INFINITY;
-    int cnt = 0;
+    int cnt = 0, incl = 0, nc = 0;
+    auto count = [&]() {
+      cnt = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) cnt += v[i] >= tf ? 1 : 0;
-    const int incl = wave_scan_incl(cnt);
-    const int nc = __builtin_amdgcn_readlane(incl, 63);
+      for (int i = 0; i < NV; ++i) cnt += v[i] >= tf ? 1 : 0;
+      incl = wave_scan_incl(cnt);
+      nc = __builtin_amdgcn_readlane(incl, 63);
+    };
+    count();
+    if (__builtin_expect(nc > 64, 0)) {
+      // several experts of many lanes (a large k): halve between a value that more
+      // than 64 reach and one that fewer than k do
+      uint32_t lo = ordered_key(-3.402823466e38f), hi = ordered_key(3.402823466e38f);
+      while (hi - lo > 1) {
+        const uint32_t c = lo + (hi - lo) / 2;
+        const float f = key_to_float(c);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) n += __popcll(__ballot(kept && v[i] >= f));
+        if (n >= a.k) lo = c;
+        else hi = c;
+        if (n >= a.k && n <= 48) break;
+      }
+      tf = key_to_float(lo);
+      if constexpr (BIAS) tf -= 4.0f * eps_abs + 4.0f * KEY_REL * fabsf(tf);
+      if (!kept) tf = INFINITY;
+      count();
+    }
 
     int e_mine = 0, rank = 64;
     float l_mine = neg_inf();
-    if (nc >= a.k && nc <= 64) {
+    if (__builtin_expect(nc >= a.k && nc <= 64, 1)) {
       int pos = incl - cnt;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (v[i] >= tf) {
-          Cand c;
-          c.c = ((uint64_t)ordered_key(v[i]) << 32) | (uint32_t)~(uint32_t)(sl.base + i);
-          c.l = l[i];
-          c.e = sl.base + i;
-          cand[pos++] = c;
+          if constexpr (BIAS) {
+            cand.key[pos] = v[i];
+            cand.b[pos] = b[i];
+          }
+          cand.l[pos] = l[i];
+          cand.e[pos] = sl.base + i;
+          ++pos;
         }
+      float *key = BIAS ? cand.key : cand.l;
+      if (lane >= nc) key[lane] = neg_inf();
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       const bool in = lane < nc;
-      const uint64_t mine = in ? cand[lane].c : 0;
-      if (in) {
-        e_mine = (int)cand[lane].e;
-        l_mine = cand[lane].l;
-      }
-      rank = 0;
-      for (int j = 0; j < nc; ++j) rank += cand[j].c > mine ? 1 : 0;
-      if constexpr (BIAS) {
-        // the candidates in order: neighbours nearer than their errors?
-        const float key = key_to_float((uint32_t)(mine >> 32));
-        const int src = __builtin_amdgcn_ds_permute(4 * (in ? rank : lane), __float_as_int(key));
-        const float ks = __int_as_float(src);
-        const float nx = __shfl_down(ks, 1);
-        const bool near = lane + 1 < nc && lane < a.k &&
-                          !(ks - nx > 2.0f * eps_abs + 2.0f * KEY_REL * fmaxf(fabsf(ks), fabsf(nx)));
-        if (__ballot(near)) {
-          z64();
-          const double d = in ? key64<BIAS, SOFT>(r, e_mine, l_mine) : -INFINITY;
-          rank = 0;
+      const float mine = key[lane];
+      l_mine = BIAS ? cand.l[lane] : mine;
+      e_mine = cand.e[lane];
+      // candidates surely above this one, and not surely below it (itself among them)
+      const float tol = BIAS ? 2.0f * eps_abs + 2.0f * KEY_REL * fabsf(mine) : 0.0f;
+      const float hi = mine + tol, lo = mine - tol;
+      int above = 0, near = 0;
+      auto four = [&](const f32x4 &o) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          above += o[j] > hi ? 1 : 0;
+          near += o[j] >= lo ? 1 : 0;
+        }
+      };
+      f32x4 o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = *(const f32x4 *)&key[4 * q];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (4 * q < nc) four(o[q]);
+      for (int j = 16; j < nc; j += 4) four(*(const f32x4 *)&key[j]);
+      rank = above;
+      if (__builtin_expect(__ballot(in && above < a.k && near - above != 1) != 0, 0)) {
+        // equal keys, or biased ones nearer than their errors: in 64 bits
+        if constexpr (!BIAS) {
+          rank = rank64(in ? (double)mine : -INFINITY, e_mine, nc);
+        } else if constexpr (!SOFT) {
+          const double s = 1.0 / (1.0 + exp64(-(double)l_mine));
+          rank = rank64(in ? s + (double)cand.b[lane] : -INFINITY, e_mine, nc);
+        } else {
+          // Z, common to all, changes a difference of keys by its error times the
+          // difference of the scores: mostly the fp32 Z settles the order
+          const double e = in ? exp64((double)l_mine - (double)r.m) : 0.0;
+          const double be = (double)cand.b[lane];
+          double p = e / (double)z, d = in ? p + be : -INFINITY;
+          int sure = 0, maybe = 0;
           for (int j = 0; j < nc; ++j) {
-            const double o = readlane_d(d, j);
-            rank += (o > d || (o == d && __builtin_amdgcn_readlane(e_mine, j) < e_mine)) ? 1 : 0;
+            const double od = readlane_d(d, j), op = readlane_d(p, j);
+            const double tol = fabs(op - p) * (double)Z_REL + 1e-14 * (fabs(d) + 1.0);
+            sure += od - d > tol ? 1 : 0;
+            maybe += od - d >= -tol ? 1 : 0;
           }
+          if (__ballot(in && sure < a.k && maybe - sure != 1)) {
+            z64();
+            d = in ? e / r.z + be : -INFINITY;
+          }
+          rank = rank64(d, e_mine, nc);
         }
       }
       if (!in) rank = 64;
@@ -478,26 +638,24 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
     float w;
     if (a.renorm) {
       // the selected scores over their sum, scaled so that the largest does not
-      // vanish: exp(l - max), or exp(l - c) / (1 + exp(l)) with c the largest
-      // logit where that is negative
+      // vanish: exp(l - max); sigmoid: exp(l) / (1 + exp(l)), times exp(-max)
+      // where the largest logit is below 0
       const float mx = wave_max_f(live ? l_mine : neg_inf());
-      float s = 0.0f;
-      if (live) {
-        if constexpr (SOFT) {
-          s = expf(l_mine - mx);
-        } else {
-          s = l_mine > 0.0f ? 1.0f / (1.0f + expf(-l_mine))
-                            : expf(l_mine - fminf(mx, 0.0f)) / (1.0f + expf(l_mine));
-        }
+      float s;
+      if constexpr (SOFT) {
+        s = exp_fast(l_mine - mx);
+      } else {
+        const float e = exp_fast(-fabsf(l_mine));
+        s = (mx < 0.0f ? exp_fast(l_mine - mx) : l_mine > 0.0f ? 1.0f : e) *
+            __builtin_amdgcn_rcpf(1.0f + e);
       }
+      s = live ? s : 0.0f;
       const float sum = wave_sum_f(s);
-      w = sum > 0.0f ? s / sum * a.scale : 0.0f;
-    } else if (!live) {
-      w = 0.0f;
+      w = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
     } else if constexpr (SOFT) {
-      w = expf(l_mine - r.m) / z * a.scale;
+      w = live ? exp_fast(l_mine - r.m) * __builtin_amdgcn_rcpf(z) * a.scale : 0.0f;
     } else {
-      w = 1.0f / (1.0f + expf(-l_mine)) * a.scale;
+      w = live ? sigmoid_fast(l_mine) * a.scale : 0.0f;
     }
     if (sel) {
       a.idx[(size_t)t * a.k + rank] = e_mine;
@@ -506,20 +664,21 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
   }
 }
 
-template <int NV>
-void launch_nv(const ScoredArgs &a, int grid, bool soft, hipStream_t s) {
+template <int NV, bool GRP>
+void launch_grp(const ScoredArgs &a, int grid, bool soft, hipStream_t s) {
   const dim3 b(64 * SR_WAVES);
   if (a.bias) {
-    if (soft)
-      k_route_scored<NV, true, true><<<grid, b, 0, s>>>(a);
-    else
-      k_route_scored<NV, true, false><<<grid, b, 0, s>>>(a);
+    if (soft) k_route_scored<NV, true, true, GRP><<<grid, b, 0, s>>>(a);
+    else k_route_scored<NV, true, false, GRP><<<grid, b, 0, s>>>(a);
   } else {
-    if (soft)
-      k_route_scored<NV, false, true><<<grid, b, 0, s>>>(a);
-    else
-      k_route_scored<NV, false, false><<<grid, b, 0, s>>>(a);
+    if (soft) k_route_scored<NV, false, true, GRP><<<grid, b, 0, s>>>(a);
+    else k_route_scored<NV, false, false, GRP><<<grid, b, 0, s>>>(a);
   }
+}
+template <int NV>
+void launch_nv(const ScoredArgs &a, int grid, bool soft, hipStream_t s) {
+  if (a.G > 1) launch_grp<NV, true>(a, grid, soft, s);
+  else launch_grp<NV, false>(a, grid, soft, s);
 }
 
 }  // namespace
@@ -546,9 +705,13 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   while (slots < a.G) slots *= 2;
   a.gl = 0;
   while ((slots << a.gl) < 64) ++a.gl;
+  a.more = a.k <= 16 ? 3 : 0;
   const int lanes = 1 << a.gl, need = (a.per + lanes - 1) / lanes;
-  const int esz = dtype == AINFER_ACT_F32 ? 4 : 2, piece = 16 / esz;
-  a.vec = a.per % piece == 0 && (uintptr_t)logits % 16 == 0 && (ld * esz) % 16 == 0;
+  // whole pieces of 4 (8 bf16 from 8 experts a lane on) experts, dwords aligned
+  if (dtype == AINFER_ACT_F32)
+    a.vec = a.per % 4 == 0;
+  else
+    a.vec = a.per % (need > 4 ? 8 : 4) == 0 && (uintptr_t)logits % 4 == 0 && ld % 2 == 0;
   const int blocks = (T + SR_WAVES - 1) / SR_WAVES;
   const int grid = blocks < SR_MAX_GRID ? blocks : SR_MAX_GRID;
   const bool soft = r.score == AINFER_SCORE_SOFTMAX;
@@ -557,6 +720,7 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   else if (need <= 4) launch_nv<4>(a, grid, soft, s);
   else if (need <= 8) launch_nv<8>(a, grid, soft, s);
   else if (need <= 16) launch_nv<16>(a, grid, soft, s);
-  else launch_nv<32>(a, grid, soft, s);
+  else if (a.G > 1) launch_grp<32, true>(a, grid, soft, s);
+  else return hipErrorInvalidValue;  // more than 1024 experts
   return hipGetLastError();
 }
