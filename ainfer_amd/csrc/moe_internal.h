@@ -396,9 +396,6 @@ struct ScoredArgs {
   float scale;
   bool vec;         // rows readable in 16-byte pieces
 };
-#ifndef SR_MAX_GRID
-#define SR_MAX_GRID 2048
-#endif
 hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, int dtype,
                                int64_t ld, const float *bias, int T, int32_t *idx, float *w,
                                hipStream_t s);

@@ -713,7 +713,10 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   else
     a.vec = a.per % (need > 4 ? 8 : 4) == 0 && (uintptr_t)logits % 4 == 0 && ld % 2 == 0;
   const int blocks = (T + SR_WAVES - 1) / SR_WAVES;
-  const int grid = blocks < SR_MAX_GRID ? blocks : SR_MAX_GRID;
+  // a wave keeps the bias over its tokens; without one a workgroup per 4 tokens.  us at
+  // T 65536, grids of 2048 and 16384: 512 experts with a bias 64 and 93, without
+  // 52 and 45 (bf16, not renormalised 70 and 53), 64 experts 38 and 31
+  const int most = bias ? 2048 : 16384, grid = blocks < most ? blocks : most;
   const bool soft = r.score == AINFER_SCORE_SOFTMAX;
   if (need <= 1) launch_nv<1>(a, grid, soft, s);
   else if (need <= 2) launch_nv<2>(a, grid, soft, s);
