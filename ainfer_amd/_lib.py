@@ -22,6 +22,7 @@ GROUP_MAX, GROUP_TOP2 = 0, 1
 LORA_MAX_PROJ = 4
 FILL_BYTES, FILL_BF16_NORMAL, FILL_FP16_ABSNORMAL, FILL_BF16_ABSNORMAL = 0, 1, 2, 3
 MAX_TOKENS = 65536
+CHUNK_TOKENS = 4096
 STACK_MAX_TOKENS = 4
 
 # every symbol include/ainfer_moe.h declares

@@ -5,6 +5,7 @@ documents; forward/route/dispatch/block_forward enqueue on a HIP stream and
 return immediately, like the C entry points they wrap.  Every call goes to
 libainfer_moe.so; there is no other implementation behind these names.
 """
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -22,6 +23,12 @@ def _stream(stream):
     if stream is None:
         stream = torch.cuda.current_stream()
     return C.c_void_p(stream.cuda_stream)
+
+
+def _on(stream):
+    """The stream as torch's current one (buffers allocated under it are its
+    own); nothing to do for None."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def fill_(kind: int, seed: int, std: float, t: torch.Tensor, stream=None):
@@ -116,7 +123,7 @@ class MoeLayer:
             _ptr(resid_in), _ptr(resid_out), T, _stream(stream)))
 
     def route(self, x, ws, want_logits=False, stream=None):
-        T, E, k = x.shape[0], self.cfg.n_experts, self.cfg.top_k
+        T, E, k = x.shape[0], self.shape.n_experts, self.shape.top_k
         dev = self.device
         idx = torch.empty(T, k, dtype=torch.int32, device=dev)
         w = torch.empty(T, k, dtype=torch.float32, device=dev)
@@ -130,7 +137,7 @@ class MoeLayer:
     def experts(self, x, idx, ws, stream=None):
         """Expert rows in slot order: [T * k + T][H] bf16 (row t * k + j =
         expert idx[t][j] on token t, row T * k + t = the shared expert)."""
-        T, k, H = x.shape[0], self.cfg.top_k, self.cfg.hidden
+        T, k, H = x.shape[0], self.shape.top_k, self.shape.hidden
         o = torch.empty(T * k + T, H, dtype=torch.bfloat16, device=self.device)
         L.check(L.lib().ainfer_moe_experts(C.byref(self.shape), C.byref(self.weights), _ptr(x),
                                            _ptr(idx), T, _ptr(o), _ptr(ws), ws.numel(),
@@ -143,8 +150,57 @@ class MoeLayer:
                                            _ptr(resid), _ptr(y), T, _stream(stream)))
         return y
 
+    def forward_scored(self, x, y, ws, routing, bias=None, resid=None, shared=None, stream=None):
+        """forward with scored routing: the layer's router logits (its
+        router_bias, where it has one, is part of them) -> route_scored(routing,
+        logits, bias) -> experts -> combine, in steps of CHUNK_TOKENS.  shared:
+        [T][H] bf16 rows that take the place of the shared expert's (for
+        example shared_adapted's)."""
+        if (routing.n_experts, routing.top_k) != (self.shape.n_experts, self.shape.top_k):
+            raise L.MoeError("routing: the layer's n_experts and top_k")
+        T, H = x.shape[0], self.shape.hidden
+        for t in (x, y, resid, shared):
+            if t is not None and not (t.shape == (T, H) and t.dtype == torch.bfloat16
+                                      and t.is_contiguous() and t.device == x.device):
+                raise L.MoeError("x, y, resid and shared: contiguous [T][H] bf16 on one device")
+        if shared is not None and self.shape.shared_inter == 0:
+            raise L.MoeError("shared: the layer has no shared expert")
+        with _on(stream):
+            for t in range(0, T, L.CHUNK_TOKENS):
+                c = slice(t, t + L.CHUNK_TOKENS)
+                idx, w, sg, logits = self.route(x[c], ws, want_logits=True)
+                route_scored(routing, logits, bias, out=(idx, w))
+                o = self.experts(x[c], idx, ws)
+                if shared is not None:
+                    o[idx.numel():].copy_(shared[c])
+                self.combine(o, w, sg, y[c], resid[c] if resid is not None else None)
+        return y
+
+    def shared_adapted(self, x, token_adapter, gate_up, down, lora_ws, stream=None):
+        """The shared expert's rows [T][H] (bf16) with each token's adapters on
+        its three projections: x quantised to int8 groups, gate and up as
+        ainfer_moe_int4_gemv_i8, their adapters, SiLU-mul, the same for down.
+        gate_up (two projections, x bf16, y fp32) and down (x and y fp32):
+        LoraAdapters or None; lora_ws: a workspace large enough for both."""
+        sh, wt = self.shape, self.weights
+        H, Is = sh.hidden, sh.shared_inter
+        if Is == 0 or x.shape[1] != H:
+            raise L.MoeError("a layer with a shared expert, x of its hidden size")
+        with _on(stream):
+            q, sq = act_quant_i8(x)
+            gate = int4_gemv_i8(wt.ws_gate, wt.ss_gate, sh.scale_dtype, q, sq, Is)
+            up = int4_gemv_i8(wt.ws_up, wt.ss_up, sh.scale_dtype, q, sq, Is)
+            if gate_up is not None:
+                gate_up.apply(x, token_adapter, [gate, up], lora_ws)
+            act = silu_mul(gate, up, gate)
+            q, sq = act_quant_i8(act)
+            out = int4_gemv_i8(wt.ws_down, wt.ss_down, sh.scale_dtype, q, sq, H)
+            if down is not None:
+                down.apply(act, token_adapter, [out], lora_ws)
+            return out.to(torch.bfloat16)
+
     def dispatch(self, idx, ws, stream=None):
-        T, E, k = idx.shape[0], self.cfg.n_experts, self.cfg.top_k
+        T, E, k = idx.shape[0], self.shape.n_experts, self.shape.top_k
         dev = self.device
         counts = torch.empty(E, dtype=torch.int32, device=dev)
         offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
@@ -257,34 +313,34 @@ _ACT = {torch.float32: L.ACT_F32, torch.bfloat16: L.ACT_BF16}
 
 
 def _rows(t, name, cols=None):
-    """A device matrix of fp32 or bf16 rows, each contiguous: (dtype, rows,
-    columns, pitch)."""
-    dt = _ACT.get(t.dtype)
-    if dt is None or not t.is_cuda or t.dim() != 2:
+    """A device matrix of fp32 or bf16 rows, each contiguous: (dtype, device,
+    rows, columns, pitch)."""
+    dt, dev = _ACT.get(t.dtype), t.get_device()
+    if dt is None or dev < 0 or t.dim() != 2:
         raise L.MoeError(f"{name}: a device matrix of fp32 or bf16 rows")
-    (n, m), (ld, one) = t.shape, t.stride()
+    n, m = t.shape
+    ld, one = t.stride()
     if (cols is not None and m != cols) or (one != 1 and m != 1):
         raise L.MoeError(f"{name}: contiguous rows" + (f" of {cols} columns" if cols else ""))
-    return dt, n, m, (ld if n > 1 else m)  # a single row has no pitch
+    return dt, dev, n, m, (ld if n > 1 else m)  # a single row has no pitch
 
 
-def _vector(t, name, dtype, n, device):
-    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+def _vector(t, name, dtype, n, dev):
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
         raise L.MoeError(f"{name}: {n} contiguous {dtype} values on the inputs' device")
 
 
-def _call(fn, device, stream, *args):
+def _call(fn, dev, stream, *args):
     """fn(*args, stream) on the device the tensors are on; its current stream
     when none is given."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _enqueue(fn, device, stream, args)
-    return _enqueue(fn, device, stream, args)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return _enqueue(fn, dev, stream, args)
+    return _enqueue(fn, dev, stream, args)
 
 
-def _enqueue(fn, device, stream, args):
-    raw = (torch._C._cuda_getCurrentRawStream(device.index) if stream is None
-           else stream.cuda_stream)
+def _enqueue(fn, dev, stream, args):
+    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
     rc = fn(*args, raw)
     if rc:
         L.check(rc)
@@ -294,17 +350,18 @@ def route_scored(routing, logits, bias=None, out=None, stream=None):
     """Scored routing of logits [T][E] (ainfer_moe_route_scored; routing: an
     L.Routing): (topk_idx [T][k] int32, topk_w [T][k] fp32), as MoeLayer.dispatch,
     experts and combine take them.  out: the two tensors to write."""
-    dt, T, E, ld = _rows(logits, "logits", routing.n_experts)
-    dev, k = logits.device, routing.top_k
+    dt, dev, T, E, ld = _rows(logits, "logits", routing.n_experts)
+    k = routing.top_k
     if bias is not None:
         _vector(bias, "bias", torch.float32, E, dev)
     if out is None:
-        idx = torch.empty(T, k, dtype=torch.int32, device=dev)
-        w = torch.empty(T, k, dtype=torch.float32, device=dev)
+        with _on(stream):
+            idx = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+            w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
     else:
         idx, w = out
         if not (idx.dtype == torch.int32 and w.dtype == torch.float32
-                and idx.shape == w.shape == (T, k) and idx.device == dev == w.device
+                and idx.shape == w.shape == (T, k) and idx.get_device() == dev == w.get_device()
                 and idx.is_contiguous() and w.is_contiguous()):
             raise L.MoeError("out: (idx int32, w fp32), [T][k] contiguous on the logits' device")
     _call(L.lib().ainfer_moe_route_scored, dev, stream, C.byref(routing), logits.data_ptr(), dt,
@@ -312,14 +369,42 @@ def route_scored(routing, logits, bias=None, out=None, stream=None):
     return idx, w
 
 
+def act_quant_i8(x, stream=None):
+    """int8 codes [T][K] and group scales [T][K / 128] of contiguous x
+    (ainfer_moe_act_quant_i8)."""
+    dt, dev, T, K, ld = _rows(x, "x")
+    if ld != K:
+        raise L.MoeError("x: contiguous")
+    with _on(stream):
+        q = torch.empty(T, K, dtype=torch.int8, device=x.device)
+        sq = torch.empty(T, K // 128, dtype=torch.float32, device=x.device)
+    _call(L.lib().ainfer_moe_act_quant_i8, dev, stream, x.data_ptr(), dt, T, K, q.data_ptr(),
+          sq.data_ptr())
+    return q, sq
+
+
+def int4_gemv_i8(packed, scales, scale_dtype, q, sq, rows, stream=None):
+    """y [T][rows] fp32 of an INT4 matrix (device addresses of its nibbles and
+    scales) and act_quant_i8's codes (ainfer_moe_int4_gemv_i8)."""
+    T, K = q.shape
+    dev = q.get_device()
+    _vector(sq.view(-1), "sq", torch.float32, T * (K // 128), dev)
+    if q.dtype != torch.int8 or not q.is_contiguous() or dev < 0:
+        raise L.MoeError("q: contiguous int8 rows on a device")
+    with _on(stream):
+        y = torch.empty(T, rows, dtype=torch.float32, device=q.device)
+    _call(L.lib().ainfer_moe_int4_gemv_i8, dev, stream, packed, scales, scale_dtype, q.data_ptr(),
+          sq.data_ptr(), rows, K, T, y.data_ptr())
+    return y
+
+
 def silu_mul(gate, up, act, stream=None):
     """act = gate / (1 + exp(-gate)) * up over rows of any pitch
-    (ainfer_moe_silu_mul)."""
-    dt, T, n, gld = _rows(gate, "gate")
-    udt, uT, _, uld = _rows(up, "up", n)
-    adt, aT, _, ald = _rows(act, "act", n)
-    dev = gate.device
-    if not (udt == dt and uT == T == aT and up.device == dev == act.device):
+    (ainfer_moe_silu_mul); act may be gate or up."""
+    dt, dev, T, n, gld = _rows(gate, "gate")
+    udt, udev, uT, _, uld = _rows(up, "up", n)
+    adt, adev, aT, _, ald = _rows(act, "act", n)
+    if not (udt == dt and uT == T == aT and udev == dev == adev):
         raise L.MoeError("gate, up and act: one shape and device, gate and up one type")
     _call(L.lib().ainfer_moe_silu_mul, dev, stream, gate.data_ptr(), gld, up.data_ptr(), uld, dt,
           T, n, act.data_ptr(), ald, adt)
@@ -339,9 +424,9 @@ class LoraAdapters:
                              f"{L.LORA_MAX_PROJ} projections")
         if x_dtype not in _ACT or y_dtype not in _ACT:
             raise L.MoeError("x and y: fp32 or bf16")
-        dev = a[0].device
+        dev = a[0].get_device()
         for t in a + b:
-            if not (t.dtype == torch.bfloat16 and t.is_cuda and t.device == dev
+            if not (t.dtype == torch.bfloat16 and t.get_device() == dev >= 0
                     and t.is_contiguous() and t.dim() == 3):
                 raise L.MoeError("a and b: contiguous [N][R][K] and [N][M][R] bf16 on one device")
         N, R, K = a[0].shape
@@ -353,7 +438,7 @@ class LoraAdapters:
         if scales is not None:
             _vector(scales, "scales", torch.float32, N, dev)
         self.tensors = (a, b, ranks, scales)
-        self.device, self.x_dtype, self.y_dtype = dev, x_dtype, y_dtype
+        self.device, self.dev, self.x_dtype, self.y_dtype = a[0].device, dev, x_dtype, y_dtype
         self.cols, self.rows = K, [t.shape[1] for t in b]
         s = L.Lora(N, R, K, len(a), _ACT[x_dtype], _ACT[y_dtype])
         for p, (ta, tb) in enumerate(zip(a, b)):
@@ -376,19 +461,20 @@ class LoraAdapters:
     def apply(self, x, token_adapter, ys, ws, stream=None):
         """ys[p] += scale * (x a^T) b^T of each token's adapter, in place
         (ainfer_moe_lora_apply); tokens without one keep their rows."""
-        dt, T, _, ld = _rows(x, "x", self.cols)
-        dev = self.device
-        if x.dtype != self.x_dtype or x.device != dev or ws.device != dev:
+        dev = self.dev
+        _, xdev, T, _, ld = _rows(x, "x", self.cols)
+        if x.dtype != self.x_dtype or xdev != dev or ws.get_device() != dev or \
+                not ws.is_contiguous():
             raise L.MoeError("x: the adapters' x type; x and the workspace on their device")
         _vector(token_adapter, "token_adapter", torch.int32, T, dev)
         if len(ys) != len(self.rows):
             raise L.MoeError("one y per projection")
         yp, yl = (C.c_void_p * len(ys))(), (C.c_int64 * len(ys))()
         for p, y in enumerate(ys):
-            _, n, _, yl[p] = _rows(y, "y", self.rows[p])
-            if n != T or y.dtype != self.y_dtype or y.device != dev:
+            _, ydev, n, _, yl[p] = _rows(y, "y", self.rows[p])
+            if n != T or y.dtype != self.y_dtype or ydev != dev:
                 raise L.MoeError("y: a row per token, of the adapters' y type and device")
             yp[p] = y.data_ptr()
         _call(L.lib().ainfer_moe_lora_apply, dev, stream, C.byref(self.struct), x.data_ptr(), ld,
-              token_adapter.data_ptr(), T, yp, yl, ws.data_ptr(), ws.numel())
+              token_adapter.data_ptr(), T, yp, yl, ws.data_ptr(), ws.nbytes)
         return ys
