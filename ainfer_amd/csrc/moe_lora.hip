@@ -313,11 +313,20 @@ __device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
-template <bool YF32>
-struct YRun {  // 4 values of y
-  uint32_t v[YF32 ? 4 : 2];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
-    if constexpr (YF32) {
+// a lane's 4 values of one token's y: neighbours (VEC), or 16 apart, one access each
+template <bool YF32, bool VEC>
+struct YRun {
+  uint32_t v[YF32 || !VEC ? 4 : 2];
+  // at: of value j
+  template <class At>
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, At at_j) {
+    const uint32_t at = at_j(0);
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = YF32 ? __builtin_amdgcn_raw_buffer_load_b32(r, at_j(j), 0, 0)
+                    : __builtin_amdgcn_raw_buffer_load_b16(r, at_j(j), 0, 0);
+    } else if constexpr (YF32) {
       const u32x4 t = buf_load16(r, at);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = t[j];
@@ -327,8 +336,31 @@ struct YRun {  // 4 values of y
       v[1] = t[1];
     }
   }
-  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t at) const {
-    if constexpr (YF32)
+  // += d, rounded once
+  __device__ __forceinline__ void add(const YRun &y, float d0, float d1, float d2, float d3) {
+    const float d[4] = {d0, d1, d2, d3};
+    if constexpr (YF32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(__uint_as_float(y.v[j]) + d[j]);
+    } else if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        v[j] = bf16x2_bits(bf16_lo(y.v[j]) + d[2 * j], bf16_hi(y.v[j]) + d[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = f32_to_bf16(bf16_lo(y.v[j]) + d[j]);
+    }
+  }
+  template <class At>
+  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, At at_j) const {
+    const uint32_t at = at_j(0);
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (YF32) __builtin_amdgcn_raw_buffer_store_b32(v[j], r, at_j(j), 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16((uint16_t)v[j], r, at_j(j), 0, 0);
+      }
+    } else if constexpr (YF32)
       __builtin_amdgcn_raw_buffer_store_b128((u32x4){v[0], v[1], v[2], v[3]}, r, at, 0, 0);
     else
       __builtin_amdgcn_raw_buffer_store_b64((u32x2){v[0], v[1]}, r, at, 0, 0);
@@ -411,9 +443,10 @@ struct PanelF32 {
 //      are read while the last ones are multiplied.  The sums meet in LDS.
 //   2. v scaled, split and laid out for the MFMA.
 //   3. units of 64 rows of B: column c of MFMA j is row 4 c + j, so that a lane
-//      ends with 4 consecutive values of y of each of its 4 tokens.  B's rows
-//      are read whole and turned in LDS as A's; what the next unit reads of B
-//      and y is in flight meanwhile.
+//      ends with 4 consecutive values of y of each of its 4 tokens (VEC: y in
+//      whole pieces of 4; else row 16 j + c, so that 16 lanes reach a line
+//      together).  B's rows are read whole and turned in LDS as A's; what the
+//      next unit reads of B and y is in flight meanwhile.
 template <int LP, bool XF32, bool YF32, bool VEC>
 __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(LoraArgs a) {
   constexpr int NRB = LP <= 2 ? 1 : LP / 2;  // blocks of 16 rows of A
@@ -513,7 +546,7 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   const __amdgpu_buffer_rsrc_t B =
       make_rsrc(a.b[p] + (size_t)ad * M * a.R, (uint32_t)M * a.R * 2);
   u32x4 w[LP];
-  YRun<YF32> y[4];
+  YRun<YF32, VEC> y[4];
   const int ysz = YF32 ? 4 : 2;
   const __amdgpu_buffer_rsrc_t Y =
       make_rsrc((const char *)a.y[p] + (size_t)t0 * a.y_ld[p] * ysz, 0x7FFFFFFFu);
@@ -522,7 +555,7 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
 #pragma unroll
   for (int i = 0; i < 4; ++i) y_tok[i] = (own >> i) & 1 ? (q_y * 4 + i) * ypitch : BUF_OOB;
   auto y_at = [&](int u, int i, int j) {
-    const int m = u * 64 + 4 * col_y + j;
+    const int m = u * 64 + (VEC ? 4 * col_y + j : 16 * j + col_y);
     return m < M ? y_tok[i] + m * ysz : BUF_OOB;
   };
   auto load_b = [&](int u) {
@@ -532,11 +565,11 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   };
   auto load_y = [&](int u) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i].load(Y, y_at(u, i, 0));
+    for (int i = 0; i < 4; ++i) y[i].load(Y, [&](int j) { return y_at(u, i, j); });
   };
   int u = u0 + wave;
   load_b(u);
-  if (VEC) load_y(u);
+  load_y(u);
   __syncthreads();  // every wave is done with its stage
   {
     f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
@@ -571,8 +604,9 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   int place[LP];
 #pragma unroll
   for (int i = 0; i < LP; ++i) {
-    const int l = i * 64 + lane_y, row = l / cpr, ch = l - row * cpr, s = row >> 2;
-    place[i] = row < 64 ? s * 4 * CP + (((row & 3) * CP + ch) ^ (s & 15)) : STAGE + lane_y;
+    const int l = i * 64 + lane_y, row = l / cpr, ch = l - row * cpr;
+    const int c = VEC ? row >> 2 : row & 15, j = VEC ? row & 3 : row >> 4;
+    place[i] = row < 64 ? c * 4 * CP + ((j * CP + ch) ^ c) : STAGE + lane_y;
   }
   u32x4 keep;  // clears B's columns from rank on (they may hold anything) in rank's block of 32
 #pragma unroll
@@ -606,50 +640,15 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
       }
     lds_order();
   };
-  if constexpr (VEC) {
-    for (; u < u_end; u += T_WAVES) {
-      f32x4 d[4];
-      product(u, d);
-      YRun<YF32> o[4];
+  for (; u < u_end; u += T_WAVES) {
+    f32x4 d[4];
+    product(u, d);
+    YRun<YF32, VEC> o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (YF32) {
+    for (int i = 0; i < 4; ++i) o[i].add(y[i], d[0][i], d[1][i], d[2][i], d[3][i]);
+    load_y(u + T_WAVES);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[i].v[j] = __float_as_uint(__uint_as_float(y[i].v[j]) + d[j][i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            o[i].v[j] = bf16x2_bits(bf16_lo(y[i].v[j]) + d[2 * j][i],
-                                    bf16_hi(y[i].v[j]) + d[2 * j + 1][i]);
-        }
-      }
-      load_y(u + T_WAVES);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i].store(Y, y_at(u, i, 0));
-    }
-  } else {
-    for (; u < u_end; u += T_WAVES) {
-      f32x4 d[4];
-      product(u, d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] = YF32 ? __builtin_amdgcn_raw_buffer_load_b32(Y, y_at(u, i, j), 0, 0)
-                      : __builtin_amdgcn_raw_buffer_load_b16(Y, y_at(u, i, j), 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (YF32)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(__uint_as_float(v[j]) + d[j][i]), Y,
-                                                  y_at(u, i, j), 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(bf16_to_f32((uint16_t)v[j]) + d[j][i]),
-                                                  Y, y_at(u, i, j), 0, 0);
-        }
-      }
-    }
+    for (int i = 0; i < 4; ++i) o[i].store(Y, [&](int j) { return y_at(u, i, j); });
   }
   if (rem) __syncthreads();  // the stage is the next adapter's
   }
