@@ -453,7 +453,7 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
   constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
   constexpr int RING = NRB < 4 ? NRB : 4;  // panels of A in flight
-  constexpr int STAGE = NRK == 4 ? 1024 : 512;  // 16-byte pieces of a wave's LDS
+  constexpr int STAGE = NRK <= 2 ? 512 : NRK * 256;  // 16-byte pieces of a wave's LDS
   constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it
   __shared__ u32x4 s_stage[T_WAVES][STAGE + 64];
   __shared__ u32x2 s_v[NRK][NS][64][2];
@@ -804,7 +804,9 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
   if (cpr <= 1) launch_tile<1>(a, grid, xf32, yf32, vec, s);
   else if (cpr <= 2) launch_tile<2>(a, grid, xf32, yf32, vec, s);
   else if (cpr <= 4) launch_tile<4>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 6) launch_tile<6>(a, grid, xf32, yf32, vec, s);
   else if (cpr <= 8) launch_tile<8>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 12) launch_tile<12>(a, grid, xf32, yf32, vec, s);
   else launch_tile<16>(a, grid, xf32, yf32, vec, s);
   return hipGetLastError();
 }
