@@ -30,7 +30,6 @@ constexpr int N_CU = 256;
 constexpr int TT = 16;       // tokens of an MFMA tile
 constexpr int R_WAVES = 4;   // waves of a workgroup: k_lora_rows
 constexpr int dec_waves(bool fused) { return fused ? 8 : 4; }  // k_lora_dec
-constexpr int T_WAVES = 8;   // k_lora_tile
 
 struct LoraArgs {
   const void *x;
@@ -40,7 +39,7 @@ struct LoraArgs {
   void *y[AINFER_LORA_MAX_PROJ];
   int64_t y_ld[AINFER_LORA_MAX_PROJ], x_ld;
   int m[AINFER_LORA_MAX_PROJ];
-  float *v;       // [P][T][R], of k_lora_rows
+  float *v;       // [P][T][R], x A^T of a first launch
   int N, R, K, P, T;
   int units;      // groups of 64 rows of y per wave
 };
@@ -447,12 +446,26 @@ struct PanelF32 {
 //      whole pieces of 4; else row 16 j + c, so that 16 lanes reach a line
 //      together).  B's rows are read whole and turned in LDS as A's; what the
 //      next unit reads of B and y is in flight meanwhile.
-template <int LP, bool XF32, bool YF32, bool VEC>
-__global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(LoraArgs a) {
+// STAGES V: 1 alone, of a.rows rows of A (blockIdx.z: projection and which), v
+// to memory; Y: 2 and 3 of that v.
+enum { STAGES_VY, STAGES_V, STAGES_Y };
+constexpr int tile_waves(int stages) { return stages == STAGES_Y ? 4 : 8; }
+// Two workgroups a CU (128 registers) where they fit: a tile with a second adapter
+// then need not wait for a first round.  4096 tokens of 24 requests, 4096 x 4096, rank
+// 64 44.4 us (46 with one), 8192 tokens of 30 79 (88).
+constexpr bool tile_two(int lp, bool yf32) { return lp <= 6 || (lp == 8 && !yf32); }
+// waves a SIMD holds: of STAGES_Y the LDS allows three workgroups, from 65 ranks two
+constexpr int tile_occupancy(int stages, int lp, bool yf32) {
+  return stages == STAGES_Y ? (lp <= 8 ? 3 : 2) : tile_two(lp, yf32) ? 4 : 2;
+}
+template <int STAGES, int LP, bool XF32, bool YF32, bool VEC>
+__global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP, YF32)) void k_lora_tile(
+    LoraArgs a) {
+  constexpr int T_WAVES = tile_waves(STAGES);
   constexpr int NRB = LP <= 2 ? 1 : LP / 2;  // blocks of 16 rows of A
   constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
   constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
-  constexpr int RING = NRB < 4 ? NRB : 4;  // panels of A in flight
+  constexpr int RING = NRB < 3 ? NRB : tile_two(LP, YF32) ? 2 : 4;  // panels of A in flight
   constexpr int STAGE = NRK <= 2 ? 512 : NRK * 256;  // 16-byte pieces of a wave's LDS
   constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it
   __shared__ u32x4 s_stage[T_WAVES][STAGE + 64];
@@ -464,16 +477,17 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   const int p = blockIdx.z % a.P, part = blockIdx.z / a.P;
   const int M = a.m[p];
   const int id = tile_ids(a, t0, lane0);
-  const int u0 = part * a.units * T_WAVES, u_end = min(u0 + a.units * T_WAVES, (M + 63) / 64);
-  if (u0 * 64 >= M) return;
+  const int row0 = STAGES == STAGES_V ? part * NRB * 16 : 0;  // of A
   uint32_t rem = (uint32_t)__ballot(id >= 0);  // 16 tokens
+  const int u0 = part * a.units * T_WAVES, u_end = min(u0 + a.units * T_WAVES, (M + 63) / 64);
+  if (STAGES != STAGES_V && u0 >= u_end) return;
   for (int nth = 0; rem; ++nth) {
   const int ad = __builtin_amdgcn_readlane(id, __builtin_ctz(rem));
   const uint32_t mask = (uint32_t)__ballot(id == ad) & rem;
   rem &= ~mask;
   if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
   const int rank = rank_of(a, ad);
-  if (rank == 0) continue;
+  if (rank <= row0) continue;
   const float scale = a.scales ? a.scales[ad] : 1.0f;
   // opaque, so that what depends on the lane is computed again for each adapter
   // and not held in registers across this loop
@@ -484,14 +498,14 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   f32x4 acc[NRB];
 #pragma unroll
   for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  {
+  if constexpr (STAGES != STAGES_Y) {
     const __amdgpu_buffer_rsrc_t A =
         make_rsrc(a.a[p] + (size_t)ad * a.R * a.K, (uint32_t)(a.R * a.K) * 2);
     const int nc = (a.K + CK - 1) / CK;
     Panel<CK> pa[RING];
     using XPanel = typename std::conditional<XF32, PanelF32, Panel<CK>>::type;
     XPanel px;
-    auto load_a = [&](int r, int c) { pa[r % RING].load(A, r * 16, c * CK, a.K, lane); };
+    auto load_a = [&](int r, int c) { pa[r % RING].load(A, row0 + r * 16, c * CK, a.K, lane); };
     // the tile's rows of x; rows past the last token are never multiplied into a
     // token's column, and read as 0
     const int xsz = XF32 ? 4 : 2;
@@ -540,6 +554,30 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
     }
   }
   const int lane_y = tid_opaque() & 63, col_y = lane_y & 15, q_y = lane_y >> 4;
+  // the sums of the waves: ranks row0 + rb * 16 + q_y * 4 .. + 3 of token col
+  auto to_red = [&]() {
+    f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
+#pragma unroll
+    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane_y] = acc[r];
+  };
+  auto from_red = [&](int rb) {
+    const f32x4 *red = (const f32x4 *)s_stage;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane_y];
+    return v;
+  };
+  float *const v_tok = a.v + ((size_t)p * a.T + t0 + col_y) * a.R;  // of token col
+  if constexpr (STAGES == STAGES_V) {
+    __syncthreads();  // every wave is done with its stage
+    to_red();
+    __syncthreads();
+    for (int rb = wave; rb < NRB; rb += T_WAVES) {
+      const f32x4 v = from_red(rb);
+      const int r0 = row0 + rb * 16 + q_y * 4;
+      if ((mask >> col_y) & 1 && r0 < a.R) *(f32x4 *)(v_tok + r0) = v;
+    }
+  } else {
   const uint32_t own = mask >> (q_y * 4);  // bit i: this lane's token q * 4 + i
   constexpr int CP = NRK * 4;              // pieces of a row of B, padded
   const int cpr = a.R / 8;
@@ -570,23 +608,22 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
   int u = u0 + wave;
   load_b(u);
   load_y(u);
-  __syncthreads();  // every wave is done with its stage
-  {
-    f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
-#pragma unroll
-    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane_y] = acc[r];
+  if constexpr (STAGES == STAGES_VY) {
+    __syncthreads();  // every wave is done with its stage
+    to_red();
+    __syncthreads();
   }
-  __syncthreads();
-  // 2. ranks rb * 16 + q_y * 4 .. + 3 of token col
+  // 2.
   for (int rb = wave; rb < 2 * NRK; rb += T_WAVES) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (rb < NRB) {
-      const f32x4 *red = (const f32x4 *)s_stage;
-#pragma unroll
-      for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane_y];
-    }
     float e[4][NS];
     const int r0 = rb * 16 + q_y * 4;
+    if constexpr (STAGES == STAGES_VY) {
+      if (rb < NRB) v = from_red(rb);
+    } else {
+      // another adapter's tokens of the tile are never multiplied into this one's
+      if ((mask >> col_y) & 1 && r0 < rank) v = *(const f32x4 *)(v_tok + r0);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_bf16(r0 + i < rank ? v[i] * scale : 0.0f, e[i]);
     const int slot = ((r0 & 31) >> 3) * 16 + col_y;
@@ -650,6 +687,7 @@ __global__ __launch_bounds__(64 * T_WAVES, LP <= 4 ? 4 : 2) void k_lora_tile(Lor
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i].store(Y, [&](int j) { return y_at(u, i, j); });
   }
+  }
   if (rem) __syncthreads();  // the stage is the next adapter's
   }
 }
@@ -683,6 +721,12 @@ constexpr int dec_waves_wanted(bool fused) { return fused ? 4096 : 8192; }
 // k_lora_rows: two rows a workgroup, four from this many rows in the call (fewer
 // workgroups for equal time: rank 128, T 256 76.9 and 77.3 us)
 constexpr int ROWS_TWO = 4096;
+// k_lora_tile in two launches where further parts of y's rows would read more of A
+// again, us in one and in two: T 300, 4096 x 4096, rank 64 (70 MB) 23.9 and 15.1, T 512,
+// rank 96 (176 MB) 33.2 and 21.7, T 1024, rank 128 (201 MB) 52.9 and 36.5, T 934, 704 x
+// 685 x 2, rank 112 (19 MB) 30.9 and 27.3, T 300, 1024 x 1024, rank 40 (11 MB) 7.2 and
+// 8.6; of tiles that fill the card, T 2048, 4096 x 1024 x 2, rank 48 (0) 25.4 and 30.4.
+constexpr size_t TILE_AGAIN = 16 << 20;
 
 template <int LR, bool FUSED>
 void launch_dec(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
@@ -705,29 +749,28 @@ void launch_dec_lr(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream
   else if (a.R <= 64) launch_dec<8, FUSED>(a, grid, xf32, yf32, s);
   else launch_dec<16, FUSED>(a, grid, xf32, yf32, s);
 }
-template <int LP, bool VEC>
-void launch_tile_y(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, hipStream_t s) {
-  const dim3 b(64 * T_WAVES);
-  if (xf32) {
-    if (yf32) k_lora_tile<LP, true, true, VEC><<<grid, b, 0, s>>>(a);
-    else k_lora_tile<LP, true, false, VEC><<<grid, b, 0, s>>>(a);
+template <int STAGES, int LP, bool XF32>
+void launch_tile(const LoraArgs &a, dim3 grid, bool yf32, bool vec, hipStream_t s) {
+  const dim3 b(64 * tile_waves(STAGES));
+  if (yf32) {
+    if (vec) k_lora_tile<STAGES, LP, XF32, true, true><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<STAGES, LP, XF32, true, false><<<grid, b, 0, s>>>(a);
   } else {
-    if (yf32) k_lora_tile<LP, false, true, VEC><<<grid, b, 0, s>>>(a);
-    else k_lora_tile<LP, false, false, VEC><<<grid, b, 0, s>>>(a);
+    if (vec) k_lora_tile<STAGES, LP, XF32, false, true><<<grid, b, 0, s>>>(a);
+    else k_lora_tile<STAGES, LP, XF32, false, false><<<grid, b, 0, s>>>(a);
   }
 }
 template <int LP>
-void launch_tile(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, bool vec, hipStream_t s) {
-  if (vec) launch_tile_y<LP, true>(a, grid, xf32, yf32, s);
-  else launch_tile_y<LP, false>(a, grid, xf32, yf32, s);
+void launch_tile_vy(const LoraArgs &a, dim3 grid, bool xf32, bool yf32, bool vec, hipStream_t s) {
+  if (xf32) launch_tile<STAGES_VY, LP, true>(a, grid, yf32, vec, s);
+  else launch_tile<STAGES_VY, LP, false>(a, grid, yf32, vec, s);
 }
 
 }  // namespace
 
-// v of k_lora_rows
+// v of the calls of two launches
 size_t lora_workspace_bytes(const ainfer_moe_lora &l, int max_tokens) {
-  const size_t T = max_tokens < DEC_MAX_T ? max_tokens : DEC_MAX_T;
-  const size_t n = T * l.n_proj * l.rank * sizeof(float);
+  const size_t n = (size_t)max_tokens * l.n_proj * l.rank * sizeof(float);
   return n > 256 ? (n + 255) & ~(size_t)255 : 256;
 }
 
@@ -786,27 +829,49 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     }
     return hipGetLastError();
   }
-  const int tiles = div_up(T, TT), units = div_up(m_most, 64);
+  const int tiles = div_up(T, TT), units = div_up(m_most, 64), cpr = l.rank / 8;
+  // a multiple of the XCDs, so that blockIdx.x alone tells the XCD
+  const int gx = div_up(tiles, N_XCD) * N_XCD;
+  // a.units and how many parts of y's rows, of about `want`
+  auto split = [&](int want, int waves) {
+    a.units = div_up(units, want * waves);
+    return div_up(units, a.units * waves);
+  };
+  // workgroups of a tile, which share its adapters: as many as two on each CU, and
+  // some (with 2 and 4, 4096 x 4096: T 4096, rank 16, 96 requests 34.0 us and 24.9, rank
+  // 32, 24 requests 30.4 and 28.2; of a second launch, which has more workgroups of
+  // less work, T 512, rank 96 21.8 and 24.7, T 300, rank 64 15.1 and 17.4)
+  auto slots = [&](int others, int least) {
+    int n = 2 * N_CU / others;
+    n = n < least ? least : n > TT ? TT : n;
+    return n < l.n_adapters ? n : l.n_adapters;
+  };
   // parts of y's rows, each of which computes v again, while tiles leave CUs idle
   int parts = N_CU / (tiles * l.n_proj);
-  parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
-  a.units = div_up(units, parts * T_WAVES);
-  parts = div_up(units, a.units * T_WAVES);
-  // workgroups of a tile, which share its adapters: as many as two on each CU, and
-  // 4 (T 4096, 16 requests: 33.3 us with 2, 27.8 with 4; 512 tokens, 4 requests
-  // 12.1 and 14.4)
-  int slots = 2 * N_CU / (tiles * l.n_proj * parts);
-  slots = slots < 4 ? 4 : slots > TT ? TT : slots;
-  if (slots > l.n_adapters) slots = l.n_adapters;
-  // a multiple of the XCDs, so that blockIdx.x alone tells the XCD
-  const dim3 grid(div_up(tiles, N_XCD) * N_XCD, slots, l.n_proj * parts);
-  const int cpr = l.rank / 8;
-  if (cpr <= 1) launch_tile<1>(a, grid, xf32, yf32, vec, s);
-  else if (cpr <= 2) launch_tile<2>(a, grid, xf32, yf32, vec, s);
-  else if (cpr <= 4) launch_tile<4>(a, grid, xf32, yf32, vec, s);
-  else if (cpr <= 6) launch_tile<6>(a, grid, xf32, yf32, vec, s);
-  else if (cpr <= 8) launch_tile<8>(a, grid, xf32, yf32, vec, s);
-  else if (cpr <= 12) launch_tile<12>(a, grid, xf32, yf32, vec, s);
-  else launch_tile<16>(a, grid, xf32, yf32, vec, s);
+  parts = split(parts < 1 ? 1 : parts > 8 ? 8 : parts, tile_waves(STAGES_VY));
+  const size_t again = (size_t)(parts - 1) * tiles * l.n_proj * l.rank * l.in * 2;
+  if (cpr > 4 && again > TILE_AGAIN) {
+    const int groups = div_up(l.rank, 32);
+    const dim3 gv(gx, slots(tiles * l.n_proj * groups, 2), l.n_proj * groups);
+    const dim3 bv(64 * tile_waves(STAGES_V));
+    if (xf32) k_lora_tile<STAGES_V, 4, true, false, false><<<gv, bv, 0, s>>>(a);
+    else k_lora_tile<STAGES_V, 4, false, false, false><<<gv, bv, 0, s>>>(a);
+    parts = 2 * N_CU / (tiles * l.n_proj);
+    parts = split(parts < 1 ? 1 : parts, tile_waves(STAGES_Y));
+    const dim3 gy(gx, slots(tiles * l.n_proj * parts, 2), l.n_proj * parts);
+    if (cpr <= 6) launch_tile<STAGES_Y, 6, false>(a, gy, yf32, vec, s);
+    else if (cpr <= 8) launch_tile<STAGES_Y, 8, false>(a, gy, yf32, vec, s);
+    else if (cpr <= 12) launch_tile<STAGES_Y, 12, false>(a, gy, yf32, vec, s);
+    else launch_tile<STAGES_Y, 16, false>(a, gy, yf32, vec, s);
+    return hipGetLastError();
+  }
+  const dim3 grid(gx, slots(tiles * l.n_proj * parts, 4), l.n_proj * parts);
+  if (cpr <= 1) launch_tile_vy<1>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 2) launch_tile_vy<2>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 4) launch_tile_vy<4>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 6) launch_tile_vy<6>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 8) launch_tile_vy<8>(a, grid, xf32, yf32, vec, s);
+  else if (cpr <= 12) launch_tile_vy<12>(a, grid, xf32, yf32, vec, s);
+  else launch_tile_vy<16>(a, grid, xf32, yf32, vec, s);
   return hipGetLastError();
 }

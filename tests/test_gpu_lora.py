@@ -233,3 +233,43 @@ def test_offsets_past_32_bits(torch, T, pitch):
     c.lora.apply(x, c.ids, [y], c.lora.workspace(T))
     torch.cuda.synchronize()
     c.compare(c.y, [y.contiguous()])
+
+
+# prompts whose A is read once, in a launch of its own: long K, ranks above 32
+TWO_LAUNCHES = [(300, 7, 64, 4096, [1027]), (300, 3, 40, 4104, [1100, 1030]),
+                (513, 2, 72, 2056, [1500]), (600, 4, 128, 1032, [2100]),
+                (401, 5, 96, 4096, [640, 1300])]
+
+
+@pytest.mark.parametrize("shape", TWO_LAUNCHES)
+@pytest.mark.parametrize("x,y", (("bf16", "bf16"), ("fp32", "fp32"), ("fp32", "bf16")))
+def test_long_prompts_of_large_ranks(torch, shape, x, y):
+    T, N, R = shape[:3]
+    ids = [(t // 37) % (N + 1) - 1 if t < 200 else (t // 5) % N for t in range(T)]
+    Case(torch, *shape, x=x, y=y, ids=ids).check()
+    c = Case(torch, *shape, x=x, y=y, ids=ids, ranks=[(R - 9 * n) if n < 4 else 0 for n in range(N)])
+    for n in range(N):                              # beyond a rank anything may stand
+        r = max(int(c.ranks[n]), 0)
+        for a, b in zip(c.a, c.b):
+            a[n, r:] = float("nan")
+            b[n, :, r:] = float("inf")
+    c.check()
+
+
+def test_workspace_of_pitched_prompts(torch):
+    """More than 256 tokens at a pitch that the tiles' 32-bit offsets cannot
+    reach, ranks that are not worth reading in every workgroup: one row of
+    scratch per token.  Nothing past the workspace is written."""
+    T, R, K, pitch = 300, 128, 1040, (1 << 26) + (1 << 23)
+    c = Case(torch, T, 3, R, K, [48])
+    xs = torch.empty((T - 1) * pitch + K, dtype=torch.bfloat16, device="cuda")
+    c.x = xs.as_strided((T, K), (pitch, 1)).copy_(c.x)
+    n = c.lora.workspace(T).numel()
+    assert n >= T * R * 4
+    buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    off = -buf.data_ptr() % 256
+    ys = [y.clone() for y in c.y]
+    c.apply(ys, buf[off:off + n])
+    torch.cuda.synchronize()
+    c.compare(c.y, ys)
+    assert (buf[:off] == 0xA5).all() and (buf[off + n:] == 0xA5).all()
