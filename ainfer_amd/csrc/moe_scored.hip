@@ -282,6 +282,37 @@ __device__ int pick_rounds(const Row &r, const Slot &s, bool kept, int k, int la
   return mine;
 }
 
+// A group's value gv of its two largest keys, and the errors tol of two such values:
+// each of up to two keys (exp alone is off by 1.01 2^-23) and the rounding of
+// their sum
+template <bool BIAS, bool SOFT>
+__device__ __forceinline__ void group_value(float m1, float m2, bool top2, float m, float eps_abs,
+                                            float &gv, float &tol) {
+  gv = m1;
+  if (top2) {
+    if constexpr (!BIAS) {  // the logits order the scores: the two largest give the sum
+      m1 = m1 == neg_inf() ? m1 : SOFT ? exp_fast(m1 - m) : sigmoid_fast(m1);
+      m2 = m2 == neg_inf() ? m2 : SOFT ? exp_fast(m2 - m) : sigmoid_fast(m2);
+    }
+    gv = m2 == neg_inf() ? m1 : m1 + m2;
+  }
+  tol = 0.0f;
+  if (BIAS || top2)
+    tol = 4.0f * (BIAS ? eps_abs : SIG_ABS) +
+          4.0f * KEY_REL * (m2 == neg_inf() ? fabsf(gv) : fabsf(m1) + fabsf(m2));
+  if (gv == neg_inf()) tol = 0.0f;
+}
+
+// A selected score relative to the largest one's, mx its logit, so that the largest
+// does not vanish: exp(l - mx); sigmoid: exp(l) / (1 + exp(l)), times exp(-mx) where
+// the largest logit is below 0
+template <bool SOFT>
+__device__ __forceinline__ float relative_score(float l, float mx) {
+  if constexpr (SOFT) return exp_fast(l - mx);
+  const float e = exp_fast(-fabsf(l));
+  return (mx < 0.0f ? exp_fast(l - mx) : l > 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 // a lane's NV logits of one row, as loaded: whole 16- or 8-byte pieces where
 // VEC allows, else one by one; what lies past the lane's experts reads as 0
 template <int NV>
@@ -289,9 +320,11 @@ struct Raw {
   uint32_t v[NV];  // fp32 bits
   __device__ __forceinline__ void load(const ScoredArgs &a, int t, const Slot &s) {
     const int esz = a.dtype == AINFER_ACT_F32 ? 4 : 2;
-    const __amdgpu_buffer_rsrc_t r =
-        make_rsrc((const char *)a.logits + (size_t)t * a.ld * esz, a.G * a.per * esz);
-    auto at = [&](int i) { return i < s.n ? (uint32_t)(s.base + i) * esz : BUF_OOB; };
+    load(a, make_rsrc((const char *)a.logits + (size_t)t * a.ld * esz, a.G * a.per * esz), 0, esz, s);
+  }
+  __device__ __forceinline__ void load(const ScoredArgs &a, __amdgpu_buffer_rsrc_t r, uint32_t row,
+                                       int esz, const Slot &s) {
+    auto at = [&](int i) { return i < s.n ? row + (uint32_t)(s.base + i) * esz : BUF_OOB; };
     if (esz == 4) {
       if constexpr (NV >= 4) {
         if (a.vec) {
@@ -463,22 +496,9 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
         m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
         m1 = fmaxf(m1, o1);
       }
-      float gv = m1;
-      if (top2) {
-        if constexpr (!BIAS) {  // the logits order the scores: the two largest give the sum
-          m1 = m1 == neg_inf() ? m1 : SOFT ? exp_fast(m1 - r.m) : sigmoid_fast(m1);
-          m2 = m2 == neg_inf() ? m2 : SOFT ? exp_fast(m2 - r.m) : sigmoid_fast(m2);
-        }
-        gv = m2 == neg_inf() ? m1 : m1 + m2;
-      }
       const bool exact = !BIAS && !top2;
-      // the errors of two values: each of up to two keys (exp alone is off by
-      // 1.01 2^-23) and the rounding of their sum
-      float tol = 0.0f;
-      if (!exact)
-        tol = 4.0f * (BIAS ? eps_abs : SIG_ABS) +
-              4.0f * KEY_REL * (m2 == neg_inf() ? fabsf(gv) : fabsf(m1) + fabsf(m2));
-      if (gv == neg_inf()) tol = 0.0f;
+      float gv, tol;
+      group_value<BIAS, SOFT>(m1, m2, top2, r.m, eps_abs, gv, tol);
       const float hi_g = gv + tol, lo_g = gv - tol;
       int above = 0, near = 0;
       for (int h = 0; h < a.G; ++h) {
@@ -637,19 +657,9 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
     const bool live = sel && l_mine != neg_inf();
     float w;
     if (a.renorm) {
-      // the selected scores over their sum, scaled so that the largest does not
-      // vanish: exp(l - max); sigmoid: exp(l) / (1 + exp(l)), times exp(-max)
-      // where the largest logit is below 0
+      // the selected scores over their sum
       const float mx = wave_max_f(live ? l_mine : neg_inf());
-      float s;
-      if constexpr (SOFT) {
-        s = exp_fast(l_mine - mx);
-      } else {
-        const float e = exp_fast(-fabsf(l_mine));
-        s = (mx < 0.0f ? exp_fast(l_mine - mx) : l_mine > 0.0f ? 1.0f : e) *
-            __builtin_amdgcn_rcpf(1.0f + e);
-      }
-      s = live ? s : 0.0f;
+      const float s = live ? relative_score<SOFT>(l_mine, mx) : 0.0f;
       const float sum = wave_sum_f(s);
       w = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
     } else if constexpr (SOFT) {
@@ -661,6 +671,273 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
       a.idx[(size_t)t * a.k + rank] = e_mine;
       a.w[(size_t)t * a.k + rank] = w;
     }
+  }
+}
+
+// ---- many tokens of few experts -------------------------------------------------
+//
+// Four tokens a wave, 16 lanes each (the slots of the groups within them), since
+// what a wave does for a token above costs the same however few its experts are.
+// k rounds of the largest key left of 16 lanes, ties to the lowest lane and there to
+// the lowest expert; lanes hold experts in ascending order.  With a bias one round
+// more: where two picks are nearer than the keys' errors, they are ranked by 64-bit
+// keys, and where the last and the next are, the rounds are run again on those.
+
+template <class F>
+__device__ __forceinline__ float reduce16(float v, F f) {
+  v = f(v, dpp_f<0xB1, 0xF>(v, v));
+  v = f(v, dpp_f<0x4E, 0xF>(v, v));
+  v = f(v, dpp_f<0x141, 0xF>(v, v));
+  return f(v, dpp_f<0x140, 0xF>(v, v));
+}
+__device__ __forceinline__ float max16(float v) {
+  return reduce16(v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float sum16(float v) {
+  return reduce16(v, [](float x, float y) { return x + y; });
+}
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint64_t max16(uint64_t v) {
+  v = max_u64(v, dpp_u64<0xB1>(v));
+  v = max_u64(v, dpp_u64<0x4E>(v));
+  v = max_u64(v, dpp_u64<0x141>(v));
+  return max_u64(v, dpp_u64<0x140>(v));
+}
+
+struct Pick {
+  int e;
+  float l;
+};
+constexpr int MP_K = 16;  // picks of a token: one a lane
+
+template <int NV, bool BIAS, bool SOFT, bool GRP>
+__global__ __launch_bounds__(64 * SR_WAVES) void k_route_many(ScoredArgs a) {
+  __shared__ Pick s_pick[SR_WAVES][4][MP_K];
+  const int lane = threadIdx.x & 63, lane16 = lane & 15, seg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = (blockIdx.x * SR_WAVES + wave) * 4, t = t0 + seg;
+  if (t0 >= a.T) return;
+  const int gl = GRP ? a.gl : 4, lanes = 1 << gl;
+  const int g = lane16 >> gl, sub = lane16 & (lanes - 1);
+  Slot sl;
+  sl.base = g * a.per + sub * NV;
+  sl.n = g < a.G && t < a.T ? min(max(a.per - sub * NV, 0), NV) : 0;
+  const int esz = a.dtype == AINFER_ACT_F32 ? 4 : 2;
+  Raw<NV> raw;
+  raw.load(a, make_rsrc((const char *)a.logits + (size_t)t0 * a.ld * esz, 0x7FFFFFFFu),
+           (uint32_t)(seg * a.ld) * esz, esz, sl);
+  float b[BIAS ? NV : 1];
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      b[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+          make_rsrc(a.bias, a.G * a.per * 4), i < sl.n ? (sl.base + i) * 4 : BUF_OOB, 0, 0));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) b[i] = clean_bias(b[i]);
+  }
+  Row r;
+  r.base = a.logits;
+  r.ld = a.ld;
+  r.t = t;
+  r.bias = a.bias;
+  r.dtype = a.dtype;
+  r.lowest = a.dtype == AINFER_ACT_F32 ? -3.402823466e38f : -3.3895313892515355e38f;
+  r.m = 0.0f;
+  float l[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    l[i] = i < sl.n ? clean_logit(__uint_as_float(raw.v[i]), r.lowest) : neg_inf();
+
+  const bool need_z = SOFT && (BIAS || !a.renorm);
+  float z = 1.0f, eps_abs = SIG_ABS;
+  if (SOFT && (need_z || GRP)) {
+    float m = l[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, l[i]);
+    m = max16(m);
+    r.m = m == neg_inf() ? 0.0f : m;
+  }
+  float v[NV];  // selection keys; -inf: masked
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = l[i];
+  if constexpr (SOFT) {
+    if (need_z) {
+      float e[NV], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) sum += e[i] = exp_fast(l[i] - r.m);
+      z = sum16(sum);
+      if (z == 0.0f) z = 1.0f;
+      if constexpr (BIAS) {
+        const float rz = 1.0f / z;
+        eps_abs = SOFT_REL * rz;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = l[i] == neg_inf() ? l[i] : fmaf(e[i], rz, b[i]);
+      }
+    }
+  } else if constexpr (BIAS) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = l[i] == neg_inf() ? l[i] : sigmoid_fast(l[i]) + b[i];
+  }
+  bool have_z64 = false;
+  auto z64 = [&]() {
+    if (SOFT && BIAS && !have_z64) {
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        s += l[i] != neg_inf() ? exp64((double)l[i] - (double)r.m) : 0.0;
+      for (int d = 1; d < 16; d *= 2) s += __shfl_xor(s, d);
+      r.z = s;
+      have_z64 = true;
+    }
+  };
+
+  bool kept = sl.n > 0;
+  if constexpr (GRP) {
+    const bool top2 = a.group_score == AINFER_GROUP_TOP2;
+    float m1 = v[0], m2 = neg_inf();
+#pragma unroll
+    for (int i = 1; i < NV; ++i) {
+      m2 = fmaxf(m2, fminf(m1, v[i]));
+      m1 = fmaxf(m1, v[i]);
+    }
+    for (int d = 1; d < lanes; d *= 2) {
+      const float o1 = step_f(m1, d), o2 = step_f(m2, d);
+      m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+      m1 = fmaxf(m1, o1);
+    }
+    const bool exact = !BIAS && !top2;
+    float gv, tol;
+    group_value<BIAS, SOFT>(m1, m2, top2, r.m, eps_abs, gv, tol);
+    const float hi_g = gv + tol, lo_g = gv - tol;
+    const int slots = 16 >> gl;
+    int above = 0, near = 1;
+    for (int d = 1; d < slots; ++d) {
+      const int h = (g + d) & (slots - 1);
+      const float o = __shfl(gv, (lane & 48) | (h << gl));
+      above += h < a.G && o > hi_g ? 1 : 0;
+      near += h < a.G && o >= lo_g ? 1 : 0;
+    }
+    bool in = near <= a.top;
+    if (__builtin_expect(__ballot(g < a.G && above < a.top && near > a.top) != 0, 0)) {
+      z64();
+      const double v64 = exact ? (double)gv : group64<BIAS, SOFT>(r, sl, lanes, top2);
+      int rank = 0;
+      for (int h = 0; h < a.G; ++h) {
+        const double o = __shfl(v64, (lane & 48) | (h << gl));
+        rank += o > v64 || (o == v64 && h < g) ? 1 : 0;
+      }
+      in = rank < a.top;
+    }
+    kept = kept && in;
+  }
+
+  // rounds: u = ordered keys (0: not there), taken ones cleared.  Bit lane of
+  // `lower` stands for the lower lanes of the same token.
+  const uint64_t lower = ((1ull << lane16) - 1) << (seg * 16);
+  Pick *pick = s_pick[wave][seg];
+  const int rounds = a.k + (BIAS ? 1 : 0);
+  bool near_in = false, near_out = false;  // two picks, or the last and the next one
+  auto select = [&](auto(&u)[NV], auto masked, auto &&see) {
+    using U = typename std::remove_reference<decltype(u[0])>::type;
+    for (int j = 0; j < rounds; ++j) {
+      U best = u[0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i) best = u[i] > best ? u[i] : best;
+      const U top = max16(best);
+      see(j, top);
+      const bool win = best == top && (__ballot(best == top) & lower) == 0;
+      int e = 0;
+      float le = neg_inf();
+      bool found = !win;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool hit = !found && u[i] == top;
+        e = hit ? i : e;
+        if (BIAS) le = hit ? l[i] : le;
+        u[i] = hit ? (U)0 : u[i];
+        found |= hit;
+      }
+      if (win && j < a.k) {
+        if (BIAS) le = top == (U)masked ? neg_inf() : le;
+        else le = key_to_float((uint32_t)top);
+        pick[j] = Pick{sl.base + e, le};
+      }
+    }
+  };
+  {
+    uint32_t u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) u[i] = kept && i < sl.n ? ordered_key(v[i]) : 0u;
+    float last = INFINITY;
+    select(u, ordered_key(neg_inf()), [&](int j, uint32_t top) {
+      if constexpr (BIAS) {
+        const float f = key_to_float(top);  // NaN: none left
+        const bool near = f != neg_inf() && last - f <= 4.0f * eps_abs + 4.0f * KEY_REL * fabsf(f);
+        near_in |= near && j < a.k;
+        near_out |= near && j == a.k;
+        last = f;
+      }
+    });
+    if constexpr (BIAS) {
+      if (__builtin_expect(__ballot(near_out) != 0, 0)) {
+        near_in = false;
+        z64();
+        uint64_t w[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          w[i] = kept && i < sl.n ? ordered_key_d(key64<BIAS, SOFT>(r, sl.base + i, l[i])) : 0ull;
+        select(w, ordered_key_d(-INFINITY), [](int, uint64_t) {});
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const bool sel = lane16 < a.k && t < a.T;
+  const Pick mine = pick[lane16 < a.k ? lane16 : 0];
+  int pos = lane16;
+  if (BIAS && __builtin_expect(__ballot(near_in) != 0, 0)) {
+    z64();
+    const double d = sel ? key64<BIAS, SOFT>(r, mine.e, mine.l) : -INFINITY;
+    pos = 0;
+    for (int j = 0; j < a.k; ++j) {
+      const double o = __shfl(d, (lane & 48) | j);
+      const int oe = __shfl(mine.e, (lane & 48) | j);
+      pos += o > d || (o == d && oe < mine.e) ? 1 : 0;
+    }
+  }
+  const bool live = sel && mine.l != neg_inf();
+  float w;
+  if (a.renorm) {
+    const float mx = max16(live ? mine.l : neg_inf());
+    const float s = live ? relative_score<SOFT>(mine.l, mx) : 0.0f;
+    const float sum = sum16(s);
+    w = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
+  } else if constexpr (SOFT) {
+    w = live ? exp_fast(mine.l - r.m) * __builtin_amdgcn_rcpf(z) * a.scale : 0.0f;
+  } else {
+    w = live ? sigmoid_fast(mine.l) * a.scale : 0.0f;
+  }
+  if (sel) {
+    a.idx[(size_t)t * a.k + pos] = mine.e;
+    a.w[(size_t)t * a.k + pos] = w;
+  }
+}
+
+template <int NV>
+void launch_many(const ScoredArgs &a, bool soft, hipStream_t s) {
+  const dim3 grid((a.T + SR_WAVES * 4 - 1) / (SR_WAVES * 4)), b(64 * SR_WAVES);
+  auto run = [&](auto kernel) { kernel<<<grid, b, 0, s>>>(a); };
+  if (a.G > 1) {
+    if (a.bias) run(soft ? k_route_many<NV, true, true, true> : k_route_many<NV, true, false, true>);
+    else run(soft ? k_route_many<NV, false, true, true> : k_route_many<NV, false, false, true>);
+  } else {
+    if (a.bias) run(soft ? k_route_many<NV, true, true, false> : k_route_many<NV, true, false, false>);
+    else run(soft ? k_route_many<NV, false, true, false> : k_route_many<NV, false, false, false>);
   }
 }
 
@@ -680,6 +957,15 @@ void launch_nv(const ScoredArgs &a, int grid, bool soft, hipStream_t s) {
   if (a.G > 1) launch_grp<NV, true>(a, grid, soft, s);
   else launch_grp<NV, false>(a, grid, soft, s);
 }
+
+// k_route_many from this many tokens on, and while the rounds over a lane's experts
+// are fewer than MANY_WORK.  us by a wave a token and by 4: T 4096 without a bias 60
+// experts 4.4 and 3.2, 40 in 8 groups 6.0 and 4.6, 128 4.9 and 4.85 (T 1024 3.6 and 4.6),
+// T 65536 28.6 and 8.9, 48 and 14.8, 34.9 and 17.6; with a bias, where a wave in a
+// hundred has to rank 64-bit keys, T 4096 64 experts 4.9 and 6.4, T 16384 10.8 and 8.4,
+// T 65536 32.9 and 19.2, 128 experts in 8 groups 51.6 and 32.8, 16 picks of 128 41.0 and
+// 45.5.
+constexpr int MANY_T = 4096, MANY_T_BIAS = 16384, MANY_WORK = 64;
 
 }  // namespace
 
@@ -701,23 +987,37 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   a.group_score = r.group_score;
   a.renorm = r.renormalize;
   a.scale = r.scale;
+  // whole pieces of 4 (8 bf16 from 8 experts a lane on) experts, dwords aligned
+  auto vec = [&](int need) {
+    if (dtype == AINFER_ACT_F32) return a.per % 4 == 0;
+    return a.per % (need > 4 ? 8 : 4) == 0 && (uintptr_t)logits % 4 == 0 && ld % 2 == 0;
+  };
   int slots = 1;
   while (slots < a.G) slots *= 2;
+  const bool soft = r.score == AINFER_SCORE_SOFTMAX;
+  if (slots <= 16 && a.k <= MP_K && T >= (bias ? MANY_T_BIAS : MANY_T) &&
+      (3 * ld + r.n_experts) * 4 < INT32_MAX) {
+    for (a.gl = 0; (slots << a.gl) < 16;) ++a.gl;
+    const int need = (a.per + (1 << a.gl) - 1) >> a.gl;
+    a.vec = vec(need);
+    if (need <= 8 && a.k * need <= MANY_WORK) {
+      if (need <= 1) launch_many<1>(a, soft, s);
+      else if (need <= 2) launch_many<2>(a, soft, s);
+      else if (need <= 4) launch_many<4>(a, soft, s);
+      else launch_many<8>(a, soft, s);
+      return hipGetLastError();
+    }
+  }
   a.gl = 0;
   while ((slots << a.gl) < 64) ++a.gl;
   a.more = a.k <= 16 ? 3 : 0;
   const int lanes = 1 << a.gl, need = (a.per + lanes - 1) / lanes;
-  // whole pieces of 4 (8 bf16 from 8 experts a lane on) experts, dwords aligned
-  if (dtype == AINFER_ACT_F32)
-    a.vec = a.per % 4 == 0;
-  else
-    a.vec = a.per % (need > 4 ? 8 : 4) == 0 && (uintptr_t)logits % 4 == 0 && ld % 2 == 0;
+  a.vec = vec(need);
   const int blocks = (T + SR_WAVES - 1) / SR_WAVES;
   // a wave keeps the bias over its tokens; without one a workgroup per 4 tokens.  us at
   // T 65536, grids of 2048 and 16384: 512 experts with a bias 64 and 93, without
   // 52 and 45 (bf16, not renormalised 70 and 53), 64 experts 38 and 31
   const int most = bias ? 2048 : 16384, grid = blocks < most ? blocks : most;
-  const bool soft = r.score == AINFER_SCORE_SOFTMAX;
   if (need <= 1) launch_nv<1>(a, grid, soft, s);
   else if (need <= 2) launch_nv<2>(a, grid, soft, s);
   else if (need <= 4) launch_nv<4>(a, grid, soft, s);

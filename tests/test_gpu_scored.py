@@ -261,3 +261,118 @@ def test_streams_and_graph(torch):
         torch.cuda.synchronize()
         eager = moe.route_scored(r, x, bias)
         assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+def check_many(torch, x, bias, k, score, G=1, top=1, gscore=GTOP2, renorm=1, scale=1.0,
+               T=16400):
+    """The rows of x over and over in a random order (many tokens of few experts
+    share a wave): each the definition's answer, whatever stands beside it."""
+    from ainfer_amd import _lib as L
+    from ainfer_amd import moe
+    B, E = x.shape
+    print(f"[case] T={T} of {B} rows E={E} k={k} score={score} G={G}/{top} gs={gscore} "
+          f"renorm={renorm} {x.dtype} bias={bias is not None}", flush=True)
+    order = torch.randint(0, B, (T,), generator=torch.Generator().manual_seed(B + E + k))
+    order[-B:] = torch.arange(B)
+    wide = torch.empty(T, E + 3, dtype=x.dtype, device="cuda")
+    idx, w = [], []
+    for rows in (x[order.cuda()], wide[:, 1:E + 1].copy_(x[order.cuda()])):
+        out = (torch.full((T + 2, k), -7, dtype=torch.int32, device="cuda"),
+               torch.full((T + 2, k), -7.0, device="cuda"))
+        moe.route_scored(L.Routing(E, k, score, G, top, gscore, renorm, scale), rows, bias,
+                         out=(out[0][:T], out[1][:T]))
+        torch.cuda.synchronize()
+        assert (out[0][T:] == -7).all() and (out[1][T:] == -7).all()
+        idx.append(out[0][:T].cpu().numpy())
+        w.append(out[1][:T].cpu().numpy())
+    assert np.array_equal(idx[0], idx[1]) and np.array_equal(w[0], w[1])
+    ri, rw = reference(x.double().cpu().numpy(), torch.finfo(x.dtype).min,
+                       None if bias is None else bias.cpu().numpy(), E, k, score, G, top, gscore,
+                       renorm, scale)
+    order = order.numpy()
+    assert np.array_equal(idx[0], ri[order])
+    assert np.all(np.abs(w[0] - rw[order]) <= RTOL * np.abs(rw[order]) + ATOL * max(1.0, abs(scale)))
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1), (16, 3, 1, 1), (23, 13, 1, 1), (60, 4, 6, 3),
+                                   (64, 8, 1, 1), (40, 6, 8, 7), (128, 16, 1, 1), (96, 6, 3, 2),
+                                   (128, 8, 8, 4), (120, 16, 5, 2), (64, 6, 16, 5), (127, 9, 1, 1),
+                                   (32, 2, 2, 1), (128, 12, 16, 16)])
+@pytest.mark.parametrize("score", (SOFT, SIG))
+@pytest.mark.parametrize("biased", (False, True))
+def test_many_tokens_of_few_experts(torch, shape, score, biased):
+    E, k, G, top = shape
+    for dtype, gscore, renorm, T in ((torch.float32, GTOP2, 1, 16400), (torch.bfloat16, GMAX, 0, 16387),
+                                     (torch.float32, GMAX, 0, 65536), (torch.bfloat16, GTOP2, 1, 20001)):
+        x = logits_of(torch, 50, E, dtype, E + k + score)
+        bias = None
+        if biased:
+            bias = logits_of(torch, 1, E, torch.float32, E + 7, 0.1 if score == SIG else 1 / E)[0]
+        check_many(torch, x, bias, k, score, G, top, gscore, renorm, 2.5, T)
+
+
+@pytest.mark.parametrize("score", (SOFT, SIG))
+@pytest.mark.parametrize("biased", (False, True))
+@pytest.mark.parametrize("G,top", ((1, 1), (4, 2), (16, 3)))
+def test_many_tokens_masks_infinities_and_ties(torch, score, biased, G, top):
+    E, k = 128, 8
+    for dtype in (torch.float32, torch.bfloat16):
+        x = logits_of(torch, 16, E, dtype, 5)
+        x[0] = -math.inf
+        x[1] = torch.finfo(dtype).min
+        x[2] = math.nan
+        x[3] = -math.inf
+        x[3, 100] = 0.5
+        x[4, :122] = torch.finfo(dtype).min
+        x[5] = 0.0
+        x[6, ::2] = 0.0
+        x[6, 1::2] = -0.0
+        x[7, [3, 9, 120]] = math.inf
+        x[8, ::3] = math.nan
+        x[8, 1::3] = -math.inf
+        x[9] = -90.0
+        x[9, 20:40] = -88.5
+        x[10] = 60.0
+        x[11, 64:] = -math.inf
+        x[12] = (x[12].float() * 8).round().to(dtype) / 8
+        x[13] = x[13] * 1e4
+        x[14] = -math.inf
+        x[14, 62:66] = 1.0
+        bias = None
+        if biased:
+            bias = logits_of(torch, 1, E, torch.float32, 3, 0.05)[0]
+            bias[[5, 70]] = -math.inf
+            bias[9] = math.nan
+            bias[[30, 125]] = math.inf
+        for gscore in (GMAX, GTOP2):
+            for renorm in (0, 1):
+                check_many(torch, x, bias, k, score, G, top, gscore, renorm)
+
+
+@pytest.mark.parametrize("score", (SOFT, SIG))
+@pytest.mark.parametrize("near", (3, 12, 40, 128))
+def test_many_tokens_keys_nearer_than_fp32(torch, score, near):
+    """One row whose biased keys lie within an fp32 step of one value, among others."""
+    E, k = 128, 6
+    x = logits_of(torch, 9, E, torch.float32, near)
+    d = x[4].double()
+    s = torch.sigmoid(d) if score == SIG else torch.softmax(d, 0)
+    bias = torch.full((E,), -2.0, device="cuda")
+    at = torch.randperm(E, generator=torch.Generator().manual_seed(near))[:near].cuda()
+    bias[at] = (0.75 - s[at]).float()
+    check_many(torch, x, bias, k, score)
+    check_many(torch, x, bias, k, score, 8, 3, GTOP2)
+    check_many(torch, x, bias, k, score, 8, 3, GMAX)
+
+
+def test_many_tokens_group_values_nearer_than_fp32(torch):
+    E, G = 128, 8
+    x = logits_of(torch, 6, E, torch.float32, 77)
+    s = torch.sigmoid(x.double())
+    for t in range(6):
+        bias = torch.full((E,), -1.0, device="cuda")
+        for g in range(G):
+            own = torch.arange(g * 16, g * 16 + 2, device="cuda")
+            bias[own] = (0.5 - s[t, own]).float()
+        check_many(torch, x, bias, 4, SIG, G, 3, GTOP2)
+        check_many(torch, x, bias, 4, SIG, G, 3, GMAX)
