@@ -391,6 +391,7 @@ struct ScoredArgs {
   int dtype, T, k;
   int G, top, per;  // groups, groups kept, experts per group
   int gl;           // log2 of the lanes that hold a group
+  int each;         // experts a lane
   int more;         // lanes above top_k that the candidates' threshold may let in
   int group_score, renorm;
   float scale;

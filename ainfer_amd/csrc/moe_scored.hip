@@ -382,8 +382,8 @@ __global__ __launch_bounds__(64 * SR_WAVES) void k_route_scored(ScoredArgs a) {
   const int lanes = 1 << gl;
   const int g = lane >> gl, sub = lane & (lanes - 1);
   Slot sl;
-  sl.base = g * a.per + sub * NV;
-  sl.n = g < a.G ? min(max(a.per - sub * NV, 0), NV) : 0;
+  sl.base = g * a.per + sub * a.each;
+  sl.n = g < a.G ? min(max(a.per - sub * a.each, 0), a.each) : 0;
   const bool full = __ballot(sl.n == NV) == ~0ull;  // every lane has NV experts
   const int step = gridDim.x * SR_WAVES;
   int t = blockIdx.x * SR_WAVES + wave;
@@ -1013,6 +1013,10 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   a.more = a.k <= 16 ? 3 : 0;
   const int lanes = 1 << a.gl, need = (a.per + lanes - 1) / lanes;
   a.vec = vec(need);
+  // experts a lane, of the NV it has room for: shared evenly, so that the maxima of many
+  // lanes bound the top-k (one group of 291 in lanes of 32: 10 maxima, 16 us; of 19: 8)
+  const int piece = !a.vec || need <= 4 ? 1 : dtype == AINFER_ACT_F32 ? 4 : 8;
+  a.each = need <= 4 ? (need > 2 ? 4 : need) : (need + piece - 1) / piece * piece;
   const int blocks = (T + SR_WAVES - 1) / SR_WAVES;
   // a wave keeps the bias over its tokens; without one a workgroup per 4 tokens.  us at
   // T 65536, grids of 2048 and 16384: 512 experts with a bias 64 and 93, without
