@@ -15,12 +15,17 @@
 //                 adapters in any order.  Its products are exact too: bf16 values
 //                 enter the MFMA as they are, fp32 values as the sum of two or three
 //                 bf16 (split_bf16).  v never leaves the CU.
-// GPU us a call (inside a graph) of the benchmark's larger shapes, and the time the
-// bytes of x, y, and each A and B used once take at 5.1 TB/s: one token 4096 x
-// 4096 rank 16 4.8 (0.1; a launch alone is 2.5), 64 tokens 4096 x (1024 + 1024) rank
-// 16 6.2 (2.2), 16 tokens 5120 x 17408 rank 64 14.8 (8.3), 1003 tokens of 7 requests
-// 1024 x 4096 rank 8 in fp32 14.6 (7.3), 4096 tokens 4096 x 4096 rank 32 of 24
-// requests 28 (19.3), of one request 22 (19.7).
+// GPU us a call (inside a graph), and the time the bytes of x, y, and each A and B
+// used once take at 5.1 TB/s: one token 4096 x 4096 rank 16 4.8 (0.1; a launch alone is
+// 2.5), 64 tokens 4096 x (1024 + 1024) rank 16 6.1 (2.2), 16 tokens 5120 x 17408 rank
+// 64 14.8 (8.3), 1003 tokens of 7 requests 1024 x 4096 rank 8 in fp32 14.3 (7.3), 4096
+// tokens 4096 x 4096 of 24 requests rank 32 28 (19.3), rank 64 40 (21.5), of one
+// request rank 32 21 (19.7).
+//
+// What bounds it: batches, the two dependent sweeps over A and B (an HBM latency each)
+// and the bytes of B.  Prompts, y's and x's bytes while a tile has one adapter; a tile
+// that lies across two requests is two workgroups, and the second shares its CU with
+// another tile's: it ends 5 us (rank 16) to 10 (rank 64) after the others.
 #include "moe_common.h"
 #include "moe_internal.h"
 
@@ -482,213 +487,213 @@ __global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP,
   const int u0 = part * a.units * T_WAVES, u_end = min(u0 + a.units * T_WAVES, (M + 63) / 64);
   if (STAGES != STAGES_V && u0 >= u_end) return;
   for (int nth = 0; rem; ++nth) {
-  const int ad = __builtin_amdgcn_readlane(id, __builtin_ctz(rem));
-  const uint32_t mask = (uint32_t)__ballot(id == ad) & rem;
-  rem &= ~mask;
-  if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
-  const int rank = rank_of(a, ad);
-  if (rank <= row0) continue;
-  const float scale = a.scales ? a.scales[ad] : 1.0f;
-  // opaque, so that what depends on the lane is computed again for each adapter
-  // and not held in registers across this loop
-  const int lane = tid_opaque() & 63;
-  u32x4 *stage = s_stage[wave];
+    const int ad = __builtin_amdgcn_readlane(id, __builtin_ctz(rem));
+    const uint32_t mask = (uint32_t)__ballot(id == ad) & rem;
+    rem &= ~mask;
+    if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
+    const int rank = rank_of(a, ad);
+    if (rank <= row0) continue;
+    const float scale = a.scales ? a.scales[ad] : 1.0f;
+    // opaque, so that what depends on the lane is computed again for each adapter
+    // and not held in registers across this loop
+    const int lane = tid_opaque() & 63;
+    u32x4 *stage = s_stage[wave];
 
-  // 1.
-  f32x4 acc[NRB];
+    // 1.
+    f32x4 acc[NRB];
 #pragma unroll
-  for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  if constexpr (STAGES != STAGES_Y) {
-    const __amdgpu_buffer_rsrc_t A =
-        make_rsrc(a.a[p] + (size_t)ad * a.R * a.K, (uint32_t)(a.R * a.K) * 2);
-    const int nc = (a.K + CK - 1) / CK;
-    Panel<CK> pa[RING];
-    using XPanel = typename std::conditional<XF32, PanelF32, Panel<CK>>::type;
-    XPanel px;
-    auto load_a = [&](int r, int c) { pa[r % RING].load(A, row0 + r * 16, c * CK, a.K, lane); };
-    // the tile's rows of x; rows past the last token are never multiplied into a
-    // token's column, and read as 0
-    const int xsz = XF32 ? 4 : 2;
-    const __amdgpu_buffer_rsrc_t X =
-        make_rsrc((const char *)a.x + (size_t)t0 * a.x_ld * xsz, 0x7FFFFFFFu);
-    const uint32_t xpitch = (uint32_t)a.x_ld * xsz;
-    uint32_t x_row[4];
+    for (int r = 0; r < NRB; ++r) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if constexpr (STAGES != STAGES_Y) {
+      const __amdgpu_buffer_rsrc_t A =
+          make_rsrc(a.a[p] + (size_t)ad * a.R * a.K, (uint32_t)(a.R * a.K) * 2);
+      const int nc = (a.K + CK - 1) / CK;
+      Panel<CK> pa[RING];
+      using XPanel = typename std::conditional<XF32, PanelF32, Panel<CK>>::type;
+      XPanel px;
+      auto load_a = [&](int r, int c) { pa[r % RING].load(A, row0 + r * 16, c * CK, a.K, lane); };
+      // the tile's rows of x; rows past the last token are never multiplied into a
+      // token's column, and read as 0
+      const int xsz = XF32 ? 4 : 2;
+      const __amdgpu_buffer_rsrc_t X =
+          make_rsrc((const char *)a.x + (size_t)t0 * a.x_ld * xsz, 0x7FFFFFFFu);
+      const uint32_t xpitch = (uint32_t)a.x_ld * xsz;
+      uint32_t x_row[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 4 + lane / 16;
-      x_row[i] = t0 + r < a.T ? r * xpitch : BUF_OOB;
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 4 + lane / 16;
+        x_row[i] = t0 + r < a.T ? r * xpitch : BUF_OOB;
+      }
+      auto load_x = [&](int c) {
+        const int k = c * CK + (lane & 15) * (16 / xsz);  // 16 lanes a row
+#pragma unroll
+        for (int i = 0; i < 4; ++i) px.v[i] = buf_load16(X, k < a.K ? x_row[i] + k * xsz : BUF_OOB);
+      };
+      // chunks from nc on read as 0, without a branch: a branch around a load or a
+      // store makes every later wait a wait for all of them
+      load_x(wave);
+#pragma unroll
+      for (int r = 0; r < RING; ++r) load_a(r, wave);
+      for (int c = wave; c < nc; c += T_WAVES) {
+        const int next = c + T_WAVES;
+        u32x4 xf[NX][KS];
+        px.to_lds(stage, lane);
+        load_x(next);
+        lds_order();
+#pragma unroll
+        for (int s = 0; s < NX; ++s) Panel<CK>::frags(stage + s * 128, lane, xf[s]);
+#pragma unroll
+        for (int r = 0; r < NRB; ++r) {
+          u32x4 *buf = stage + XPART;
+          pa[r % RING].to_lds(buf, lane);
+          if (r + RING < NRB) load_a(r + RING, c);
+          else load_a((r + RING) % NRB, next);
+          lds_order();
+          u32x4 af[KS];
+          Panel<CK>::frags(buf, lane, af);
+#pragma unroll
+          for (int s = 0; s < NX; ++s)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) acc[r] = mfma_bf16_16x16x32(af[k], xf[s][k], acc[r]);
+          lds_order();
+        }
+      }
     }
-    auto load_x = [&](int c) {
-      const int k = c * CK + (lane & 15) * (16 / xsz);  // 16 lanes a row
+    const int lane_y = tid_opaque() & 63, col_y = lane_y & 15, q_y = lane_y >> 4;
+    // the sums of the waves: ranks row0 + rb * 16 + q_y * 4 .. + 3 of token col
+    auto to_red = [&]() {
+      f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
 #pragma unroll
-      for (int i = 0; i < 4; ++i) px.v[i] = buf_load16(X, k < a.K ? x_row[i] + k * xsz : BUF_OOB);
+      for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane_y] = acc[r];
     };
-    // chunks from nc on read as 0, without a branch: a branch around a load or a
-    // store makes every later wait a wait for all of them
-    load_x(wave);
+    auto from_red = [&](int rb) {
+      const f32x4 *red = (const f32x4 *)s_stage;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < RING; ++r) load_a(r, wave);
-    for (int c = wave; c < nc; c += T_WAVES) {
-      const int next = c + T_WAVES;
-      u32x4 xf[NX][KS];
-      px.to_lds(stage, lane);
-      load_x(next);
-      lds_order();
-#pragma unroll
-      for (int s = 0; s < NX; ++s) Panel<CK>::frags(stage + s * 128, lane, xf[s]);
-#pragma unroll
-      for (int r = 0; r < NRB; ++r) {
-        u32x4 *buf = stage + XPART;
-        pa[r % RING].to_lds(buf, lane);
-        if (r + RING < NRB) load_a(r + RING, c);
-        else load_a((r + RING) % NRB, next);
-        lds_order();
-        u32x4 af[KS];
-        Panel<CK>::frags(buf, lane, af);
-#pragma unroll
-        for (int s = 0; s < NX; ++s)
-#pragma unroll
-          for (int k = 0; k < KS; ++k) acc[r] = mfma_bf16_16x16x32(af[k], xf[s][k], acc[r]);
-        lds_order();
+      for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane_y];
+      return v;
+    };
+    float *const v_tok = a.v + ((size_t)p * a.T + t0 + col_y) * a.R;  // of token col
+    if constexpr (STAGES == STAGES_V) {
+      __syncthreads();  // every wave is done with its stage
+      to_red();
+      __syncthreads();
+      for (int rb = wave; rb < NRB; rb += T_WAVES) {
+        const f32x4 v = from_red(rb);
+        const int r0 = row0 + rb * 16 + q_y * 4;
+        if ((mask >> col_y) & 1 && r0 < a.R) *(f32x4 *)(v_tok + r0) = v;
       }
-    }
-  }
-  const int lane_y = tid_opaque() & 63, col_y = lane_y & 15, q_y = lane_y >> 4;
-  // the sums of the waves: ranks row0 + rb * 16 + q_y * 4 .. + 3 of token col
-  auto to_red = [&]() {
-    f32x4 *red = (f32x4 *)s_stage;  // [T_WAVES][NRB][64]
-#pragma unroll
-    for (int r = 0; r < NRB; ++r) red[(wave * NRB + r) * 64 + lane_y] = acc[r];
-  };
-  auto from_red = [&](int rb) {
-    const f32x4 *red = (const f32x4 *)s_stage;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < T_WAVES; ++w) v += red[(w * NRB + rb) * 64 + lane_y];
-    return v;
-  };
-  float *const v_tok = a.v + ((size_t)p * a.T + t0 + col_y) * a.R;  // of token col
-  if constexpr (STAGES == STAGES_V) {
-    __syncthreads();  // every wave is done with its stage
-    to_red();
-    __syncthreads();
-    for (int rb = wave; rb < NRB; rb += T_WAVES) {
-      const f32x4 v = from_red(rb);
-      const int r0 = row0 + rb * 16 + q_y * 4;
-      if ((mask >> col_y) & 1 && r0 < a.R) *(f32x4 *)(v_tok + r0) = v;
-    }
-  } else {
-  const uint32_t own = mask >> (q_y * 4);  // bit i: this lane's token q * 4 + i
-  constexpr int CP = NRK * 4;              // pieces of a row of B, padded
-  const int cpr = a.R / 8;
-  const __amdgpu_buffer_rsrc_t B =
-      make_rsrc(a.b[p] + (size_t)ad * M * a.R, (uint32_t)M * a.R * 2);
-  u32x4 w[LP];
-  YRun<YF32, VEC> y[4];
-  const int ysz = YF32 ? 4 : 2;
-  const __amdgpu_buffer_rsrc_t Y =
-      make_rsrc((const char *)a.y[p] + (size_t)t0 * a.y_ld[p] * ysz, 0x7FFFFFFFu);
-  const uint32_t ypitch = (uint32_t)a.y_ld[p] * ysz;
-  uint32_t y_tok[4];  // this lane's tokens q * 4 + i, or past the buffer
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y_tok[i] = (own >> i) & 1 ? (q_y * 4 + i) * ypitch : BUF_OOB;
-  auto y_at = [&](int u, int i, int j) {
-    const int m = u * 64 + (VEC ? 4 * col_y + j : 16 * j + col_y);
-    return m < M ? y_tok[i] + m * ysz : BUF_OOB;
-  };
-  auto load_b = [&](int u) {
-#pragma unroll
-    for (int i = 0; i < LP; ++i)  // piece i * 64 + lane of the unit
-      w[i] = buf_load16(B, (uint32_t)(u * cpr + i) * 1024 + lane_y * 16);
-  };
-  auto load_y = [&](int u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i].load(Y, [&](int j) { return y_at(u, i, j); });
-  };
-  int u = u0 + wave;
-  load_b(u);
-  load_y(u);
-  if constexpr (STAGES == STAGES_VY) {
-    __syncthreads();  // every wave is done with its stage
-    to_red();
-    __syncthreads();
-  }
-  // 2.
-  for (int rb = wave; rb < 2 * NRK; rb += T_WAVES) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    float e[4][NS];
-    const int r0 = rb * 16 + q_y * 4;
-    if constexpr (STAGES == STAGES_VY) {
-      if (rb < NRB) v = from_red(rb);
     } else {
-      // another adapter's tokens of the tile are never multiplied into this one's
-      if ((mask >> col_y) & 1 && r0 < rank) v = *(const f32x4 *)(v_tok + r0);
-    }
+      const uint32_t own = mask >> (q_y * 4);  // bit i: this lane's token q * 4 + i
+      constexpr int CP = NRK * 4;              // pieces of a row of B, padded
+      const int cpr = a.R / 8;
+      const __amdgpu_buffer_rsrc_t B =
+          make_rsrc(a.b[p] + (size_t)ad * M * a.R, (uint32_t)M * a.R * 2);
+      u32x4 w[LP];
+      YRun<YF32, VEC> y[4];
+      const int ysz = YF32 ? 4 : 2;
+      const __amdgpu_buffer_rsrc_t Y =
+          make_rsrc((const char *)a.y[p] + (size_t)t0 * a.y_ld[p] * ysz, 0x7FFFFFFFu);
+      const uint32_t ypitch = (uint32_t)a.y_ld[p] * ysz;
+      uint32_t y_tok[4];  // this lane's tokens q * 4 + i, or past the buffer
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split_bf16(r0 + i < rank ? v[i] * scale : 0.0f, e[i]);
-    const int slot = ((r0 & 31) >> 3) * 16 + col_y;
+      for (int i = 0; i < 4; ++i) y_tok[i] = (own >> i) & 1 ? (q_y * 4 + i) * ypitch : BUF_OOB;
+      auto y_at = [&](int u, int i, int j) {
+        const int m = u * 64 + (VEC ? 4 * col_y + j : 16 * j + col_y);
+        return m < M ? y_tok[i] + m * ysz : BUF_OOB;
+      };
+      auto load_b = [&](int u) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      s_v[rb >> 1][s][slot][(r0 >> 2) & 1] =
-          (u32x2){pack_hi(e[0][s], e[1][s]), pack_hi(e[2][s], e[3][s])};
-  }
-  __syncthreads();
-
-  // 3.
-  // piece i * 64 + lane of a unit: its place in the stage.  4 rows (a column of
-  // the MFMAs) are 4 CP pieces, turned by the column so that neither side meets a
-  // bank twice.
-  int place[LP];
+        for (int i = 0; i < LP; ++i)  // piece i * 64 + lane of the unit
+          w[i] = buf_load16(B, (uint32_t)(u * cpr + i) * 1024 + lane_y * 16);
+      };
+      auto load_y = [&](int u) {
 #pragma unroll
-  for (int i = 0; i < LP; ++i) {
-    const int l = i * 64 + lane_y, row = l / cpr, ch = l - row * cpr;
-    const int c = VEC ? row >> 2 : row & 15, j = VEC ? row & 3 : row >> 4;
-    place[i] = row < 64 ? c * 4 * CP + ((j * CP + ch) ^ c) : STAGE + lane_y;
-  }
-  u32x4 keep;  // clears B's columns from rank on (they may hold anything) in rank's block of 32
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = q_y * 8 + 2 * i, n = rank & 31;
-    keep[i] = (r < n ? 0xFFFFu : 0u) | (r + 1 < n ? 0xFFFF0000u : 0u);
-  }
-  u32x4 vf[NRK][NS];
-#pragma unroll
-  for (int rb = 0; rb < NRK; ++rb)
-#pragma unroll
-    for (int s = 0; s < NS; ++s) vf[rb][s] = *(const u32x4 *)s_v[rb][s][lane_y];
-
-  // d = v B^T of unit u, and the next unit's rows on their way
-  auto product = [&](int u, f32x4 (&d)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < LP; ++i) stage[place[i]] = w[i];
-    load_b(u + T_WAVES);
-    lds_order();
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int rb = 0; rb < NRK; ++rb) {
-        u32x4 b = stage[col_y * 4 * CP + ((j * CP + rb * 4 + q_y) ^ col_y)];
-        // from rank on B may hold anything: its block of 32 is masked, later ones are left out
-        if (rb * 32 + 32 > rank) b = rb * 32 < rank ? b & keep : (u32x4){0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) d[j] = mfma_bf16_16x16x32(vf[rb][s], b, d[j]);
+        for (int i = 0; i < 4; ++i) y[i].load(Y, [&](int j) { return y_at(u, i, j); });
+      };
+      int u = u0 + wave;
+      load_b(u);
+      load_y(u);
+      if constexpr (STAGES == STAGES_VY) {
+        __syncthreads();  // every wave is done with its stage
+        to_red();
+        __syncthreads();
       }
-    lds_order();
-  };
-  for (; u < u_end; u += T_WAVES) {
-    f32x4 d[4];
-    product(u, d);
-    YRun<YF32, VEC> o[4];
+      // 2.
+      for (int rb = wave; rb < 2 * NRK; rb += T_WAVES) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        float e[4][NS];
+        const int r0 = rb * 16 + q_y * 4;
+        if constexpr (STAGES == STAGES_VY) {
+          if (rb < NRB) v = from_red(rb);
+        } else {
+          // another adapter's tokens of the tile are never multiplied into this one's
+          if ((mask >> col_y) & 1 && r0 < rank) v = *(const f32x4 *)(v_tok + r0);
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i].add(y[i], d[0][i], d[1][i], d[2][i], d[3][i]);
-    load_y(u + T_WAVES);
+        for (int i = 0; i < 4; ++i) split_bf16(r0 + i < rank ? v[i] * scale : 0.0f, e[i]);
+        const int slot = ((r0 & 31) >> 3) * 16 + col_y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i].store(Y, [&](int j) { return y_at(u, i, j); });
-  }
-  }
-  if (rem) __syncthreads();  // the stage is the next adapter's
+        for (int s = 0; s < NS; ++s)
+          s_v[rb >> 1][s][slot][(r0 >> 2) & 1] =
+              (u32x2){pack_hi(e[0][s], e[1][s]), pack_hi(e[2][s], e[3][s])};
+      }
+      __syncthreads();
+
+      // 3.
+      // piece i * 64 + lane of a unit: its place in the stage.  4 rows (a column of
+      // the MFMAs) are 4 CP pieces, turned by the column so that neither side meets a
+      // bank twice.
+      int place[LP];
+#pragma unroll
+      for (int i = 0; i < LP; ++i) {
+        const int l = i * 64 + lane_y, row = l / cpr, ch = l - row * cpr;
+        const int c = VEC ? row >> 2 : row & 15, j = VEC ? row & 3 : row >> 4;
+        place[i] = row < 64 ? c * 4 * CP + ((j * CP + ch) ^ c) : STAGE + lane_y;
+      }
+      u32x4 keep;  // clears B's columns from rank on (they may hold anything) in rank's block of 32
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = q_y * 8 + 2 * i, n = rank & 31;
+        keep[i] = (r < n ? 0xFFFFu : 0u) | (r + 1 < n ? 0xFFFF0000u : 0u);
+      }
+      u32x4 vf[NRK][NS];
+#pragma unroll
+      for (int rb = 0; rb < NRK; ++rb)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) vf[rb][s] = *(const u32x4 *)s_v[rb][s][lane_y];
+
+      // d = v B^T of unit u, and the next unit's rows on their way
+      auto product = [&](int u, f32x4 (&d)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < LP; ++i) stage[place[i]] = w[i];
+        load_b(u + T_WAVES);
+        lds_order();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int rb = 0; rb < NRK; ++rb) {
+            u32x4 b = stage[col_y * 4 * CP + ((j * CP + rb * 4 + q_y) ^ col_y)];
+            // from rank on B may hold anything: its block of 32 is masked, later ones are left out
+            if (rb * 32 + 32 > rank) b = rb * 32 < rank ? b & keep : (u32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) d[j] = mfma_bf16_16x16x32(vf[rb][s], b, d[j]);
+          }
+        lds_order();
+      };
+      for (; u < u_end; u += T_WAVES) {
+        f32x4 d[4];
+        product(u, d);
+        YRun<YF32, VEC> o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i].add(y[i], d[0][i], d[1][i], d[2][i], d[3][i]);
+        load_y(u + T_WAVES);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i].store(Y, [&](int j) { return y_at(u, i, j); });
+      }
+    }
+    if (rem) __syncthreads();  // the stage is the next adapter's
   }
 }
 
@@ -809,7 +814,8 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     const int groups = div_up(m_most, 64);
     auto grid = [&](bool fused) {
       const int waves = dec_waves(fused);
-      a.units = div_up(groups * T * l.n_proj, dec_waves_wanted(fused));
+      const int64_t all = (int64_t)groups * T * l.n_proj;  // past 2^31 at pitched large calls
+      a.units = (int)((all + dec_waves_wanted(fused) - 1) / dec_waves_wanted(fused));
       return dim3(T, div_up(groups, a.units * waves), l.n_proj);
     };
     const size_t bytes_a = (size_t)l.rank * l.in * 2;
