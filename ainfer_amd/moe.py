@@ -153,7 +153,8 @@ class MoeLayer:
     def forward_scored(self, x, y, ws, routing, bias=None, resid=None, shared=None, stream=None):
         """forward with scored routing: the layer's router logits (its
         router_bias, where it has one, is part of them) -> route_scored(routing,
-        logits, bias) -> experts -> combine, in steps of CHUNK_TOKENS.  shared:
+        logits, bias) -> experts -> combine, in steps of CHUNK_TOKENS (ws: for
+        that many tokens, or T where it is less).  shared:
         [T][H] bf16 rows that take the place of the shared expert's (for
         example shared_adapted's)."""
         if (routing.n_experts, routing.top_k) != (self.shape.n_experts, self.shape.top_k):

@@ -205,3 +205,13 @@ def test_refusals(torch, world):
                  lambda: w.layer.shared_adapted(x, ids, w.gu, None, wsl[:16])):
         with pytest.raises(L.MoeError):
             call()
+
+
+def test_no_tokens(torch, world):
+    w = world
+    x, ids, wsl, ws = inputs(torch, w, 1, 1)
+    empty = torch.empty(0, 1024, dtype=torch.bfloat16, device="cuda")
+    rows = w.layer.shared_adapted(empty, ids[:0], w.gu, w.down, wsl)
+    assert rows.shape == (0, 1024)
+    y = w.layer.forward_scored(empty, torch.empty_like(empty), ws, w.r, w.bias, shared=rows)
+    assert y.shape == (0, 1024)

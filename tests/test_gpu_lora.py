@@ -273,3 +273,33 @@ def test_workspace_of_pitched_prompts(torch):
     torch.cuda.synchronize()
     c.compare(c.y, ys)
     assert (buf[:off] == 0xA5).all() and (buf[off + n:] == 0xA5).all()
+
+
+def test_two_launches_on_two_streams_and_in_a_graph(torch):
+    """Calls at once on two streams, each with its own scratch; replays of a
+    captured call with eager calls between them."""
+    a = Case(torch, 300, 7, 64, 4096, [1027], seed=1)
+    b = Case(torch, 411, 4, 96, 2048, [1500], x="fp32", seed=2)
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    ys = [[y.clone() for y in c.y] for c in (a, b)]
+    ws = [c.lora.workspace(c.T) for c in (a, b)]
+    torch.cuda.synchronize()
+    for c, y, w, s in zip((a, b), ys, ws, side):
+        c.apply(y, w, stream=s)
+    torch.cuda.synchronize()
+    for c, y in zip((a, b), ys):
+        c.compare(c.y, y)
+    work = [y.clone() for y in a.y]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.apply(work, ws[0])
+    for rep in range(3):
+        for y, y0 in zip(work, a.y):
+            y.copy_(y0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for y, want in zip(work, ys[0]):
+            assert torch.equal(y, want), rep
+        b.apply([y.clone() for y in b.y], ws[1])
+        ws[0].fill_(rep)
+        torch.cuda.synchronize()

@@ -1,9 +1,10 @@
 """Scored routing (ainfer_moe_route_scored) against its definition in 64 bits.
 
 Bar: expert indices equal; weights within RTOL of the 64-bit value.  The weights
-are a few fp32 operations: exp and the reciprocal or division to 2^-22 each, the
-argument of exp rounded once (2^-24 of up to 80, which e^-80 caps: 2^-17.7), sums of
-at most 1024 positive terms (2^-18, softmax over all experts): below 2^-16 in all.
+are a few fp32 operations: the hardware's exp2 of an argument off by 1.125 2^-23 of
+itself in all ((1.125 d + 1) 2^-23 for exp(-d), d up to 80: 2^-16.5; larger ones are
+covered by ATOL), reciprocals to 2^-22, sums of at most 1024 positive terms, which
+carry the errors of their large ones (2^-19): below 2^-16 in all.
 ATOL covers what fp32 cannot hold (values below its normal range)."""
 import math
 
@@ -376,3 +377,30 @@ def test_many_tokens_group_values_nearer_than_fp32(torch):
             bias[own] = (0.5 - s[t, own]).float()
         check_many(torch, x, bias, 4, SIG, G, 3, GTOP2)
         check_many(torch, x, bias, 4, SIG, G, 3, GMAX)
+
+
+def test_many_tokens_on_another_stream_and_in_a_graph(torch):
+    from ainfer_amd import _lib as L
+    from ainfer_amd import moe
+    r = L.Routing(64, 6, SIG, 4, 2, GTOP2, 1, 2.5)
+    x = logits_of(torch, 20000, 64, torch.float32, 8)
+    bias = logits_of(torch, 1, 64, torch.float32, 9, 0.1)[0]
+    want = moe.route_scored(r, x, bias)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = moe.route_scored(r, x, bias, stream=side)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    parts = [moe.route_scored(r, x[i:i + 999], bias) for i in range(0, 20000, 999)]
+    assert torch.equal(torch.cat([p[0] for p in parts]), want[0])  # a wave a token: the same picks
+    out = (torch.empty_like(want[0]), torch.empty_like(want[1]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moe.route_scored(r, x, bias, out=out)
+    for rep in range(3):
+        x.copy_(logits_of(torch, 20000, 64, torch.float32, 20 + rep))
+        out[0].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = moe.route_scored(r, x, bias)
+        assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
