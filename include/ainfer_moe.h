@@ -432,8 +432,10 @@ int ainfer_moe_set_strict(int32_t on);
  *               lower index first, and only where fewer than top_k are left
  *   topk_w[t][j] scale * s, or scale * s / (sum of the selected s) with
  *               renormalize; 0 for a masked expert, also where all are masked
- * Scores and sums are fp32; where two keys or group values are too near for
- * fp32 the comparison is redone in fp64.  The rows are what
+ * Scores and sums are fp32 (weights within 2^-16 of the formula's, relative,
+ * where they are not below 2^-80 of the largest); where two keys or group values
+ * are too near for fp32 the comparison is redone in fp64, so topk_idx does not
+ * depend on the size of the call.  The rows are what
  * ainfer_moe_dispatch, _experts and _combine take.  No reference counterpart
  * (the reference is dense). */
 enum { AINFER_SCORE_SOFTMAX = 0, AINFER_SCORE_SIGMOID = 1 };
@@ -464,11 +466,14 @@ int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logit
  * adapter is outside [0, n_adapters) keeps its rows of y untouched (they are
  * not read either), as does one whose adapter has rank 0.  Tokens of a batch
  * may name adapters in any order.  Rows r >= rank_a of a and columns
- * r >= rank_a of b may hold anything.  x, a and b enter exactly; v and the
- * products are fp32 sums, v is scaled in fp32 and enters the second product as
- * the sum of three bf16 values (its 24 bits) where y is fp32, of two (2^-16 of
- * it) where y is bf16; y is rounded once.  No reference counterpart (the
- * reference serves one model to one request). */
+ * r >= rank_a of b may hold anything, and so may unused adapters; an infinity or
+ * NaN in use gives its tokens infinities or NaN, and no other token.  x, a and b
+ * enter exactly; v and the products are fp32 sums and v is scaled in fp32.  It
+ * enters the second product in fp32 up to 256 tokens, above as the sum of three
+ * bf16 values (its 24 bits) where y is fp32, of two (2^-16 of it) where y is bf16;
+ * y is rounded once.  The same call gives the same bits; calls of other token
+ * counts add in other orders.  No reference counterpart (the reference serves one
+ * model to one request). */
 #define AINFER_LORA_MAX_PROJ 4
 typedef struct ainfer_moe_lora {
   int32_t n_adapters;  /* N, 1..4096                                         */
