@@ -467,10 +467,13 @@ template <int STAGES, int LP, bool XF32, bool YF32, bool VEC>
 __global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP, YF32)) void k_lora_tile(
     LoraArgs a) {
   constexpr int T_WAVES = tile_waves(STAGES);
-  constexpr int NRB = LP <= 2 ? 1 : LP / 2;  // blocks of 16 rows of A
+  // blocks of 16 rows of A (4 also for 33 to 48 rows: two panels in flight divide them)
+  constexpr int NRB = LP <= 2 ? 1 : LP == 6 ? 4 : LP / 2;
   constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
   constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
-  constexpr int RING = NRB < 3 ? NRB : tile_two(LP, YF32) ? 2 : 4;  // panels of A in flight
+  // panels of A in flight; a block's place among them is the same in every chunk
+  constexpr int RING = NRB < 3 ? NRB : tile_two(LP, YF32) ? 2 : NRB % 4 ? 3 : 4;
+  static_assert(NRB % RING == 0, "");
   constexpr int STAGE = NRK <= 2 ? 512 : NRK * 256;  // 16-byte pieces of a wave's LDS
   constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it
   __shared__ u32x4 s_stage[T_WAVES][STAGE + 64];

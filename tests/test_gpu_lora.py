@@ -303,3 +303,14 @@ def test_two_launches_on_two_streams_and_in_a_graph(torch):
         b.apply([y.clone() for y in b.y], ws[1])
         ws[0].fill_(rep)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("R", (8, 16, 24, 32, 40, 48, 56, 64, 72, 80, 88, 96, 104, 112, 120, 128))
+@pytest.mark.parametrize("x,y", (("bf16", "fp32"), ("bf16", "bf16"), ("fp32", "fp32"),
+                                 ("fp32", "bf16")))
+def test_prompts_of_every_rank(torch, R, x, y):
+    """One launch and two, several chunks of K a wave, with and without the other."""
+    Case(torch, 700, 3, R, 2312, [100], x=x, y=y).check()
+    Case(torch, 290, 3, R, 4104, [70, 516], x=x, y=y, ids=[t // 60 % 4 - 1 for t in range(290)]).check()
+    Case(torch, 1500, 3, R, 1160, [136], x=x, y=y).check()
+    Case(torch, 330, 3, R, 1160, [2100], x=x, y=y).check()
