@@ -439,10 +439,10 @@ struct PanelF32 {
 };
 
 // One adapter's tokens of a tile of 16, all of K, then all of this workgroup's
-// rows of y.  blockIdx.x: tile (fastest, so that the first adapters of all tiles
-// start first; a workgroup of an adapter that a tile lacks ends after one load),
-// blockIdx.y: which distinct adapter of the tile, blockIdx.z: projection and
-// part of its rows.
+// rows of y.  blockIdx.x: tile, blockIdx.y: projection and part of its rows,
+// blockIdx.z: which distinct adapter of the tile (slowest, so that the first adapters
+// of all tiles and parts start first, on CUs of their own; a workgroup of an adapter
+// that a tile lacks ends after one load).
 //   1. v = A x^T: a wave takes every T_WAVES-th chunk of CK columns; A's next rows
 //      are read while the last ones are multiplied.  The sums meet in LDS.
 //   2. v scaled, split and laid out for the MFMA.
@@ -451,7 +451,7 @@ struct PanelF32 {
 //      whole pieces of 4; else row 16 j + c, so that 16 lanes reach a line
 //      together).  B's rows are read whole and turned in LDS as A's; what the
 //      next unit reads of B and y is in flight meanwhile.
-// STAGES V: 1 alone, of a.rows rows of A (blockIdx.z: projection and which), v
+// STAGES V: 1 alone, of 32 rows of A (blockIdx.y: projection and which), v
 // to memory; Y: 2 and 3 of that v.
 enum { STAGES_VY, STAGES_V, STAGES_Y };
 constexpr int tile_waves(int stages) { return stages == STAGES_Y ? 4 : 8; }
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // neighbouring tiles on one XCD, whose L2 then holds their adapters
   const int t0 = xcd_remap(blockIdx.x, gridDim.x) * TT;
-  const int p = blockIdx.z % a.P, part = blockIdx.z / a.P;
+  const int p = blockIdx.y % a.P, part = blockIdx.y / a.P;
   const int M = a.m[p];
   const int id = tile_ids(a, t0, lane0);
   const int row0 = STAGES == STAGES_V ? part * NRB * 16 : 0;  // of A
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP,
     const int ad = __builtin_amdgcn_readlane(id, __builtin_ctz(rem));
     const uint32_t mask = (uint32_t)__ballot(id == ad) & rem;
     rem &= ~mask;
-    if (nth % (int)gridDim.y != (int)blockIdx.y) continue;
+    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int rank = rank_of(a, ad);
     if (rank <= row0) continue;
     const float scale = a.scales ? a.scales[ad] : 1.0f;
@@ -855,26 +855,35 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     n = n < least ? least : n > TT ? TT : n;
     return n < l.n_adapters ? n : l.n_adapters;
   };
-  // parts of y's rows, each of which computes v again, while tiles leave CUs idle
-  int parts = N_CU / (tiles * l.n_proj);
-  parts = split(parts < 1 ? 1 : parts > 8 ? 8 : parts, tile_waves(STAGES_VY));
+  // parts of y's rows, each of which computes v again, while tiles leave CUs idle: on
+  // half of them (the others are for second adapters of a tile), and fewer where v is
+  // most of the work.  us with 1, 2, 4 parts: T 1024, 4096 x 4096, rank 32, 16.6, 13.9,
+  // 18.4, T 1003, 1024 x 4096 fp32, rank 8, 14.3, 12.1, 13.2; T 998, 2136 x 1195 of fp32,
+  // rank 56, with 1 and 2 17.4 and 22.3; T 1641, 576 x 4239 of fp32, rank 24, 27.7 and 21.3
+  const int64_t v_bytes = (int64_t)l.in * (l.rank * 2 + TT * (xf32 ? 4 : 2));
+  const int64_t y_bytes = (int64_t)m_most * (l.rank * 2 + TT * 2 * ysz);
+  const int idle = N_CU / (tiles * l.n_proj);
+  int64_t most = 2 * idle * y_bytes / (5 * v_bytes);
+  if (most > idle / 2) most = idle / 2;
+  if (idle >= 2 && y_bytes > 4 * v_bytes && most < 2) most = 2;
+  int parts = split(most < 1 ? 1 : most > 8 ? 8 : (int)most, tile_waves(STAGES_VY));
   const size_t again = (size_t)(parts - 1) * tiles * l.n_proj * l.rank * l.in * 2;
   if (cpr > 4 && again > TILE_AGAIN) {
     const int groups = div_up(l.rank, 32);
-    const dim3 gv(gx, slots(tiles * l.n_proj * groups, 2), l.n_proj * groups);
+    const dim3 gv(gx, l.n_proj * groups, slots(tiles * l.n_proj * groups, 2));
     const dim3 bv(64 * tile_waves(STAGES_V));
     if (xf32) k_lora_tile<STAGES_V, 4, true, false, false><<<gv, bv, 0, s>>>(a);
     else k_lora_tile<STAGES_V, 4, false, false, false><<<gv, bv, 0, s>>>(a);
     parts = 2 * N_CU / (tiles * l.n_proj);
     parts = split(parts < 1 ? 1 : parts, tile_waves(STAGES_Y));
-    const dim3 gy(gx, slots(tiles * l.n_proj * parts, 2), l.n_proj * parts);
+    const dim3 gy(gx, l.n_proj * parts, slots(tiles * l.n_proj * parts, 2));
     if (cpr <= 6) launch_tile<STAGES_Y, 6, false>(a, gy, yf32, vec, s);
     else if (cpr <= 8) launch_tile<STAGES_Y, 8, false>(a, gy, yf32, vec, s);
     else if (cpr <= 12) launch_tile<STAGES_Y, 12, false>(a, gy, yf32, vec, s);
     else launch_tile<STAGES_Y, 16, false>(a, gy, yf32, vec, s);
     return hipGetLastError();
   }
-  const dim3 grid(gx, slots(tiles * l.n_proj * parts, 4), l.n_proj * parts);
+  const dim3 grid(gx, l.n_proj * parts, slots(tiles * l.n_proj * parts, 4));
   if (cpr <= 1) launch_tile_vy<1>(a, grid, xf32, yf32, vec, s);
   else if (cpr <= 2) launch_tile_vy<2>(a, grid, xf32, yf32, vec, s);
   else if (cpr <= 4) launch_tile_vy<4>(a, grid, xf32, yf32, vec, s);
