@@ -314,3 +314,13 @@ def test_prompts_of_every_rank(torch, R, x, y):
     Case(torch, 290, 3, R, 4104, [70, 516], x=x, y=y, ids=[t // 60 % 4 - 1 for t in range(290)]).check()
     Case(torch, 1500, 3, R, 1160, [136], x=x, y=y).check()
     Case(torch, 330, 3, R, 1160, [2100], x=x, y=y).check()
+
+
+@pytest.mark.parametrize("R", (8, 16, 24, 32, 40, 64, 72, 96, 120, 128))
+@pytest.mark.parametrize("x,y", (("bf16", "fp32"), ("bf16", "bf16"), ("fp32", "fp32"),
+                                 ("fp32", "bf16")))
+def test_batches_of_every_rank(torch, R, x, y):
+    Case(torch, 3, 2, R, 20488, [130], x=x, y=y, ids=[1, 0, 1]).check()
+    Case(torch, 1, 2, R, 16384, [64, 1], x=x, y=y, ids=[1]).check()
+    Case(torch, 41, 5, R, 2312, [70, 516], x=x, y=y).check()
+    Case(torch, 200, 9, R, 1160, [100], x=x, y=y).check()

@@ -113,7 +113,7 @@ def logits_of(torch, T, E, dtype, seed, std=1.5):
 SHAPES = [(1, 1, 1, 1, 1), (1, 256, 8, 8, 4), (7, 60, 4, 6, 3), (333, 64, 8, 1, 1),
           (130, 512, 10, 1, 1), (65, 1024, 32, 1, 1), (33, 1024, 32, 64, 8), (5, 23, 13, 1, 1),
           (40, 96, 6, 3, 2), (9, 1023, 7, 33, 5), (17, 960, 16, 48, 3), (64, 40, 1, 8, 1),
-          (12, 64, 6, 64, 6), (21, 1024, 9, 2, 1), (3, 65, 32, 5, 3), (257, 160, 8, 8, 3)]
+          (12, 64, 6, 64, 6), (30, 873, 9, 3, 1), (30, 864, 9, 3, 2), (19, 300, 11, 1, 1), (21, 1024, 9, 2, 1), (3, 65, 32, 5, 3), (257, 160, 8, 8, 3)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -286,13 +286,13 @@ def check_many(torch, x, bias, k, score, G=1, top=1, gscore=GTOP2, renorm=1, sca
         assert (out[0][T:] == -7).all() and (out[1][T:] == -7).all()
         idx.append(out[0][:T].cpu().numpy())
         w.append(out[1][:T].cpu().numpy())
-    assert np.array_equal(idx[0], idx[1]) and np.array_equal(w[0], w[1])
     ri, rw = reference(x.double().cpu().numpy(), torch.finfo(x.dtype).min,
                        None if bias is None else bias.cpu().numpy(), E, k, score, G, top, gscore,
                        renorm, scale)
     order = order.numpy()
-    assert np.array_equal(idx[0], ri[order])
-    assert np.all(np.abs(w[0] - rw[order]) <= RTOL * np.abs(rw[order]) + ATOL * max(1.0, abs(scale)))
+    for i, v in zip(idx, w):
+        assert np.array_equal(i, ri[order])
+        assert np.all(np.abs(v - rw[order]) <= RTOL * np.abs(rw[order]) + ATOL * max(1.0, abs(scale)))
 
 
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1), (16, 3, 1, 1), (23, 13, 1, 1), (60, 4, 6, 3),
