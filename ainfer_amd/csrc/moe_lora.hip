@@ -18,7 +18,7 @@
 // GPU us a call (inside a graph), and the time the bytes of x, y, and each A and B
 // used once take at 5.1 TB/s: one token 4096 x 4096 rank 16 4.8 (0.1; a launch alone is
 // 2.5), 64 tokens 4096 x (1024 + 1024) rank 16 6.1 (2.2), 16 tokens 5120 x 17408 rank
-// 64 14.8 (8.3), 1003 tokens of 7 requests 1024 x 4096 rank 8 in fp32 14.3 (7.3), 4096
+// 64 14.8 (8.3), 1003 tokens of 7 requests 1024 x 4096 rank 8 in fp32 12.1 (7.3), 4096
 // tokens 4096 x 4096 of 24 requests rank 32 28 (19.3), rank 64 40 (21.5), of one
 // request rank 32 21 (19.7).
 //
@@ -704,11 +704,11 @@ __global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP,
 
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Up to this many tokens a call is taken as a batch of requests.  GPU us of one
-// projection, 4096 x 4096, rank 16: every token another of 64 adapters, 256 tokens
-// 14.7 by tokens and 37 by tiles, 1024 tokens 34 and 85; 4 requests' prompts, 128
-// tokens 12.8 and 10.5, 256 15.0 and 10.8, 512 18.6 and 14.4, 1024 25 and 15; at
-// rank 64 256 tokens of 4 requests 23 and 16, 512 35 and 27.
+// Up to this many tokens a call is taken as a batch of requests.  GPU us by tokens and
+// by tiles: every token another of 64 adapters, 256 tokens 4096 x 4096 rank 16 14.6 and
+// 32, 1024 x 4096 rank 8 fp32 7.8 and 25.5, 2048 x (2048 + 2048) rank 64 35 and 51;
+// prompts of 4 requests, 128 tokens rank 16 8.3 and 7.2, 256 9.9 and 7.6, rank 8 5.8 and
+// 7.1, rank 64 20 and 14; of 16 requests 256 tokens 11.2 and 11.3, 6.4 and 9.4, 22 and 16.
 constexpr int DEC_MAX_T = 256;
 
 // v in every workgroup of a token, or by k_lora_rows first.  us, K 4096, M 4096
@@ -722,10 +722,10 @@ bool fuse(size_t bytes_a, int tokens, int workgroups) {
   const size_t again = (size_t)(workgroups - 1) * tokens * bytes_a;
   return bytes_a <= FUSED_BYTES && again * (workgroups > 8 ? 2 : 1) <= FUSED_AGAIN;
 }
-// about this many waves of k_lora_dec: fused, more workgroups read A more often
-// (rank 16, T 128 13.6 us at 8192, 10.3 at 4096); alone, more loads are in flight
-// (rank 32, T 256 27.3 at 4096, 23.8 at 8192, 25.5 at 16384)
-constexpr int dec_waves_wanted(bool fused) { return fused ? 4096 : 8192; }
+// Workgroups of k_lora_dec: fused, two on each CU, all at once, as each reads A (T 192
+// rank 16, 4096 x 4096, 3 and 2 a token: 15.6 and 12.8 us); alone, about this many waves,
+// for the loads in flight (rank 32, T 256 27.3 at 4096, 23.8 at 8192, 25.5 at 16384)
+constexpr int DEC_WAVES_WANTED = 8192;
 // k_lora_rows: two rows a workgroup, four from this many rows in the call (fewer
 // workgroups for equal time: rank 128, T 256 76.9 and 77.3 us)
 constexpr int ROWS_TWO = 4096;
@@ -817,8 +817,13 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
     const int groups = div_up(m_most, 64);
     auto grid = [&](bool fused) {
       const int waves = dec_waves(fused);
-      const int64_t all = (int64_t)groups * T * l.n_proj;  // past 2^31 at pitched large calls
-      a.units = (int)((all + dec_waves_wanted(fused) - 1) / dec_waves_wanted(fused));
+      if (fused) {
+        const int each = 2 * N_CU / (T * l.n_proj);  // workgroups a token
+        a.units = div_up(groups, waves * (each < 1 ? 1 : each));
+      } else {
+        const int64_t all = (int64_t)groups * T * l.n_proj;  // past 2^31 at pitched large calls
+        a.units = (int)((all + DEC_WAVES_WANTED - 1) / DEC_WAVES_WANTED);
+      }
       return dim3(T, div_up(groups, a.units * waves), l.n_proj);
     };
     const size_t bytes_a = (size_t)l.rank * l.in * 2;
