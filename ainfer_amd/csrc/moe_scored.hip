@@ -28,7 +28,7 @@
 // k_route_many: many tokens of few experts, four a wave.
 //
 // What bounds it: the instructions issued.  65536 tokens of 512 experts with a bias
-// (softmax, top-10) take 60 us where their bytes take 27: 315 vector and 287 scalar
+// (softmax, top-10) take 58 us where their bytes take 27: 315 vector and 287 scalar
 // instructions a token, next token's logits in flight meanwhile; 64 experts 19.  One
 // token takes 4.4 us, of which a launch alone is 2.5; 4096 tokens of 256 experts in 8
 // groups 7.1.
@@ -1030,8 +1030,11 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   const int blocks = (T + SR_WAVES - 1) / SR_WAVES;
   // a wave keeps the bias over its tokens; without one a workgroup per 4 tokens.  us at
   // T 65536, grids of 2048 and 16384: 512 experts with a bias 64 and 93, without
-  // 52 and 45 (bf16, not renormalised 70 and 53), 64 experts 38 and 31
-  const int most = bias ? 2048 : 16384, grid = blocks < most ? blocks : most;
+  // 52 and 45 (bf16, not renormalised 70 and 53), 64 experts 38 and 31.  With 8 experts a
+  // lane 1280 are resident at once (about 90 registers): 512 experts softmax 58.2 (2048
+  // 60.3), sigmoid 50.2 (53.2); 256 experts in 8 groups 57 (2048 56)
+  const int most = !bias ? 16384 : need > 4 && need <= 8 ? 1280 : 2048;
+  const int grid = blocks < most ? blocks : most;
   if (need <= 1) launch_nv<1>(a, grid, soft, s);
   else if (need <= 2) launch_nv<2>(a, grid, soft, s);
   else if (need <= 4) launch_nv<4>(a, grid, soft, s);
