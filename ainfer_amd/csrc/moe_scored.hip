@@ -28,7 +28,7 @@
 // k_route_many: many tokens of few experts, four a wave.
 //
 // What bounds it: the instructions issued.  65536 tokens of 512 experts with a bias
-// (softmax, top-10) take 58 us where their bytes take 27: 315 vector and 287 scalar
+// (softmax, top-10) take 58 us where their bytes take 27: 308 vector and 283 scalar
 // instructions a token, next token's logits in flight meanwhile; 64 experts 19.  One
 // token takes 4.4 us, of which a launch alone is 2.5; 4096 tokens of 256 experts in 8
 // groups 7.1.
