@@ -1169,7 +1169,8 @@ int ainfer_moe_route_scored(const ainfer_moe_routing *r, const void *logits, int
   if (T == 0) return AINFER_OK;
   if (!logits || !topk_idx || !topk_w) return AINFER_ERR_NULL;
   if (ld < r->n_experts || ld > MAX_LD || mis(logits, act_size(logits_dtype)) || mis(bias, 4) ||
-      mis(topk_idx, 4) || mis(topk_w, 4))
+      mis(topk_idx, 4) || mis(topk_w, 4) || (const void *)topk_idx == topk_w ||
+      logits == topk_idx || logits == topk_w)
     return AINFER_ERR_ARG;
   HIP_TRY(launch_route_scored(*r, logits, logits_dtype, ld, bias, T, topk_idx, topk_w,
                               (hipStream_t)stream));
@@ -1200,6 +1201,11 @@ int ainfer_moe_lora_apply(const ainfer_moe_lora *l, const void *x, int64_t x_ld,
         y_ld[p] > MAX_LD)
       return AINFER_ERR_ARG;
   if (mis(ws, 256) || ws_bytes < lora_workspace_bytes(*l, T)) return AINFER_ERR_WORKSPACE;
+  for (int p = 0; p < l->n_proj; ++p) {
+    if (y[p] == x || y[p] == ws || ws == x) return AINFER_ERR_ARG;
+    for (int q = 0; q < p; ++q)
+      if (y[p] == y[q]) return AINFER_ERR_ARG;
+  }
   HIP_TRY(launch_lora(*l, x, x_ld, token_adapter, T, y, y_ld, ws, (hipStream_t)stream));
   return AINFER_OK;
 }
@@ -1215,6 +1221,10 @@ int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64
   const int isz = act_size(in_dtype);
   if (gate_ld < I || up_ld < I || act_ld < I || gate_ld > MAX_LD || up_ld > MAX_LD ||
       act_ld > MAX_LD || mis(gate, isz) || mis(up, isz) || mis(act, act_size(act_dtype)))
+    return AINFER_ERR_ARG;
+  // in place only where every element of act lies on its own input
+  if ((act == gate && (act_dtype != in_dtype || (T > 1 && act_ld != gate_ld))) ||
+      (act == up && (act_dtype != in_dtype || (T > 1 && act_ld != up_ld))))
     return AINFER_ERR_ARG;
   HIP_TRY(launch_silu_rows(gate, gate_ld, up, up_ld, in_dtype, T, I, act, act_ld, act_dtype,
                            (hipStream_t)stream));

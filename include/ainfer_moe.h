@@ -452,7 +452,7 @@ typedef struct ainfer_moe_routing {
 } ainfer_moe_routing;
 /* logits [T] rows of E values (AINFER_ACT_F32 or AINFER_ACT_BF16), row t at
  * t * ld elements (ld >= E); bias [E] fp32 or NULL; topk_idx, topk_w
- * [T][top_k].  No workspace. */
+ * [T][top_k], none of the three overlapping.  No workspace. */
 int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logits,
                             int32_t logits_dtype, int64_t ld, const float *bias, int32_t T,
                             int32_t *topk_idx, float *topk_w, void *stream);
@@ -495,7 +495,8 @@ typedef struct ainfer_moe_lora {
 size_t ainfer_moe_lora_workspace_bytes(const ainfer_moe_lora *lora, int32_t max_tokens);
 /* x: T rows of K values, row t at t * x_ld elements, 16-byte aligned rows;
  * token_adapter [T] int32; y[p]: T rows of M_p values at t * y_ld[p] elements
- * (aligned to their type; rows must not overlap x, a, b or each other). */
+ * (aligned to their type; rows must not overlap x, a, b or each other: the same
+ * address for two of x, the y and the workspace is refused). */
 int ainfer_moe_lora_apply(const ainfer_moe_lora *lora, const void *x, int64_t x_ld,
                           const int32_t *token_adapter, int32_t T, void *const *y,
                           const int64_t *y_ld, void *workspace, size_t workspace_bytes,
@@ -505,7 +506,8 @@ int ainfer_moe_lora_apply(const ainfer_moe_lora *lora, const void *x, int64_t x_
  * u = up[t][i], computed in fp32.  Row t of gate, up and act starts at t * its
  * ld elements (so gate and up may be the halves of one [T][2 * I] buffer);
  * in_dtype of gate and up, act_dtype of act: AINFER_ACT_F32 or
- * AINFER_ACT_BF16.  act may be gate or up itself (same pointer, type and ld).
+ * AINFER_ACT_BF16.  act may be gate or up itself (same pointer, type and
+ * ld; with another type or ld it is refused), and must not overlap them otherwise.
  * Replaces SiluMul, tools/cmdlist/kernels.cpp:29-37, where the projections
  * around it are calls of their own (an adapted MLP). */
 int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,

@@ -144,3 +144,20 @@ def test_python_wrappers_refuse_host_tensors(L):
     with pytest.raises(L.MoeError):
         moe.LoraAdapters([torch.zeros(1, 8, 8, dtype=torch.bfloat16)],
                          [torch.zeros(1, 8, 8, dtype=torch.bfloat16)])
+
+
+def test_overlapping_operands(L):
+    """The same address for two operands that a call reads and writes in
+    different orders."""
+    ys = (0x10000, 0x20000)
+    good = dict(x=C.c_void_p(0x40000), ws=C.c_void_p(0x30000))
+    for kw in (dict(y=(0x10000, 0x10000)), dict(y=(0x40000, 0x20000)), dict(y=(0x10000, 0x30000)),
+               dict(x=C.c_void_p(0x30000))):
+        assert apply(L, lora(L), **{**good, "y": ys, **kw}) == L.ERR_ARG, kw
+    at = dict(logits=C.c_void_p(0x10000), idx=C.c_void_p(0x20000), w=C.c_void_p(0x30000))
+    for kw in (dict(w=at["idx"]), dict(w=at["logits"]), dict(idx=at["logits"])):
+        assert route(L, routing(L), **{**at, **kw}) == L.ERR_ARG, kw
+    up, act = C.c_void_p(0x10000), FAKE
+    for kw in (dict(up=up, act=act, adt=1), dict(up=up, act=act, ald=104),
+               dict(gate=up, act=act, adt=1), dict(gate=up, act=act, ald=104)):
+        assert silu(L, **kw) == L.ERR_ARG, kw
