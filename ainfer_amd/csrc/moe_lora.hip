@@ -13,7 +13,7 @@
 //                 v_mfma_f32_16x16x32_bf16, once per distinct adapter among them,
 //                 other tokens' columns ignored: no sorting, tokens may name
 //                 adapters in any order.  Its products are exact too: bf16 values
-//                 enter the MFMA as they are, fp32 values as the sum of two or three
+//                 enter the MFMA as they are, fp32 values (x, and v) as the sum of three
 //                 bf16 (split_bf16).  v never leaves the CU.
 // GPU us a call (inside a graph), and the time the bytes of x, y, and each A and B
 // used once take at 5.1 TB/s: one token 4096 x 4096 rank 16 4.8 (0.1; a launch alone is
@@ -301,13 +301,12 @@ __global__ __launch_bounds__(64 * dec_waves(FUSED)) void k_lora_dec(LoraArgs a) 
 
 // ---- prompts ------------------------------------------------------------------
 
-// N values that sum to x, each exact in bf16 (x's bits from the top, 8 at a
-// time: N = 3 holds all 24, N = 2 x to 2^-16), as fp32 with the low half clear.
-// inf and NaN stay in the first.
-template <int N>
-__device__ __forceinline__ void split_bf16(float x, float (&s)[N]) {
+// NS values that sum to x, each exact in bf16 (x's 24 bits from the top, 8 at a
+// time), as fp32 with the low half clear.  inf and NaN stay in the first.
+constexpr int NS = 3;
+__device__ __forceinline__ void split_bf16(float x, float (&s)[NS]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < NS; ++i) {
     s[i] = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
     x = x == s[i] ? 0.0f : x - s[i];
   }
@@ -425,11 +424,11 @@ struct PanelF32 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i * 4 + lane / 16, piece = (lane & 15) >> 1;
-      float e[4][3];
+      float e[4][NS];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split_bf16(__uint_as_float(v[i][j]), e[j]);
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
+      for (int s = 0; s < NS; ++s) {
         u32x2 w = {pack_hi(e[0][s], e[1][s]), pack_hi(e[2][s], e[3][s])};
         u32x4 *row = buf + s * 128 + r * 8;
         ((u32x2 *)(row + (piece ^ Panel<CK>::swz(r))))[lane & 1] = w;
@@ -457,22 +456,26 @@ enum { STAGES_VY, STAGES_V, STAGES_Y };
 constexpr int tile_waves(int stages) { return stages == STAGES_Y ? 4 : 8; }
 // Two workgroups a CU (128 registers) where they fit: a tile with a second adapter
 // then need not wait for a first round.  4096 tokens of 24 requests, 4096 x 4096, rank
-// 64 44.4 us (46 with one), 8192 tokens of 30 79 (88).
-constexpr bool tile_two(int lp, bool yf32) { return lp <= 6 || (lp == 8 && !yf32); }
+// 64 44.4 us (46 with one), 8192 tokens of 30 79 (88).  Ranks 49 to 64 with y in single
+// values fit only with v's parts read from LDS for every product: 4096 x 4097 50 to 56
+// (55 to 57 with one), 2048 tokens of 12, 2048 x 2049, rank 56 22.5 (18.3).
+constexpr bool tile_two(int lp, bool yf32, bool vec) {
+  return lp <= 6 || (lp == 8 && !yf32 && vec);
+}
 // waves a SIMD holds: of STAGES_Y the LDS allows three workgroups, from 65 ranks two
-constexpr int tile_occupancy(int stages, int lp, bool yf32) {
-  return stages == STAGES_Y ? (lp <= 8 ? 3 : 2) : tile_two(lp, yf32) ? 4 : 2;
+constexpr int tile_occupancy(int stages, int lp, bool yf32, bool vec) {
+  return stages == STAGES_Y ? (lp <= 8 ? 3 : 2) : tile_two(lp, yf32, vec) ? 4 : 2;
 }
 template <int STAGES, int LP, bool XF32, bool YF32, bool VEC>
-__global__ __launch_bounds__(64 * tile_waves(STAGES), tile_occupancy(STAGES, LP, YF32)) void k_lora_tile(
-    LoraArgs a) {
+__global__ __launch_bounds__(64 * tile_waves(STAGES),
+                             tile_occupancy(STAGES, LP, YF32, VEC)) void k_lora_tile(LoraArgs a) {
   constexpr int T_WAVES = tile_waves(STAGES);
   // blocks of 16 rows of A (4 also for 33 to 48 rows: two panels in flight divide them)
   constexpr int NRB = LP <= 2 ? 1 : LP == 6 ? 4 : LP / 2;
-  constexpr int NRK = (NRB + 1) / 2, NS = YF32 ? 3 : 2;
-  constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? 3 : 1;
+  constexpr int NRK = (NRB + 1) / 2;
+  constexpr int CK = XF32 ? 64 : 128, KS = CK / 32, NX = XF32 ? NS : 1;
   // panels of A in flight; a block's place among them is the same in every chunk
-  constexpr int RING = NRB < 3 ? NRB : tile_two(LP, YF32) ? 2 : NRB % 4 ? 3 : 4;
+  constexpr int RING = NRB < 3 ? NRB : tile_two(LP, YF32, VEC) ? 2 : NRB % 4 ? 3 : 4;
   static_assert(NRB % RING == 0, "");
   constexpr int STAGE = NRK <= 2 ? 512 : NRK * 256;  // 16-byte pieces of a wave's LDS
   constexpr int XPART = XF32 ? 384 : 256;  // the x panel's share of it

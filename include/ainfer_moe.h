@@ -468,11 +468,9 @@ int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logit
  * may name adapters in any order.  Rows r >= rank_a of a and columns
  * r >= rank_a of b may hold anything, and so may unused adapters; an infinity or
  * NaN in use gives its tokens infinities or NaN, and no other token.  x, a and b
- * enter exactly; v and the products are fp32 sums and v is scaled in fp32.  It
- * enters the second product in fp32 up to 256 tokens, above as the sum of three
- * bf16 values (its 24 bits) where y is fp32, of two (2^-16 of it) where y is bf16;
- * y is rounded once.  The same call gives the same bits; calls of other token
- * counts add in other orders.  No reference counterpart (the reference serves one
+ * enter exactly; v and the products are fp32 sums and v is scaled in fp32 and enters
+ * the second product with its 24 bits; y is rounded once.  The same call gives the
+ * same bits; calls of other token counts add in other orders.  No reference counterpart (the reference serves one
  * model to one request). */
 #define AINFER_LORA_MAX_PROJ 4
 typedef struct ainfer_moe_lora {
