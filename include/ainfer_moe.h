@@ -417,8 +417,10 @@ int ainfer_moe_set_strict(int32_t on);
  *   masked e    logit_e <= the lowest finite value of its type, or NaN, or
  *               bias_e NaN or -inf
  *   s_e         SIGMOID 1 / (1 + exp(-logit_e)); SOFTMAX exp(logit_e) / sum
- *               of exp over the unmasked experts; a logit of +inf counts as
- *               the largest finite one
+ *               of exp over the experts whose logit is not masked (a bias, one
+ *               of -inf or NaN too, takes part in the selection only and
+ *               leaves every score as it is); a logit of +inf counts as the
+ *               largest finite one
  *   key_e       logit_e without a bias (both scores rise with it), s_e +
  *               bias_e with one (bias clamped to +-1e38), in the order of the
  *               64-bit values
