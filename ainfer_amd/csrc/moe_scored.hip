@@ -145,9 +145,9 @@ constexpr float SIG_ABS = 0x1p-22f, SOFT_REL = 0x1.2p-19f;
 constexpr float Z_REL = 0x1.1p-19f;  // of Z and p = e / Z in fp64: (8.8 + 5.5 + 1) 2^-23
 constexpr float BIAS_MOST = 1e38f;
 
-// a logit as the definition takes it: -inf where masked, +inf the largest
+// a logit as the definition takes it: -inf where masked, +inf the largest of its type
 __device__ __forceinline__ float clean_logit(float x, float lowest) {
-  return x > lowest ? fminf(x, 3.402823466e38f) : neg_inf();
+  return x > lowest ? fminf(x, -lowest) : neg_inf();
 }
 __device__ __forceinline__ float clean_bias(float b) {
   return b > neg_inf() ? fminf(fmaxf(b, -BIAS_MOST), BIAS_MOST) : neg_inf();

@@ -420,7 +420,7 @@ int ainfer_moe_set_strict(int32_t on);
  *               of exp over the experts whose logit is not masked (a bias, one
  *               of -inf or NaN too, takes part in the selection only and
  *               leaves every score as it is); a logit of +inf counts as the
- *               largest finite one
+ *               largest finite value of its type
  *   key_e       logit_e without a bias (both scores rise with it), s_e +
  *               bias_e with one (bias clamped to +-1e38), in the order of the
  *               64-bit values

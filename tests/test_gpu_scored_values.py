@@ -44,3 +44,16 @@ def test_a_bias_selects_and_changes_no_score(torch):
     row = [math.log(v) for v in (3.5, 0.5, 4.0, 8.0)]
     check(torch, row, [0.0, 0.0, 0.1, -INF], 1, SOFT, [(2, 0.25)], G=2, top=1)
     check(torch, row, [0.03, 0.0, 0.0, -INF], 1, SOFT, [(0, 0.21875)], G=2, top=1, gscore=GTOP2)
+
+
+@pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
+def test_an_infinite_logit_is_the_largest_of_its_type(torch, dtype):
+    """It ties with the largest finite value, the lower index first."""
+    most = torch.finfo(getattr(torch, dtype)).max
+    for rest in (0, 5, 300):
+        row = [most, INF, most] + [0.0] * rest
+        for score, w in ((SOFT, 1 / 3), (SIG, 1.0)):
+            check(torch, row, None, 2, score, [(0, w), (1, w)], dtype=dtype)
+            check(torch, row, [0.0] * len(row), 2, score, [(0, w), (1, w)], dtype=dtype)
+            check(torch, row[1:], None, 2, score, [(0, w if score == SIG else 1 / 2),
+                                                   (1, w if score == SIG else 1 / 2)], dtype=dtype)
