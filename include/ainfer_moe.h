@@ -434,8 +434,10 @@ int ainfer_moe_set_strict(int32_t on);
  *               lower index first, and only where fewer than top_k are left
  *   topk_w[t][j] scale * s, or scale * s / (sum of the selected s) with
  *               renormalize; 0 for a masked expert, also where all are masked
- * Scores and sums are fp32 (weights within 2^-16 of the formula's, relative,
- * where they are not below 2^-80 of the largest); where two keys or group values
+ * Scores and sums are fp32.  Weights are within 2^-16 of the formula's, relative;
+ * with renormalize those below 2^-80 of the largest may be 0 instead, without it
+ * those of a score below 2^-126 (fp32's smallest normal value: a sigmoid from a
+ * logit of -87.4 down), whatever scale is.  Where two keys or group values
  * are too near for fp32 the comparison is redone in fp64, so topk_idx does not
  * depend on the size of the call.  The rows are what
  * ainfer_moe_dispatch, _experts and _combine take.  No reference counterpart

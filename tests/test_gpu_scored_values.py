@@ -57,3 +57,27 @@ def test_an_infinite_logit_is_the_largest_of_its_type(torch, dtype):
             check(torch, row, [0.0] * len(row), 2, score, [(0, w), (1, w)], dtype=dtype)
             check(torch, row[1:], None, 2, score, [(0, w if score == SIG else 1 / 2),
                                                    (1, w if score == SIG else 1 / 2)], dtype=dtype)
+
+
+def test_scores_at_the_end_of_fp32(torch):
+    """Not renormalised: full relative accuracy down to 2^-126, below it the weight may
+    be 0 times scale, which is off by less than 2^-126 of it."""
+    low = 2.0 ** -126
+
+    def sig(l):
+        return 1 / (1 + math.exp(-l))
+
+    for scale in (1.0, 2.0 ** 100):
+        check(torch, [-87.0, -86.5, -300.0, -80.0], None, 3, SIG,
+              [(3, sig(-80.0) * scale), (1, sig(-86.5) * scale), (0, sig(-87.0) * scale)], scale=scale)
+        check(torch, [-88.5, -90.0, -100.0, -88.0], None, 4, SIG,
+              [(e, sig(l) * scale) for e, l in ((3, -88.0), (0, -88.5), (1, -90.0), (2, -100.0))],
+              scale=scale, atol=low * scale)
+        check(torch, [-87.0, 0.0, -40.0], None, 3, SOFT,
+              [(1, scale), (2, math.exp(-40.0) * scale), (0, math.exp(-87.0) * scale)], scale=scale)
+        check(torch, [-88.0, 0.0, -103.0], None, 3, SOFT,
+              [(1, scale), (0, math.exp(-88.0) * scale), (2, math.exp(-103.0) * scale)],
+              scale=scale, atol=low * scale)
+    # renormalised, such scores keep their ratios
+    check(torch, [-89.0, -90.0], None, 2, SIG, [(0, 1 / (1 + math.exp(-1))),
+                                                (1, 1 / (1 + math.exp(1)))], renorm=1)
