@@ -701,6 +701,11 @@ int do_route(const ainfer_moe_shape *s, const ainfer_moe_weights *w, const void 
 bool mis(const void *p, uintptr_t align) { return ((uintptr_t)p & (align - 1)) != 0; }
 bool is_act(int32_t dtype) { return dtype == AINFER_ACT_F32 || dtype == AINFER_ACT_BF16; }
 int act_size(int32_t dtype) { return dtype == AINFER_ACT_F32 ? 4 : 2; }
+// two runs of bytes with one in common
+bool meet(const void *p, size_t n, const void *q, size_t m) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return p && q && (a < b ? b - a < n : a - b < m);
+}
 // row pitches (in elements) whose products with a token count stay far from 2^63
 constexpr int64_t MAX_LD = (int64_t)1 << 40;
 
@@ -1169,8 +1174,12 @@ int ainfer_moe_route_scored(const ainfer_moe_routing *r, const void *logits, int
   if (T == 0) return AINFER_OK;
   if (!logits || !topk_idx || !topk_w) return AINFER_ERR_NULL;
   if (ld < r->n_experts || ld > MAX_LD || mis(logits, act_size(logits_dtype)) || mis(bias, 4) ||
-      mis(topk_idx, 4) || mis(topk_w, 4) || (const void *)topk_idx == topk_w ||
-      logits == topk_idx || logits == topk_w)
+      mis(topk_idx, 4) || mis(topk_w, 4))
+    return AINFER_ERR_ARG;
+  // logits [T][E] may have a pitch, with other rows between theirs; the others are whole
+  const size_t out = (size_t)T * r->top_k * 4, all = (size_t)r->n_experts * 4;
+  if (meet(topk_idx, out, topk_w, out) || meet(bias, all, topk_idx, out) ||
+      meet(bias, all, topk_w, out) || logits == topk_idx || logits == topk_w)
     return AINFER_ERR_ARG;
   HIP_TRY(launch_route_scored(*r, logits, logits_dtype, ld, bias, T, topk_idx, topk_w,
                               (hipStream_t)stream));
@@ -1201,8 +1210,15 @@ int ainfer_moe_lora_apply(const ainfer_moe_lora *l, const void *x, int64_t x_ld,
         y_ld[p] > MAX_LD)
       return AINFER_ERR_ARG;
   if (mis(ws, 256) || ws_bytes < lora_workspace_bytes(*l, T)) return AINFER_ERR_WORKSPACE;
+  // what is written (every y, the workspace) at the address of another operand
+  auto read = [&](const void *out) {
+    bool hit = out == x || out == token_adapter || out == l->ranks || out == l->scales;
+    for (int p = 0; p < l->n_proj; ++p) hit |= out == l->a[p] || out == l->b[p];
+    return hit;
+  };
+  if (read(ws)) return AINFER_ERR_ARG;
   for (int p = 0; p < l->n_proj; ++p) {
-    if (y[p] == x || y[p] == ws || ws == x) return AINFER_ERR_ARG;
+    if (read(y[p]) || y[p] == ws) return AINFER_ERR_ARG;
     for (int q = 0; q < p; ++q)
       if (y[p] == y[q]) return AINFER_ERR_ARG;
   }

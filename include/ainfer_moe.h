@@ -456,7 +456,8 @@ typedef struct ainfer_moe_routing {
 } ainfer_moe_routing;
 /* logits [T] rows of E values (AINFER_ACT_F32 or AINFER_ACT_BF16), row t at
  * t * ld elements (ld >= E); bias [E] fp32 or NULL; topk_idx, topk_w
- * [T][top_k], none of the three overlapping.  No workspace. */
+ * [T][top_k].  Neither of these two may overlap the other, bias (both refused) or
+ * logits (refused at the same address).  No workspace. */
 int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logits,
                             int32_t logits_dtype, int64_t ld, const float *bias, int32_t T,
                             int32_t *topk_idx, float *topk_w, void *stream);
@@ -497,8 +498,8 @@ typedef struct ainfer_moe_lora {
 size_t ainfer_moe_lora_workspace_bytes(const ainfer_moe_lora *lora, int32_t max_tokens);
 /* x: T rows of K values, row t at t * x_ld elements, 16-byte aligned rows;
  * token_adapter [T] int32; y[p]: T rows of M_p values at t * y_ld[p] elements
- * (aligned to their type; rows must not overlap x, a, b or each other: the same
- * address for two of x, the y and the workspace is refused). */
+ * (aligned to their type).  No y may overlap another, nor a y or the workspace
+ * anything that is read: one that starts at another operand's address is refused. */
 int ainfer_moe_lora_apply(const ainfer_moe_lora *lora, const void *x, int64_t x_ld,
                           const int32_t *token_adapter, int32_t T, void *const *y,
                           const int64_t *y_ld, void *workspace, size_t workspace_bytes,
