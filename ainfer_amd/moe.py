@@ -154,9 +154,11 @@ class MoeLayer:
         """forward with scored routing: the layer's router logits (its
         router_bias, where it has one, is part of them) -> route_scored(routing,
         logits, bias) -> experts -> combine, in steps of CHUNK_TOKENS (ws: for
-        that many tokens, or T where it is less).  shared:
-        [T][H] bf16 rows that take the place of the shared expert's (for
-        example shared_adapted's)."""
+        that many tokens, or T where it is less).  W4A16 layers only, as
+        ainfer_moe_experts.  shared: [T][H] bf16 rows that take the place of the
+        shared expert's (for example shared_adapted's)."""
+        if self.shape.precision != L.PRECISION_W4A16:
+            raise L.MoeError("forward_scored: a W4A16 layer (the expert stage has no W4A8 form)")
         if (routing.n_experts, routing.top_k) != (self.shape.n_experts, self.shape.top_k):
             raise L.MoeError("routing: the layer's n_experts and top_k")
         T, H = x.shape[0], self.shape.hidden
