@@ -161,11 +161,13 @@ class MoeLayer:
             raise L.MoeError("forward_scored: a W4A16 layer (the expert stage has no W4A8 form)")
         if (routing.n_experts, routing.top_k) != (self.shape.n_experts, self.shape.top_k):
             raise L.MoeError("routing: the layer's n_experts and top_k")
-        T, H = x.shape[0], self.shape.hidden
+        T, H, dev = x.shape[0], self.shape.hidden, x.get_device()
         for t in (x, y, resid, shared):
             if t is not None and not (t.shape == (T, H) and t.dtype == torch.bfloat16
-                                      and t.is_contiguous() and t.device == x.device):
+                                      and t.is_contiguous() and t.get_device() == dev >= 0):
                 raise L.MoeError("x, y, resid and shared: contiguous [T][H] bf16 on one device")
+        if ws.get_device() != dev:
+            raise L.MoeError("ws: on the inputs' device")
         if shared is not None and self.shape.shared_inter == 0:
             raise L.MoeError("shared: the layer has no shared expert")
         with _on(stream):

@@ -40,3 +40,33 @@ def test_w4a8_layer(world):
     with pytest.raises(L.MoeError, match="W4A16"):
         layer.forward_scored(rows, rows.clone(), None, routing)
     assert calls == []
+
+
+class OnDevice:
+    """Stands for a [rows][cols] tensor on a GPU of some index."""
+
+    def __init__(self, dev, rows=3, cols=128, dtype=torch.bfloat16):
+        self.dev, self.shape, self.dtype = dev, (rows, cols) if cols else (rows,), dtype
+
+    def get_device(self):
+        return self.dev
+
+    def is_contiguous(self):
+        return True
+
+    def __getitem__(self, rows):
+        return self
+
+
+def test_host_tensors(world):
+    """The stages take addresses: a host one would reach the GPU."""
+    L, moe, layer, calls, rows, routing = world
+    host = rows.clone()
+    gpu = OnDevice(0)
+    for kw in (dict(x=host, y=host, ws=host), dict(x=gpu, y=host, ws=gpu),
+               dict(x=gpu, y=gpu, ws=host), dict(x=gpu, y=OnDevice(1), ws=gpu),
+               dict(x=gpu, y=gpu, ws=OnDevice(1)), dict(x=gpu, y=gpu, ws=gpu, shared=host),
+               dict(x=gpu, y=gpu, ws=gpu, resid=OnDevice(1))):
+        with pytest.raises(L.MoeError):
+            layer.forward_scored(routing=routing, **kw)
+        assert calls == [], kw
