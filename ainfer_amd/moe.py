@@ -170,7 +170,7 @@ class MoeLayer:
             raise L.MoeError("ws: on the inputs' device")
         if shared is not None and self.shape.shared_inter == 0:
             raise L.MoeError("shared: the layer has no shared expert")
-        with _on(stream):
+        with torch.cuda.device(dev), _on(stream):
             for t in range(0, T, L.CHUNK_TOKENS):
                 c = slice(t, t + L.CHUNK_TOKENS)
                 idx, w, sg, logits = self.route(x[c], ws, want_logits=True)

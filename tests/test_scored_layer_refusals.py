@@ -70,3 +70,20 @@ def test_host_tensors(world):
         with pytest.raises(L.MoeError):
             layer.forward_scored(routing=routing, **kw)
         assert calls == [], kw
+
+
+def test_runs_on_the_tensors_device(world, monkeypatch):
+    """Every stage goes to the current stream of the device that x is on, whichever is
+    the current one."""
+    L, moe, layer, calls, rows, routing = world
+
+    @contextlib.contextmanager
+    def device(dev):
+        calls.append(dev)
+        yield
+        calls.append("left")
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    x = OnDevice(1)
+    assert layer.forward_scored(x, x, x, routing) is x
+    assert calls == [1, "route", "route_scored", "experts", "combine", "left"]
