@@ -168,6 +168,10 @@ class MoeLayer:
                 raise L.MoeError("x, y, resid and shared: contiguous [T][H] bf16 on one device")
         if ws.get_device() != dev:
             raise L.MoeError("ws: on the inputs' device")
+        if bias is not None:
+            _vector(bias, "bias", torch.float32, routing.n_experts, dev)
+        L.check(L.lib().ainfer_moe_route_scored(C.byref(routing), None, L.ACT_F32, 0, None, 0, None,
+                                                None, None))  # no tokens: routing's own checks
         if shared is not None and self.shape.shared_inter == 0:
             raise L.MoeError("shared: the layer has no shared expert")
         with torch.cuda.device(dev), _on(stream):

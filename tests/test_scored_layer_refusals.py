@@ -72,6 +72,23 @@ def test_host_tensors(world):
         assert calls == [], kw
 
 
+def test_routing_and_bias_are_checked_first(world):
+    L, moe, layer, calls, rows, routing = world
+    gpu = OnDevice(0)
+    for bad in (dict(n_groups=3), dict(score=7), dict(scale=float("nan")), dict(top_groups=2)):
+        r = L.Routing.from_buffer_copy(routing)
+        for name, v in bad.items():
+            setattr(r, name, v)
+        with pytest.raises(L.MoeError):
+            layer.forward_scored(gpu, gpu, gpu, r)
+        assert calls == [], bad
+    for bias in (torch.zeros(8), OnDevice(1, 8, 0, torch.float32), OnDevice(0, 7, 0, torch.float32),
+                 OnDevice(0, 8, 0)):
+        with pytest.raises(L.MoeError):
+            layer.forward_scored(gpu, gpu, gpu, routing, bias)
+        assert calls == []
+
+
 def test_runs_on_the_tensors_device(world, monkeypatch):
     """Every stage goes to the current stream of the device that x is on, whichever is
     the current one."""
