@@ -150,13 +150,17 @@ class MoeLayer:
                                            _ptr(resid), _ptr(y), T, _stream(stream)))
         return y
 
-    def forward_scored(self, x, y, ws, routing, bias=None, resid=None, shared=None, stream=None):
+    def forward_scored(self, x, y, ws, routing, bias=None, resid=None, shared=None, stream=None,
+                       shared_tokens=None):
         """forward with scored routing: the layer's router logits (its
         router_bias, where it has one, is part of them) -> route_scored(routing,
         logits, bias) -> experts -> combine, in steps of CHUNK_TOKENS (ws: for
         that many tokens, or T where it is less).  W4A16 layers only, as
         ainfer_moe_experts.  shared: [T][H] bf16 rows that take the place of the
-        shared expert's (for example shared_adapted's)."""
+        shared expert's (for example shared_adapted's, whose activations are
+        int8); shared_tokens: [T] bool, the tokens they do so for (token_adapter >= 0,
+        say, so that a token without an adapter has the layer's own W4A16 row
+        whoever shares its batch), None for all."""
         if self.shape.precision != L.PRECISION_W4A16:
             raise L.MoeError("forward_scored: a W4A16 layer (the expert stage has no W4A8 form)")
         if (routing.n_experts, routing.top_k) != (self.shape.n_experts, self.shape.top_k):
@@ -174,13 +178,20 @@ class MoeLayer:
                                                 None, None))  # no tokens: routing's own checks
         if shared is not None and self.shape.shared_inter == 0:
             raise L.MoeError("shared: the layer has no shared expert")
+        if shared_tokens is not None:
+            if shared is None:
+                raise L.MoeError("shared_tokens: the tokens of shared")
+            _vector(shared_tokens, "shared_tokens", torch.bool, T, dev)
         with torch.cuda.device(dev), _on(stream):
             for t in range(0, T, L.CHUNK_TOKENS):
                 c = slice(t, t + L.CHUNK_TOKENS)
                 idx, w, sg, logits = self.route(x[c], ws, want_logits=True)
                 route_scored(routing, logits, bias, out=(idx, w))
                 o = self.experts(x[c], idx, ws)
-                if shared is not None:
+                if shared_tokens is not None:
+                    own = o[idx.numel():]
+                    torch.where(shared_tokens[c, None], shared[c], own, out=own)
+                elif shared is not None:
                     o[idx.numel():].copy_(shared[c])
                 self.combine(o, w, sg, y[c], resid[c] if resid is not None else None)
         return y
@@ -189,6 +200,10 @@ class MoeLayer:
         """The shared expert's rows [T][H] (bf16) with each token's adapters on
         its three projections: x quantised to int8 groups, gate and up as
         ainfer_moe_int4_gemv_i8, their adapters, SiLU-mul, the same for down.
+        That is W4A8 arithmetic whatever the layer's precision: rows of a W4A16 layer
+        differ from its own shared expert's by the rounding of x and act to int8,
+        without an adapter too (forward_scored's shared_tokens keeps the
+        layer's own for those).
         gate_up (two projections, x bf16, y fp32) and down (x and y fp32):
         LoraAdapters or None; lora_ws: a workspace large enough for both."""
         sh, wt = self.shape, self.weights
