@@ -19,13 +19,16 @@
 // used once take at 5.1 TB/s: one token 4096 x 4096 rank 16 4.8 (0.1; a launch alone is
 // 2.5), 64 tokens 4096 x (1024 + 1024) rank 16 6.1 (2.2), 16 tokens 5120 x 17408 rank
 // 64 14.8 (8.3), 1003 tokens of 7 requests 1024 x 4096 rank 8 in fp32 12.1 (7.3), 4096
-// tokens 4096 x 4096 of 24 requests rank 32 28 (19.3), rank 64 40 (21.5), of one
-// request rank 32 21 (19.7).
+// tokens 4096 x 4096 of 24 requests rank 32 29 (19.3), rank 64 45 (21.5), of one
+// request rank 32 21 (19.7), 1024 tokens of 16 requests rank 128 34 (10).
 //
 // What bounds it: batches, the two dependent sweeps over A and B (an HBM latency each)
 // and the bytes of B.  Prompts, y's and x's bytes while a tile has one adapter; a tile
 // that lies across two requests is two workgroups, and the second shares its CU with
-// another tile's: it ends 5 us (rank 16) to 10 (rank 64) after the others.
+// another tile's: it ends 5 us (rank 16) to 10 (rank 64) after the others.  From 33 ranks
+// on, A and B: every tile of 16 tokens takes its adapter's whole rows through L2 and LDS
+// (2 MB at rank 128, 1.3 M reads of 128 bytes a call of 1024 tokens) for one column block
+// of the MFMAs.
 #include "moe_common.h"
 #include "moe_internal.h"
 

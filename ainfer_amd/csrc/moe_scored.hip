@@ -27,11 +27,13 @@
 //
 // k_route_many: many tokens of few experts, four a wave.
 //
-// What bounds it: the instructions issued.  65536 tokens of 512 experts with a bias
-// (softmax, top-10) take 58 us where their bytes take 27: 308 vector and 283 scalar
-// instructions a token, next token's logits in flight meanwhile; 64 experts 19.  One
-// token takes 4.4 us, of which a launch alone is 2.5; 4096 tokens of 256 experts in 8
-// groups 7.1.
+// What bounds it.  65536 tokens of 512 experts with a bias (softmax, top-10) take 58 us:
+// 36 to issue 308 vector instructions a token, meanwhile the bytes' 27 (the next token's
+// logits are in flight), and the rest latency: 283 scalar instructions a token, most of
+// which wait for the one before, at five waves a SIMD.  k_route_many issues vector
+// instructions most of its time: 64 experts with a bias 19 us, 17 of them (148 a token),
+// 60 without 9.0, 7 (62); their bytes 4.  One token takes 4.4 us, of which a launch alone
+// is 2.5; 4096 tokens of 256 experts in 8 groups 7.1.
 #include "moe_common.h"
 #include "moe_internal.h"
 #include "moe_topk.h"
@@ -1032,7 +1034,7 @@ hipError_t launch_route_scored(const ainfer_moe_routing &r, const void *logits, 
   // T 65536, grids of 2048 and 16384: 512 experts with a bias 64 and 93, without
   // 52 and 45 (bf16, not renormalised 70 and 53), 64 experts 38 and 31.  With 8 experts a
   // lane 1280 are resident at once (about 90 registers): 512 experts softmax 58.2 (2048
-  // 60.3), sigmoid 50.2 (53.2); 256 experts in 8 groups 57 (2048 56)
+  // 60.3), sigmoid 50.2 (53.2)
   const int most = !bias ? 16384 : need > 4 && need <= 8 ? 1280 : 2048;
   const int grid = blocks < most ? blocks : most;
   if (need <= 1) launch_nv<1>(a, grid, soft, s);
