@@ -475,8 +475,8 @@ int ainfer_moe_route_scored(const ainfer_moe_routing *routing, const void *logit
  * NaN in use gives its tokens infinities or NaN, and no other token.  x, a and b
  * enter exactly; v and the products are fp32 sums and v is scaled in fp32 and enters
  * the second product with its 24 bits; y is rounded once.  The same call gives the
- * same bits; calls of other token counts add in other orders.  No reference counterpart (the reference serves one
- * model to one request). */
+ * same bits; calls of other token counts add in other orders.  No reference
+ * counterpart (the reference serves one model to one request). */
 #define AINFER_LORA_MAX_PROJ 4
 typedef struct ainfer_moe_lora {
   int32_t n_adapters;  /* N, 1..4096                                         */
