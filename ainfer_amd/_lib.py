@@ -20,6 +20,8 @@ ACT_F32, ACT_BF16 = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
 LORA_MAX_PROJ = 4
+FP8_SCALE_ANY, FP8_SCALE_POW2 = 0, 1
+MAX_ROWS = 1 << 21
 FILL_BYTES, FILL_BF16_NORMAL, FILL_FP16_ABSNORMAL, FILL_BF16_ABSNORMAL = 0, 1, 2, 3
 MAX_TOKENS = 65536
 CHUNK_TOKENS = 4096
@@ -37,6 +39,10 @@ EXPORTS = (
     "ainfer_moe_act_quant_i8", "ainfer_moe_int4_gemv_i8",
     "ainfer_moe_route_scored", "ainfer_moe_lora_workspace_bytes", "ainfer_moe_lora_apply",
     "ainfer_moe_silu_mul",
+    "ainfer_moe_act_quant_fp8", "ainfer_moe_weight_quant_fp8", "ainfer_moe_fp8_product",
+    "ainfer_moe_silu_mul_fp8", "ainfer_moe_silu_mul_backward",
+    "ainfer_moe_sort_workspace_bytes", "ainfer_moe_sort_rows", "ainfer_moe_unpermute",
+    "ainfer_moe_unpermute_backward",
     "ainfer_moe_profile_enable", "ainfer_moe_profile_read", "ainfer_moe_profile_kernel", "ainfer_moe_debug_spin_limit",
     "ainfer_moe_set_strict",
     "ainfer_moe_mfma_probe", "ainfer_moe_read_probe",
@@ -73,6 +79,18 @@ class Lora(C.Structure):
                 ("out", C.c_int32 * LORA_MAX_PROJ), ("a", C.c_void_p * LORA_MAX_PROJ),
                 ("b", C.c_void_p * LORA_MAX_PROJ), ("ranks", C.c_void_p),
                 ("scales", C.c_void_p)]
+
+
+class Fp8(C.Structure):
+    """Weights in e4m3 with a scale for each 128 x 128 block (ainfer_moe_fp8)."""
+    _fields_ = [("n_experts", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32),
+                ("y_dtype", C.c_int32), ("w", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class Sorting(C.Structure):
+    """Token rows sorted by expert (ainfer_moe_sorting)."""
+    _fields_ = [("n_experts", C.c_int32), ("top_k", C.c_int32), ("hidden", C.c_int32),
+                ("x_dtype", C.c_int32), ("fp8", C.c_int32), ("scale_kind", C.c_int32)]
 
 
 class MoeError(RuntimeError):
@@ -124,6 +142,20 @@ def lib():
         L.ainfer_moe_lora_apply.argtypes = [C.POINTER(Lora), P, I64, P, I32, C.POINTER(P),
                                             C.POINTER(I64), P, SZ, P]
         L.ainfer_moe_silu_mul.argtypes = [P, I64, P, I64, I32, I32, I32, P, I64, I32, P]
+        L.ainfer_moe_act_quant_fp8.argtypes = [P, I64, I32, P, I32, I32, I32, P, I64, P, P]
+        L.ainfer_moe_weight_quant_fp8.argtypes = [P, I32, I32, I32, I32, I32, P, P, P]
+        L.ainfer_moe_fp8_product.argtypes = [C.POINTER(Fp8), P, I64, P, P, I32, P, I64, P]
+        L.ainfer_moe_silu_mul_fp8.argtypes = [P, I64, P, I64, I32, P, I32, I32, I32, P, I64, P, P]
+        L.ainfer_moe_silu_mul_backward.argtypes = [P, I64, P, I64, P, I64, I32, P, I32, I32, P, I64,
+                                                   P, I64, P]
+        L.ainfer_moe_sort_workspace_bytes.restype = SZ
+        L.ainfer_moe_sort_workspace_bytes.argtypes = [I32, I32, I32]
+        L.ainfer_moe_sort_rows.argtypes = [C.POINTER(Sorting), P, I64, P, I32, P, P, P, I64, P, P,
+                                           SZ, P]
+        L.ainfer_moe_unpermute.argtypes = [P, I64, I32, I32, P, P, I32, I32, I32, P, I64, P, I64,
+                                           I32, P]
+        L.ainfer_moe_unpermute_backward.argtypes = [P, I64, I32, P, I64, I32, I32, P, P, I32, I32,
+                                                    I32, P, I64, P, P]
         L.ainfer_moe_profile_enable.argtypes = [I32]
         L.ainfer_moe_profile_kernel.argtypes = [C.POINTER(C.c_float), C.POINTER(I32)]
         L.ainfer_moe_mfma_probe.argtypes = [I32, I32, I32, P, C.POINTER(C.c_float)]

@@ -720,6 +720,41 @@ int check_lora(const ainfer_moe_lora *l) {
   if (!is_act(l->x_dtype) || !is_act(l->y_dtype)) return AINFER_ERR_ARG;
   return AINFER_OK;
 }
+
+// ---- experts in 8-bit floating point, tokens sorted by expert ------------------
+// the same for up to AINFER_MOE_MAX_ROWS rows
+constexpr int64_t MAX_ROW_LD = (int64_t)1 << 36;
+bool is_scale_kind(int32_t kind) {
+  return kind == AINFER_FP8_SCALE_ANY || kind == AINFER_FP8_SCALE_POW2;
+}
+// a pitch that fits rows of `cols` elements
+bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > MAX_ROW_LD; }
+// Whether `rows` rows that are written meet n bytes at p: all of their bytes where
+// the rows are whole, their first address where a pitch leaves room between them.
+bool over(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, const void *p,
+          size_t n) {
+  if (!out || !p) return false;
+  if (rows == 1 || ld == cols) return meet(out, (size_t)(rows * cols * size), p, n);
+  return out == p;
+}
+int check_fp8(const ainfer_moe_fp8 *w) {
+  if (!w) return AINFER_ERR_NULL;
+  if (w->n_experts < 1 || w->n_experts > 1024 || w->rows < 1 || w->rows > (1 << 20) ||
+      w->cols < 16 || w->cols > 65536 || w->cols % 16 ||
+      (int64_t)w->n_experts * w->rows * w->cols > (int64_t)1 << 38)
+    return AINFER_ERR_SHAPE;
+  if (!is_act(w->y_dtype)) return AINFER_ERR_ARG;
+  return AINFER_OK;
+}
+int check_sorting(const ainfer_moe_sorting *s) {
+  if (!s) return AINFER_ERR_NULL;
+  if (s->n_experts < 1 || s->n_experts > 1024 || s->top_k < 1 || s->top_k > 32 ||
+      s->hidden < 1 || s->hidden > 65536 || (s->fp8 && s->hidden % 16))
+    return AINFER_ERR_SHAPE;
+  if (!is_act(s->x_dtype) || (s->fp8 != 0 && s->fp8 != 1) || !is_scale_kind(s->scale_kind))
+    return AINFER_ERR_ARG;
+  return AINFER_OK;
+}
 }  // namespace
 
 extern "C" {
@@ -1244,6 +1279,228 @@ int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64
     return AINFER_ERR_ARG;
   HIP_TRY(launch_silu_rows(gate, gate_ld, up, up_ld, in_dtype, T, I, act, act_ld, act_dtype,
                            (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_silu_mul_backward(const void *dact, int64_t dact_ld, const void *gate,
+                                 int64_t gate_ld, const void *up, int64_t up_ld, int32_t dtype,
+                                 const int32_t *n_live, int32_t N, int32_t I, void *dgate,
+                                 int64_t dgate_ld, void *dup, int64_t dup_ld, void *stream) {
+  if (N < 0 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
+  if (I <= 0 || I > 65536) return AINFER_ERR_SHAPE;
+  if (!is_act(dtype)) return AINFER_ERR_ARG;
+  if (N == 0) return AINFER_OK;
+  if (!dact || !gate || !up || !dgate || !dup) return AINFER_ERR_NULL;
+  const int sz = act_size(dtype);
+  if (bad_ld(dact_ld, I) || bad_ld(gate_ld, I) || bad_ld(up_ld, I) || bad_ld(dgate_ld, I) ||
+      bad_ld(dup_ld, I) || mis(dact, sz) || mis(gate, sz) || mis(up, sz) || mis(dgate, sz) ||
+      mis(dup, sz) || mis(n_live, 4) || dgate == dup)
+    return AINFER_ERR_ARG;
+  // in place only where every element lies on its own input
+  const void *in[3] = {dact, gate, up};
+  const int64_t in_ld[3] = {dact_ld, gate_ld, up_ld};
+  for (int i = 0; i < 3; ++i)
+    if ((in[i] == dgate && N > 1 && in_ld[i] != dgate_ld) ||
+        (in[i] == dup && N > 1 && in_ld[i] != dup_ld))
+      return AINFER_ERR_ARG;
+  if (over(dgate, N, dgate_ld, I, sz, n_live, 4) || over(dup, N, dup_ld, I, sz, n_live, 4))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_silu_backward(dact, dact_ld, gate, gate_ld, up, up_ld, dtype, n_live, N, I, dgate,
+                               dgate_ld, dup, dup_ld, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_act_quant_fp8(const void *x, int64_t x_ld, int32_t x_dtype, const int32_t *n_live,
+                             int32_t N, int32_t K, int32_t scale_kind, uint8_t *q, int64_t q_ld,
+                             float *sq, void *stream) {
+  if (N < 0 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
+  if (K < 16 || K > 65536 || K % 16) return AINFER_ERR_SHAPE;
+  if (!is_act(x_dtype) || !is_scale_kind(scale_kind)) return AINFER_ERR_ARG;
+  if (N == 0) return AINFER_OK;
+  if (!x || !q || !sq) return AINFER_ERR_NULL;
+  const int xsz = act_size(x_dtype);
+  if (bad_ld(x_ld, K) || bad_ld(q_ld, K) || q_ld % 16 || mis(x, xsz) || mis(q, 16) || mis(sq, 4) ||
+      mis(n_live, 4))
+    return AINFER_ERR_ARG;
+  const size_t scales = (size_t)N * ((K + 127) / 128) * 4;
+  if (q == x || (const void *)sq == x || meet(sq, scales, n_live, 4) ||
+      over(x, N, x_ld, K, xsz, sq, scales) || over(q, N, q_ld, K, 1, sq, scales) ||
+      over(q, N, q_ld, K, 1, n_live, 4))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_act_quant_fp8(x, x_ld, x_dtype, n_live, N, K, scale_kind, q, q_ld, sq,
+                               (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,
+                            int32_t in_dtype, const int32_t *n_live, int32_t N, int32_t I,
+                            int32_t scale_kind, uint8_t *q, int64_t q_ld, float *sq,
+                            void *stream) {
+  if (N < 0 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
+  if (I < 16 || I > 65536 || I % 16) return AINFER_ERR_SHAPE;
+  if (!is_act(in_dtype) || !is_scale_kind(scale_kind)) return AINFER_ERR_ARG;
+  if (N == 0) return AINFER_OK;
+  if (!gate || !up || !q || !sq) return AINFER_ERR_NULL;
+  const int sz = act_size(in_dtype);
+  if (bad_ld(gate_ld, I) || bad_ld(up_ld, I) || bad_ld(q_ld, I) || q_ld % 16 || mis(gate, sz) ||
+      mis(up, sz) || mis(q, 16) || mis(sq, 4) || mis(n_live, 4))
+    return AINFER_ERR_ARG;
+  const size_t scales = (size_t)N * ((I + 127) / 128) * 4;
+  if (q == gate || q == up || (const void *)sq == gate || (const void *)sq == up ||
+      meet(sq, scales, n_live, 4) || over(gate, N, gate_ld, I, sz, sq, scales) ||
+      over(up, N, up_ld, I, sz, sq, scales) || over(q, N, q_ld, I, 1, sq, scales) ||
+      over(q, N, q_ld, I, 1, n_live, 4))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_silu_mul_fp8(gate, gate_ld, up, up_ld, in_dtype, n_live, N, I, scale_kind, q, q_ld,
+                              sq, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_weight_quant_fp8(const void *w, int32_t w_dtype, int32_t E, int32_t M, int32_t K,
+                                int32_t scale_kind, uint8_t *q, float *scales, void *stream) {
+  const ainfer_moe_fp8 d = {E, M, K, w_dtype, q, scales};
+  int rc = check_fp8(&d);
+  if (rc) return rc;
+  if (!is_scale_kind(scale_kind)) return AINFER_ERR_ARG;
+  if (!w || !q || !scales) return AINFER_ERR_NULL;
+  if (mis(w, act_size(w_dtype)) || mis(q, 16) || mis(scales, 4)) return AINFER_ERR_ARG;
+  const size_t n = (size_t)E * M * K, sn = (size_t)E * ((M + 127) / 128) * ((K + 127) / 128) * 4;
+  if (meet(w, n * act_size(w_dtype), q, n) || meet(w, n * act_size(w_dtype), scales, sn) ||
+      meet(q, n, scales, sn))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_weight_quant_fp8(w, w_dtype, E, M, K, scale_kind, q, scales, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_ld, const float *sq,
+                           const int32_t *offsets, int32_t N, void *y, int64_t y_ld,
+                           void *stream) {
+  int rc = check_fp8(w);
+  if (rc) return rc;
+  if (N < 0 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
+  if (N == 0) return AINFER_OK;
+  if (!w->w || !w->scales || !q || !sq || !y || (!offsets && w->n_experts != 1))
+    return AINFER_ERR_NULL;
+  const int M = w->rows, K = w->cols, ysz = act_size(w->y_dtype);
+  if (bad_ld(q_ld, K) || q_ld % 16 || bad_ld(y_ld, M) || mis(w->w, 16) || mis(q, 16) ||
+      mis(w->scales, 4) || mis(sq, 4) || mis(offsets, 4) || mis(y, ysz))
+    return AINFER_ERR_ARG;
+  const size_t G = (K + 127) / 128, E = w->n_experts;
+  if (over(y, N, y_ld, M, ysz, w->w, E * M * K) ||
+      over(y, N, y_ld, M, ysz, w->scales, E * ((M + 127) / 128) * G * 4) ||
+      over(y, N, y_ld, M, ysz, sq, N * G * 4) || over(y, N, y_ld, M, ysz, offsets, (E + 1) * 4) ||
+      y == q)
+    return AINFER_ERR_ARG;
+  const Fp8Args a = {w->w, w->scales, q, sq, offsets, y, q_ld, y_ld, w->n_experts, M, K, N};
+  HIP_TRY(launch_fp8_product(a, w->y_dtype, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+size_t ainfer_moe_sort_workspace_bytes(int32_t max_tokens, int32_t top_k, int32_t n_experts) {
+  if (max_tokens < 0 || max_tokens > AINFER_MOE_MAX_TOKENS || top_k < 1 || top_k > 32 ||
+      n_experts < 1 || n_experts > 1024)
+    return 0;
+  return sort_workspace_bytes(max_tokens > 0 ? max_tokens : 1, top_k, n_experts);
+}
+
+int ainfer_moe_sort_rows(const ainfer_moe_sorting *s, const void *x, int64_t x_ld,
+                         const int32_t *topk_idx, int32_t T, int32_t *offsets, int32_t *pos,
+                         void *rows, int64_t rows_ld, float *row_scales, void *ws, size_t ws_bytes,
+                         void *stream) {
+  int rc = check_sorting(s);
+  if (rc) return rc;
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS) return AINFER_ERR_TOKENS;
+  if (!offsets) return AINFER_ERR_NULL;
+  if (mis(offsets, 4)) return AINFER_ERR_ARG;
+  const int k = s->top_k, H = s->hidden, xsz = act_size(s->x_dtype), rsz = s->fp8 ? 1 : xsz;
+  const int64_t P = (int64_t)T * k;
+  const size_t n = (size_t)P * 4, no = ((size_t)s->n_experts + 1) * 4,
+               ns = (size_t)P * ((H + 127) / 128) * 4;
+  if (T > 0) {
+    if (!topk_idx || !pos || !ws || (rows && (!x || (s->fp8 && !row_scales))))
+      return AINFER_ERR_NULL;
+    if (mis(topk_idx, 4) || mis(pos, 4)) return AINFER_ERR_ARG;
+    if (rows && (bad_ld(x_ld, H) || bad_ld(rows_ld, H) || mis(x, xsz) ||
+                 (s->fp8 && (rows_ld % 16 || mis(rows, 16) || mis(row_scales, 4))) || mis(rows, rsz)))
+      return AINFER_ERR_ARG;
+    if (mis(ws, 256) || ws_bytes < sort_workspace_bytes(T, k, s->n_experts))
+      return AINFER_ERR_WORKSPACE;
+    // what is written (offsets, pos, the workspace, rows, their scales) over another operand
+    const size_t nw = sort_workspace_bytes(T, k, s->n_experts);
+    float *sc = rows && s->fp8 ? row_scales : nullptr;
+    if (meet(offsets, no, pos, n) || meet(offsets, no, topk_idx, n) || meet(pos, n, topk_idx, n) ||
+        meet(ws, nw, offsets, no) || meet(ws, nw, pos, n) || meet(ws, nw, topk_idx, n) ||
+        meet(sc, ns, offsets, no) || meet(sc, ns, pos, n) || meet(sc, ns, topk_idx, n) ||
+        meet(sc, ns, ws, nw))
+      return AINFER_ERR_ARG;
+    if (rows) {
+      auto hit = [&](const void *p, size_t bytes) {
+        return over(rows, P, rows_ld, H, rsz, p, bytes) || over(x, T, x_ld, H, xsz, p, bytes);
+      };
+      if (rows == x || hit(offsets, no) || hit(pos, n) || hit(ws, nw) || hit(sc, ns) ||
+          over(rows, P, rows_ld, H, rsz, topk_idx, n) ||
+          (x_ld == H && over(rows, P, rows_ld, H, rsz, x, (size_t)T * H * xsz)))
+        return AINFER_ERR_ARG;
+    }
+  }
+  HIP_TRY(launch_sort_rows(*s, x, x_ld, topk_idx, T, offsets, pos, T > 0 ? rows : nullptr, rows_ld,
+                           row_scales, ws, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_unpermute(const void *rows, int64_t rows_ld, int32_t rows_dtype, int32_t N,
+                         const int32_t *pos, const float *w, int32_t T, int32_t top_k, int32_t H,
+                         const void *resid, int64_t resid_ld, void *y, int64_t y_ld,
+                         int32_t y_dtype, void *stream) {
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS || N < 0 || N > AINFER_MOE_MAX_ROWS)
+    return AINFER_ERR_TOKENS;
+  if (top_k < 1 || top_k > 32 || H < 1 || H > 65536) return AINFER_ERR_SHAPE;
+  if (!is_act(rows_dtype) || !is_act(y_dtype)) return AINFER_ERR_ARG;
+  if (T == 0) return AINFER_OK;
+  if ((!rows && N > 0) || !pos || !y) return AINFER_ERR_NULL;
+  const int rsz = act_size(rows_dtype), ysz = act_size(y_dtype);
+  if (bad_ld(rows_ld, H) || bad_ld(y_ld, H) || (resid && bad_ld(resid_ld, H)) || mis(rows, rsz) ||
+      mis(pos, 4) || mis(w, 4) || mis(resid, ysz) || mis(y, ysz))
+    return AINFER_ERR_ARG;
+  const size_t n = (size_t)T * top_k * 4;
+  if (y == rows || over(y, T, y_ld, H, ysz, pos, n) || over(y, T, y_ld, H, ysz, w, n) ||
+      (rows_ld == H && over(y, T, y_ld, H, ysz, rows, (size_t)N * H * rsz)) ||
+      (resid == y && T > 1 && resid_ld != y_ld))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_unpermute(rows, rows_ld, rows_dtype, N, pos, w, T, top_k, H, resid, resid_ld, y,
+                           y_ld, y_dtype, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
+int ainfer_moe_unpermute_backward(const void *dy, int64_t dy_ld, int32_t dy_dtype, const void *rows,
+                                  int64_t rows_ld, int32_t rows_dtype, int32_t N,
+                                  const int32_t *pos, const float *w, int32_t T, int32_t top_k,
+                                  int32_t H, void *drows, int64_t drows_ld, float *dw,
+                                  void *stream) {
+  if (T < 0 || T > AINFER_MOE_MAX_TOKENS || N < 0 || N > AINFER_MOE_MAX_ROWS)
+    return AINFER_ERR_TOKENS;
+  if (top_k < 1 || top_k > 32 || H < 1 || H > 65536) return AINFER_ERR_SHAPE;
+  if (!is_act(rows_dtype) || !is_act(dy_dtype)) return AINFER_ERR_ARG;
+  if (T == 0 || (!drows && !dw)) return AINFER_OK;
+  if (!dy || !pos || (dw && !rows && N > 0)) return AINFER_ERR_NULL;
+  const int rsz = act_size(rows_dtype), ysz = act_size(dy_dtype);
+  if (bad_ld(dy_ld, H) || (dw && bad_ld(rows_ld, H)) || (drows && bad_ld(drows_ld, H)) ||
+      mis(dy, ysz) || mis(rows, rsz) || mis(drows, rsz) || mis(pos, 4) || mis(w, 4) || mis(dw, 4))
+    return AINFER_ERR_ARG;
+  const size_t n = (size_t)T * top_k * 4;
+  if (meet(dw, n, pos, n) || meet(dw, n, w, n) || over(dy, T, dy_ld, H, ysz, dw, n) ||
+      (dw && N > 0 && over(rows, N, rows_ld, H, rsz, dw, n)) || (drows && drows == dy))
+    return AINFER_ERR_ARG;
+  if (drows && N > 0) {
+    if (over(drows, N, drows_ld, H, rsz, pos, n) || over(drows, N, drows_ld, H, rsz, w, n) ||
+        over(drows, N, drows_ld, H, rsz, dw, n) ||
+        (dw && drows == rows) ||
+        (dy_ld == H && over(drows, N, drows_ld, H, rsz, dy, (size_t)T * H * ysz)) ||
+        (dw && rows_ld == H && over(drows, N, drows_ld, H, rsz, rows, (size_t)N * H * rsz)))
+      return AINFER_ERR_ARG;
+  }
+  HIP_TRY(launch_unpermute_backward(dy, dy_ld, dy_dtype, rows, rows_ld, rows_dtype, N, pos, w, T,
+                                    top_k, H, drows, drows_ld, dw, (hipStream_t)stream));
   return AINFER_OK;
 }
 

@@ -409,3 +409,43 @@ hipError_t launch_lora(const ainfer_moe_lora &l, const void *x, int64_t x_ld, co
 // ---- gated activation (moe_silu.hip) ----------------------------------------
 hipError_t launch_silu_rows(const void *g, int64_t gld, const void *u, int64_t uld, int in_dtype,
                             int T, int I, void *y, int64_t yld, int out_dtype, hipStream_t s);
+hipError_t launch_silu_backward(const void *d, int64_t dld, const void *g, int64_t gld,
+                                const void *u, int64_t uld, int dtype, const int32_t *live, int N,
+                                int I, void *dg, int64_t dgld, void *du, int64_t duld,
+                                hipStream_t s);
+
+// ---- experts in 8-bit floating point (moe_fp8.hip, moe_fp8_product.hip) -------
+// live: device count of the rows in use, or NULL: all N
+hipError_t launch_act_quant_fp8(const void *x, int64_t xld, int dtype, const int32_t *live, int N,
+                                int K, int scale_kind, uint8_t *q, int64_t qld, float *sq,
+                                hipStream_t s);
+hipError_t launch_silu_mul_fp8(const void *g, int64_t gld, const void *u, int64_t uld, int dtype,
+                               const int32_t *live, int N, int I, int scale_kind, uint8_t *q,
+                               int64_t qld, float *sq, hipStream_t s);
+hipError_t launch_weight_quant_fp8(const void *w, int dtype, int E, int M, int K, int scale_kind,
+                                   uint8_t *q, float *scales, hipStream_t s);
+struct Fp8Args {
+  const uint8_t *w;        // [E][M][K]
+  const float *scales;     // [E][ceil(M / 128)][ceil(K / 128)]
+  const uint8_t *q;        // N rows of K codes
+  const float *sq;         // [N][ceil(K / 128)]
+  const int32_t *offsets;  // [E + 1], or null: one matrix for all rows
+  void *y;
+  int64_t q_ld, y_ld;
+  int E, M, K, N;
+};
+hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s);
+
+// ---- tokens sorted by expert and back (moe_sort.hip) ---------------------------
+size_t sort_workspace_bytes(int T, int k, int E);
+hipError_t launch_sort_rows(const ainfer_moe_sorting &d, const void *x, int64_t xld,
+                            const int32_t *idx, int T, int32_t *offsets, int32_t *pos, void *rows,
+                            int64_t rld, float *row_scales, void *ws, hipStream_t s);
+hipError_t launch_unpermute(const void *rows, int64_t rld, int rows_dtype, int N,
+                            const int32_t *pos, const float *w, int T, int k, int H,
+                            const void *resid, int64_t sld, void *y, int64_t yld, int y_dtype,
+                            hipStream_t s);
+hipError_t launch_unpermute_backward(const void *dy, int64_t yld, int y_dtype, const void *rows,
+                                     int64_t rld, int rows_dtype, int N, const int32_t *pos,
+                                     const float *w, int T, int k, int H, void *drows, int64_t dld,
+                                     float *dw, hipStream_t s);

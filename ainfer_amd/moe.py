@@ -502,3 +502,328 @@ class LoraAdapters:
         _call(L.lib().ainfer_moe_lora_apply, dev, stream, C.byref(self.struct), x.data_ptr(), ld,
               token_adapter.data_ptr(), T, yp, yl, ws.data_ptr(), ws.nbytes)
         return ys
+
+
+# ---- experts in 8-bit floating point -------------------------------------------
+_CODES = (torch.float8_e4m3fn, torch.uint8)
+
+
+def _codes(t, name, cols=None):
+    """A device matrix of e4m3 codes (as float8_e4m3fn or uint8), rows contiguous:
+    (device, rows, columns, pitch)."""
+    dev = t.get_device()
+    if t.dtype not in _CODES or dev < 0 or t.dim() != 2:
+        raise L.MoeError(f"{name}: a device matrix of float8_e4m3fn or uint8 codes")
+    n, m = t.shape
+    ld, one = t.stride()
+    if (cols is not None and m != cols) or (one != 1 and m != 1):
+        raise L.MoeError(f"{name}: contiguous rows" + (f" of {cols} columns" if cols else ""))
+    return dev, n, m, (ld if n > 1 else m)
+
+
+def _scales(t, name, n, cols, dev):
+    if not (t.dtype == torch.float32 and t.shape == (n, -(-cols // 128))
+            and t.get_device() == dev and t.is_contiguous()):
+        raise L.MoeError(f"{name}: contiguous fp32 [{n}][{-(-cols // 128)}] on the rows' device")
+
+
+def _live(live, dev):
+    """The address of a device count of rows: the last value of an int32 vector
+    (sort_rows' offsets, say)."""
+    if live is None:
+        return None
+    if live.dtype != torch.int32 or live.dim() != 1 or live.get_device() != dev or \
+            not live.is_contiguous() or live.numel() == 0:
+        raise L.MoeError("live: a contiguous int32 vector on the rows' device")
+    return live.data_ptr() + 4 * (live.numel() - 1)
+
+
+def _kind(pow2):
+    return L.FP8_SCALE_POW2 if pow2 else L.FP8_SCALE_ANY
+
+
+def _new_codes(n, cols, device):
+    return (torch.empty(n, cols, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(n, -(-cols // 128), dtype=torch.float32, device=device))
+
+
+def act_quant_fp8(x, q=None, sq=None, pow2=False, live=None, stream=None):
+    """e4m3 codes [N][K] and scales [N][ceil(K / 128)] of the rows of x
+    (ainfer_moe_act_quant_fp8), in q and sq where these are given.  live: an int32
+    vector whose last value is how many rows to take (sort_rows' offsets)."""
+    dt, dev, n, K, ld = _rows(x, "x")
+    if (q is None) != (sq is None):
+        raise L.MoeError("q and sq: both or neither")
+    if q is None:
+        with _on(stream):
+            q, sq = _new_codes(n, K, x.device)
+    qdev, qn, _, qld = _codes(q, "q", K)
+    if qdev != dev or qn != n:
+        raise L.MoeError("q: a row for each of x's, on its device")
+    _scales(sq, "sq", n, K, dev)
+    _call(L.lib().ainfer_moe_act_quant_fp8, dev, stream, x.data_ptr(), ld, dt, _live(live, dev), n,
+          K, _kind(pow2), q.data_ptr(), qld, sq.data_ptr())
+    return q, sq
+
+
+def silu_mul_fp8(gate, up, q=None, sq=None, pow2=False, live=None, stream=None):
+    """act_quant_fp8 of silu_mul's fp32 values (ainfer_moe_silu_mul_fp8)."""
+    dt, dev, n, I, gld = _rows(gate, "gate")
+    udt, udev, un, _, uld = _rows(up, "up", I)
+    if not (udt == dt and un == n and udev == dev):
+        raise L.MoeError("gate and up: one shape, type and device")
+    if (q is None) != (sq is None):
+        raise L.MoeError("q and sq: both or neither")
+    if q is None:
+        with _on(stream):
+            q, sq = _new_codes(n, I, gate.device)
+    qdev, qn, _, qld = _codes(q, "q", I)
+    if qdev != dev or qn != n:
+        raise L.MoeError("q: a row for each of gate's, on its device")
+    _scales(sq, "sq", n, I, dev)
+    _call(L.lib().ainfer_moe_silu_mul_fp8, dev, stream, gate.data_ptr(), gld, up.data_ptr(), uld, dt,
+          _live(live, dev), n, I, _kind(pow2), q.data_ptr(), qld, sq.data_ptr())
+    return q, sq
+
+
+def silu_mul_backward(dact, gate, up, dgate, dup, live=None, stream=None):
+    """The gradients of silu_mul to gate and up (ainfer_moe_silu_mul_backward), rows of
+    any pitch and one type; dgate and dup may be dact, gate or up."""
+    dt, dev, n, I, dld = _rows(dact, "dact")
+    args = [dact.data_ptr(), dld]
+    for t, name in ((gate, "gate"), (up, "up"), (dgate, "dgate"), (dup, "dup")):
+        tdt, tdev, tn, _, ld = _rows(t, name, I)
+        if not (tdt == dt and tdev == dev and tn == n):
+            raise L.MoeError("dact, gate, up, dgate and dup: one shape, type and device")
+        args += [t.data_ptr(), ld]
+    _call(L.lib().ainfer_moe_silu_mul_backward, dev, stream, *args[:6], dt, _live(live, dev), n, I,
+          *args[6:])
+    return dgate, dup
+
+
+class Fp8Weights:
+    """The weights of E experts' projection (or one matrix, E = 1) as e4m3 codes
+    w [E][M][K] (float8_e4m3fn or uint8) and fp32 scales
+    [E][ceil(M / 128)][ceil(K / 128)], resident on one device."""
+
+    def __init__(self, w, scales, y_dtype=None):
+        dev = w.get_device()
+        if not (w.dtype in _CODES and w.dim() == 3 and dev >= 0 and w.is_contiguous()):
+            raise L.MoeError("w: contiguous [E][M][K] codes on a device")
+        E, M, K = w.shape
+        if not (scales.dtype == torch.float32 and scales.get_device() == dev
+                and scales.shape == (E, -(-M // 128), -(-K // 128)) and scales.is_contiguous()):
+            raise L.MoeError("scales: contiguous fp32 [E][ceil(M / 128)][ceil(K / 128)] beside w")
+        if y_dtype is not None and y_dtype not in _ACT:
+            raise L.MoeError("y: fp32 or bf16")
+        self.w, self.scales, self.dev, self.y_dtype = w, scales, dev, y_dtype
+        self.structs = {dt: L.Fp8(E, M, K, code, w.data_ptr(), scales.data_ptr())
+                        for dt, code in _ACT.items()}
+        # no rows: the sizes' own checks
+        L.check(L.lib().ainfer_moe_fp8_product(C.byref(self.structs[torch.float32]), None, 0, None,
+                                               None, 0, None, 0, None))
+
+    @classmethod
+    def quantise(cls, w, pow2=False, y_dtype=None, stream=None):
+        """From w [E][M][K] fp32 or bf16 (ainfer_moe_weight_quant_fp8)."""
+        dev = w.get_device()
+        if not (w.dtype in _ACT and w.dim() == 3 and dev >= 0 and w.is_contiguous()):
+            raise L.MoeError("w: contiguous [E][M][K] fp32 or bf16 on a device")
+        E, M, K = w.shape
+        with _on(stream):
+            q = torch.empty(E, M, K, dtype=torch.float8_e4m3fn, device=w.device)
+            s = torch.empty(E, -(-M // 128), -(-K // 128), dtype=torch.float32, device=w.device)
+        _call(L.lib().ainfer_moe_weight_quant_fp8, dev, stream, w.data_ptr(), _ACT[w.dtype], E, M, K,
+              _kind(pow2), q.data_ptr(), s.data_ptr())
+        return cls(q, s, y_dtype)
+
+    def transposed(self):
+        """[E][K][M], for the gradient to x (laid out once; M a multiple of 16)."""
+        w = self.w.view(torch.uint8).transpose(1, 2).contiguous()
+        return Fp8Weights(w, self.scales.transpose(1, 2).contiguous(), self.y_dtype)
+
+    def product(self, q, sq, y=None, offsets=None, stream=None):
+        """y [N][M] = x W^T for codes q [N][K] and scales sq of rows sorted by expert
+        (offsets [E + 1] int32; may be left out with one expert), in fp32 or bf16
+        (ainfer_moe_fp8_product).  Rows outside the offsets keep what y holds."""
+        E, M, K = self.w.shape
+        dev, n, _, ld = _codes(q, "q", K)
+        if dev != self.dev:
+            raise L.MoeError("q: on the weights' device")
+        _scales(sq, "sq", n, K, dev)
+        if offsets is None:
+            if E != 1:
+                raise L.MoeError("offsets: the experts' rows")
+        else:
+            _vector(offsets, "offsets", torch.int32, E + 1, dev)
+        if y is None:
+            with _on(stream):
+                y = torch.empty(n, M, dtype=self.y_dtype or torch.bfloat16, device=q.device)
+        _, ydev, yn, _, yld = _rows(y, "y", M)
+        if ydev != dev or yn != n:
+            raise L.MoeError("y: a row for each of q's, on its device")
+        _call(L.lib().ainfer_moe_fp8_product, dev, stream, C.byref(self.structs[y.dtype]),
+              q.data_ptr(), ld, sq.data_ptr(), offsets.data_ptr() if offsets is not None else None,
+              n, y.data_ptr(), yld)
+        return y
+
+
+# ---- tokens sorted by expert and back --------------------------------------------
+def sort_workspace(max_tokens, top_k, n_experts, device="cuda"):
+    """Scratch of sort_rows with up to max_tokens tokens (no initialisation)."""
+    n = L.lib().ainfer_moe_sort_workspace_bytes(max_tokens, top_k, n_experts)
+    if n == 0:
+        raise L.MoeError("invalid sizes for a sort workspace")
+    ws = torch.empty(n + 256, dtype=torch.uint8, device=device)
+    off = (-ws.data_ptr()) % 256
+    return ws[off:off + n]
+
+
+def sort_rows(x, idx, n_experts, ws, fp8=False, pow2=False, out=None, stream=None):
+    """The rows of x [T][H] in the order of their experts (idx [T][k] int32; ids outside
+    [0, n_experts) are dropped): (rows [T * k][H], row_scales or None, offsets [E + 1], pos
+    [T][k]) (ainfer_moe_sort_rows).  fp8: rows as e4m3 codes with their scales.  out: the
+    four tensors to write; its rows' type then decides instead of fp8."""
+    dt, dev, T, H, ld = _rows(x, "x")
+    if not (idx.dtype == torch.int32 and idx.dim() == 2 and idx.shape[0] == T
+            and idx.get_device() == dev and idx.is_contiguous()):
+        raise L.MoeError("idx: contiguous int32 [T][k] on x's device")
+    if ws.get_device() != dev or not ws.is_contiguous():
+        raise L.MoeError("ws: on x's device")
+    k = idx.shape[1]
+    if out is None:
+        with _on(stream):
+            if fp8:
+                rows, sc = _new_codes(T * k, H, x.device)
+            else:
+                rows, sc = torch.empty(T * k, H, dtype=x.dtype, device=x.device), None
+            offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=x.device)
+            pos = torch.empty(T, k, dtype=torch.int32, device=x.device)
+    else:
+        rows, sc, offsets, pos = out
+        fp8 = rows.dtype in _CODES
+    if fp8:
+        rdev, rn, _, rld = _codes(rows, "rows", H)
+        if sc is None:
+            raise L.MoeError("row_scales: fp32, beside rows of codes")
+        _scales(sc, "row_scales", T * k, H, dev)
+    else:
+        _, rdev, rn, _, rld = _rows(rows, "rows", H)
+        if rows.dtype != x.dtype or sc is not None:
+            raise L.MoeError("rows: x's type without scales, or codes with them")
+    if rdev != dev or rn != T * k:
+        raise L.MoeError("rows: T * k of them, on x's device")
+    _vector(offsets, "offsets", torch.int32, n_experts + 1, dev)
+    if not (pos.dtype == torch.int32 and pos.shape == (T, k) and pos.get_device() == dev
+            and pos.is_contiguous()):
+        raise L.MoeError("pos: contiguous int32 [T][k] on x's device")
+    d = L.Sorting(n_experts, k, H, dt, int(fp8), _kind(pow2))
+    _call(L.lib().ainfer_moe_sort_rows, dev, stream, C.byref(d), x.data_ptr(), ld, idx.data_ptr(), T,
+          offsets.data_ptr(), pos.data_ptr(), rows.data_ptr(), rld,
+          sc.data_ptr() if fp8 else None, ws.data_ptr(), ws.nbytes)
+    return rows, sc, offsets, pos
+
+
+def _pairs(pos, w, T, dev):
+    """k of pos [T][k] (and w [T][k], or None) on device dev."""
+    if not (pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape[0] == T
+            and pos.get_device() == dev and pos.is_contiguous()):
+        raise L.MoeError("pos: contiguous int32 [T][k] on the rows' device")
+    if w is not None and not (w.dtype == torch.float32 and w.shape == pos.shape
+                              and w.get_device() == dev and w.is_contiguous()):
+        raise L.MoeError("w: contiguous fp32, of pos's shape, on its device")
+    return pos.shape[1]
+
+
+def unpermute(rows, pos, w, y, resid=None, stream=None):
+    """y[t] = sum_j w[t][j] rows[pos[t][j]] (+ resid[t]) (ainfer_moe_unpermute); w None: 1,
+    the gradient of sort_rows to x.  resid may be y."""
+    rdt, dev, n, H, rld = _rows(rows, "rows")
+    ydt, ydev, T, _, yld = _rows(y, "y", H)
+    k = _pairs(pos, w, T, dev)
+    if ydev != dev:
+        raise L.MoeError("y: on the rows' device")
+    sld = 0
+    if resid is not None:
+        sdt, sdev, sT, _, sld = _rows(resid, "resid", H)
+        if not (sdt == ydt and sdev == dev and sT == T):
+            raise L.MoeError("resid: y's shape, type and device")
+    _call(L.lib().ainfer_moe_unpermute, dev, stream, rows.data_ptr(), rld, rdt, n, pos.data_ptr(),
+          w.data_ptr() if w is not None else None, T, k, H,
+          resid.data_ptr() if resid is not None else None, sld, y.data_ptr(), yld, ydt)
+    return y
+
+
+def unpermute_backward(dy, rows, pos, w, drows=None, dw=None, stream=None):
+    """drows[pos[t][j]] = w[t][j] dy[t] and dw[t][j] = <dy[t], rows[pos[t][j]]>
+    (ainfer_moe_unpermute_backward), in drows and dw; one that is None is left out."""
+    ydt, dev, T, H, yld = _rows(dy, "dy")
+    rdt, rdev, n, _, rld = _rows(rows, "rows", H)
+    k = _pairs(pos, w, T, dev)
+    if rdev != dev:
+        raise L.MoeError("rows: on dy's device")
+    dld = 0
+    if drows is not None:
+        ddt, ddev, dn, _, dld = _rows(drows, "drows", H)
+        if not (ddt == rdt and ddev == dev and dn == n):
+            raise L.MoeError("drows: the rows' shape, type and device")
+    if dw is not None and not (dw.dtype == torch.float32 and dw.shape == pos.shape
+                               and dw.get_device() == dev and dw.is_contiguous()):
+        raise L.MoeError("dw: contiguous fp32, of pos's shape, on its device")
+    _call(L.lib().ainfer_moe_unpermute_backward, dev, stream, dy.data_ptr(), yld, ydt,
+          rows.data_ptr(), rld, rdt, n, pos.data_ptr(), w.data_ptr() if w is not None else None, T,
+          k, H, drows.data_ptr() if drows is not None else None, dld,
+          dw.data_ptr() if dw is not None else None)
+    return drows, dw
+
+
+class Fp8Experts:
+    """The routed experts' MLP with 8-bit floating point weights: gate_up [E][2 I][H]
+    (gate rows, then up rows) and down [E][H][I], Fp8Weights on one device.  Takes the
+    routing of route_scored or MoeLayer.route; ids outside [0, E) (experts of other GPUs)
+    add nothing.  train: also lays out the transposed weights, for backward."""
+
+    def __init__(self, gate_up, down, pow2=False, train=False):
+        E, I2, H = gate_up.w.shape
+        if down.w.shape != (E, H, I2 // 2) or I2 % 2 or gate_up.dev != down.dev:
+            raise L.MoeError("gate_up [E][2 I][H] and down [E][H][I] on one device")
+        self.gate_up, self.down, self.pow2 = gate_up, down, pow2
+        self.n_experts, self.inter, self.hidden = E, I2 // 2, H
+        self.back = (gate_up.transposed(), down.transposed()) if train else None
+
+    def forward(self, x, idx, w, y=None, resid=None, stream=None, keep=False):
+        """y[t] = sum_j w[t][j] expert_{idx[t][j]}(x[t]) (+ resid[t]), x and y [T][H] bf16 or
+        fp32 rows: rows sorted and quantised, gate and up, gated activation quantised,
+        down, weighted sums.  keep: (y, what backward needs) instead of y."""
+        T, k = idx.shape
+        I, dev = self.inter, self.gate_up.dev
+        with torch.cuda.device(dev), _on(stream):
+            ws = sort_workspace(T, k, self.n_experts, x.device)
+            q, sq, offsets, pos = sort_rows(x, idx, self.n_experts, ws, fp8=True, pow2=self.pow2)
+            h = self.gate_up.product(q, sq, offsets=offsets)
+            a, sa = silu_mul_fp8(h[:, :I], h[:, I:], pow2=self.pow2, live=offsets)
+            o = self.down.product(a, sa, offsets=offsets)
+            if y is None:
+                y = torch.empty_like(x)
+            unpermute(o, pos, w, y, resid)
+        return (y, (h, o, offsets, pos, w)) if keep else y
+
+    def backward(self, dy, kept, stream=None):
+        """(dx [T][H] of dy's type, dw [T][k] fp32) from dy [T][H] and forward's kept
+        tensors.  The weights are constants; the products' gradients are quantised to
+        e4m3 as the activations are, and each rounding passes its gradient on."""
+        if self.back is None:
+            raise L.MoeError("experts laid out with train=True")
+        h, o, offsets, pos, w = kept
+        I = self.inter
+        with torch.cuda.device(self.gate_up.dev), _on(stream):
+            do, dw = unpermute_backward(dy, o, pos, w, torch.empty_like(o), torch.empty_like(w))
+            q, sq = act_quant_fp8(do, pow2=self.pow2, live=offsets)
+            dact = self.back[1].product(q, sq, offsets=offsets,
+                                        y=torch.empty(len(q), I, dtype=h.dtype, device=h.device))
+            dh = torch.empty_like(h)
+            silu_mul_backward(dact, h[:, :I], h[:, I:], dh[:, :I], dh[:, I:], live=offsets)
+            q, sq = act_quant_fp8(dh, pow2=self.pow2, live=offsets)
+            drows = self.back[0].product(q, sq, offsets=offsets)
+            dx = unpermute(drows, pos, None, torch.empty_like(dy))
+        return dx, dw

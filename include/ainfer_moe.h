@@ -517,6 +517,118 @@ int ainfer_moe_silu_mul(const void *gate, int64_t gate_ld, const void *up, int64
                         int32_t in_dtype, int32_t T, int32_t I, void *act, int64_t act_ld,
                         int32_t act_dtype, void *stream);
 
+/* ---- experts in 8-bit floating point ---------------------------------------
+ * Weights and activations as e4m3 codes (OCP FP8 E4M3FN: 448 is the largest
+ * value, no infinities) with fp32 scales, one for every 128 consecutive columns
+ * of a row of activations and one for every 128 x 128 block of a weight matrix;
+ * the last block of a row, or of the rows, may be smaller.  Rows of activations
+ * stand in the order of their experts, as ainfer_moe_sort_rows writes them.  No
+ * reference counterpart (its weights are INT4, its activations int8).
+ *
+ * Quantising a block of values x:  m = max |x| (NaN left out),
+ *   s = 1 where m is 0, else max(m / 448, 2^-126) (SCALE_ANY), or the least power of
+ *       two that is not below that (SCALE_POW2; x / s is then exact);
+ *   q = x / s (fp32) rounded to the nearest e4m3 value, ties to even.
+ * A NaN gives a NaN code; a block with an infinity has an infinite scale, and what is
+ * computed with it is NaN. */
+#define AINFER_MOE_MAX_ROWS (1 << 21) /* sorted rows: up to 32 for each of 65536 tokens */
+enum { AINFER_FP8_SCALE_ANY = 0, AINFER_FP8_SCALE_POW2 = 1 };
+
+/* q [N] rows of K codes, sq [N][ceil(K / 128)] of x: N rows of K values (AINFER_ACT_F32
+ * or _BF16).  K a multiple of 16, 16..65536; row r at r * its ld elements; q 16-byte
+ * aligned, q_ld a multiple of 16.  n_live: device count of the rows to take (the last
+ * value of the offsets of ainfer_moe_sort_rows, say; rows behind it are left as they
+ * are), or NULL: N. */
+int ainfer_moe_act_quant_fp8(const void *x, int64_t x_ld, int32_t x_dtype, const int32_t *n_live,
+                             int32_t N, int32_t K, int32_t scale_kind, uint8_t *q, int64_t q_ld,
+                             float *sq, void *stream);
+/* The gated activation written as codes and scales: those of ainfer_moe_silu_mul's fp32
+ * values (gate, up: rows of I values of in_dtype, I as K above). */
+int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,
+                            int32_t in_dtype, const int32_t *n_live, int32_t N, int32_t I,
+                            int32_t scale_kind, uint8_t *q, int64_t q_ld, float *sq, void *stream);
+/* Weights w [E][M][K] (fp32 or bf16) as q [E][M][K] and scales
+ * [E][ceil(M / 128)][ceil(K / 128)]; sizes as in ainfer_moe_fp8. */
+int ainfer_moe_weight_quant_fp8(const void *w, int32_t w_dtype, int32_t E, int32_t M, int32_t K,
+                                int32_t scale_kind, uint8_t *q, float *scales, void *stream);
+
+typedef struct ainfer_moe_fp8 {
+  int32_t n_experts;   /* E, 1..1024                                         */
+  int32_t rows;        /* M, 1..1048576                                      */
+  int32_t cols;        /* K, multiple of 16, 16..65536; E M K at most 2^38   */
+  int32_t y_dtype;     /* AINFER_ACT_F32 or AINFER_ACT_BF16                  */
+  const uint8_t *w;    /* [E][M][K] e4m3, 16-byte aligned                    */
+  const float *scales; /* [E][ceil(M / 128)][ceil(K / 128)]                  */
+} ainfer_moe_fp8;
+/* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
+ *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
+ * sums in fp32, y rounded once.  q: N rows of K codes at q_ld elements (16-byte aligned, a
+ * multiple of 16), sq [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one
+ * expert: all N rows), y: N rows of M values at y_ld elements.  Rows of y outside
+ * [offsets[0], offsets[E]) are left as they were; offsets outside [0, N] are taken as
+ * its ends, and rows of experts that overlap are unspecified.  A NaN code or scale
+ * reaches the values whose sums it is in.  y must not overlap anything that is read.
+ * The gradient to x is the same call with the transposed weights: [E][K][M] codes and
+ * [E][ceil(K / 128)][ceil(M / 128)] scales, as blocks are square. */
+int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_ld,
+                           const float *sq, const int32_t *offsets, int32_t N, void *y,
+                           int64_t y_ld, void *stream);
+
+/* Gradient of ainfer_moe_silu_mul, computed in fp32: with sig = 1 / (1 + exp(-gate)),
+ *   dgate = dact * up * sig * (1 + gate * (1 - sig)),   dup = dact * gate * sig.
+ * N rows of I values (I up to 65536) of one type; dgate and dup may be dact, gate or up
+ * themselves (same pointer and ld), and must not overlap them or each other otherwise. */
+int ainfer_moe_silu_mul_backward(const void *dact, int64_t dact_ld, const void *gate,
+                                 int64_t gate_ld, const void *up, int64_t up_ld, int32_t dtype,
+                                 const int32_t *n_live, int32_t N, int32_t I, void *dgate,
+                                 int64_t dgate_ld, void *dup, int64_t dup_ld, void *stream);
+
+/* ---- tokens sorted by expert and back ---------------------------------------
+ * The caller's own form of the layer's dispatch and combine: any number of tokens, any
+ * ids (those outside [0, E) are dropped: experts of other GPUs, padded tokens; one id
+ * may stand twice in a token's row), and the rows are moved too.
+ *   offsets[e]  how many pairs (t, j) name an expert below e; E + 1 values
+ *   pos[t][j]   the pair's row: pairs by expert, then token, then slot; -1 if dropped
+ *   rows[pos[t][j]] = x[t], as it is or (fp8) quantised as by ainfer_moe_act_quant_fp8,
+ *               its scales in row_scales [T * k][ceil(H / 128)]
+ * Rows from offsets[E] on are left as they were. */
+typedef struct ainfer_moe_sorting {
+  int32_t n_experts;  /* E, 1..1024                                          */
+  int32_t top_k;      /* k, 1..32                                            */
+  int32_t hidden;     /* H, 1..65536; a multiple of 16 with fp8              */
+  int32_t x_dtype;    /* AINFER_ACT_F32 or AINFER_ACT_BF16                   */
+  int32_t fp8;        /* 0: rows of x's type; 1: e4m3 codes and scales       */
+  int32_t scale_kind; /* AINFER_FP8_SCALE_* (fp8)                            */
+} ainfer_moe_sorting;
+/* Scratch of calls with up to max_tokens tokens (0: a size out of range); 256-byte
+ * aligned, no initialisation; calls that share it must be stream-ordered. */
+size_t ainfer_moe_sort_workspace_bytes(int32_t max_tokens, int32_t top_k, int32_t n_experts);
+/* topk_idx [T][k]; x: T rows at x_ld elements; rows: T * k rows at rows_ld elements
+ * (fp8: 16-byte aligned, rows_ld a multiple of 16), or NULL: offsets and pos alone.
+ * Nothing that is written may overlap another operand. */
+int ainfer_moe_sort_rows(const ainfer_moe_sorting *sorting, const void *x, int64_t x_ld,
+                         const int32_t *topk_idx, int32_t T, int32_t *offsets, int32_t *pos,
+                         void *rows, int64_t rows_ld, float *row_scales, void *workspace,
+                         size_t workspace_bytes, void *stream);
+/* y[t] = sum_j w[t][j] * rows[pos[t][j]] (+ resid[t]): fp32 fma in slot order, rounded
+ * once.  rows: N rows of H values; pairs whose pos is outside [0, N) are left out, and
+ * their w is not used.  w [T][k] or NULL: 1, which makes this the gradient of
+ * ainfer_moe_sort_rows to x (rows: its rows' gradient).  resid (y's type) or NULL; it may
+ * be y itself. */
+int ainfer_moe_unpermute(const void *rows, int64_t rows_ld, int32_t rows_dtype, int32_t N,
+                         const int32_t *pos, const float *w, int32_t T, int32_t top_k, int32_t H,
+                         const void *resid, int64_t resid_ld, void *y, int64_t y_ld,
+                         int32_t y_dtype, void *stream);
+/* Its gradients: drows[pos[t][j]] = w[t][j] * dy[t] (rows' type) and dw[t][j] =
+ * sum_h dy[t][h] * rows[pos[t][j]][h] (fp32 sums in one order; 0 where pos is outside [0, N)).
+ * Either of drows and dw may be NULL (rows is read for dw alone); no row may stand
+ * twice in pos.  Rows of drows that pos does not name are left as they were. */
+int ainfer_moe_unpermute_backward(const void *dy, int64_t dy_ld, int32_t dy_dtype,
+                                  const void *rows, int64_t rows_ld, int32_t rows_dtype, int32_t N,
+                                  const int32_t *pos, const float *w, int32_t T, int32_t top_k,
+                                  int32_t H, void *drows, int64_t drows_ld, float *dw,
+                                  void *stream);
+
 /* ---- synthetic data (counter-based, bit-identical to the CPU oracle) --- */
 enum {
   AINFER_FILL_BYTES = 0,      /* uniform random bytes (packed int4 weights)  */
