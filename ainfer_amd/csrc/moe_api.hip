@@ -1382,7 +1382,8 @@ int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_
   if (!w->w || !w->scales || !q || !sq || !y || (!offsets && w->n_experts != 1))
     return AINFER_ERR_NULL;
   const int M = w->rows, K = w->cols, ysz = act_size(w->y_dtype);
-  if (bad_ld(q_ld, K) || q_ld % 16 || bad_ld(y_ld, M) || mis(w->w, 16) || mis(q, 16) ||
+  // a tile's rows of codes are addressed with 32-bit offsets
+  if (bad_ld(q_ld, K) || q_ld % 16 || q_ld > 1 << 24 || bad_ld(y_ld, M) || mis(w->w, 16) || mis(q, 16) ||
       mis(w->scales, 4) || mis(sq, 4) || mis(offsets, 4) || mis(y, ysz))
     return AINFER_ERR_ARG;
   const size_t G = (K + 127) / 128, E = w->n_experts;

@@ -563,7 +563,7 @@ typedef struct ainfer_moe_fp8 {
 /* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
  *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
  * sums in fp32, y rounded once.  q: N rows of K codes at q_ld elements (16-byte aligned, a
- * multiple of 16), sq [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one
+ * multiple of 16, at most 2^24), sq [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one
  * expert: all N rows), y: N rows of M values at y_ld elements.  Rows of y outside
  * [offsets[0], offsets[E]) are left as they were; offsets outside [0, N] are taken as
  * its ends, and rows of experts that overlap are unspecified.  A NaN code or scale

@@ -108,7 +108,7 @@ def test_product(L):
     refused(call, (dict(N=-1), dict(N=L.MAX_ROWS + 1)), L.ERR_TOKENS)
     refused(call, (dict(struct=False), dict(w=None), dict(s=None), dict(q=None), dict(sq=None),
                    dict(offsets=None), dict(y=None)), L.ERR_NULL)
-    refused(call, (dict(dtype=2), dict(dtype=-1), dict(q_ld=256), dict(q_ld=280), dict(y_ld=129),
+    refused(call, (dict(dtype=2), dict(dtype=-1), dict(q_ld=256), dict(q_ld=280), dict(q_ld=(1 << 24) + 16), dict(y_ld=129),
                    dict(y_ld=1 << 40), dict(w=A + 8), dict(q=D + 8), dict(s=B + 2), dict(sq=E + 2),
                    dict(offsets=F + 2), dict(y=G + 1), dict(y=D), dict(y=A), dict(y=A + 256),
                    dict(y=B), dict(y=E), dict(y=F), dict(y=F - 1024), dict(y=A, y_ld=140),
