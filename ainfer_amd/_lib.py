@@ -39,7 +39,8 @@ EXPORTS = (
     "ainfer_moe_act_quant_i8", "ainfer_moe_int4_gemv_i8",
     "ainfer_moe_route_scored", "ainfer_moe_lora_workspace_bytes", "ainfer_moe_lora_apply",
     "ainfer_moe_silu_mul",
-    "ainfer_moe_act_quant_fp8", "ainfer_moe_weight_quant_fp8", "ainfer_moe_fp8_product",
+    "ainfer_moe_act_quant_fp8", "ainfer_moe_weight_quant_fp8", "ainfer_moe_fp8_packed_bytes",
+    "ainfer_moe_fp8_pack", "ainfer_moe_fp8_product",
     "ainfer_moe_silu_mul_fp8", "ainfer_moe_silu_mul_backward",
     "ainfer_moe_sort_workspace_bytes", "ainfer_moe_sort_rows", "ainfer_moe_unpermute",
     "ainfer_moe_unpermute_backward",
@@ -84,7 +85,7 @@ class Lora(C.Structure):
 class Fp8(C.Structure):
     """Weights in e4m3 with a scale for each 128 x 128 block (ainfer_moe_fp8)."""
     _fields_ = [("n_experts", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32),
-                ("y_dtype", C.c_int32), ("w", C.c_void_p), ("scales", C.c_void_p)]
+                ("y_dtype", C.c_int32), ("packed", C.c_void_p), ("scales", C.c_void_p)]
 
 
 class Sorting(C.Structure):
@@ -144,6 +145,9 @@ def lib():
         L.ainfer_moe_silu_mul.argtypes = [P, I64, P, I64, I32, I32, I32, P, I64, I32, P]
         L.ainfer_moe_act_quant_fp8.argtypes = [P, I64, I32, P, I32, I32, I32, P, I64, P, P]
         L.ainfer_moe_weight_quant_fp8.argtypes = [P, I32, I32, I32, I32, I32, P, P, P]
+        L.ainfer_moe_fp8_packed_bytes.restype = SZ
+        L.ainfer_moe_fp8_packed_bytes.argtypes = [I32, I32, I32]
+        L.ainfer_moe_fp8_pack.argtypes = [P, I32, I32, I32, I32, P, SZ, P]
         L.ainfer_moe_fp8_product.argtypes = [C.POINTER(Fp8), P, I64, P, P, I32, P, I64, P]
         L.ainfer_moe_silu_mul_fp8.argtypes = [P, I64, P, I64, I32, P, I32, I32, I32, P, I64, P, P]
         L.ainfer_moe_silu_mul_backward.argtypes = [P, I64, P, I64, P, I64, I32, P, I32, I32, P, I64,

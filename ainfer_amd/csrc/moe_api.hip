@@ -737,14 +737,17 @@ bool over(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, con
   if (rows == 1 || ld == cols) return meet(out, (size_t)(rows * cols * size), p, n);
   return out == p;
 }
+int check_fp8_sizes(int32_t E, int32_t M, int32_t K) {
+  if (E < 1 || E > 1024 || M < 1 || M > (1 << 20) || K < 16 || K > 65536 || K % 16 ||
+      (int64_t)E * M * K > (int64_t)1 << 38)
+    return AINFER_ERR_SHAPE;
+  return AINFER_OK;
+}
 int check_fp8(const ainfer_moe_fp8 *w) {
   if (!w) return AINFER_ERR_NULL;
-  if (w->n_experts < 1 || w->n_experts > 1024 || w->rows < 1 || w->rows > (1 << 20) ||
-      w->cols < 16 || w->cols > 65536 || w->cols % 16 ||
-      (int64_t)w->n_experts * w->rows * w->cols > (int64_t)1 << 38)
-    return AINFER_ERR_SHAPE;
-  if (!is_act(w->y_dtype)) return AINFER_ERR_ARG;
-  return AINFER_OK;
+  int rc = check_fp8_sizes(w->n_experts, w->rows, w->cols);
+  if (rc) return rc;
+  return is_act(w->y_dtype) ? AINFER_OK : AINFER_ERR_ARG;
 }
 int check_sorting(const ainfer_moe_sorting *s) {
   if (!s) return AINFER_ERR_NULL;
@@ -1358,10 +1361,9 @@ int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, i
 
 int ainfer_moe_weight_quant_fp8(const void *w, int32_t w_dtype, int32_t E, int32_t M, int32_t K,
                                 int32_t scale_kind, uint8_t *q, float *scales, void *stream) {
-  const ainfer_moe_fp8 d = {E, M, K, w_dtype, q, scales};
-  int rc = check_fp8(&d);
+  int rc = check_fp8_sizes(E, M, K);
   if (rc) return rc;
-  if (!is_scale_kind(scale_kind)) return AINFER_ERR_ARG;
+  if (!is_act(w_dtype) || !is_scale_kind(scale_kind)) return AINFER_ERR_ARG;
   if (!w || !q || !scales) return AINFER_ERR_NULL;
   if (mis(w, act_size(w_dtype)) || mis(q, 16) || mis(scales, 4)) return AINFER_ERR_ARG;
   const size_t n = (size_t)E * M * K, sn = (size_t)E * ((M + 127) / 128) * ((K + 127) / 128) * 4;
@@ -1372,6 +1374,24 @@ int ainfer_moe_weight_quant_fp8(const void *w, int32_t w_dtype, int32_t E, int32
   return AINFER_OK;
 }
 
+size_t ainfer_moe_fp8_packed_bytes(int32_t E, int32_t M, int32_t K) {
+  return check_fp8_sizes(E, M, K) == AINFER_OK ? fp8_packed_bytes(E, M, K) : 0;
+}
+
+int ainfer_moe_fp8_pack(const uint8_t *w, int32_t E, int32_t M, int32_t K, int32_t transpose,
+                        uint8_t *packed, size_t packed_bytes, void *stream) {
+  int rc = check_fp8_sizes(E, M, K);
+  if (rc) return rc;
+  if (transpose != 0 && transpose != 1) return AINFER_ERR_ARG;
+  if (!w || !packed) return AINFER_ERR_NULL;
+  const size_t n = fp8_packed_bytes(E, M, K);
+  if (mis(packed, 16) || (!transpose && mis(w, 16)) || packed_bytes < n ||
+      meet(w, (size_t)E * M * K, packed, n))
+    return AINFER_ERR_ARG;
+  HIP_TRY(launch_fp8_pack(w, E, M, K, transpose, packed, (hipStream_t)stream));
+  return AINFER_OK;
+}
+
 int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_ld, const float *sq,
                            const int32_t *offsets, int32_t N, void *y, int64_t y_ld,
                            void *stream) {
@@ -1379,20 +1399,20 @@ int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_
   if (rc) return rc;
   if (N < 0 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
   if (N == 0) return AINFER_OK;
-  if (!w->w || !w->scales || !q || !sq || !y || (!offsets && w->n_experts != 1))
+  if (!w->packed || !w->scales || !q || !sq || !y || (!offsets && w->n_experts != 1))
     return AINFER_ERR_NULL;
   const int M = w->rows, K = w->cols, ysz = act_size(w->y_dtype);
   // a tile's rows of codes are addressed with 32-bit offsets
-  if (bad_ld(q_ld, K) || q_ld % 16 || q_ld > 1 << 24 || bad_ld(y_ld, M) || mis(w->w, 16) || mis(q, 16) ||
+  if (bad_ld(q_ld, K) || q_ld % 16 || q_ld > 1 << 24 || bad_ld(y_ld, M) || mis(w->packed, 16) || mis(q, 16) ||
       mis(w->scales, 4) || mis(sq, 4) || mis(offsets, 4) || mis(y, ysz))
     return AINFER_ERR_ARG;
   const size_t G = (K + 127) / 128, E = w->n_experts;
-  if (over(y, N, y_ld, M, ysz, w->w, E * M * K) ||
+  if (over(y, N, y_ld, M, ysz, w->packed, fp8_packed_bytes(w->n_experts, M, K)) ||
       over(y, N, y_ld, M, ysz, w->scales, E * ((M + 127) / 128) * G * 4) ||
       over(y, N, y_ld, M, ysz, sq, N * G * 4) || over(y, N, y_ld, M, ysz, offsets, (E + 1) * 4) ||
       y == q)
     return AINFER_ERR_ARG;
-  const Fp8Args a = {w->w, w->scales, q, sq, offsets, y, q_ld, y_ld, w->n_experts, M, K, N};
+  const Fp8Args a = {w->packed, w->scales, q, sq, offsets, y, q_ld, y_ld, w->n_experts, M, K, N};
   HIP_TRY(launch_fp8_product(a, w->y_dtype, (hipStream_t)stream));
   return AINFER_OK;
 }

@@ -6,6 +6,14 @@
 // rows of x, so a group's dot comes out whole and enters the fp32 sum as
 // fma(s_x s_w, dot, sum).  Weights are its first operand: a lane's four results are
 // four neighbouring columns of one row of y, with one scale for all four.
+//
+// Weights are laid out once (ainfer_moe_fp8_pack) as this instruction takes them: 64 rows x
+// 128 columns are four tiles of 16 rows, each 2 KB in the order of the lanes, so that a wave's
+// load is 1 KB of neighbouring bytes.  (Read from plain rows, 16 neighbouring lanes touch 16
+// rows, which the CU's address unit takes one by one: the whole kernel ran at 1394 TFLOP/s
+// for 8192^3 where it reaches 2622 without those loads.)  Row r of tile i is row 16 (r / 4) +
+// 4 i + r % 4 of the 64, so that the lane that holds four results of each tile holds 16
+// neighbouring columns of a row of y.  Rows and columns behind the matrix are zeros.
 #include <algorithm>
 
 #include "moe_common.h"
@@ -101,56 +109,84 @@ __device__ __forceinline__ Tile find_tile(const int32_t *offsets, int E, int N, 
   return found;
 }
 
-// 16 bytes of codes, none behind the row's K columns
-__device__ __forceinline__ u32x4 codes_at(const uint8_t *row, int col, int K) {
-  return col < K ? *(const u32x4 *)(row + col) : u32x4{0, 0, 0, 0};
+// the packed tile i of rows 64 mb .. +63 and group g
+__device__ __forceinline__ const uint8_t *tile_at(const Fp8Args &a, int e, int mb, int g, int i) {
+  const int G = (a.K + 127) >> 7, MB64 = (a.M + 63) >> 6;
+  return a.w + (((int64_t)e * MB64 + mb) * G + g) * 8192 + i * 2048;
 }
 
-// 16 weight rows x at most 16 rows of x: four waves take every fourth group of 128
+// ---- rows -------------------------------------------------------------------------
+// 16 weight rows x at most 16 NS rows of x: four waves take every fourth group of 128
 // columns, and their sums are added in the waves' order.
-template <bool F32>
+template <bool F32, int NS>
 __global__ __launch_bounds__(256) void k_fp8_rows(Fp8Args a, int64_t items) {
-  __shared__ f32x4 sums[4][64];
+  __shared__ f32x4 sums[3][NS][64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slabs = (a.M + 15) / 16, G = (a.K + 127) / 128, MB = (a.M + 127) / 128;
+  const int slabs = (a.M + 63) / 64 * 4, G = (a.K + 127) / 128, MB = (a.M + 127) / 128;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const Tile t = find_tile<16>(a.offsets, a.E, a.N, it / slabs);
+    const Tile t = find_tile<16 * NS>(a.offsets, a.E, a.N, it / slabs);
     if (t.n == 0) return;  // no tile from here on
-    const int m0 = (int)(it % slabs) * 16;
-    const uint8_t *wr = a.w + ((int64_t)t.e * a.M + min(m0 + c, a.M - 1)) * a.K;
-    const float *sw = a.scales + ((int64_t)t.e * MB + m0 / 128) * G;
-    const int64_t row = t.r0 + min(c, t.n - 1);
-    const uint8_t *xr = a.q + row * a.q_ld;
-    const float *sx = a.sq + row * G;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int g = wave; g < G; g += 4) {
-      const int col = g * 128 + qd * 16;
-      const Codes wv = {{codes_at(wr, col, a.K), codes_at(wr, col + 64, a.K)}};
-      const Codes xv = {{codes_at(xr, col, a.K), codes_at(xr, col + 64, a.K)}};
-      const f32x4 dot = group_dot<F32>(wv, xv);
-      const float s = sx[g] * sw[g];
+    const int slab = (int)(it % slabs), mb = slab >> 2, i = slab & 3;
+    const uint8_t *wt = tile_at(a, t.e, mb, 0, i) + lane * 16;
+    const float *sw = a.scales + ((int64_t)t.e * MB + mb / 2) * G;
+    const uint8_t *xr[NS];
+    const float *sx[NS];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(s, dot[i], acc[i]);
+    for (int j = 0; j < NS; ++j) {
+      const int64_t row = t.r0 + min(16 * j + c, t.n - 1);
+      xr[j] = a.q + row * a.q_ld;
+      sx[j] = a.sq + row * G;
     }
-    sums[wave][lane] = acc;
-    __syncthreads();
-    if (wave == 0 && c < t.n) {
+    f32x4 acc[NS];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = m0 + 4 * qd + i;
-        const float v = (sums[0][lane][i] + sums[1][lane][i]) + (sums[2][lane][i] + sums[3][lane][i]);
-        if (m < a.M) {
-          const int64_t at = row * a.y_ld + m;
-          if constexpr (F32) ((float *)a.y)[at] = v;
-          else ((uint16_t *)a.y)[at] = f32_to_bf16(v);
+    for (int j = 0; j < NS; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto group = [&](int g) __attribute__((always_inline)) {
+      const int col = g * 128 + qd * 16;
+      Codes w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w.v[h] = __builtin_nontemporal_load((const u32x4 *)(wt + (int64_t)g * 8192 + h * 1024));
+      const float s = sw[g];
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        Codes x;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          x.v[h] = col + 64 * h < a.K ? *(const u32x4 *)(xr[j] + col + 64 * h) : u32x4{0, 0, 0, 0};
+        const f32x4 d = group_dot<F32>(w, x);
+        const float f = sx[j][g] * s;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, d[r], acc[j][r]);
+      }
+    };
+    int g = wave;
+    for (; g + 12 < G; g += 16) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) group(g + 4 * u);
+    }
+    for (; g < G; g += 4) group(g);
+    if (wave > 0) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) sums[wave - 1][j][lane] = acc[j];
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int m = mb * 64 + 16 * qd + 4 * i;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        if (16 * j + c >= t.n) continue;
+        const int64_t at = (int64_t)(t.r0 + 16 * j + c) * a.y_ld + m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = ((acc[j][r] + sums[0][j][lane][r]) + sums[1][j][lane][r]) + sums[2][j][lane][r];
+          if (m + r < a.M) store_one<F32>(a.y, at + r, v);
         }
       }
     }
     __syncthreads();
   }
 }
-
 
 // ---- tiles ------------------------------------------------------------------------
 // 256 weight rows x NS * 16 rows of x in a workgroup of four waves, each 64 of the weight
@@ -162,13 +198,24 @@ __global__ __launch_bounds__(256) void k_fp8_rows(Fp8Args a, int64_t items) {
 // 64, so that a lane ends with 16 neighbouring columns of a row of y.
 constexpr int TILE_M = 256;
 
-__device__ const uint8_t fp8_zeros[16] __attribute__((aligned(16))) = {};
+// Lane l's 16 or 4 bytes at `off` of the buffer to the wave's LDS address + 16 l or 4 l (zeros
+// where off is behind the buffer).  The compiler counts the copy among the loads in flight but
+// is not told what it writes, so that it waits for none of them before a read of the ring:
+// step() does.  (A global_load_lds would do that too, but counts as an access of both
+// memories, for which the compiler waits until nothing is in flight.)
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ void dma_x4(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void dma_x1(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 4, off, 0, 0, 0);
+}
 
 template <int NS>
 struct Stage {
-  static constexpr int X = NS * 16 * 128;           // codes: 128 bytes a row
-  static constexpr int SDMA = (NS * 16 + 63) / 64;  // scales, by 64 lanes of 4 bytes each
-  static constexpr int BYTES = X + SDMA * 256;
+  static constexpr int DMA = NS == 1 ? 1 : NS / 2;  // 16-byte copies a lane, of four waves
+  static constexpr int X = DMA * 4096;              // codes: 128 bytes a row
+  static constexpr int BYTES = X + 1024;            // scales: one a lane
 };
 
 // where the rows of each expert's tiles are: tiles before expert e, by 256 threads
@@ -221,69 +268,42 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
   const int tid = tid_opaque(), lane = tid & 63,
             col = lane & 15, qd = lane >> 4;  // per item: nothing is kept across items
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = (a.K + 127) >> 7, groups = (G + 1) & ~1, MB = (a.M + 127) >> 7;
-  // weights: a scalar base at the wave's first row, a 32-bit offset for each tile's row
-  const int mw = m0 + wave * 64;
-  const uint8_t *wbase = a.w + ((int64_t)e * a.M + min(mw, a.M - 1)) * a.K;
-  uint32_t woff[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 16 * (col >> 2) + 4 * i + (col & 3);
-    woff[i] = (uint32_t)max(0, min(r, a.M - 1 - mw)) * (uint32_t)a.K;
-  }
-  const float *sw = a.scales + ((int64_t)e * MB + min(mw >> 7, MB - 1)) * G;
+  const int G = (a.K + 127) >> 7, MB = (a.M + 127) >> 7;
+  int zero = 0;  // opaque: a vector load is in the counts below, a scalar one would not be
+  asm volatile("" : "+v"(zero));
+  const int mw = m0 + wave * 64, mbw = min(mw >> 6, ((a.M + 63) >> 6) - 1);
+  const uint8_t *wbase = tile_at(a, e, mbw, 0, 2);
+  const float *sw = a.scales + ((int64_t)e * MB + (mbw >> 1)) * G;
   // rows of x by DMA: slot s of 16 bytes holds chunk (s & 7) ^ (row & 7) of row s >> 3
-  constexpr int DMA = NS * 16 * 8 / 64;  // of 64 lanes each, over four waves
-  constexpr int PER = (DMA + 3) / 4;
-  const uint64_t xbase = sbase64(a.q + (int64_t)r0 * a.q_ld);
-  const uint64_t sbase = sbase64(a.sq + (int64_t)r0 * G);
-  uint32_t xoff[PER], xcol[PER];
+  const __amdgpu_buffer_rsrc_t xbuf =
+      make_rsrc(a.q + (int64_t)r0 * a.q_ld, (uint32_t)(n - 1) * (uint32_t)a.q_ld + (uint32_t)a.K);
+  const __amdgpu_buffer_rsrc_t sbuf = make_rsrc(a.sq + (int64_t)r0 * G, (uint32_t)(n * G) * 4u);
+  uint32_t xoff[St::DMA];
+  const uint32_t xcol = (uint32_t)(((lane & 7) ^ (lane >> 3)) * 16);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int s = (i * 4 + wave) * 64 + lane, row = s >> 3;
-    xcol[i] = (uint32_t)(((s & 7) ^ (row & 7)) * 16);
-    xoff[i] = (uint32_t)min(row, n - 1) * (uint32_t)a.q_ld;
-  }
-  // scales of x: place p of the stage's 16 NS floats is row 16 (p % NS) + p / NS
-  constexpr int SDMA = St::SDMA;
-  uint32_t soff;
-  {
-    const int p = wave * 64 + lane;
-    const int row = 16 * (p % NS) + p / NS;
-    soff = (uint32_t)min(row, n - 1) * (uint32_t)G * 4u;
-  }
-  // Columns behind the row (a last group that is not full, and a last one of an odd number)
-  // are zeros in x and any columns of the same row in w: a NaN among those is one of y too.
-  auto issue = [&](int g, int stage) __attribute__((always_inline)) {
-    const uint32_t base = lds0 + stage * St::BYTES;
-    const bool whole = (g + 1) * 128 <= a.K;
+  for (int i = 0; i < St::DMA; ++i)
+    xoff[i] = (uint32_t)min((i * 4 + wave) * 8 + (lane >> 3), n - 1) * (uint32_t)a.q_ld + xcol;
+  // scales: place p of the stage's is row 16 (p % NS) + p / NS
+  const int sp = wave * 64 + lane;
+  const uint32_t soff = (uint32_t)min(16 * (sp % NS) + sp / NS, n - 1) * (uint32_t)G * 4u;
+  auto issue = [&](int g, uint32_t stage) __attribute__((always_inline)) {
+    const bool past = g * 128 + xcol >= (uint32_t)a.K;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (DMA >= 4 * (i + 1) || i * 4 + wave < DMA) {
-        const uint32_t to = base + (uint32_t)((i * 4 + wave) * 1024);
-        if (whole)
-          dma16s(xoff[i] + xcol[i], xbase + (uint64_t)g * 128u, to);
-        else
-          dma16(g * 128 + xcol[i] < (uint32_t)a.K ? (const uint8_t *)xbase + g * 128 + xoff[i] + xcol[i]
-                                                  : fp8_zeros, to);
-      }
-    }
-    if (wave < SDMA) {
-      const uint32_t to = base + St::X + (uint32_t)(wave * 256);
-      if (g < G) dma4s(soff, sbase + (uint64_t)g * 4u, to);
-      else dma4s(0u, (uint64_t)(uintptr_t)fp8_zeros, to);
-    }
+    for (int i = 0; i < St::DMA; ++i)
+      dma_x4(xbuf, past ? BUF_OOB : xoff[i] + g * 128, stage + (uint32_t)((i * 4 + wave) * 1024));
+    dma_x1(sbuf, soff + g * 4, stage + St::X + (uint32_t)(wave * 256));
+    // the loads of weights stay behind the copies: step() counts on it
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto load_w = [&](int g, Codes (&w)[4]) __attribute__((always_inline)) {
-    g = min(g, G - 1);
-    const uint8_t *p = wbase + (int64_t)g * 128;
-    const uint32_t c0 = g * 128 + qd * 16 < a.K ? qd * 16 : 0;
-    const uint32_t c1 = g * 128 + qd * 16 + 64 < a.K ? qd * 16 + 64 : 0;
+  const uint32_t wlane = (uint32_t)lane * 16u;
+  auto load_w = [&](int g, Codes (&w)[4], float &s) __attribute__((always_inline)) {
+    s = sw[g + zero];
+    const uint8_t *p = wbase + (int64_t)g * 8192;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i].v[0] = *(const u32x4 *)(p + (woff[i] + c0));
-      w[i].v[1] = *(const u32x4 *)(p + (woff[i] + c1));
-    }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[i].v[h] = *(const u32x4 *)(p + wlane + ((i - 2) * 2048 + h * 1024));
   };
   f32x4 acc[NS][4];
 #pragma unroll
@@ -291,34 +311,43 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const uint32_t xr0 = (uint32_t)(col * 128 + ((qd ^ (col & 7)) << 4));
-  float swv = 0.f;  // lane l: the weights' scale of group 64 (g / 64) + l
+  const uint32_t xs0 = (uint32_t)(St::X + col * NS * 4);
 
-  auto step = [&](int g, Codes (&w)[4], Codes (&next)[4]) __attribute__((always_inline)) {
-    if ((g & 63) == 0) swv = sw[min(g + lane, G - 1)];
-    wait_vm<0>();  // this thread's DMA of group g
+  // Group g: its loads were issued two groups ago, and behind its DMA there are its own
+  // nine loads of weights and all of the next group's.  The loop's last steps load the last
+  // group again, so that these counts are the same in every one of them.  (A load whose
+  // value nothing takes would not be there to be counted: the steps behind the loop issue
+  // none, and wait for what is left.)
+  uint32_t here = 0, fill = 2 * St::BYTES;  // the stages of groups g and g + 2
+  auto step = [&](int g, Codes (&w)[4], float s, auto loads, Codes (&next)[4], float &snext)
+                  __attribute__((always_inline)) {
+    constexpr bool LOADS = decltype(loads)::value;
+    if constexpr (LOADS) wait_vm<18 + St::DMA + 1>();
+    else wait_vm<0>();
     block_barrier();
-    if (g + 1 < groups) {
-      issue(g + 1, (g + 1) & 1);
-      load_w(g + 1, next);
+    if constexpr (LOADS) {
+      issue(min(g + 2, G - 1), lds0 + fill);
+      load_w(min(g + 2, G - 1), next, snext);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const uint8_t *st = lds + (g & 1) * St::BYTES;
-    const float s = __uint_as_float(
-        __builtin_amdgcn_readlane((int)__float_as_uint(swv), g & 63));
+    const uint8_t *st = lds + here;
+    here = here == 2 * St::BYTES ? 0 : here + St::BYTES;
+    fill = fill == 2 * St::BYTES ? 0 : fill + St::BYTES;
     // One product and the four fmas of the one two before it at a time: the fmas run under
     // the products.  The barriers keep the compiler from reading all rows first (spills).
-    Codes x[2];
+    constexpr int XB = F32 ? 1 : 2;  // fp32: the registers are the conversions'
+    Codes x[XB];
     float f[2];
     f32x4 d[3];
     auto read_row = [&](int j) {
-      x[j & 1] = {{*(const u32x4 *)(st + xr0 + j * 2048), *(const u32x4 *)(st + (xr0 ^ 64) + j * 2048)}};
-      f[j & 1] = *(const float *)(st + St::X + (col * NS + j) * 4) * s;
+      x[j % XB] = {{*(const u32x4 *)(st + xr0 + j * 2048), *(const u32x4 *)(st + (xr0 ^ 64) + j * 2048)}};
+      f[j & 1] = *(const float *)(st + xs0 + j * 4) * s;
     };
     read_row(0);
 #pragma unroll
     for (int t = 0; t < 4 * NS + 2; ++t) {
       const int j = t >> 2, i = t & 3;
-      if (t < 4 * NS) d[t % 3] = group_dot<F32>(w[i], x[j & 1]);
+      if (t < 4 * NS) d[t % 3] = group_dot<F32>(w[i], x[j % XB]);
       if (t >= 2) {
         const int u = t - 2;
 #pragma unroll
@@ -327,17 +356,30 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
         // no instruction: the sums are due here, not after the next group's branch
         asm volatile("" : "+v"(acc[u >> 2][u & 3]));
       }
-      if (i == 1 && j + 1 < NS) read_row(j + 1);  // f of row j - 1 has been used
+      // (f of row j - 1 has been used)
+      if (i == (XB == 2 ? 1 : 3) && j + 1 < NS) read_row(j + 1);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  Codes w0[4], w1[4];
-  block_barrier();  // the ring's last readers, of the item before
-  issue(0, 0);
-  load_w(0, w0);
-  for (int g = 0; g < groups; g += 2) {
-    step(g, w0, w1);
-    step(g + 1, w1, w0);
+  Codes w0[4], w1[4], w2[4];
+  float s0, s1, s2;
+  // the ring's last readers and copies, of the item before
+  wait_vm<0>();
+  block_barrier();
+  issue(0, lds0);
+  load_w(0, w0, s0);
+  __builtin_amdgcn_sched_barrier(0);
+  issue(min(1, G - 1), lds0 + St::BYTES);
+  load_w(min(1, G - 1), w1, s1);
+  int g = 0;  // (without breaks, for which the compiler would wait for every load)
+  for (; g + 3 <= G; g += 3) {
+    step(g, w0, s0, std::true_type(), w2, s2);
+    step(g + 1, w1, s1, std::true_type(), w0, s0);
+    step(g + 2, w2, s2, std::true_type(), w1, s1);
+  }
+  if (g < G) {
+    step(g, w0, s0, std::false_type(), w2, s2);
+    if (g + 1 < G) step(g + 1, w1, s1, std::false_type(), w0, s0);
   }
 
   // 16 neighbouring columns of row 16 j + col
@@ -365,7 +407,7 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
 // the 64 workgroups of an XCD read few tiles and few weights at a time from its L2.
 template <bool F32, int NT>
 __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Stage<NT / 16>::BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[3 * Stage<NT / 16>::BYTES];
   __shared__ TileMap map;
   const int mb = (a.M + TILE_M - 1) / TILE_M;
   const int64_t items = (int64_t)map_tiles(a, NT, map) * mb;
@@ -393,8 +435,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
     n = __builtin_amdgcn_readfirstlane(min(NT, n - t * NT));
     const int ns = (n + 15) / 16;
     if constexpr (NT > 64) {
-      if (ns > 6) run_tile<F32, 8>(a, lds0, lds, e, r0, n, m0);
-      else if (ns > 4) run_tile<F32, 6>(a, lds0, lds, e, r0, n, m0);
+      if (ns > 4) run_tile<F32, 6>(a, lds0, lds, e, r0, n, m0);
     }
     if (ns <= 4) {
       if (ns > 2) run_tile<F32, 4>(a, lds0, lds, e, r0, n, m0);
@@ -402,27 +443,73 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
       else run_tile<F32, 1>(a, lds0, lds, e, r0, n, m0);
     }
   }
+  wait_vm<0>();  // no copy into this workgroup's LDS outlives it
 }
 
 }  // namespace
 
 hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
   const bool f32 = y_dtype == AINFER_ACT_F32;
-  if (a.N > 8 * a.E) {
-    const int nt = f32 ? 64 : 128;
+  if (a.N > 64 * a.E) {
+    const int nt = f32 ? 64 : 96;
     const int64_t most = (int64_t)(a.N / nt + std::min(a.E, a.N)) * ((a.M + TILE_M - 1) / TILE_M);
     const int grid = (int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD);
     if (f32) k_fp8_tiles<true, 64><<<grid, 256, 0, s>>>(a);
-    else k_fp8_tiles<false, 128><<<grid, 256, 0, s>>>(a);
+    else k_fp8_tiles<false, 96><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
   }
   // at most: full tiles, and one that is not full for each expert
-  const int64_t tiles = a.offsets ? a.N / 16 + std::min(a.E, a.N) : (a.N + 15) / 16;
-  const int64_t items = tiles * ((a.M + 15) / 16);
-  const int grid = (int)std::min<int64_t>(items, 1 << 20);
-  if (f32)
-    k_fp8_rows<true><<<grid, 256, 0, s>>>(a, items);
-  else
-    k_fp8_rows<false><<<grid, 256, 0, s>>>(a, items);
+  auto rows = [&](auto ns_c) {
+    constexpr int NS = decltype(ns_c)::value;
+    const int64_t tiles = a.offsets ? a.N / (16 * NS) + std::min(a.E, a.N) : (a.N + 16 * NS - 1) / (16 * NS);
+    const int64_t items = tiles * ((a.M + 63) / 64 * 4);
+    const int grid = (int)std::min<int64_t>(items, 1 << 20);
+    if (f32) k_fp8_rows<true, NS><<<grid, 256, 0, s>>>(a, items);
+    else k_fp8_rows<false, NS><<<grid, 256, 0, s>>>(a, items);
+  };
+  if (a.N > 32 * a.E) rows(std::integral_constant<int, 4>());
+  else if (a.N > 16 * a.E) rows(std::integral_constant<int, 2>());
+  else rows(std::integral_constant<int, 1>());
+  return hipGetLastError();
+}
+
+// A thread writes 16 codes: of a row's neighbouring columns, or (TRANS) of 16 rows.
+template <bool TRANS>
+__global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t *w, int M, int K, int64_t chunks,
+                                                  uint8_t *packed) {
+  const int G = (K + 127) >> 7, MB64 = (M + 63) >> 6;
+  for (int64_t c = blockIdx.x * 256ll + threadIdx.x; c < chunks; c += gridDim.x * 256ll) {
+    const int lane = (int)(c & 63), h = (int)(c >> 6) & 1, i = (int)(c >> 7) & 3;
+    const int64_t t = c >> 9, em = t / G;
+    const int g = (int)(t - em * G), mb = (int)(em % MB64);
+    const int64_t e = em / MB64;
+    const int r = lane & 15, m = mb * 64 + 16 * (r >> 2) + 4 * i + (r & 3);
+    const int k = g * 128 + 64 * h + 16 * (lane >> 4);
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (m < M && k < K) {
+      if constexpr (TRANS) {
+        const uint8_t *from = w + (e * K + k) * M + m;
+#pragma unroll
+        for (int b = 0; b < 16; ++b) v[b >> 2] |= (uint32_t)from[(int64_t)b * M] << (8 * (b & 3));
+      } else {
+        const u32x4 x = *(const u32x4 *)(w + (e * M + m) * K + k);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) v[d] = x[d];
+      }
+    }
+    *(u32x4 *)(packed + c * 16) = u32x4{v[0], v[1], v[2], v[3]};
+  }
+}
+
+size_t fp8_packed_bytes(int E, int M, int K) {
+  return (size_t)E * ((M + 63) / 64) * ((K + 127) / 128) * 8192;
+}
+
+hipError_t launch_fp8_pack(const uint8_t *w, int E, int M, int K, int transpose, uint8_t *packed,
+                           hipStream_t s) {
+  const int64_t chunks = (int64_t)(fp8_packed_bytes(E, M, K) / 16);
+  const int grid = (int)std::min<int64_t>((chunks + 255) / 256, 1 << 20);
+  if (transpose) k_fp8_pack<true><<<grid, 256, 0, s>>>(w, M, K, chunks, packed);
+  else k_fp8_pack<false><<<grid, 256, 0, s>>>(w, M, K, chunks, packed);
   return hipGetLastError();
 }

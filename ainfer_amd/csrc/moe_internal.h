@@ -425,7 +425,7 @@ hipError_t launch_silu_mul_fp8(const void *g, int64_t gld, const void *u, int64_
 hipError_t launch_weight_quant_fp8(const void *w, int dtype, int E, int M, int K, int scale_kind,
                                    uint8_t *q, float *scales, hipStream_t s);
 struct Fp8Args {
-  const uint8_t *w;        // [E][M][K]
+  const uint8_t *w;        // packed
   const float *scales;     // [E][ceil(M / 128)][ceil(K / 128)]
   const uint8_t *q;        // N rows of K codes
   const float *sq;         // [N][ceil(K / 128)]
@@ -434,6 +434,10 @@ struct Fp8Args {
   int64_t q_ld, y_ld;
   int E, M, K, N;
 };
+// rows of 64 and columns of 128, the last ones filled with zeros (moe_fp8_product.hip)
+size_t fp8_packed_bytes(int E, int M, int K);
+hipError_t launch_fp8_pack(const uint8_t *w, int E, int M, int K, int transpose, uint8_t *packed,
+                           hipStream_t s);
 hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s);
 
 // ---- tokens sorted by expert and back (moe_sort.hip) ---------------------------

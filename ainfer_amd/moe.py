@@ -601,12 +601,28 @@ def silu_mul_backward(dact, gate, up, dgate, dup, live=None, stream=None):
     return dgate, dup
 
 
-class Fp8Weights:
-    """The weights of E experts' projection (or one matrix, E = 1) as e4m3 codes
-    w [E][M][K] (float8_e4m3fn or uint8) and fp32 scales
-    [E][ceil(M / 128)][ceil(K / 128)], resident on one device."""
+def weight_quant_fp8(w, pow2=False, stream=None):
+    """e4m3 codes [E][M][K] and scales [E][ceil(M / 128)][ceil(K / 128)] of w [E][M][K] fp32 or
+    bf16 (ainfer_moe_weight_quant_fp8)."""
+    dev = w.get_device()
+    if not (w.dtype in _ACT and w.dim() == 3 and dev >= 0 and w.is_contiguous()):
+        raise L.MoeError("w: contiguous [E][M][K] fp32 or bf16 on a device")
+    E, M, K = w.shape
+    with _on(stream):
+        q = torch.empty(E, M, K, dtype=torch.float8_e4m3fn, device=w.device)
+        s = torch.empty(E, -(-M // 128), -(-K // 128), dtype=torch.float32, device=w.device)
+    _call(L.lib().ainfer_moe_weight_quant_fp8, dev, stream, w.data_ptr(), _ACT[w.dtype], E, M, K,
+          _kind(pow2), q.data_ptr(), s.data_ptr())
+    return q, s
 
-    def __init__(self, w, scales, y_dtype=None):
+
+class Fp8Weights:
+    """The weights of E experts' projection (or one matrix, E = 1), resident on one
+    device: e4m3 codes w [E][M][K] (float8_e4m3fn or uint8) laid out for the product
+    (w itself is not kept), and their fp32 scales [E][ceil(M / 128)][ceil(K / 128)].
+    transpose: the weights are W^T, [E][K][M], for the gradient to x (M a multiple of 16)."""
+
+    def __init__(self, w, scales, y_dtype=torch.bfloat16, transpose=False, stream=None):
         dev = w.get_device()
         if not (w.dtype in _CODES and w.dim() == 3 and dev >= 0 and w.is_contiguous()):
             raise L.MoeError("w: contiguous [E][M][K] codes on a device")
@@ -614,39 +630,27 @@ class Fp8Weights:
         if not (scales.dtype == torch.float32 and scales.get_device() == dev
                 and scales.shape == (E, -(-M // 128), -(-K // 128)) and scales.is_contiguous()):
             raise L.MoeError("scales: contiguous fp32 [E][ceil(M / 128)][ceil(K / 128)] beside w")
-        if y_dtype is not None and y_dtype not in _ACT:
+        if y_dtype not in _ACT:
             raise L.MoeError("y: fp32 or bf16")
-        self.w, self.scales, self.dev, self.y_dtype = w, scales, dev, y_dtype
-        self.structs = {dt: L.Fp8(E, M, K, code, w.data_ptr(), scales.data_ptr())
+        if transpose:
+            M, K = K, M
+        n = L.lib().ainfer_moe_fp8_packed_bytes(E, M, K)
+        if n == 0:
+            raise L.MoeError("weight sizes outside the supported range")
+        with torch.cuda.device(dev), _on(stream):
+            self.packed = torch.empty(n, dtype=torch.uint8, device=w.device)
+            self.scales = scales.transpose(1, 2).contiguous() if transpose else scales
+        _call(L.lib().ainfer_moe_fp8_pack, dev, stream, w.data_ptr(), E, M, K, int(transpose),
+              self.packed.data_ptr(), n)
+        self.shape, self.dev, self.y_dtype = (E, M, K), dev, y_dtype
+        self.structs = {dt: L.Fp8(E, M, K, code, self.packed.data_ptr(), self.scales.data_ptr())
                         for dt, code in _ACT.items()}
-        # no rows: the sizes' own checks
-        L.check(L.lib().ainfer_moe_fp8_product(C.byref(self.structs[torch.float32]), None, 0, None,
-                                               None, 0, None, 0, None))
-
-    @classmethod
-    def quantise(cls, w, pow2=False, y_dtype=None, stream=None):
-        """From w [E][M][K] fp32 or bf16 (ainfer_moe_weight_quant_fp8)."""
-        dev = w.get_device()
-        if not (w.dtype in _ACT and w.dim() == 3 and dev >= 0 and w.is_contiguous()):
-            raise L.MoeError("w: contiguous [E][M][K] fp32 or bf16 on a device")
-        E, M, K = w.shape
-        with _on(stream):
-            q = torch.empty(E, M, K, dtype=torch.float8_e4m3fn, device=w.device)
-            s = torch.empty(E, -(-M // 128), -(-K // 128), dtype=torch.float32, device=w.device)
-        _call(L.lib().ainfer_moe_weight_quant_fp8, dev, stream, w.data_ptr(), _ACT[w.dtype], E, M, K,
-              _kind(pow2), q.data_ptr(), s.data_ptr())
-        return cls(q, s, y_dtype)
-
-    def transposed(self):
-        """[E][K][M], for the gradient to x (laid out once; M a multiple of 16)."""
-        w = self.w.view(torch.uint8).transpose(1, 2).contiguous()
-        return Fp8Weights(w, self.scales.transpose(1, 2).contiguous(), self.y_dtype)
 
     def product(self, q, sq, y=None, offsets=None, stream=None):
         """y [N][M] = x W^T for codes q [N][K] and scales sq of rows sorted by expert
         (offsets [E + 1] int32; may be left out with one expert), in fp32 or bf16
         (ainfer_moe_fp8_product).  Rows outside the offsets keep what y holds."""
-        E, M, K = self.w.shape
+        E, M, K = self.shape
         dev, n, _, ld = _codes(q, "q", K)
         if dev != self.dev:
             raise L.MoeError("q: on the weights' device")
@@ -658,7 +662,7 @@ class Fp8Weights:
             _vector(offsets, "offsets", torch.int32, E + 1, dev)
         if y is None:
             with _on(stream):
-                y = torch.empty(n, M, dtype=self.y_dtype or torch.bfloat16, device=q.device)
+                y = torch.empty(n, M, dtype=self.y_dtype, device=q.device)
         _, ydev, yn, _, yld = _rows(y, "y", M)
         if ydev != dev or yn != n:
             raise L.MoeError("y: a row for each of q's, on its device")
@@ -781,15 +785,18 @@ class Fp8Experts:
     """The routed experts' MLP with 8-bit floating point weights: gate_up [E][2 I][H]
     (gate rows, then up rows) and down [E][H][I], Fp8Weights on one device.  Takes the
     routing of route_scored or MoeLayer.route; ids outside [0, E) (experts of other GPUs)
-    add nothing.  train: also lays out the transposed weights, for backward."""
+    add nothing.  back: the two transposed, Fp8Weights(..., transpose=True), for backward."""
 
-    def __init__(self, gate_up, down, pow2=False, train=False):
-        E, I2, H = gate_up.w.shape
-        if down.w.shape != (E, H, I2 // 2) or I2 % 2 or gate_up.dev != down.dev:
+    def __init__(self, gate_up, down, back=None, pow2=False):
+        E, I2, H = gate_up.shape
+        I = I2 // 2
+        if down.shape != (E, H, I) or I2 % 2 or gate_up.dev != down.dev:
             raise L.MoeError("gate_up [E][2 I][H] and down [E][H][I] on one device")
-        self.gate_up, self.down, self.pow2 = gate_up, down, pow2
-        self.n_experts, self.inter, self.hidden = E, I2 // 2, H
-        self.back = (gate_up.transposed(), down.transposed()) if train else None
+        if back is not None and not (back[0].shape == (E, H, I2) and back[1].shape == (E, I, H)
+                                     and back[0].dev == back[1].dev == down.dev):
+            raise L.MoeError("back: gate_up and down transposed, beside them")
+        self.gate_up, self.down, self.back, self.pow2 = gate_up, down, back, pow2
+        self.n_experts, self.inter, self.hidden = E, I, H
 
     def forward(self, x, idx, w, y=None, resid=None, stream=None, keep=False):
         """y[t] = sum_j w[t][j] expert_{idx[t][j]}(x[t]) (+ resid[t]), x and y [T][H] bf16 or
@@ -813,7 +820,7 @@ class Fp8Experts:
         tensors.  The weights are constants; the products' gradients are quantised to
         e4m3 as the activations are, and each rounding passes its gradient on."""
         if self.back is None:
-            raise L.MoeError("experts laid out with train=True")
+            raise L.MoeError("experts with transposed weights (back)")
         h, o, offsets, pos, w = kept
         I = self.inter
         with torch.cuda.device(self.gate_up.dev), _on(stream):

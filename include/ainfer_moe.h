@@ -552,12 +552,20 @@ int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, i
 int ainfer_moe_weight_quant_fp8(const void *w, int32_t w_dtype, int32_t E, int32_t M, int32_t K,
                                 int32_t scale_kind, uint8_t *q, float *scales, void *stream);
 
+/* Weights laid out for the product, once: W[e][m][k] = w[e][m][k] (w 16-byte aligned), or
+ * w[e][k][m] with transpose, as tiles of 64 x 128 in the order of the matrix instructions'
+ * lanes.  ainfer_moe_fp8_packed_bytes (0: a size out of range) is E M K with M rounded up to
+ * 64 and K to 128; what is behind the matrix is filled with zeros.  packed 16-byte aligned. */
+size_t ainfer_moe_fp8_packed_bytes(int32_t E, int32_t M, int32_t K);
+int ainfer_moe_fp8_pack(const uint8_t *w, int32_t E, int32_t M, int32_t K, int32_t transpose,
+                        uint8_t *packed, size_t packed_bytes, void *stream);
+
 typedef struct ainfer_moe_fp8 {
   int32_t n_experts;   /* E, 1..1024                                         */
   int32_t rows;        /* M, 1..1048576                                      */
   int32_t cols;        /* K, multiple of 16, 16..65536; E M K at most 2^38   */
   int32_t y_dtype;     /* AINFER_ACT_F32 or AINFER_ACT_BF16                  */
-  const uint8_t *w;    /* [E][M][K] e4m3, 16-byte aligned                    */
+  const uint8_t *packed; /* as ainfer_moe_fp8_pack writes them               */
   const float *scales; /* [E][ceil(M / 128)][ceil(K / 128)]                  */
 } ainfer_moe_fp8;
 /* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
@@ -568,8 +576,9 @@ typedef struct ainfer_moe_fp8 {
  * [offsets[0], offsets[E]) are left as they were; offsets outside [0, N] are taken as
  * its ends, and rows of experts that overlap are unspecified.  A NaN code or scale
  * reaches the values whose sums it is in.  y must not overlap anything that is read.
- * The gradient to x is the same call with the transposed weights: [E][K][M] codes and
- * [E][ceil(K / 128)][ceil(M / 128)] scales, as blocks are square. */
+ * The gradient to x is the same call with the transposed weights (M a multiple of 16):
+ * ainfer_moe_fp8_pack(w, E, K, M, 1, ...) and scales [E][ceil(K / 128)][ceil(M / 128)], as
+ * blocks are square. */
 int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_ld,
                            const float *sq, const int32_t *offsets, int32_t N, void *y,
                            int64_t y_ld, void *stream);

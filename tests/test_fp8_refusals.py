@@ -95,6 +95,24 @@ def test_weight_quant(L):
                    dict(q=A), dict(q=A + 16), dict(s=A), dict(s=B + 64)), L.ERR_ARG)
 
 
+def pack(L, w=A, E_=2, M=130, K=272, t=0, p=B, n=1 << 30):
+    return L.lib().ainfer_moe_fp8_pack(w, E_, M, K, t, p, n, None)
+
+
+def test_pack(L):
+    call = lambda **kw: pack(L, **kw)  # noqa: E731
+    refused(call, SIZES, L.ERR_SHAPE)
+    refused(call, (dict(w=None), dict(p=None)), L.ERR_NULL)
+    n = L.lib().ainfer_moe_fp8_packed_bytes(2, 130, 272)
+    assert n == 2 * 192 * 384
+    refused(call, (dict(t=2), dict(t=-1), dict(w=A + 8), dict(p=B + 8), dict(n=n - 1), dict(p=A),
+                   dict(p=A + 65536), dict(w=B + 16)), L.ERR_ARG)
+    for kw in SIZES:
+        d = dict(E_=2, M=130, K=272)
+        d.update(kw)
+        assert L.lib().ainfer_moe_fp8_packed_bytes(d["E_"], d["M"], d["K"]) == 0
+
+
 def product(L, E_=2, M=130, K=272, dtype=1, w=A, s=B, q=D, q_ld=272, sq=E, offsets=F, N=5, y=G,
             y_ld=130, struct=True):
     d = L.Fp8(E_, M, K, dtype, w, s)

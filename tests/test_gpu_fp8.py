@@ -135,16 +135,35 @@ def test_weight_quant(torch, E, M, K, dtype):
     for pow2 in (False, True):
         w = torch.randn(E, M, K, generator=gen(torch, M + K), device="cuda").to(getattr(torch, dtype))
         w[0, 0, 0] = 0
-        f = moe.Fp8Weights.quantise(w, pow2=pow2)
+        q, scales = moe.weight_quant_fp8(w, pow2=pow2)
         b = torch.nn.functional.pad(w.float().cpu(), (0, -K % 128, 0, -M % 128))
         b = b.view(E, R.groups(M), 128, R.groups(K), 128)
         s = R.scale_of(b.abs().amax((2, 4)), pow2)
-        assert torch.equal(f.scales.cpu(), s)
+        assert torch.equal(scales.cpu(), s)
         want = (b / s[:, :, None, :, None]).reshape(E, R.groups(M) * 128, -1)[:, :M, :K]
-        same_codes(torch, f.w, want.to(R.E4M3))
-        t = f.transposed() if M % 16 == 0 else None
-        if t is not None:
-            same_codes(torch, t.w.view(R.E4M3), f.w.transpose(1, 2).cpu())
+        same_codes(torch, q, want.to(R.E4M3))
+
+
+@pytest.mark.parametrize("E,M,K", ((1, 1, 16), (2, 64, 128), (3, 130, 144), (1, 65, 272), (2, 304, 400)))
+def test_pack(torch, E, M, K):
+    """Tiles of 64 x 128: tile i's row r is row 16 (r / 4) + 4 i + r % 4, two halves of 64
+    columns, 16 of each quarter to lane 16 quarter + r; zeros behind the matrix."""
+    from ainfer_amd import _lib as L
+    from ainfer_amd import moe
+    w = torch.randint(0, 256, (E, M, K), device="cuda", dtype=torch.uint8)
+    mb, G = -(-M // 64), R.groups(K)
+    full = torch.zeros(E, mb * 64, G * 128, dtype=torch.uint8, device="cuda")
+    full[:, :M, :K] = w
+    # [e][mb][r / 4][i][r % 4][g][half][quarter][16] -> [e][mb][g][i][half][quarter][r][16]
+    want = full.view(E, mb, 4, 4, 4, G, 2, 4, 16).permute(0, 1, 5, 3, 6, 7, 2, 4, 8).reshape(-1)
+    f = moe.Fp8Weights(w, torch.ones(E, R.groups(M), G, device="cuda"))
+    assert f.packed.numel() == want.numel() == L.lib().ainfer_moe_fp8_packed_bytes(E, M, K)
+    assert torch.equal(f.packed, want)
+    t = w.transpose(1, 2).contiguous()
+    s = torch.rand(E, G, R.groups(M), device="cuda")
+    b = moe.Fp8Weights(t, s, transpose=True)
+    assert torch.equal(b.packed, want) and torch.equal(b.scales, s.transpose(1, 2))
+    assert b.shape == (E, M, K)
 
 
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))

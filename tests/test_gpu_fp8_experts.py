@@ -21,14 +21,20 @@ def torch():
     return torch
 
 
-def experts(torch, E, H, I, pow2=False, train=True, y_dtype=None):
+def experts(torch, E, H, I, pow2=False, y_dtype=None):
+    """(experts with their transposed weights, the weights' 64-bit values)"""
     from ainfer_amd import moe
     g = torch.Generator(device="cuda")
     g.manual_seed(E + H)
-    gu = torch.randn(E, 2 * I, H, generator=g, device="cuda") * H ** -0.5
-    dn = torch.randn(E, H, I, generator=g, device="cuda") * I ** -0.5
-    return moe.Fp8Experts(moe.Fp8Weights.quantise(gu, pow2, y_dtype),
-                          moe.Fp8Weights.quantise(dn, pow2, y_dtype), pow2=pow2, train=train)
+    fwd, back, dense = [], [], []
+    for M, K in ((2 * I, H), (H, I)):
+        w = torch.randn(E, M, K, generator=g, device="cuda") * K ** -0.5
+        q, s = moe.weight_quant_fp8(w, pow2)
+        dt = y_dtype or torch.bfloat16
+        fwd.append(moe.Fp8Weights(q, s, dt))
+        back.append(moe.Fp8Weights(q, s, dt, transpose=True))
+        dense.append(q.double() * R.wide(R.wide(s.double(), 2, K), 1, M))
+    return moe.Fp8Experts(*fwd, back=back, pow2=pow2), dense
 
 
 def routed(torch, T, k, E, H, dtype, seed=0):
@@ -42,14 +48,8 @@ def routed(torch, T, k, E, H, dtype, seed=0):
     return x, idx, w
 
 
-def dense(torch, f):
-    """The weights of an Fp8Weights as 64-bit values."""
-    E, M, K = f.w.shape
-    return f.w.double() * R.wide(R.wide(f.scales.double(), 2, K), 1, M)
-
-
-def plain(torch, ex, x, idx, w):
-    gu, dn = dense(torch, ex.gate_up), dense(torch, ex.down)
+def plain(torch, ex, dense, x, idx, w):
+    gu, dn = dense
     I = ex.inter
     y = torch.zeros(x.shape, dtype=torch.float64, device="cuda")
     for e in range(ex.n_experts):
@@ -69,11 +69,11 @@ def test_forward(torch, T, k, E, H, I, dtype):
     print(f"[case] experts {T} {k} {E} {H} {I} {dtype}", flush=True)
     dt = getattr(torch, dtype)
     for pow2 in (False, True):
-        ex = experts(torch, E, H, I, pow2)
+        ex, dense = experts(torch, E, H, I, pow2)
         x, idx, w = routed(torch, T, k, E, H, dt)
         idx[::3, 0] = E + 2  # experts of another GPU
         y = ex.forward(x, idx, w)
-        ref = plain(torch, ex, x, idx, w)
+        ref = plain(torch, ex, dense, x, idx, w)
         assert (y.double() - ref).norm() <= 0.14 * ref.norm()
         q, sq, off, pos = moe.sort_rows(x, idx, E, moe.sort_workspace(T, k, E), fp8=True, pow2=pow2)
         h = ex.gate_up.product(q, sq, offsets=off)
@@ -86,7 +86,7 @@ def test_forward(torch, T, k, E, H, I, dtype):
 
 
 def test_no_tokens_and_no_kept_pairs(torch):
-    ex = experts(torch, 4, 256, 128)
+    ex, _ = experts(torch, 4, 256, 128)
     x, idx, w = routed(torch, 5, 2, 4, 256, torch.bfloat16)
     assert ex.forward(x[:0], idx[:0], w[:0]).shape == (0, 256)
     y, kept = ex.forward(x, torch.full_like(idx, 9), w, keep=True)
@@ -101,7 +101,7 @@ def test_no_tokens_and_no_kept_pairs(torch):
 def test_backward(torch, T, k, E, H, I):
     """dw against <dy, the rows that forward kept>, dx against the 64-bit chain from the
     kept rows, with the weights' values."""
-    ex = experts(torch, E, H, I, y_dtype=torch.float32)
+    ex, (gu, dn) = experts(torch, E, H, I, y_dtype=torch.float32)
     x, idx, w = routed(torch, T, k, E, H, torch.float32)
     idx[::3, 0] = -1
     g = torch.Generator(device="cuda")
@@ -115,7 +115,6 @@ def test_backward(torch, T, k, E, H, I):
     terms = dy.double()[:, None, :] * o.double()[at]
     want = torch.where(there, terms.sum(2), 0.0)
     assert ((dw.double() - want).abs() <= (H + 8) * 2.0 ** -24 * terms.abs().sum(2) + 1e-30).all()
-    gu, dn = dense(torch, ex.gate_up), dense(torch, ex.down)
     ref = torch.zeros_like(dx, dtype=torch.float64)
     for e in range(E):
         t, j = torch.nonzero(idx == e, as_tuple=True)
@@ -129,7 +128,7 @@ def test_backward(torch, T, k, E, H, I):
 
 def test_gradient_of_the_routing_weights_by_differences(torch):
     """The output is linear in w: one step is the slope."""
-    ex = experts(torch, 8, 256, 128, y_dtype=torch.float32)
+    ex, _ = experts(torch, 8, 256, 128, y_dtype=torch.float32)
     x, idx, w = routed(torch, 60, 3, 8, 256, torch.float32)
     dy = torch.randn(60, 256, device="cuda")
     y, kept = ex.forward(x, idx, w, keep=True)
@@ -142,7 +141,7 @@ def test_gradient_of_the_routing_weights_by_differences(torch):
 
 def test_captured_step(torch):
     """A forward and backward step in a graph, replayed on new tokens."""
-    ex = experts(torch, 8, 256, 128)
+    ex, _ = experts(torch, 8, 256, 128)
     for T in (2, 300):
         x, idx, w = routed(torch, T, 3, 8, 256, torch.bfloat16)
         dy = torch.randn(T, 256, device="cuda").to(torch.bfloat16)
