@@ -68,155 +68,11 @@ __device__ __forceinline__ f32x4 group_dot(const Codes &a, const Codes &b) {
   }
 }
 
-struct Tile {
-  int e, r0, n;  // expert, first row, rows; n = 0: none
-};
-
-// Tile `tile` of NT rows, in the order of the experts' rows.  offsets (what the caller
-// gives) are taken as rows of [0, N), whatever they hold.  256 threads, E <= 1024.
-template <int NT>
-__device__ __forceinline__ Tile find_tile(const int32_t *offsets, int E, int N, int64_t tile) {
-  __shared__ Tile found;
-  __shared__ int32_t part[4];
-  if (!offsets) {
-    const int64_t r0 = tile * NT;
-    return Tile{0, (int)r0, (int)min((int64_t)NT, max((int64_t)0, N - r0))};
-  }
-  const int tid = threadIdx.x, wave = tid >> 6;
-  int start[4], rows[4], tiles = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = min(tid * 4 + i, E - 1);
-    start[i] = max(0, min(offsets[e], N));
-    rows[i] = tid * 4 + i < E ? max(0, min(offsets[e + 1], N) - start[i]) : 0;
-    tiles += (rows[i] + NT - 1) / NT;
-  }
-  const int incl = wave_scan_incl(tiles);
-  __syncthreads();  // the last call's readers of found and part
-  if (tid == 0) found = Tile{0, 0, 0};
-  if ((tid & 63) == 63) part[wave] = incl;
-  __syncthreads();
-  int64_t at = tile - (incl - tiles);
-  for (int w = 0; w < wave; ++w) at -= part[w];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = (rows[i] + NT - 1) / NT;
-    if (at >= 0 && at < c)
-      found = Tile{tid * 4 + i, start[i] + (int)at * NT, min(NT, rows[i] - (int)at * NT)};
-    at -= c;
-  }
-  __syncthreads();
-  return found;
-}
-
 // the packed tile i of rows 64 mb .. +63 and group g
 __device__ __forceinline__ const uint8_t *tile_at(const Fp8Args &a, int e, int mb, int g, int i) {
   const int G = (a.K + 127) >> 7, MB64 = (a.M + 63) >> 6;
   return a.w + (((int64_t)e * MB64 + mb) * G + g) * 8192 + i * 2048;
 }
-
-// ---- rows -------------------------------------------------------------------------
-// 16 weight rows x at most 16 NS rows of x: four waves take every fourth group of 128
-// columns, and their sums are added in the waves' order.
-template <bool F32, int NS>
-__global__ __launch_bounds__(256) void k_fp8_rows(Fp8Args a, int64_t items) {
-  __shared__ f32x4 sums[3][NS][64];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slabs = (a.M + 63) / 64 * 4, G = (a.K + 127) / 128, MB = (a.M + 127) / 128;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const Tile t = find_tile<16 * NS>(a.offsets, a.E, a.N, it / slabs);
-    if (t.n == 0) return;  // no tile from here on
-    const int slab = (int)(it % slabs), mb = slab >> 2, i = slab & 3;
-    const uint8_t *wt = tile_at(a, t.e, mb, 0, i) + lane * 16;
-    const float *sw = a.scales + ((int64_t)t.e * MB + mb / 2) * G;
-    const uint8_t *xr[NS];
-    const float *sx[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const int64_t row = t.r0 + min(16 * j + c, t.n - 1);
-      xr[j] = a.q + row * a.q_ld;
-      sx[j] = a.sq + row * G;
-    }
-    f32x4 acc[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto group = [&](int g) __attribute__((always_inline)) {
-      const int col = g * 128 + qd * 16;
-      Codes w;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w.v[h] = __builtin_nontemporal_load((const u32x4 *)(wt + (int64_t)g * 8192 + h * 1024));
-      const float s = sw[g];
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        Codes x;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          x.v[h] = col + 64 * h < a.K ? *(const u32x4 *)(xr[j] + col + 64 * h) : u32x4{0, 0, 0, 0};
-        const f32x4 d = group_dot<F32>(w, x);
-        const float f = sx[j][g] * s;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, d[r], acc[j][r]);
-      }
-    };
-    int g = wave;
-    for (; g + 12 < G; g += 16) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) group(g + 4 * u);
-    }
-    for (; g < G; g += 4) group(g);
-    if (wave > 0) {
-#pragma unroll
-      for (int j = 0; j < NS; ++j) sums[wave - 1][j][lane] = acc[j];
-    }
-    __syncthreads();
-    if (wave == 0) {
-      const int m = mb * 64 + 16 * qd + 4 * i;
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        if (16 * j + c >= t.n) continue;
-        const int64_t at = (int64_t)(t.r0 + 16 * j + c) * a.y_ld + m;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = ((acc[j][r] + sums[0][j][lane][r]) + sums[1][j][lane][r]) + sums[2][j][lane][r];
-          if (m + r < a.M) store_one<F32>(a.y, at + r, v);
-        }
-      }
-    }
-    __syncthreads();
-  }
-}
-
-// ---- tiles ------------------------------------------------------------------------
-// 256 weight rows x NS * 16 rows of x in a workgroup of four waves, each 64 of the weight
-// rows: weights go from global memory into registers (no wave shares them), one group
-// ahead; rows of x and their scales go through two stages of LDS by DMA, shared by the
-// waves.  Two workgroups fit a CU, so that one's waits run under the other's products.
-//
-// Weight row r of a wave's tile i (four tiles of 16) is row 16 (r / 4) + 4 i + r % 4 of the
-// 64, so that a lane ends with 16 neighbouring columns of a row of y.
-constexpr int TILE_M = 256;
-
-// Lane l's 16 or 4 bytes at `off` of the buffer to the wave's LDS address + 16 l or 4 l (zeros
-// where off is behind the buffer).  The compiler counts the copy among the loads in flight but
-// is not told what it writes, so that it waits for none of them before a read of the ring:
-// step() does.  (A global_load_lds would do that too, but counts as an access of both
-// memories, for which the compiler waits until nothing is in flight.)
-typedef __attribute__((address_space(3))) void lds_void;
-__device__ __forceinline__ void dma_x4(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 16, off, 0, 0, 0);
-}
-__device__ __forceinline__ void dma_x1(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 4, off, 0, 0, 0);
-}
-
-template <int NS>
-struct Stage {
-  static constexpr int DMA = NS == 1 ? 1 : NS / 2;  // 16-byte copies a lane, of four waves
-  static constexpr int X = DMA * 4096;              // codes: 128 bytes a row
-  static constexpr int BYTES = X + 1024;            // scales: one a lane
-};
 
 // where the rows of each expert's tiles are: tiles before expert e, by 256 threads
 struct TileMap {
@@ -260,6 +116,196 @@ __device__ __forceinline__ int map_tiles(const Fp8Args &a, int nt, TileMap &map)
   __syncthreads();
   return __builtin_amdgcn_readfirstlane(map.before[a.E]);
 }
+
+// the last expert that starts at or before the tile: the one that holds it
+__device__ __forceinline__ int expert_of_tile(const TileMap &map, int E, int tile) {
+  int lo = 0, hi = E;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (map.before[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Lane l's 16 or 4 bytes at `off` of the buffer to the wave's LDS address + 16 l or 4 l (zeros
+// where off is behind the buffer).  The compiler counts the copy among the loads in flight but
+// is not told what it writes, so that it waits for none of them before a read of the ring:
+// step() does.  (A global_load_lds would do that too, but counts as an access of both
+// memories, for which the compiler waits until nothing is in flight.)
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ void dma_x4(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void dma_x1(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void *)(uintptr_t)to, 4, off, 0, 0, 0);
+}
+
+// ---- split ------------------------------------------------------------------------
+// 16 R weight rows x 16 NS rows of x in a workgroup of four waves that take every fourth
+// group of 128 columns each; their sums are added in the waves' order.  For calls with too few
+// 256-row tiles to fill the CUs.  Each wave copies its own rows of x into LDS of its own
+// (no barriers), three stages, two groups ahead, and loads its weights into registers.
+template <int NS>
+struct Share {
+  static constexpr int X = NS * 2048;
+  static constexpr int BYTES = X + 256;  // a stage of one wave: codes, scales
+};
+
+template <bool F32, int R, int NS>
+__global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
+  using Sh = Share<NS>;
+  constexpr int RING = 4 * 3 * Sh::BYTES, SUMS = 3 * R * NS * 1024;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[RING > SUMS ? RING : SUMS];
+  __shared__ TileMap map;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, qd = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int slabs = (a.M + 63) / 64 * (4 / R), G = (a.K + 127) >> 7, MB = (a.M + 127) >> 7;
+  const uint8_t *mine = lds + wave * 3 * Sh::BYTES;
+  const uint32_t mine0 = (uint32_t)(uintptr_t)lds + (uint32_t)(wave * 3 * Sh::BYTES);
+  const int64_t items = (int64_t)map_tiles(a, 16 * NS, map) * slabs;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int tile = (int)(it / slabs), e = expert_of_tile(map, a.E, tile);
+    int r0, n;
+    clamp_rows(a, e, r0, n);
+    const int before = __builtin_amdgcn_readfirstlane(tile - map.before[e]) * 16 * NS;
+    r0 = __builtin_amdgcn_readfirstlane(r0 + before);
+    n = __builtin_amdgcn_readfirstlane(min(16 * NS, n - before));
+    const int slab = (int)(it % slabs), mb = slab / (4 / R), i0 = slab % (4 / R) * R;
+    const uint8_t *wbase = tile_at(a, e, mb, 0, i0) + lane * 16;
+    int zero = 0;  // opaque: a vector load is in the counts below, a scalar one would not be
+    asm volatile("" : "+v"(zero));
+    const float *sw = a.scales + ((int64_t)e * MB + (mb >> 1)) * G + zero;
+    const __amdgpu_buffer_rsrc_t xbuf =
+        make_rsrc(a.q + (int64_t)r0 * a.q_ld, (uint32_t)(n - 1) * (uint32_t)a.q_ld + (uint32_t)a.K);
+    const __amdgpu_buffer_rsrc_t sbuf = make_rsrc(a.sq + (int64_t)r0 * G, (uint32_t)(n * G) * 4u);
+    // as in the tiles: chunk (s & 7) ^ (row & 7) of row s >> 3 in slot s
+    uint32_t xoff[2 * NS];
+    const uint32_t xcol = (uint32_t)(((lane & 7) ^ (lane >> 3)) * 16);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i)
+      xoff[i] = (uint32_t)min(8 * i + (lane >> 3), n - 1) * (uint32_t)a.q_ld + xcol;
+    const uint32_t soff = (uint32_t)min(16 * (lane % NS) + lane / NS, n - 1) * (uint32_t)G * 4u;
+    struct Group {
+      Codes w[R];
+      float s;
+    };
+    const int mineG = (G - wave + 3) / 4;  // groups wave, wave + 4, ...
+    auto issue = [&](int u, int stage, Group &next) __attribute__((always_inline)) {
+      const int g = wave + 4 * u;
+      const bool past = g * 128 + xcol >= (uint32_t)a.K;
+      const uint32_t to = mine0 + (uint32_t)(stage * Sh::BYTES);
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i)
+        dma_x4(xbuf, past ? BUF_OOB : xoff[i] + g * 128, to + (uint32_t)(i * 1024));
+      dma_x1(sbuf, soff + g * 4, to + Sh::X);
+      // the loads of weights stay behind the copies: step() counts on it
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      next.s = sw[g];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          next.w[i].v[h] = __builtin_nontemporal_load(
+              (const u32x4 *)(wbase + (int64_t)g * 8192 + i * 2048 + h * 1024));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x4 acc[NS][R];
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+      for (int i = 0; i < R; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t xr0 = (uint32_t)(col * 128 + ((qd ^ (col & 7)) << 4));
+    // the wave's group u, in a stage; behind its DMA there are its own 2 R + 1 loads and all
+    // of the next group's
+    auto step = [&](int u, int stage, Group &c, auto loads, int fill, Group &next)
+                    __attribute__((always_inline)) {
+      constexpr bool LOADS = decltype(loads)::value;
+      if constexpr (LOADS) {
+        wait_vm<2 * (2 * R + 1) + 2 * NS + 1>();
+        issue(min(u + 2, mineG - 1), fill, next);
+      } else {
+        wait_vm<0>();
+      }
+      const uint8_t *st = mine + stage * Sh::BYTES;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const Codes x = {{*(const u32x4 *)(st + xr0 + j * 2048), *(const u32x4 *)(st + (xr0 ^ 64) + j * 2048)}};
+        const float f = *(const float *)(st + Sh::X + (col * NS + j) * 4) * c.s;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const f32x4 d = group_dot<F32>(c.w[i], x);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(f, d[r], acc[j][i][r]);
+        }
+      }
+      // the stage has been read before it is filled again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    Group c0, c1, c2;
+    if (mineG > 0) {
+      issue(0, 0, c0);
+      issue(min(1, mineG - 1), 1, c1);
+    }
+    int u = 0;
+    for (; u + 3 <= mineG; u += 3) {
+      step(u, 0, c0, std::true_type(), 2, c2);
+      step(u + 1, 1, c1, std::true_type(), 0, c0);
+      step(u + 2, 2, c2, std::true_type(), 1, c1);
+    }
+    if (u < mineG) {
+      step(u, 0, c0, std::false_type(), 2, c2);
+      if (u + 1 < mineG) step(u + 1, 1, c1, std::false_type(), 0, c0);
+    }
+    wait_vm<0>();  // no copy into the ring is in flight
+    __syncthreads();
+    f32x4 *sums = (f32x4 *)lds;
+    if (wave > 0) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j)
+#pragma unroll
+        for (int i = 0; i < R; ++i) sums[((wave - 1) * NS * R + j * R + i) * 64 + lane] = acc[j][i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int m = mb * 64 + 16 * qd + 4 * i0;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        if (16 * j + col >= n) continue;
+        const int64_t at = (int64_t)(r0 + 16 * j + col) * a.y_ld + m;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          f32x4 v = acc[j][i];
+#pragma unroll
+          for (int w = 0; w < 3; ++w) v += sums[(w * NS * R + j * R + i) * 64 + lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (m + 4 * i + r < a.M) store_one<F32>(a.y, at + 4 * i + r, v[r]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- tiles ------------------------------------------------------------------------
+// 256 weight rows x NS * 16 rows of x in a workgroup of four waves, each 64 of the weight
+// rows: weights go from global memory into registers (no wave shares them), one group
+// ahead; rows of x and their scales go through two stages of LDS by DMA, shared by the
+// waves.  Two workgroups fit a CU, so that one's waits run under the other's products.
+//
+// Weight row r of a wave's tile i (four tiles of 16) is row 16 (r / 4) + 4 i + r % 4 of the
+// 64, so that a lane ends with 16 neighbouring columns of a row of y.
+constexpr int TILE_M = 256;
+
+template <int NS>
+struct Stage {
+  static constexpr int DMA = NS == 1 ? 1 : NS / 2;  // 16-byte copies a lane, of four waves
+  static constexpr int X = DMA * 4096;              // codes: 128 bytes a row
+  static constexpr int BYTES = X + 1024;            // scales: one a lane
+};
 
 template <bool F32, int NS>
 __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const uint8_t *lds,
@@ -416,13 +462,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
   for (int64_t it = items * xcd / N_XCD + blockIdx.x / N_XCD; it < end; it += slots) {
     const int tile = (int)(it / mb);
-    int lo = 0, hi = a.E;  // the last expert that starts at or before the tile
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (map.before[mid] <= tile) lo = mid;
-      else hi = mid;
-    }
-    const int e = __builtin_amdgcn_readfirstlane(lo);
+    const int e = expert_of_tile(map, a.E, tile);
     int r0, n;
     clamp_rows(a, e, r0, n);
     const int first = __builtin_amdgcn_readfirstlane(map.before[e]);
@@ -450,26 +490,49 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
 
 hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
   const bool f32 = y_dtype == AINFER_ACT_F32;
-  if (a.N > 64 * a.E) {
-    const int nt = f32 ? 64 : 96;
-    const int64_t most = (int64_t)(a.N / nt + std::min(a.E, a.N)) * ((a.M + TILE_M - 1) / TILE_M);
+  const int nt = f32 ? 64 : 96, G = (a.K + 127) / 128;
+  // what the host knows: at most `used` experts with rows, `each` rows of one on average
+  const int64_t used = std::min(a.E, a.N), each = a.N / used;
+  const int64_t slabs = (a.M + 63) / 64, mb = (a.M + TILE_M - 1) / TILE_M;
+  auto row_tiles = [&](int rows) { return std::max<int64_t>(used, (a.N + rows - 1) / rows); };
+  // Tiles or split, us (bf16; rows x K -> M).  A tile's workgroup takes its K groups one by one,
+  // 0.22 + 0.115 us for each 16 rows of x (latency) while its CU is not full, and a split
+  // item's four waves 7.5e-6 us a column, so few items of many rows are split:
+  //   256 x 4096 -> 4096 20.5 split, 32.7 tiles; 512 x 4096 -> 4096 36.0, 35.8;
+  //   256 x 5120 -> 17408 119, 47; 8 experts of 32 rows, 4096 -> 2048 17.2, 28.5;
+  //   64 experts of 32 rows, 4096 -> 2048 114, 98; 96 of 21, 2560 -> 1792 96, 89.
+  // With few rows an expert both read weights at the speed of the memory, and the split form
+  // gets more of it where its waves have 8 groups or more: 16 experts of 4 rows, 4096 -> 2048
+  // 25, 31; 64 of 8 86, 95; but 256 of 1, 2048 -> 1024 47, 44, and 512 of 1, 1024 -> 2048 32, 28.
+  const int64_t items2 = row_tiles(32) * slabs, tile_items = row_tiles(nt) * mb;
+  const int64_t ns = std::min<int64_t>(nt / 16, (each + 15) / 16);
+  const int64_t few = (226 + 120 * ns) * std::max<int64_t>(512, tile_items) / 512 * (f32 ? 13 : 10) / 10;
+  if (items2 > few && (each > 12 || G < 32)) {
+    // at most: full tiles, and one that is not full for each expert
+    const int64_t most = (a.N / nt + used) * mb;
     const int grid = (int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD);
     if (f32) k_fp8_tiles<true, 64><<<grid, 256, 0, s>>>(a);
     else k_fp8_tiles<false, 96><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
   }
-  // at most: full tiles, and one that is not full for each expert
-  auto rows = [&](auto ns_c) {
-    constexpr int NS = decltype(ns_c)::value;
-    const int64_t tiles = a.offsets ? a.N / (16 * NS) + std::min(a.E, a.N) : (a.N + 16 * NS - 1) / (16 * NS);
-    const int64_t items = tiles * ((a.M + 63) / 64 * 4);
-    const int grid = (int)std::min<int64_t>(items, 1 << 20);
-    if (f32) k_fp8_rows<true, NS><<<grid, 256, 0, s>>>(a, items);
-    else k_fp8_rows<false, NS><<<grid, 256, 0, s>>>(a, items);
+  auto split = [&](auto r_c, auto ns_c) {
+    constexpr int R = decltype(r_c)::value, NS = decltype(ns_c)::value;
+    const int64_t items = (a.N / (16 * NS) + used) * slabs * (4 / R);
+    const int grid = (int)std::min<int64_t>(items, R == 4 ? 512 : 1024);
+    if (f32) k_fp8_split<true, R, NS><<<grid, 256, 0, s>>>(a);
+    else k_fp8_split<false, R, NS><<<grid, 256, 0, s>>>(a);
   };
-  if (a.N > 32 * a.E) rows(std::integral_constant<int, 4>());
-  else if (a.N > 16 * a.E) rows(std::integral_constant<int, 2>());
-  else rows(std::integral_constant<int, 1>());
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
+  using four = std::integral_constant<int, 4>;
+  // Larger items read less, smaller ones are more: 16 weight rows for a single tile of rows
+  // (1 x 5120 -> 17408 17.5, 19.2 with 32); tiles of 32 rows from 128 items of them on
+  // (32 x 4096 -> 4096 9.0 with 16, 10.5; 64 x 4096 -> 4096 12.2, 10.3), 64 weight rows
+  // from 256 on (64 x 4096 -> 4096 10.3 with 32, 13.5; 128 x 4096 -> 4096 15.8, 13.2).
+  if (each > 16 && items2 >= 256) split(four(), two());
+  else if (each > 16 && items2 >= 128) split(two(), two());
+  else if (row_tiles(16) > 1) split(two(), one());
+  else split(one(), one());
   return hipGetLastError();
 }
 
