@@ -302,7 +302,7 @@ constexpr int TILE_M = 256;
 
 template <int NS>
 struct Stage {
-  static constexpr int DMA = NS == 1 ? 1 : NS / 2;  // 16-byte copies a lane, of four waves
+  static constexpr int DMA = (NS + 1) / 2;          // 16-byte copies a lane, of four waves
   static constexpr int X = DMA * 4096;              // codes: 128 bytes a row
   static constexpr int BYTES = X + 1024;            // scales: one a lane
 };
@@ -471,16 +471,18 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
     const int band = (int)(local / (8 * mb)), in_band = (int)(local - (int64_t)band * 8 * mb);
     const int wide = min(8, tiles - 8 * band);
     const int t = 8 * band + in_band % wide, m0 = in_band / wide * TILE_M;
-    r0 = __builtin_amdgcn_readfirstlane(r0 + t * NT);
-    n = __builtin_amdgcn_readfirstlane(min(NT, n - t * NT));
-    const int ns = (n + 15) / 16;
-    if constexpr (NT > 64) {
-      if (ns > 4) run_tile<F32, 6>(a, lds0, lds, e, r0, n, m0);
-    }
-    if (ns <= 4) {
-      if (ns > 2) run_tile<F32, 4>(a, lds0, lds, e, r0, n, m0);
-      else if (ns == 2) run_tile<F32, 2>(a, lds0, lds, e, r0, n, m0);
-      else run_tile<F32, 1>(a, lds0, lds, e, r0, n, m0);
+    // the expert's 16s of rows shared evenly by its tiles
+    const int units = (n + 15) / 16;
+    const int u0 = (int)((int64_t)units * t / tiles), ns = (int)((int64_t)units * (t + 1) / tiles) - u0;
+    r0 = __builtin_amdgcn_readfirstlane(r0 + 16 * u0);
+    n = __builtin_amdgcn_readfirstlane(min(16 * ns, n - 16 * u0));
+    switch (__builtin_amdgcn_readfirstlane(ns)) {
+    case 1: run_tile<F32, 1>(a, lds0, lds, e, r0, n, m0); break;
+    case 2: run_tile<F32, 2>(a, lds0, lds, e, r0, n, m0); break;
+    case 3: run_tile<F32, 3>(a, lds0, lds, e, r0, n, m0); break;
+    case 4: run_tile<F32, 4>(a, lds0, lds, e, r0, n, m0); break;
+    case 5: if constexpr (NT > 64) run_tile<F32, 5>(a, lds0, lds, e, r0, n, m0); break;
+    case 6: if constexpr (NT > 64) run_tile<F32, 6>(a, lds0, lds, e, r0, n, m0); break;
     }
   }
   wait_vm<0>();  // no copy into this workgroup's LDS outlives it
