@@ -35,19 +35,23 @@ template <bool F32>
 __device__ __forceinline__ float load_one(const void *p, int64_t at) {
   return F32 ? ((const float *)p)[at] : bf16_to_f32(((const uint16_t *)p)[at]);
 }
-template <bool F32, int N>
+template <bool F32, int N, bool NT = false>
 __device__ __forceinline__ void store_row(void *p, int64_t at, const float (&v)[N]) {
   if constexpr (F32) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *(f32x4_any *)((float *)p + at + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    for (int i = 0; i < N; i += 4) {
+      const f32x4 w = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+      if constexpr (NT) __builtin_nontemporal_store(w, (f32x4_any *)((float *)p + at + i));
+      else *(f32x4_any *)((float *)p + at + i) = w;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 8) {
       u32x4 w;
 #pragma unroll
       for (int d = 0; d < 4; ++d) w[d] = bf16x2_bits(v[i + 2 * d], v[i + 2 * d + 1]);
-      *(u32x4_any *)((uint16_t *)p + at + i) = w;
+      if constexpr (NT) __builtin_nontemporal_store(w, (u32x4_any *)((uint16_t *)p + at + i));
+      else *(u32x4_any *)((uint16_t *)p + at + i) = w;
     }
   }
 }

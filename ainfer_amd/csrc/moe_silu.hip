@@ -31,18 +31,6 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float (&v)[8]) 
   }
 }
 template <bool F32>
-__device__ __forceinline__ void store8(void *p, int64_t at, const float (&v)[8]) {
-  if constexpr (F32) {
-    *(f32x4_any *)((float *)p + at) = f32x4{v[0], v[1], v[2], v[3]};
-    *(f32x4_any *)((float *)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  } else {
-    u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = bf16x2_bits(v[2 * i], v[2 * i + 1]);
-    *(u32x4_any *)((uint16_t *)p + at) = w;
-  }
-}
-template <bool F32>
 __device__ __forceinline__ float load1(const void *p, int64_t at) {
   return F32 ? ((const float *)p)[at] : bf16_to_f32(((const uint16_t *)p)[at]);
 }
@@ -92,6 +80,33 @@ __device__ __forceinline__ void silu_grad(float d, float g, float u, float &dg, 
   du = d * (g * sig);
 }
 
+// eight values read and written past the caches where that is one piece of 16 bytes a lane
+// (32768 x 1024 bf16: 60.3 us, 66.0 with ordinary accesses; with fp32's two pieces a lane
+// 177 instead of 155 us for 40000 x 1000)
+template <bool F32>
+__device__ __forceinline__ void load8_once(const void *p, int64_t at, float (&v)[8]) {
+  if constexpr (F32) {
+    load8<F32>(p, at, v);
+  } else {
+    const u32x4 a = __builtin_nontemporal_load((const u32x4_any *)((const uint16_t *)p + at));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = __uint_as_float(i & 1 ? a[i / 2] & 0xFFFF0000u : a[i / 2] << 16);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void store8_once(void *p, int64_t at, const float (&v)[8]) {
+  if constexpr (F32) {
+    *(f32x4_any *)((float *)p + at) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4_any *)((float *)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = bf16x2_bits(v[2 * i], v[2 * i + 1]);
+    __builtin_nontemporal_store(w, (u32x4_any *)((uint16_t *)p + at));
+  }
+}
+
 // a lane takes 8 values of a row, the last lane of a row what is left of it
 template <bool F32>
 __global__ __launch_bounds__(256) void k_silu_bwd(const void *d, int64_t dld, const void *g,
@@ -106,9 +121,9 @@ __global__ __launch_bounds__(256) void k_silu_bwd(const void *d, int64_t dld, co
     const int64_t dgat = row * dgld + col, duat = row * duld + col;
     if (I - col >= 8) {
       float dv[8], gv[8], uv[8];
-      load8<F32>(d, dat, dv);
-      load8<F32>(g, gat, gv);
-      load8<F32>(u, uat, uv);
+      load8_once<F32>(d, dat, dv);
+      load8_once<F32>(g, gat, gv);
+      load8_once<F32>(u, uat, uv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float a, b;
@@ -116,8 +131,8 @@ __global__ __launch_bounds__(256) void k_silu_bwd(const void *d, int64_t dld, co
         gv[i] = a;
         uv[i] = b;
       }
-      store8<F32>(dg, dgat, gv);
-      store8<F32>(du, duat, uv);
+      store8_once<F32>(dg, dgat, gv);
+      store8_once<F32>(du, duat, uv);
     } else {
       for (int i = 0; i < I - col; ++i) {
         float a, b;
