@@ -307,7 +307,7 @@ struct Stage {
   static constexpr int BYTES = X + 1024;            // scales: one a lane
 };
 
-template <bool F32, int NS>
+template <bool F32, int NS, int AHEAD>
 __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const uint8_t *lds,
                                          int e, int r0, int n, int m0) {
   using St = Stage<NS>;
@@ -359,26 +359,27 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
   const uint32_t xr0 = (uint32_t)(col * 128 + ((qd ^ (col & 7)) << 4));
   const uint32_t xs0 = (uint32_t)(St::X + col * NS * 4);
 
-  // Group g: its loads were issued two groups ago, and behind its DMA there are its own
-  // nine loads of weights and all of the next group's.  The loop's last steps load the last
-  // group again, so that these counts are the same in every one of them.  (A load whose
-  // value nothing takes would not be there to be counted: the steps behind the loop issue
-  // none, and wait for what is left.)
-  uint32_t here = 0, fill = 2 * St::BYTES;  // the stages of groups g and g + 2
+  // Group g: its loads were issued AHEAD groups ago, and behind its DMA there are its own
+  // nine loads of weights and (AHEAD 2) all of the next group's.  The loop's last steps load
+  // the last group again, so that these counts are the same in every one of them.  (A load
+  // whose value nothing takes would not be there to be counted: the steps behind the loop
+  // issue none, and wait for what is left.)
+  constexpr int NEWER = 9 + (AHEAD > 1 ? St::DMA + 1 + 9 : 0);
+  uint32_t here = 0, fill = AHEAD * St::BYTES;  // the stages of groups g and g + AHEAD
   auto step = [&](int g, Codes (&w)[4], float s, auto loads, Codes (&next)[4], float &snext)
                   __attribute__((always_inline)) {
     constexpr bool LOADS = decltype(loads)::value;
-    if constexpr (LOADS) wait_vm<18 + St::DMA + 1>();
+    if constexpr (LOADS) wait_vm<NEWER>();
     else wait_vm<0>();
     block_barrier();
     if constexpr (LOADS) {
-      issue(min(g + 2, G - 1), lds0 + fill);
-      load_w(min(g + 2, G - 1), next, snext);
+      issue(min(g + AHEAD, G - 1), lds0 + fill);
+      load_w(min(g + AHEAD, G - 1), next, snext);
     }
     __builtin_amdgcn_sched_barrier(0);
     const uint8_t *st = lds + here;
-    here = here == 2 * St::BYTES ? 0 : here + St::BYTES;
-    fill = fill == 2 * St::BYTES ? 0 : fill + St::BYTES;
+    here = here == AHEAD * St::BYTES ? 0 : here + St::BYTES;
+    fill = fill == AHEAD * St::BYTES ? 0 : fill + St::BYTES;
     // One product and the four fmas of the one two before it at a time: the fmas run under
     // the products.  The barriers keep the compiler from reading all rows first (spills).
     constexpr int XB = F32 ? 1 : 2;  // fp32: the registers are the conversions'
@@ -407,25 +408,38 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  Codes w0[4], w1[4], w2[4];
-  float s0, s1, s2;
+  // (loops without breaks, for which the compiler would wait for every load)
+  using yes = std::true_type;
+  using no = std::false_type;
+  Codes w0[4], w1[4];
+  float s0, s1;
   // the ring's last readers and copies, of the item before
   wait_vm<0>();
   block_barrier();
   issue(0, lds0);
   load_w(0, w0, s0);
   __builtin_amdgcn_sched_barrier(0);
-  issue(min(1, G - 1), lds0 + St::BYTES);
-  load_w(min(1, G - 1), w1, s1);
-  int g = 0;  // (without breaks, for which the compiler would wait for every load)
-  for (; g + 3 <= G; g += 3) {
-    step(g, w0, s0, std::true_type(), w2, s2);
-    step(g + 1, w1, s1, std::true_type(), w0, s0);
-    step(g + 2, w2, s2, std::true_type(), w1, s1);
-  }
-  if (g < G) {
-    step(g, w0, s0, std::false_type(), w2, s2);
-    if (g + 1 < G) step(g + 1, w1, s1, std::false_type(), w0, s0);
+  int g = 0;
+  if constexpr (AHEAD > 1) {
+    Codes w2[4];
+    float s2;
+    issue(min(1, G - 1), lds0 + St::BYTES);
+    load_w(min(1, G - 1), w1, s1);
+    for (; g + 3 <= G; g += 3) {
+      step(g, w0, s0, yes(), w2, s2);
+      step(g + 1, w1, s1, yes(), w0, s0);
+      step(g + 2, w2, s2, yes(), w1, s1);
+    }
+    if (g < G) {
+      step(g, w0, s0, no(), w2, s2);
+      if (g + 1 < G) step(g + 1, w1, s1, no(), w0, s0);
+    }
+  } else {
+    for (; g + 2 <= G; g += 2) {
+      step(g, w0, s0, yes(), w1, s1);
+      step(g + 1, w1, s1, yes(), w0, s0);
+    }
+    if (g < G) step(g, w0, s0, no(), w1, s1);
   }
 
   // 16 neighbouring columns of row 16 j + col
@@ -451,9 +465,9 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
 
 // Items (tile, 256 weight rows) of an expert in bands of 8 tiles, tiles first, so that
 // the 64 workgroups of an XCD read few tiles and few weights at a time from its L2.
-template <bool F32, int NT>
+template <bool F32, int NT, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[3 * Stage<NT / 16>::BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[(AHEAD + 1) * Stage<NT / 16>::BYTES];
   __shared__ TileMap map;
   const int mb = (a.M + TILE_M - 1) / TILE_M;
   const int64_t items = (int64_t)map_tiles(a, NT, map) * mb;
@@ -476,13 +490,19 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
     const int u0 = (int)((int64_t)units * t / tiles), ns = (int)((int64_t)units * (t + 1) / tiles) - u0;
     r0 = __builtin_amdgcn_readfirstlane(r0 + 16 * u0);
     n = __builtin_amdgcn_readfirstlane(min(16 * ns, n - 16 * u0));
+    auto run = [&](auto ns_c) {
+      constexpr int NS = decltype(ns_c)::value;
+      if constexpr (NS * 16 <= NT) run_tile<F32, NS, AHEAD>(a, lds0, lds, e, r0, n, m0);
+    };
     switch (__builtin_amdgcn_readfirstlane(ns)) {
-    case 1: run_tile<F32, 1>(a, lds0, lds, e, r0, n, m0); break;
-    case 2: run_tile<F32, 2>(a, lds0, lds, e, r0, n, m0); break;
-    case 3: run_tile<F32, 3>(a, lds0, lds, e, r0, n, m0); break;
-    case 4: run_tile<F32, 4>(a, lds0, lds, e, r0, n, m0); break;
-    case 5: if constexpr (NT > 64) run_tile<F32, 5>(a, lds0, lds, e, r0, n, m0); break;
-    case 6: if constexpr (NT > 64) run_tile<F32, 6>(a, lds0, lds, e, r0, n, m0); break;
+    case 1: run(std::integral_constant<int, 1>()); break;
+    case 2: run(std::integral_constant<int, 2>()); break;
+    case 3: run(std::integral_constant<int, 3>()); break;
+    case 4: run(std::integral_constant<int, 4>()); break;
+    case 5: run(std::integral_constant<int, 5>()); break;
+    case 6: run(std::integral_constant<int, 6>()); break;
+    case 7: run(std::integral_constant<int, 7>()); break;
+    case 8: run(std::integral_constant<int, 8>()); break;
     }
   }
   wait_vm<0>();  // no copy into this workgroup's LDS outlives it
@@ -510,11 +530,21 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
   const int64_t ns = std::min<int64_t>(nt / 16, (each + 15) / 16);
   const int64_t few = (226 + 120 * ns) * std::max<int64_t>(512, tile_items) / 512 * (f32 ? 13 : 10) / 10;
   if (items2 > few && (each > 12 || G < 32)) {
-    // at most: full tiles, and one that is not full for each expert
-    const int64_t most = (a.N / nt + used) * mb;
-    const int grid = (int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD);
-    if (f32) k_fp8_tiles<true, 64><<<grid, 256, 0, s>>>(a);
-    else k_fp8_tiles<false, 96><<<grid, 256, 0, s>>>(a);
+    // Higher tiles bring fewer bytes for a product through the CU's L1, which bounds large
+    // calls, and leave registers for one group ahead instead of two, which costs calls that
+    // do not fill the CUs.  us, 96 rows with two groups ahead and 128 with one: 8192^3 626,
+    // 520; 64 experts of 512 rows, 4096 -> 2048 408, 345; of 256 218, 197; of 32 107, 107; 1024 x
+    // 4096 -> 4096 38.8, 47; 256 x 5120 -> 17408 49.3, 58.  fp32, 64 rows with two and one: 8192 x
+    // 4096 -> 4096 309, 274; 64 experts of 256 rows 341, 310; of 128 176, 181.
+    // (at most: full tiles, and one that is not full for each expert)
+    auto tiles = [&](auto kernel, int rows) {
+      const int64_t most = (a.N / rows + used) * mb;
+      kernel<<<(int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, 0, s>>>(a);
+    };
+    if (f32 && row_tiles(64) * mb >= 2048) tiles(k_fp8_tiles<true, 64, 1>, 64);
+    else if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
+    else if (row_tiles(128) * mb >= 512) tiles(k_fp8_tiles<false, 128, 1>, 128);
+    else tiles(k_fp8_tiles<false, 96, 2>, 96);
     return hipGetLastError();
   }
   auto split = [&](auto r_c, auto ns_c) {
