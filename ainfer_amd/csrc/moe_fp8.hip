@@ -9,7 +9,7 @@ namespace {
 
 // 8 neighbouring lanes take the 128 columns of a group, 16 each (K is a multiple of
 // 16, so a lane's columns are all inside the row or all behind it).
-// up != null: the values are silu(x) * up.
+// SILU: the values are silu(x) * up.
 template <bool F32, bool SILU>
 __global__ __launch_bounds__(256) void k_quant_rows(const void *x, int64_t xld, const void *up,
                                                     int64_t uld, const int32_t *live, int N, int K,
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void k_quant_rows(const void *x, int64_t xld, 
         float u[16];
         load_row<F32>(up, row * uld + col, u);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) v[d] = silu_mul(v[d], u[d]);
+        for (int d = 0; d < 16; ++d) v[d] = silu_mul_near(v[d], u[d]);
       }
     } else {
 #pragma unroll

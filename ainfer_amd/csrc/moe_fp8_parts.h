@@ -90,14 +90,48 @@ __device__ __forceinline__ float max_of_8_lanes(float m) {
 }
 // e4m3 codes of v / s, nearest even.  |v / s| is at most 448 (1 + 2^-23) by the scale's
 // choice, so no conversion overflows; NaN (and inf / inf) become e4m3's NaN.
+//
+// The fp32 quotient is the correctly rounded one, without a division for each value: from r,
+// the rounded 1 / s, v r is within two units of the last place, and each step q + (v - q s) r
+// brings it nearer until the second one rounds correctly (P. Markstein, Computation of
+// elementary functions on the IBM RISC System/6000 processor, 1990).  Below 2^-100 the
+// remainders would lose bits under fp32's smallest value, and the values are divided.  An
+// infinite s takes r = 0 and no remainder: finite values become 0.
 template <int N>
 __device__ __forceinline__ void fp8_codes(const float (&v)[N], float s, uint32_t (&q)[N / 4]) {
+  float x[N];
+  if (s < 0x1p-100f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = v[i] / s;
+  } else {
+    const float r = 1.0f / s, d = s == INFINITY ? 0.0f : s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float y = v[i] * r;
+      y = fmaf(fmaf(-y, d, v[i]), r, y);
+      x[i] = copysignf(fmaf(fmaf(-y, d, v[i]), r, y), v[i]);  // -0 stays -0
+    }
+  }
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] / s, v[4 * i + 1] / s, 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] / s, v[4 * i + 3] / s, w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
     q[i] = (uint32_t)w;
   }
+}
+
+// g / (1 + exp(-g)) * u to 2^-21: exp(-g) as 2^(h + l), h + l = -g log2 e with the rounding
+// of h in l, by the hardware's exp2 and a factor 1 + l ln 2 (3 2^-24 together), the sum
+// 2^-24, the hardware's reciprocal 2^-23 and two products 2^-24 each.  The exponent's g is
+// kept within +-200, where exp(-g) is 0 or infinite.  (With silu_mul's expf and division, and
+// a division for each code, 32768 x 1024 bf16 took 56.8 us, now 40.4.)
+__device__ __forceinline__ float silu_mul_near(float g, float u) {
+  const float c = fminf(fmaxf(g, -200.0f), 200.0f);
+  const float h = c * -1.44269502162933349609f;             // -log2 e, rounded
+  const float l = fmaf(c, -1.44269502162933349609f, -h) + c * -1.92596299112661746e-8f;
+  float e = __builtin_amdgcn_exp2f(h);
+  e = fmaf(e, l * 0.69314718056f, e);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
 }  // namespace

@@ -7,6 +7,7 @@ libainfer_moe.so; there is no other implementation behind these names.
 """
 import contextlib
 import ctypes as C
+import functools
 
 import numpy as np
 import torch
@@ -683,6 +684,12 @@ def sort_workspace(max_tokens, top_k, n_experts, device="cuda"):
     return ws[off:off + n]
 
 
+@functools.lru_cache(maxsize=256)
+def _sorting(*fields):
+    """The description of sorts of these sizes and types."""
+    return L.Sorting(*fields)
+
+
 def sort_rows(x, idx, n_experts, ws, fp8=False, pow2=False, out=None, stream=None):
     """The rows of x [T][H] in the order of their experts (idx [T][k] int32; ids outside
     [0, n_experts) are dropped): (rows [T * k][H], row_scales or None, offsets [E + 1], pos
@@ -721,7 +728,7 @@ def sort_rows(x, idx, n_experts, ws, fp8=False, pow2=False, out=None, stream=Non
     if not (pos.dtype == torch.int32 and pos.shape == (T, k) and pos.get_device() == dev
             and pos.is_contiguous()):
         raise L.MoeError("pos: contiguous int32 [T][k] on x's device")
-    d = L.Sorting(n_experts, k, H, dt, int(fp8), _kind(pow2))
+    d = _sorting(n_experts, k, H, dt, int(fp8), _kind(pow2))
     _call(L.lib().ainfer_moe_sort_rows, dev, stream, C.byref(d), x.data_ptr(), ld, idx.data_ptr(), T,
           offsets.data_ptr(), pos.data_ptr(), rows.data_ptr(), rld,
           sc.data_ptr() if fp8 else None, ws.data_ptr(), ws.nbytes)

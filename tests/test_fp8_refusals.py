@@ -204,3 +204,22 @@ def test_unpermute_backward(L):
                    dict(dr=D), dict(dr=E), dict(dr=G)), L.ERR_ARG)
     assert back_grad(L, T=0, dy=None, pos=None, rows=None) == L.OK
     assert back_grad(L, dr=None, dw=None) == L.OK
+
+
+def test_host_tensors_and_wrong_types():
+    """The Python surface refuses tensors that the kernels could not read."""
+    import torch
+    from ainfer_amd import _lib as L
+    from ainfer_amd import moe
+    x, i = torch.zeros(4, 64), torch.zeros(4, 2, dtype=torch.int32)
+    w = torch.zeros(1, 64, 64, dtype=torch.uint8)
+    b = torch.zeros(256, dtype=torch.uint8)
+    for call in (lambda: moe.act_quant_fp8(x), lambda: moe.silu_mul_fp8(x, x),
+                 lambda: moe.silu_mul_backward(x, x, x, x, x),
+                 lambda: moe.weight_quant_fp8(x[None]),
+                 lambda: moe.Fp8Weights(w, torch.zeros(1, 1, 1)),
+                 lambda: moe.sort_rows(x, i, 8, b), lambda: moe.unpermute(x, i, None, x),
+                 lambda: moe.unpermute_backward(x, x, i, None, x),
+                 lambda: moe.sort_workspace(4, 2, 0), lambda: moe.sort_workspace(-1, 2, 8)):
+        with pytest.raises(L.MoeError):
+            call()

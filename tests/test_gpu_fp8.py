@@ -88,6 +88,29 @@ def test_act_quant_values(torch, pow2):
 
 
 @pytest.mark.parametrize("pow2", (False, True))
+def test_act_quant_next_to_ties(torch, pow2):
+    """Values next to the borders between codes: a quotient that is off by one unit of the
+    last place takes the other code."""
+    from ainfer_amd import moe
+    g = torch.Generator().manual_seed(11)
+    n = 4000
+    most = torch.exp2(torch.rand(n, generator=g) * 200 - 130) * (1 + torch.rand(n, generator=g))
+    s = R.scale_of(most, pow2)
+    codes = torch.arange(0x7F, dtype=torch.uint8).view(R.E4M3).double()  # 0 to 448
+    border = (codes[:-1] + codes[1:]) / 2
+    near = (border * s.double()[:, None]).float()                        # [n][126]
+    sign = torch.where(torch.rand(n, 126, generator=g) < 0.5, -1.0, 1.0)
+    up = torch.nextafter(near, torch.full_like(near, 3e38))
+    down = torch.nextafter(near, torch.zeros_like(near))
+    rows = torch.cat([torch.cat([most[:, None], t * sign, most[:, None]], 1) for t in (near, up, down)], 1)
+    rows = rows.clamp(-most[:, None], most[:, None])
+    wq, ws = R.quantised(rows, pow2)
+    q, sq = moe.act_quant_fp8(rows.cuda(), pow2=pow2)
+    assert torch.equal(sq.cpu(), ws)
+    same_codes(torch, q, wq)
+
+
+@pytest.mark.parametrize("pow2", (False, True))
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
 @pytest.mark.parametrize("n,I", ((1, 16), (3, 144), (128, 512), (70, 1040), (1000, 128)))
 def test_silu_mul_fp8(torch, n, I, dtype, pow2):
@@ -272,6 +295,42 @@ COUNTS = ([1, 0, 3], [0, 0, 0, 1], [5, 17, 0, 16, 1], [128, 129, 127], [1] * 40,
 def test_product_grouped(torch, counts, M, K, dtype):
     q, sq, w, scales, offsets = state(torch, counts, M, K, sum(counts) + M, extra=7)
     check(torch, q, sq, w, scales, offsets, getattr(torch, dtype))
+
+
+def spread(seed, E, most):
+    """Rows of E experts: none for some, 1, 15, 16, 17 and every other number up to most."""
+    import random
+    r = random.Random(seed)
+    some = [0, 1, 15, 16, 17, 31, 32, 33, 127, 128, 129, most]
+    return [r.choice(some) if r.random() < 0.3 else r.randint(0, most) for _ in range(E)]
+
+
+# (rows of each expert, M, K): large enough for the tiled forms.  128 rows a tile and one group
+# ahead from 512 tiles on, else 96 and two (bf16); 64 rows, one group ahead from 2048 tiles on
+# (fp32); K of one to six groups, whole and not
+TILED = tuple((spread(K, 64, 300), M, K) for M in (1030, 2100)
+              for K in (16, 128, 144, 256, 400, 512, 640, 752)) + (
+    ([5000], 7000, 272), ([5000], 7001, 128), ([1, 4000, 0, 1000], 7000, 400),
+    ([64] * 40 + [0] * 30 + [200] * 30, 1030, 384), ([2000, 3], 4100, 2048), ([7] * 300, 1500, 272),
+    ([0] * 500 + [3000] + [0] * 523, 2049, 272), ([40] * 1024, 300, 144))
+
+
+@pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
+@pytest.mark.parametrize("case", range(len(TILED)))
+def test_product_tiled(torch, case, dtype):
+    counts, M, K = TILED[case]
+    q, sq, w, scales, offsets = state(torch, counts, M, K, case, pad=(16, 0), extra=5)
+    # NaN codes between pitched rows, behind the last row and in what no expert holds
+    base = q.as_strided((q.shape[0], K + 16), (K + 16, 1)).view(torch.uint8)
+    base[:, K:] = 0x7F
+    base[-5:] = 0x7F
+    sq[-5:] = float("nan")
+    y = check(torch, q, sq, w, scales, offsets, getattr(torch, dtype))
+    again = y.clone().fill_(3)
+    from ainfer_amd import moe
+    moe.Fp8Weights(w, scales).product(q, sq, again, offsets)
+    n = int(offsets[-1])
+    assert torch.equal(again[:n], y[:n]) and (again[n:] == 3).all()
 
 
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
