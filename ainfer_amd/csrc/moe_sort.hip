@@ -2,7 +2,7 @@
 // ainfer_moe_unpermute, ainfer_moe_unpermute_backward).
 //
 // The sort is a counting sort that keeps pairs of one expert in the order (token,
-// slot): chunks of SORT_CHUNK pairs are counted per expert, and a chunk's first place
+// slot): chunks of pairs are counted per expert, and a chunk's first place
 // for an expert is what all chunks have of smaller ones plus what earlier chunks
 // have of the same.  Only integers are added in any order, so the result is one.
 #include <algorithm>
@@ -13,7 +13,9 @@
 
 namespace {
 
-constexpr int SORT_CHUNK = 1024;  // pairs of a chunk: 4 waves, 4 rounds of 64 each
+// A chunk is 4 waves x `rounds` of 64 pairs, 1024 pairs while that makes at most 256 chunks:
+// every workgroup reads the counts of all of them.
+int sort_rounds(int64_t n) { return 4 * (int)std::max<int64_t>(1, (n + 262143) / 262144); }
 // Up to this many pairs every workgroup counts them all itself instead of adding a launch's
 // counts: eager calls 15.2 -> 12.7 us at 4000 pairs, 15.0 -> 14.6 at 8000, 16.5 -> 24.9 at 15000.
 constexpr int SORT_OWN = 8192;
@@ -26,17 +28,19 @@ __device__ __forceinline__ int expert_of(const int32_t *idx, int64_t i, int64_t 
 
 // counts[chunk][Ep], Ep = E rounded up to 4
 __global__ __launch_bounds__(256) void k_sort_count(const int32_t *idx, int64_t n, int E, int Ep,
-                                                    int32_t *counts) {
+                                                    int rounds, int32_t *counts) {
   __shared__ int32_t h[1024];
   for (int e = threadIdx.x; e < Ep; e += 256) h[e] = 0;
-  const int64_t c0 = (int64_t)blockIdx.x * SORT_CHUNK;
-  int ids[SORT_CHUNK / 256];
-#pragma unroll
-  for (int r = 0; r < SORT_CHUNK / 256; ++r) ids[r] = expert_of(idx, c0 + r * 256 + threadIdx.x, n, E);
   __syncthreads();
+  const int64_t c0 = (int64_t)blockIdx.x * rounds * 256;
+  for (int r0 = 0; r0 < rounds; r0 += 4) {
+    int ids[4];
 #pragma unroll
-  for (int r = 0; r < SORT_CHUNK / 256; ++r)
-    if (ids[r] < E) atomicAdd(&h[ids[r]], 1);
+    for (int r = 0; r < 4; ++r) ids[r] = expert_of(idx, c0 + (r0 + r) * 256 + threadIdx.x, n, E);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (ids[r] < E) atomicAdd(&h[ids[r]], 1);
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < Ep; e += 256) counts[(int64_t)blockIdx.x * Ep + e] = h[e];
 }
@@ -48,25 +52,27 @@ __global__ __launch_bounds__(256) void k_sort_count(const int32_t *idx, int64_t 
 // pairs itself, which saves a launch while they are few.
 template <bool COUNT>
 __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t n, int E, int Ep,
-                                                    const int32_t *counts, int chunks,
+                                                    int rounds, const int32_t *counts, int chunks,
                                                     int32_t *offsets, int32_t *pos) {
   __shared__ int32_t at[4][1024];  // next place of each wave and expert
   __shared__ int32_t all[1024], before[1024];  // pairs of every chunk, and of those before this
   __shared__ int32_t part[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int64_t c0 = (int64_t)blockIdx.x * SORT_CHUNK + wave * (SORT_CHUNK / 4);
-  int ids[SORT_CHUNK / 256];
-#pragma unroll
-  for (int r = 0; r < SORT_CHUNK / 256; ++r) ids[r] = expert_of(idx, c0 + r * 64 + lane, n, E);
+  const int64_t c0 = ((int64_t)blockIdx.x * 4 + wave) * rounds * 64;
   for (int e = tid; e < 1024; e += 256) {
     all[e] = before[e] = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) at[w][e] = 0;
   }
   __syncthreads();
+  for (int r0 = 0; r0 < rounds; r0 += 4) {
+    int ids[4];
 #pragma unroll
-  for (int r = 0; r < SORT_CHUNK / 256; ++r)
-    if (ids[r] < E) atomicAdd(&at[wave][ids[r]], 1);
+    for (int r = 0; r < 4; ++r) ids[r] = expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (ids[r] < E) atomicAdd(&at[wave][ids[r]], 1);
+  }
   const int columns = Ep / 4, groups = max(1, 256 / columns), mine = tid / columns;
   if constexpr (COUNT) {
     for (int64_t i = tid; i < n; i += 4 * 256) {
@@ -77,7 +83,7 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
       for (int u = 0; u < 4; ++u)
         if (e[u] < E) {
           atomicAdd(&all[e[u]], 1);
-          if (i + u * 256 < (int64_t)blockIdx.x * SORT_CHUNK) atomicAdd(&before[e[u]], 1);
+          if (i + u * 256 < (int64_t)blockIdx.x * rounds * 256) atomicAdd(&before[e[u]], 1);
         }
     }
   } else if (mine < groups) {
@@ -140,22 +146,27 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
   }
   __syncthreads();
   const int bits = 32 - __clz(E);  // of ids 0..E
+  for (int r0 = 0; r0 < rounds; r0 += 4) {
+    int ids[4];
 #pragma unroll
-  for (int r = 0; r < SORT_CHUNK / 256; ++r) {
-    uint64_t same = ~0ull;
-    for (int b = 0; b < bits; ++b) {
-      const bool on = ids[r] >> b & 1;
-      const uint64_t m = __ballot(on);
-      same &= on ? m : ~m;
+    for (int r = 0; r < 4; ++r) ids[r] = expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      uint64_t same = ~0ull;  // the lanes with this lane's id
+      for (int b = 0; b < bits; ++b) {
+        const bool on = ids[r] >> b & 1;
+        const uint64_t m = __ballot(on);
+        same &= on ? m : ~m;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1)), number = __popcll(same);
+      const int64_t i = c0 + (r0 + r) * 64 + lane;
+      const bool kept = ids[r] < E;
+      const int p = kept ? at[wave][ids[r]] + rank : -1;
+      if (i < n) pos[i] = p;
+      __builtin_amdgcn_wave_barrier();
+      if (kept && rank == 0) at[wave][ids[r]] = p + number;
+      __builtin_amdgcn_wave_barrier();
     }
-    const int rank = __popcll(same & ((1ull << lane) - 1)), number = __popcll(same);
-    const int64_t i = c0 + r * 64 + lane;
-    const bool kept = ids[r] < E;
-    const int p = kept ? at[wave][ids[r]] + rank : -1;
-    if (i < n) pos[i] = p;
-    __builtin_amdgcn_wave_barrier();
-    if (kept && rank == 0) at[wave][ids[r]] = p + number;
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -503,7 +514,8 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(const void *dy, int64_t y
 }  // namespace
 
 size_t sort_workspace_bytes(int T, int k, int E) {
-  const size_t chunks = ((size_t)T * k + SORT_CHUNK - 1) / SORT_CHUNK;
+  // (fewer tokens than T never have more chunks than T and 256)
+  const size_t chunks = std::min<size_t>(256, ((size_t)T * k + 1023) / 1024);
   return (chunks * ((E + 3) & ~3) * 4 + 255) & ~(size_t)255;
 }
 
@@ -512,7 +524,7 @@ hipError_t launch_sort_rows(const ainfer_moe_sorting &d, const void *x, int64_t 
                             int64_t rld, float *row_scales, void *ws, hipStream_t s) {
   const int k = d.top_k, E = d.n_experts, H = d.hidden;
   const int64_t n = (int64_t)T * k;
-  const int chunks = (int)((n + SORT_CHUNK - 1) / SORT_CHUNK);
+  const int rounds = sort_rounds(n), chunks = (int)((n + rounds * 256 - 1) / (rounds * 256));
   const int pow2 = d.scale_kind == AINFER_FP8_SCALE_POW2;
   const bool f32 = d.x_dtype == AINFER_ACT_F32;
   if (n <= SORT_FEW) {
@@ -531,10 +543,10 @@ hipError_t launch_sort_rows(const ainfer_moe_sorting &d, const void *x, int64_t 
   int32_t *counts = (int32_t *)ws;
   const int Ep = (E + 3) & ~3;
   if (n <= SORT_OWN) {
-    k_sort_place<true><<<chunks, 256, 0, s>>>(idx, n, E, Ep, nullptr, chunks, offsets, pos);
+    k_sort_place<true><<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, nullptr, chunks, offsets, pos);
   } else {
-    k_sort_count<<<chunks, 256, 0, s>>>(idx, n, E, Ep, counts);
-    k_sort_place<false><<<chunks, 256, 0, s>>>(idx, n, E, Ep, counts, chunks, offsets, pos);
+    k_sort_count<<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts);
+    k_sort_place<false><<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts, chunks, offsets, pos);
   }
   if (!rows) return hipGetLastError();
   auto grid = [](int64_t items) { return (int)std::min<int64_t>((items + 255) / 256, 8192); };

@@ -35,7 +35,8 @@ def ids(torch, T, k, E, seed, kind="any"):
 
 
 SIZES = ((1, 1, 1), (1, 8, 256), (2, 3, 5), (7, 32, 1024), (64, 8, 64), (129, 10, 512), (300, 6, 96),
-         (1003, 7, 1024), (4096, 8, 64), (5000, 32, 33))
+         (1003, 7, 1024), (2048, 1, 7), (2049, 1, 7), (1024, 8, 64), (1025, 8, 64), (4096, 8, 64),
+         (5000, 32, 33), (8193, 32, 100), (16385, 17, 3))
 
 
 @pytest.mark.parametrize("kind", ("any", "dropped", "one", "none"))
@@ -103,6 +104,23 @@ def test_sort_no_tokens(torch):
     idx = torch.empty(0, 2, dtype=torch.int32, device="cuda")
     moe.sort_rows(x, idx, 8, moe.sort_workspace(0, 2, 8), out=(x, None, off, idx.clone()))
     assert (off == 0).all()
+
+
+def test_sort_places_alone(torch):
+    """Without rows: offsets and places, through the C entry."""
+    import ctypes as C
+    from ainfer_amd import _lib as L
+    from ainfer_amd import moe
+    for T, k, E in ((3, 4, 8), (600, 4, 8), (5000, 4, 8)):
+        idx = ids(torch, T, k, E, T, "dropped")
+        ws = moe.sort_workspace(T, k, E)
+        off, pos = (torch.empty(n, dtype=torch.int32, device="cuda") for n in ((E + 1,), (T, k)))
+        d = L.Sorting(E, k, 64, L.ACT_BF16, 0, 0)
+        L.check(L.lib().ainfer_moe_sort_rows(
+            C.byref(d), None, 0, idx.data_ptr(), T, off.data_ptr(), pos.data_ptr(), None, 0, None,
+            ws.data_ptr(), ws.nbytes, torch.cuda.current_stream().cuda_stream))
+        woff, wpos, _ = R.sort(idx, E)
+        assert torch.equal(off.cpu(), woff) and torch.equal(pos.cpu(), wpos)
 
 
 def test_sort_largest(torch):
