@@ -737,6 +737,15 @@ bool over(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, con
   if (rows == 1 || ld == cols) return meet(out, (size_t)(rows * cols * size), p, n);
   return out == p;
 }
+// Whether rows that are written meet rows that are read: all bytes where both are whole, the
+// first addresses else.
+bool over_rows(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, const void *in,
+               int64_t in_rows, int64_t in_ld, int64_t in_cols, int in_size) {
+  if (!out || !in) return false;
+  if (in_rows == 1 || in_ld == in_cols)
+    return over(out, rows, ld, cols, size, in, (size_t)(in_rows * in_cols * in_size));
+  return out == in;
+}
 int check_fp8_sizes(int32_t E, int32_t M, int32_t K) {
   if (E < 1 || E > 1024 || M < 1 || M > (1 << 20) || K < 16 || K > 65536 || K % 16 ||
       (int64_t)E * M * K > (int64_t)1 << 38)
@@ -1326,7 +1335,7 @@ int ainfer_moe_act_quant_fp8(const void *x, int64_t x_ld, int32_t x_dtype, const
       mis(n_live, 4))
     return AINFER_ERR_ARG;
   const size_t scales = (size_t)N * ((K + 127) / 128) * 4;
-  if (q == x || (const void *)sq == x || meet(sq, scales, n_live, 4) ||
+  if (over_rows(q, N, q_ld, K, 1, x, N, x_ld, K, xsz) || meet(sq, scales, n_live, 4) ||
       over(x, N, x_ld, K, xsz, sq, scales) || over(q, N, q_ld, K, 1, sq, scales) ||
       over(q, N, q_ld, K, 1, n_live, 4))
     return AINFER_ERR_ARG;
@@ -1349,8 +1358,8 @@ int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, i
       mis(up, sz) || mis(q, 16) || mis(sq, 4) || mis(n_live, 4))
     return AINFER_ERR_ARG;
   const size_t scales = (size_t)N * ((I + 127) / 128) * 4;
-  if (q == gate || q == up || (const void *)sq == gate || (const void *)sq == up ||
-      meet(sq, scales, n_live, 4) || over(gate, N, gate_ld, I, sz, sq, scales) ||
+  if (over_rows(q, N, q_ld, I, 1, gate, N, gate_ld, I, sz) ||
+      over_rows(q, N, q_ld, I, 1, up, N, up_ld, I, sz) || meet(sq, scales, n_live, 4) || over(gate, N, gate_ld, I, sz, sq, scales) ||
       over(up, N, up_ld, I, sz, sq, scales) || over(q, N, q_ld, I, 1, sq, scales) ||
       over(q, N, q_ld, I, 1, n_live, 4))
     return AINFER_ERR_ARG;
@@ -1403,14 +1412,14 @@ int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_
     return AINFER_ERR_NULL;
   const int M = w->rows, K = w->cols, ysz = act_size(w->y_dtype);
   // a tile's rows of codes are addressed with 32-bit offsets
-  if (bad_ld(q_ld, K) || q_ld % 16 || q_ld > 1 << 24 || bad_ld(y_ld, M) || mis(w->packed, 16) || mis(q, 16) ||
-      mis(w->scales, 4) || mis(sq, 4) || mis(offsets, 4) || mis(y, ysz))
+  if (bad_ld(q_ld, K) || q_ld % 16 || q_ld > 1 << 24 || bad_ld(y_ld, M) || mis(w->packed, 16) ||
+      mis(q, 16) || mis(w->scales, 4) || mis(sq, 4) || mis(offsets, 4) || mis(y, ysz))
     return AINFER_ERR_ARG;
   const size_t G = (K + 127) / 128, E = w->n_experts;
   if (over(y, N, y_ld, M, ysz, w->packed, fp8_packed_bytes(w->n_experts, M, K)) ||
       over(y, N, y_ld, M, ysz, w->scales, E * ((M + 127) / 128) * G * 4) ||
       over(y, N, y_ld, M, ysz, sq, N * G * 4) || over(y, N, y_ld, M, ysz, offsets, (E + 1) * 4) ||
-      y == q)
+      over_rows(y, N, y_ld, M, ysz, q, N, q_ld, K, 1))
     return AINFER_ERR_ARG;
   const Fp8Args a = {w->packed, w->scales, q, sq, offsets, y, q_ld, y_ld, w->n_experts, M, K, N};
   HIP_TRY(launch_fp8_product(a, w->y_dtype, (hipStream_t)stream));
@@ -1458,9 +1467,8 @@ int ainfer_moe_sort_rows(const ainfer_moe_sorting *s, const void *x, int64_t x_l
       auto hit = [&](const void *p, size_t bytes) {
         return over(rows, P, rows_ld, H, rsz, p, bytes) || over(x, T, x_ld, H, xsz, p, bytes);
       };
-      if (rows == x || hit(offsets, no) || hit(pos, n) || hit(ws, nw) || hit(sc, ns) ||
-          over(rows, P, rows_ld, H, rsz, topk_idx, n) ||
-          (x_ld == H && over(rows, P, rows_ld, H, rsz, x, (size_t)T * H * xsz)))
+      if (over_rows(rows, P, rows_ld, H, rsz, x, T, x_ld, H, xsz) || hit(offsets, no) || hit(pos, n) || hit(ws, nw) || hit(sc, ns) ||
+          over(rows, P, rows_ld, H, rsz, topk_idx, n))
         return AINFER_ERR_ARG;
     }
   }
@@ -1484,8 +1492,8 @@ int ainfer_moe_unpermute(const void *rows, int64_t rows_ld, int32_t rows_dtype, 
       mis(pos, 4) || mis(w, 4) || mis(resid, ysz) || mis(y, ysz))
     return AINFER_ERR_ARG;
   const size_t n = (size_t)T * top_k * 4;
-  if (y == rows || over(y, T, y_ld, H, ysz, pos, n) || over(y, T, y_ld, H, ysz, w, n) ||
-      (rows_ld == H && over(y, T, y_ld, H, ysz, rows, (size_t)N * H * rsz)) ||
+  if (over_rows(y, T, y_ld, H, ysz, rows, N, rows_ld, H, rsz) ||
+      over(y, T, y_ld, H, ysz, pos, n) || over(y, T, y_ld, H, ysz, w, n) ||
       (resid == y && T > 1 && resid_ld != y_ld))
     return AINFER_ERR_ARG;
   HIP_TRY(launch_unpermute(rows, rows_ld, rows_dtype, N, pos, w, T, top_k, H, resid, resid_ld, y,
@@ -1515,9 +1523,8 @@ int ainfer_moe_unpermute_backward(const void *dy, int64_t dy_ld, int32_t dy_dtyp
   if (drows && N > 0) {
     if (over(drows, N, drows_ld, H, rsz, pos, n) || over(drows, N, drows_ld, H, rsz, w, n) ||
         over(drows, N, drows_ld, H, rsz, dw, n) ||
-        (dw && drows == rows) ||
-        (dy_ld == H && over(drows, N, drows_ld, H, rsz, dy, (size_t)T * H * ysz)) ||
-        (dw && rows_ld == H && over(drows, N, drows_ld, H, rsz, rows, (size_t)N * H * rsz)))
+        over_rows(drows, N, drows_ld, H, rsz, dy, T, dy_ld, H, ysz) ||
+        (dw && over_rows(drows, N, drows_ld, H, rsz, rows, N, rows_ld, H, rsz)))
       return AINFER_ERR_ARG;
   }
   HIP_TRY(launch_unpermute_backward(dy, dy_ld, dy_dtype, rows, rows_ld, rows_dtype, N, pos, w, T,

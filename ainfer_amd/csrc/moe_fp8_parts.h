@@ -94,13 +94,14 @@ __device__ __forceinline__ float max_of_8_lanes(float m) {
 // The fp32 quotient is the correctly rounded one, without a division for each value: from r,
 // the rounded 1 / s, v r is within two units of the last place, and each step q + (v - q s) r
 // brings it nearer until the second one rounds correctly (P. Markstein, Computation of
-// elementary functions on the IBM RISC System/6000 processor, 1990).  Below 2^-100 the
-// remainders would lose bits under fp32's smallest value, and the values are divided.  An
-// infinite s takes r = 0 and no remainder: finite values become 0.
+// elementary functions on the IBM RISC System/6000 processor, 1990).  The remainders are exact
+// while no bit of theirs is under fp32's 2^-149: quotients that decide on a code are 2^-11 or
+// more, so their last bits times s's are 2^-34-23 s or more.  Below s = 2^-90 the values are
+// divided.  An infinite s takes r = 0 and no remainder: finite values become 0.
 template <int N>
 __device__ __forceinline__ void fp8_codes(const float (&v)[N], float s, uint32_t (&q)[N / 4]) {
   float x[N];
-  if (s < 0x1p-100f) {
+  if (s < 0x1p-90f) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = v[i] / s;
   } else {
@@ -120,10 +121,11 @@ __device__ __forceinline__ void fp8_codes(const float (&v)[N], float s, uint32_t
   }
 }
 
-// g / (1 + exp(-g)) * u to 2^-21: exp(-g) as 2^(h + l), h + l = -g log2 e with the rounding
+// g / (1 + exp(-g)) * u to 2^-21 of itself and 2^-119 of u: exp(-g) as 2^(h + l), h + l = -g log2 e with the rounding
 // of h in l, by the hardware's exp2 and a factor 1 + l ln 2 (3 2^-24 together), the sum
 // 2^-24, the hardware's reciprocal 2^-23 and two products 2^-24 each.  The exponent's g is
-// kept within +-200, where exp(-g) is 0 or infinite.  (With silu_mul's expf and division, and
+// kept within +-200, where exp(-g) is 0 or infinite; from exp(-g) = 2^126 on the reciprocal may
+// be 0 (g 2^-126 is what is lost, g being -87 to -89 there, and less below).  (With silu_mul's expf and division, and
 // a division for each code, 32768 x 1024 bf16 took 56.8 us, now 40.4.)
 __device__ __forceinline__ float silu_mul_near(float g, float u) {
   const float c = fminf(fmaxf(g, -200.0f), 200.0f);

@@ -38,7 +38,8 @@ def test_act_quant(L):
                    dict(x_ld=-512), dict(x_ld=1 << 40), dict(q_ld=511), dict(q_ld=520),
                    dict(q_ld=1 << 40), dict(x=A + 2), dict(x=A + 1, dtype=1), dict(q=D + 8),
                    dict(sq=E + 2), dict(live=B + 2), dict(q=A), dict(sq=A), dict(sq=D + 2032),
-                   dict(sq=A + 8188), dict(live=E + 60), dict(live=D + 4)), L.ERR_ARG)
+                   dict(sq=A + 8188), dict(live=E + 60), dict(live=D + 4), dict(q=A + 512),
+                   dict(x=D + 1024), dict(q=A + 8176, q_ld=512)), L.ERR_ARG)
     assert quant(L, N=0, x=None, q=None, sq=None) == L.OK
 
 
@@ -55,7 +56,7 @@ def test_silu_mul_fp8(L):
     refused(call, (dict(dtype=2), dict(kind=3), dict(g_ld=511), dict(u_ld=511), dict(q_ld=500),
                    dict(q_ld=520), dict(g=A + 2), dict(u=B + 1), dict(q=D + 4), dict(sq=E + 1),
                    dict(live=G + 1), dict(q=A), dict(q=B), dict(sq=A), dict(sq=B), dict(live=E),
-                   dict(live=D), dict(sq=D + 16)), L.ERR_ARG)
+                   dict(live=D), dict(sq=D + 16), dict(q=A + 16), dict(u=D - 16)), L.ERR_ARG)
     assert silu(L, N=0, g=None, u=None, q=None, sq=None) == L.OK
 
 
@@ -126,8 +127,8 @@ def test_product(L):
     refused(call, (dict(N=-1), dict(N=L.MAX_ROWS + 1)), L.ERR_TOKENS)
     refused(call, (dict(struct=False), dict(w=None), dict(s=None), dict(q=None), dict(sq=None),
                    dict(offsets=None), dict(y=None)), L.ERR_NULL)
-    refused(call, (dict(dtype=2), dict(dtype=-1), dict(q_ld=256), dict(q_ld=280), dict(q_ld=(1 << 24) + 16), dict(y_ld=129),
-                   dict(y_ld=1 << 40), dict(w=A + 8), dict(q=D + 8), dict(s=B + 2), dict(sq=E + 2),
+    refused(call, (dict(dtype=2), dict(dtype=-1), dict(q_ld=256), dict(q_ld=280), dict(q_ld=(1 << 24) + 16),
+                   dict(y_ld=129), dict(y_ld=1 << 40), dict(y=D + 16), dict(q=G + 1280), dict(w=A + 8), dict(q=D + 8), dict(s=B + 2), dict(sq=E + 2),
                    dict(offsets=F + 2), dict(y=G + 1), dict(y=D), dict(y=A), dict(y=A + 256),
                    dict(y=B), dict(y=E), dict(y=F), dict(y=F - 1024), dict(y=A, y_ld=140),
                    dict(y=F, y_ld=140)), L.ERR_ARG)

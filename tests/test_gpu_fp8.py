@@ -110,6 +110,34 @@ def test_act_quant_next_to_ties(torch, pow2):
     same_codes(torch, q, wq)
 
 
+def test_act_quant_quotients_next_to_half_units(torch):
+    """Small scales and quotients a few 2^-24ths of a unit from half a unit above a border
+    between two codes: a quotient rounded the other way is the border itself and takes the
+    even code.  v = (S h - j 2^-24) units for scales of S units, h the border plus half a unit
+    of its last place, 2^24 h = A: S = j / A modulo 2^24."""
+    from ainfer_amd import moe
+    rows = []
+    for power in (-103, -100, -99, -98, -97, -94, -91, -89):
+        for num in (1, 3, 5, 7, 9, 11, 13, 15):                       # border num / 1024
+            high = num.bit_length() - 1
+            A = (num << 24 >> high) + 1
+            for j in range(-200, 201):
+                S = j * pow(A, -1, 1 << 24) % (1 << 24)
+                if S < 1 << 23:
+                    continue
+                V = (S * A - j) >> 24
+                s, v = (x * 2.0 ** (power - 23) for x in (S, V * 2.0 ** (high - 10)))
+                most = torch.tensor(448 * s, dtype=torch.float32)
+                if V < 1 << 24 and (most / 448).item() == s:
+                    rows.append([most.item(), v, -v, 0.0] * 4)
+    rows = torch.tensor(rows, dtype=torch.float64).float()
+    assert len(rows) > 1000
+    wq, ws = R.quantised(rows, False)
+    q, sq = moe.act_quant_fp8(rows.cuda())
+    assert torch.equal(sq.cpu(), ws)
+    same_codes(torch, q, wq)
+
+
 @pytest.mark.parametrize("pow2", (False, True))
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
 @pytest.mark.parametrize("n,I", ((1, 16), (3, 144), (128, 512), (70, 1040), (1000, 128)))
