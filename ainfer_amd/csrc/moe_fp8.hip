@@ -1,6 +1,14 @@
 // moe_fp8.hip - rows and weights quantised to e4m3 with a scale for each block of
 // 128 (ainfer_moe_act_quant_fp8, ainfer_moe_weight_quant_fp8), and the gated
-// activation written so (ainfer_moe_silu_mul_fp8).
+// activation written so (ainfer_moe_silu_mul_fp8): s = max |x| / 448, q = e4m3(x / s).
+//
+// One pass, bound by memory (a large copy reaches 4.95 TB/s): a group's values stay in its
+// lanes' registers between the maximum and the codes.  32768 x 4096 bf16 79 us, 5.1 TB/s; fp32
+// 129, 5.2; the gated activation of 32768 x 1024 bf16 40, 4.2 (the
+// activation's instructions come on top), fp32 56, 5.4; 64 x 2048 x 4096 bf16 weights 300,
+// 5.4.  128 x 512: 3.5 us, an empty launch takes 2.5.
+// The codes are written through the caches: past them 32768 x 1024 takes 35 us, but with the
+// product that reads the codes 236 instead of 220.
 #include "moe_common.h"
 #include "moe_internal.h"
 #include "moe_fp8_parts.h"

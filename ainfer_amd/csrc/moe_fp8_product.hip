@@ -10,8 +10,7 @@
 // Weights are laid out once (ainfer_moe_fp8_pack) as this instruction takes them: 64 rows x
 // 128 columns are four tiles of 16 rows, each 2 KB in the order of the lanes, so that a wave's
 // load is 1 KB of neighbouring bytes.  (Read from plain rows, 16 neighbouring lanes touch 16
-// rows, which the CU's address unit takes one by one: the whole kernel ran at 1394 TFLOP/s
-// for 8192^3 where it reaches 2622 without those loads.)  Row r of tile i is row 16 (r / 4) +
+// rows, which the CU's address unit takes one by one: 8192^3 ran at 1394 TFLOP/s.)  Row r of tile i is row 16 (r / 4) +
 // 4 i + r % 4 of the 64, so that the lane that holds four results of each tile holds 16
 // neighbouring columns of a row of y.  Rows and columns behind the matrix are zeros.
 #include <algorithm>
@@ -144,7 +143,8 @@ __device__ __forceinline__ void dma_x1(__amdgpu_buffer_rsrc_t b, uint32_t off, u
 // ---- split ------------------------------------------------------------------------
 // 16 R weight rows x 16 NS rows of x in a workgroup of four waves that take every fourth
 // group of 128 columns each; their sums are added in the waves' order.  For calls with too few
-// 256-row tiles to fill the CUs.  Each wave copies its own rows of x into LDS of its own
+// 256-row tiles to fill the CUs.  One row is bound by the weights: 5120 -> 17408 17.5 us, 5.1
+// TB/s.  Each wave copies its own rows of x into LDS of its own
 // (no barriers), three stages, two groups ahead, and loads its weights into registers.
 template <int NS>
 struct Share {
@@ -292,9 +292,16 @@ __global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
 
 // ---- tiles ------------------------------------------------------------------------
 // 256 weight rows x NS * 16 rows of x in a workgroup of four waves, each 64 of the weight
-// rows: weights go from global memory into registers (no wave shares them), one group
-// ahead; rows of x and their scales go through two stages of LDS by DMA, shared by the
-// waves.  Two workgroups fit a CU, so that one's waits run under the other's products.
+// rows: weights go from global memory into registers (no wave shares them); rows of x and
+// their scales go through AHEAD + 1 stages of LDS by DMA, shared by the waves; both are sent
+// for AHEAD groups before they are used.  Two workgroups fit a CU, so that one's waits run
+// under the other's products.  (One workgroup of eight waves with 256 x 192: 8192^3 637 instead
+// of 580 us.)
+//
+// Bound by the loads' way through a CU's L1: a group of 256 x 128 is 48 KB for 128 products, and
+// 8192^3 brings 48 bytes a ns to each CU (without the loads the products alone run at 2622
+// TFLOP/s).  8192^3 520 us, 2110 TFLOP/s (a library's bf16 product 1366); 4096 x 5120 -> 17408 378, 1930; 64 experts of 512 rows, 4096 -> 2048 345, 1590: there the
+// weights come from memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 274, 1000.
 //
 // Weight row r of a wave's tile i (four tiles of 16) is row 16 (r / 4) + 4 i + r % 4 of the
 // 64, so that a lane ends with 16 neighbouring columns of a row of y.

@@ -5,6 +5,13 @@
 // slot): chunks of pairs are counted per expert, and a chunk's first place
 // for an expert is what all chunks have of smaller ones plus what earlier chunks
 // have of the same.  Only integers are added in any order, so the result is one.
+//
+// What bounds each, and us alone on the GPU: up to 2048 pairs one launch of latency (1 token of
+// 4096 columns as codes 4.8; an empty launch takes 2.5); above, places are two launches of
+// latency (40960 pairs of 512 experts 3.9 + 7.6, 65536 of 64 4.8 + 5.3) and the rows a pass
+// at the speed of the memory: 4096 tokens of 2048 bf16 to 10 rows of codes 19.8, 103 MB; 8192
+// of 4096 bf16 to 4 rows each 52, 6.4 TB/s.  Weighted sums of 4096 tokens, 10 rows of 2048 bf16
+// 34.9, 5.3 TB/s; their gradients, 8 rows of 4096 bf16 110, 5.2.
 #include <algorithm>
 
 #include "moe_common.h"
@@ -170,10 +177,11 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
   }
 }
 
-// Few pairs (SORT_FEW at most; 4000 of them 16.1 instead of 12.7 us): everything in one launch.  Workgroup (t, y) takes token t and
-// every gridDim.y-th part of its columns, and counts the smaller pairs for the token's k
-// itself; workgroup (T, 0) writes offsets.  MODE: bytes of an element of rows that are moved
-// as they are, or 8 (bf16) and 9 (fp32) for rows that are quantised; 0 for none.
+// Few pairs (SORT_FEW at most; 4000 of them 16.1 instead of 12.7 us): everything in one
+// launch.  Workgroup (t, y) takes token t and every gridDim.y-th part of its columns, and
+// counts the smaller pairs for the token's k itself; workgroup (T, 0) writes offsets.  MODE:
+// bytes of an element of rows that are moved as they are, or 8 (bf16) and 9 (fp32) for rows
+// that are quantised; 0 for none.
 constexpr int SORT_FEW = 2048;
 
 template <int MODE>

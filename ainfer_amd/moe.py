@@ -568,7 +568,8 @@ def act_quant_fp8(x, q=None, sq=None, pow2=False, live=None, stream=None):
 
 
 def silu_mul_fp8(gate, up, q=None, sq=None, pow2=False, live=None, stream=None):
-    """act_quant_fp8 of silu_mul's fp32 values (ainfer_moe_silu_mul_fp8)."""
+    """e4m3 codes and scales of gate / (1 + exp(-gate)) * up (ainfer_moe_silu_mul_fp8), as
+    act_quant_fp8 writes them."""
     dt, dev, n, I, gld = _rows(gate, "gate")
     udt, udev, un, _, uld = _rows(up, "up", I)
     if not (udt == dt and un == n and udev == dev):
@@ -620,7 +621,7 @@ def weight_quant_fp8(w, pow2=False, stream=None):
 class Fp8Weights:
     """The weights of E experts' projection (or one matrix, E = 1), resident on one
     device: e4m3 codes w [E][M][K] (float8_e4m3fn or uint8) laid out for the product
-    (w itself is not kept), and their fp32 scales [E][ceil(M / 128)][ceil(K / 128)].
+    (w itself is not kept), and their fp32 scales [E][ceil(M / 128)][ceil(K / 128)] (kept).
     transpose: the weights are W^T, [E][K][M], for the gradient to x (M a multiple of 16)."""
 
     def __init__(self, w, scales, y_dtype=torch.bfloat16, transpose=False, stream=None):
@@ -650,7 +651,8 @@ class Fp8Weights:
     def product(self, q, sq, y=None, offsets=None, stream=None):
         """y [N][M] = x W^T for codes q [N][K] and scales sq of rows sorted by expert
         (offsets [E + 1] int32; may be left out with one expert), in fp32 or bf16
-        (ainfer_moe_fp8_product).  Rows outside the offsets keep what y holds."""
+        (ainfer_moe_fp8_product).  Rows outside the offsets keep what y holds (a new y has
+    anything there)."""
         E, M, K = self.shape
         dev, n, _, ld = _codes(q, "q", K)
         if dev != self.dev:

@@ -538,12 +538,14 @@ enum { AINFER_FP8_SCALE_ANY = 0, AINFER_FP8_SCALE_POW2 = 1 };
  * or _BF16).  K a multiple of 16, 16..65536; row r at r * its ld elements; q 16-byte
  * aligned, q_ld a multiple of 16.  n_live: device count of the rows to take (the last
  * value of the offsets of ainfer_moe_sort_rows, say; rows behind it are left as they
- * are), or NULL: N. */
+ * are), or NULL: N.  Nothing that is written may overlap another operand, here and below
+ * where it is not said otherwise. */
 int ainfer_moe_act_quant_fp8(const void *x, int64_t x_ld, int32_t x_dtype, const int32_t *n_live,
                              int32_t N, int32_t K, int32_t scale_kind, uint8_t *q, int64_t q_ld,
                              float *sq, void *stream);
-/* The gated activation written as codes and scales: those of ainfer_moe_silu_mul's fp32
- * values (gate, up: rows of I values of in_dtype, I as K above). */
+/* The gated activation gate / (1 + exp(-gate)) * up written as codes and scales, from fp32
+ * values within 2^-21 of themselves + 2^-119 |up| (not ainfer_moe_silu_mul's bits).  gate, up:
+ * rows of I values of in_dtype, I as K above. */
 int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, int64_t up_ld,
                             int32_t in_dtype, const int32_t *n_live, int32_t N, int32_t I,
                             int32_t scale_kind, uint8_t *q, int64_t q_ld, float *sq, void *stream);
@@ -570,9 +572,12 @@ typedef struct ainfer_moe_fp8 {
 } ainfer_moe_fp8;
 /* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
  *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
- * sums in fp32, y rounded once.  q: N rows of K codes at q_ld elements (16-byte aligned, a
- * multiple of 16, at most 2^24), sq [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one
- * expert: all N rows), y: N rows of M values at y_ld elements.  Rows of y outside
+ * sums in fp32, y rounded once.  With bf16 y the matrix instruction drops what is more than 13
+ * bits below the largest of eight neighbouring products: at most 7 * 2^-13 of the sum of
+ * magnitudes, 1.4e-5 of it for normal values; with fp32 y products are whole.  q: N rows of K
+ * codes at q_ld elements (16-byte aligned, a multiple of 16, at most 2^24), sq
+ * [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one expert: all N rows), y: N
+ * rows of M values at y_ld elements.  Rows of y outside
  * [offsets[0], offsets[E]) are left as they were; offsets outside [0, N] are taken as
  * its ends, and rows of experts that overlap are unspecified.  A NaN code or scale
  * reaches the values whose sums it is in.  y must not overlap anything that is read.
