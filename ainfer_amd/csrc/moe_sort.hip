@@ -7,8 +7,8 @@
 // have of the same.  Only integers are added in any order, so the result is one.
 //
 // What bounds each, and us alone on the GPU: up to 2048 pairs one launch of latency (1 token of
-// 4096 columns as codes 4.8; an empty launch takes 2.5); above, places are two launches of
-// latency (40960 pairs of 512 experts 3.9 + 7.6, 65536 of 64 4.8 + 5.3) and the rows a pass
+// 4096 columns as codes 4.8; an empty launch takes 2.5); above, places are a launch of counting
+// in LDS, or two of latency (65536 pairs of 64 experts 4.8 + 5.3), and the rows a pass
 // at the speed of the memory: 4096 tokens of 2048 bf16 to 10 rows of codes 19.8, 103 MB; 8192
 // of 4096 bf16 to 4 rows each 52, 6.4 TB/s.  Weighted sums of 4096 tokens, 10 rows of 2048 bf16
 // 34.9, 5.3 TB/s; their gradients, 8 rows of 4096 bf16 110, 5.2.
@@ -23,9 +23,6 @@ namespace {
 // A chunk is 4 waves x `rounds` of 64 pairs, 1024 pairs while that makes at most 256 chunks:
 // every workgroup reads the counts of all of them.
 int sort_rounds(int64_t n) { return 4 * (int)std::max<int64_t>(1, (n + 262143) / 262144); }
-// Up to this many pairs every workgroup counts them all itself instead of adding a launch's
-// counts: eager calls 15.2 -> 12.7 us at 4000 pairs, 15.0 -> 14.6 at 8000, 16.5 -> 24.9 at 15000.
-constexpr int SORT_OWN = 8192;
 
 // the expert of a pair, E for one that is dropped
 __device__ __forceinline__ int expert_of(const int32_t *idx, int64_t i, int64_t n, int E) {
@@ -52,16 +49,73 @@ __global__ __launch_bounds__(256) void k_sort_count(const int32_t *idx, int64_t 
   for (int e = threadIdx.x; e < Ep; e += 256) counts[(int64_t)blockIdx.x * Ep + e] = h[e];
 }
 
+// The places of a chunk's pairs: waves 0 to 3 of a workgroup have them in order, `rounds` of
+// 64 each (from c0, the wave's first).
+struct ChunkPlaces {
+  int32_t at[4][1024];  // next place of each wave and expert
+};
+__device__ __forceinline__ void count_chunk(ChunkPlaces &c, const int32_t *idx, int64_t c0,
+                                            int64_t n, int E, int rounds) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave >= 4) return;
+  for (int r0 = 0; r0 < rounds; r0 += 4) {
+    int ids[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      ids[r] = r0 + r < rounds ? expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E) : E;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (ids[r] < E) atomicAdd(&c.at[wave][ids[r]], 1);
+  }
+}
+// the four waves' counts of expert e become their first places
+__device__ __forceinline__ void first_places(ChunkPlaces &c, int e, int first) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int n = c.at[w][e];
+    c.at[w][e] = first;
+    first += n;
+  }
+}
+__device__ __forceinline__ void place_chunk(ChunkPlaces &c, const int32_t *idx, int64_t c0,
+                                            int64_t n, int E, int rounds, int32_t *pos) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave >= 4) return;
+  const int bits = 32 - __clz(E);  // of ids 0..E
+  for (int r0 = 0; r0 < rounds; r0 += 4) {
+    int ids[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      ids[r] = r0 + r < rounds ? expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E) : E;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r0 + r >= rounds) break;
+      uint64_t same = ~0ull;  // the lanes with this lane's id
+      for (int b = 0; b < bits; ++b) {
+        const bool on = ids[r] >> b & 1;
+        const uint64_t m = __ballot(on);
+        same &= on ? m : ~m;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1)), number = __popcll(same);
+      const int64_t i = c0 + (r0 + r) * 64 + lane;
+      const bool kept = ids[r] < E;
+      const int p = kept ? c.at[wave][ids[r]] + rank : -1;
+      if (i < n) pos[i] = p;
+      __builtin_amdgcn_wave_barrier();
+      if (kept && rank == 0) c.at[wave][ids[r]] = p + number;
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
 // pos of a chunk's pairs; the last workgroup writes offsets.  The chunks' counts are read in
 // columns of four experts by groups of threads that take every so many-th chunk, several
 // loads at once (one thread for each column, one chunk after the other: 18.5 instead of
-// 6.9 us for 40 chunks of 512 experts).  COUNT: there are none, every workgroup counts all
-// pairs itself, which saves a launch while they are few.
-template <bool COUNT>
+// 6.9 us for 40 chunks of 512 experts).
 __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t n, int E, int Ep,
                                                     int rounds, const int32_t *counts, int chunks,
                                                     int32_t *offsets, int32_t *pos) {
-  __shared__ int32_t at[4][1024];  // next place of each wave and expert
+  __shared__ ChunkPlaces places;
   __shared__ int32_t all[1024], before[1024];  // pairs of every chunk, and of those before this
   __shared__ int32_t part[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -69,31 +123,12 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
   for (int e = tid; e < 1024; e += 256) {
     all[e] = before[e] = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) at[w][e] = 0;
+    for (int w = 0; w < 4; ++w) places.at[w][e] = 0;
   }
   __syncthreads();
-  for (int r0 = 0; r0 < rounds; r0 += 4) {
-    int ids[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) ids[r] = expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (ids[r] < E) atomicAdd(&at[wave][ids[r]], 1);
-  }
+  count_chunk(places, idx, c0, n, E, rounds);
   const int columns = Ep / 4, groups = max(1, 256 / columns), mine = tid / columns;
-  if constexpr (COUNT) {
-    for (int64_t i = tid; i < n; i += 4 * 256) {
-      int e[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) e[u] = expert_of(idx, i + u * 256, n, E);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (e[u] < E) {
-          atomicAdd(&all[e[u]], 1);
-          if (i + u * 256 < (int64_t)blockIdx.x * rounds * 256) atomicAdd(&before[e[u]], 1);
-        }
-    }
-  } else if (mine < groups) {
+  if (mine < groups) {
     const int e = (tid - mine * columns) * 4;
     int4 sum = {0, 0, 0, 0}, low = {0, 0, 0, 0};
     const int32_t *p = counts + e;
@@ -140,41 +175,74 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
     const int e = tid * 4 + i;
     if (e < E) {
       if (last) offsets[e] = first;
-      int p = first + before[e];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int c = at[w][e];
-        at[w][e] = p;
-        p += c;
-      }
+      first_places(places, e, first + before[e]);
     }
     first += own[i];
     if (last && e == E - 1) offsets[E] = first;
   }
   __syncthreads();
-  const int bits = 32 - __clz(E);  // of ids 0..E
-  for (int r0 = 0; r0 < rounds; r0 += 4) {
-    int ids[4];
+  place_chunk(places, idx, c0, n, E, rounds, pos);
+}
+
+// Up to SORT_OWN pairs, in one launch: a workgroup of 16 waves counts all pairs itself, all
+// of them in the low half of a word and those of earlier chunks in the high half, four words
+// an expert for neighbouring lanes (pairs that all name one expert would take 64 turns of
+// the LDS at one word).  Its chunk is 256 pairs, placed by four of its waves.  Counting takes
+// 0.1 us for 1000 pairs; us of this launch, and of two that share the counts: 2400 pairs of 64
+// experts 7.4, 9.3 (each with a launch of short rows); 16000 8.6, 11.1; 40960 of 512
+// 11.5, 14.2, by a power law 12.5, 14.4, all of one 16.8, 14.8; 65528 of 64 13.4, 11.6.
+constexpr int SORT_OWN = 40960;  // 16 bits hold it
+typedef int32_t i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+__global__ __launch_bounds__(1024) void k_sort_own(const int32_t *idx, int n, int E,
+                                                   int32_t *offsets, int32_t *pos) {
+  constexpr int COPY = 1024 + 8;
+  __shared__ ChunkPlaces places;
+  __shared__ uint32_t h[4 * COPY];
+  __shared__ int32_t part[16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int first_pair = blockIdx.x * 256;
+  for (int i = tid; i < 4 * COPY; i += 1024) h[i] = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ids[r] = expert_of(idx, c0 + (r0 + r) * 64 + lane, n, E);
+  for (int w = 0; w < 4; ++w) places.at[w][tid] = 0;
+  __syncthreads();
+  count_chunk(places, idx, first_pair + wave * 64, n, E, 1);
+  uint32_t *mine = h + (lane & 3) * COPY;
+  for (int i = tid * 4; i < n; i += 4 * 4096) {
+    i32x4_any v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      uint64_t same = ~0ull;  // the lanes with this lane's id
-      for (int b = 0; b < bits; ++b) {
-        const bool on = ids[r] >> b & 1;
-        const uint64_t m = __ballot(on);
-        same &= on ? m : ~m;
+    for (int u = 0; u < 4; ++u) {
+      const int at = i + u * 4096;
+      v[u] = i32x4_any{-1, -1, -1, -1};
+      if (at + 4 <= n) {
+        v[u] = *(const i32x4_any *)(idx + at);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 3; ++d)
+          if (at + d < n) v[u][d] = idx[at + d];
       }
-      const int rank = __popcll(same & ((1ull << lane) - 1)), number = __popcll(same);
-      const int64_t i = c0 + (r0 + r) * 64 + lane;
-      const bool kept = ids[r] < E;
-      const int p = kept ? at[wave][ids[r]] + rank : -1;
-      if (i < n) pos[i] = p;
-      __builtin_amdgcn_wave_barrier();
-      if (kept && rank == 0) at[wave][ids[r]] = p + number;
-      __builtin_amdgcn_wave_barrier();
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if ((uint32_t)v[u][d] < (uint32_t)E)
+          atomicAdd(&mine[v[u][d]], i + u * 4096 + d < first_pair ? 0x10001u : 1u);
   }
+  __syncthreads();
+  const uint32_t c = (h[tid] + h[COPY + tid]) + (h[2 * COPY + tid] + h[3 * COPY + tid]);
+  const int own = c & 0xFFFF, incl = wave_scan_incl(own);
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int first = incl - own;
+  for (int w = 0; w < wave; ++w) first += part[w];
+  if (tid < E) first_places(places, tid, first + (int)(c >> 16));
+  if (blockIdx.x + 1 == gridDim.x && tid < E) {
+    offsets[tid] = first;
+    if (tid == E - 1) offsets[E] = first + own;
+  }
+  __syncthreads();
+  place_chunk(places, idx, first_pair + wave * 64, n, E, 1, pos);
 }
 
 // Few pairs (SORT_FEW at most; 4000 of them 16.1 instead of 12.7 us): everything in one
@@ -548,13 +616,13 @@ hipError_t launch_sort_rows(const ainfer_moe_sorting &d, const void *x, int64_t 
     else few(f32 ? k_sort_few<4> : k_sort_few<2>);
     return hipGetLastError();
   }
-  int32_t *counts = (int32_t *)ws;
-  const int Ep = (E + 3) & ~3;
   if (n <= SORT_OWN) {
-    k_sort_place<true><<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, nullptr, chunks, offsets, pos);
+    k_sort_own<<<(int)((n + 255) / 256), 1024, 0, s>>>(idx, (int)n, E, offsets, pos);
   } else {
+    int32_t *counts = (int32_t *)ws;
+    const int Ep = (E + 3) & ~3;
     k_sort_count<<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts);
-    k_sort_place<false><<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts, chunks, offsets, pos);
+    k_sort_place<<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts, chunks, offsets, pos);
   }
   if (!rows) return hipGetLastError();
   auto grid = [](int64_t items) { return (int)std::min<int64_t>((items + 255) / 256, 8192); };

@@ -36,7 +36,8 @@ def ids(torch, T, k, E, seed, kind="any"):
 
 SIZES = ((1, 1, 1), (1, 8, 256), (2, 3, 5), (7, 32, 1024), (64, 8, 64), (129, 10, 512), (300, 6, 96),
          (1003, 7, 1024), (2048, 1, 7), (2049, 1, 7), (1024, 8, 64), (1025, 8, 64), (4096, 8, 64),
-         (5000, 32, 33), (8193, 32, 100), (16385, 17, 3))
+         (5000, 32, 33), (8193, 32, 100), (16385, 17, 3), (2560, 16, 600), (2731, 15, 1024),
+         (4099, 10, 8))
 
 
 @pytest.mark.parametrize("kind", ("any", "dropped", "one", "none"))
