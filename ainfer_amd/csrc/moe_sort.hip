@@ -11,7 +11,7 @@
 // in LDS, or two of latency (65536 pairs of 64 experts 4.8 + 5.3), and the rows a pass
 // at the speed of the memory: 4096 tokens of 2048 bf16 to 10 rows of codes 19.8, 103 MB; 8192
 // of 4096 bf16 to 4 rows each 52, 6.4 TB/s.  Weighted sums of 4096 tokens, 10 rows of 2048 bf16
-// 34.9, 5.3 TB/s; their gradients, 8 rows of 4096 bf16 110, 5.2.
+// 34.9, 5.3 TB/s; their gradients, 8 rows of 4096 bf16 108.5, 5.3.
 #include <algorithm>
 
 #include "moe_common.h"
@@ -309,8 +309,8 @@ __global__ __launch_bounds__(256) void k_sort_few(const int32_t *idx, int T, int
         for (int d = 0; d < 16; ++d) v[d] = 0.0f;
       }
     } else if constexpr (MODE != 0) {
-      if (c < pieces && H - c * PER >= PER)
-        raw = *(const u32x4_any *)((const uint8_t *)x + (t * xld + c * PER) * MODE);
+      if (c < pieces && H >= PER)
+        raw = *(const u32x4_any *)((const uint8_t *)x + (t * xld + min(c * PER, H - PER)) * MODE);
     }
   };
   load();
@@ -350,17 +350,15 @@ __global__ __launch_bounds__(256) void k_sort_few(const int32_t *idx, int T, int
         }
       } else {
         if (c >= pieces) continue;
-        const int left = H - c * PER;
+        const int col = min(c * PER, H - PER);  // the last piece: the row's last 16 bytes
         for (int j = 0; j < k; ++j) {
           const int64_t p = at[j];
           if (p < 0) continue;
-          uint8_t *to = rows + (p * rld + c * PER) * MODE;
-          if (left >= PER) {
-            *(u32x4_any *)to = raw;
+          if (H >= PER) {
+            *(u32x4_any *)(rows + (p * rld + col) * MODE) = raw;
           } else {
             using el = typename std::conditional<MODE == 4, uint32_t, uint16_t>::type;
-            const el *from = (const el *)((const uint8_t *)x + (t * xld + c * PER) * MODE);
-            for (int d = 0; d < left; ++d) ((el *)to)[d] = from[d];
+            for (int d = 0; d < H; ++d) ((el *)rows)[p * rld + d] = ((const el *)x)[t * xld + d];
           }
         }
       }
@@ -369,7 +367,7 @@ __global__ __launch_bounds__(256) void k_sort_few(const int32_t *idx, int T, int
 }
 
 // Rows as they are: a lane takes 16 bytes of a token's row to its k places (SIZE: bytes of an
-// element), past the caches (ordinary stores: 68 instead of 51 us for 8192 rows of 4096 bf16,
+// element; the last piece of a row is its last 16), past the caches (ordinary stores: 68 instead of 51 us for 8192 rows of 4096 bf16,
 // half of 8 places each; 268 MB written).
 template <int SIZE>
 __global__ __launch_bounds__(256) void k_move_rows(const uint8_t *x, int64_t xld,
@@ -379,11 +377,9 @@ __global__ __launch_bounds__(256) void k_move_rows(const uint8_t *x, int64_t xld
   const int64_t per_row = (H + PER - 1) / PER, items = per_row * T;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < items; i += gridDim.x * 256ll) {
     const int64_t t = i / per_row;
-    const int col = (int)(i - t * per_row) * PER;
-    const uint8_t *src = x + (t * xld + col) * SIZE;
-    const int left = H - col;
-    if (left >= PER) {
-      const u32x4 v = *(const u32x4_any *)src;
+    if (H >= PER) {
+      const int col = min((int)(i - t * per_row) * PER, H - PER);
+      const u32x4 v = *(const u32x4_any *)(x + (t * xld + col) * SIZE);
       for (int j = 0; j < k; ++j) {
         const int p = pos[t * k + j];
         if (p >= 0) __builtin_nontemporal_store(v, (u32x4_any *)(rows + (p * rld + col) * SIZE));
@@ -393,7 +389,7 @@ __global__ __launch_bounds__(256) void k_move_rows(const uint8_t *x, int64_t xld
       for (int j = 0; j < k; ++j) {
         const int p = pos[t * k + j];
         if (p >= 0)
-          for (int d = 0; d < left; ++d) ((el *)(rows + (p * rld + col) * SIZE))[d] = ((const el *)src)[d];
+          for (int d = 0; d < H; ++d) ((el *)rows)[p * rld + d] = ((const el *)x)[t * xld + d];
       }
     }
   }
@@ -453,7 +449,9 @@ struct Eight {
 };
 
 // y[t] = sum_j w[t][j] rows[pos[t][j]] (+ resid[t]), fp32 fma in slot order.  A lane takes
-// eight columns of a token; two rows are on their way at a time.
+// eight columns of a token; two rows are on their way at a time.  The last lane of a row that
+// is no multiple of 8 reads the rows' last eight columns (column by column: 219 tokens, 5 rows of
+// 5353, 11.6 instead of 7.5 us).
 template <bool RF32, bool YF32>
 __global__ __launch_bounds__(256) void k_unpermute(const void *rows, int64_t rld, int N,
                                                    const int32_t *pos, const float *w, int T, int k,
@@ -465,7 +463,8 @@ __global__ __launch_bounds__(256) void k_unpermute(const void *rows, int64_t rld
     const int64_t t = i / per_row;
     const int col = (int)(i - t * per_row) * 8, left = H - col;
     float a[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8];
-    if (left >= 8) {
+    if (H >= 8) {
+      const int at = min(col, H - 8);  // the last lane of a row takes its last eight columns
       for (int j0 = 0; j0 < k; j0 += U) {
         Eight<RF32> v[U];
         float f[U];
@@ -478,7 +477,7 @@ __global__ __launch_bounds__(256) void k_unpermute(const void *rows, int64_t rld
             there[u] = (uint64_t)p < (uint64_t)N;
             if (there[u]) {
               f[u] = w ? w[t * k + j0 + u] : 1.0f;
-              v[u].load(rows, p * rld + col);
+              v[u].load(rows, p * rld + at);
             }
           }
         }
@@ -489,12 +488,21 @@ __global__ __launch_bounds__(256) void k_unpermute(const void *rows, int64_t rld
             for (int d = 0; d < 8; ++d) a[d] = fmaf(f[u], v[u].get(d), a[d]);
           }
       }
-      if (resid) {
-        load_row<YF32>(resid, t * sld + col, r);
+      if (left >= 8) {
+        if (resid) {
+          load_row<YF32>(resid, t * sld + col, r);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) a[d] += r[d];
+          for (int d = 0; d < 8; ++d) a[d] += r[d];
+        }
+        store_row<YF32>(y, t * yld + col, a);
+      } else {  // its own columns alone: resid may be y
+#pragma unroll
+        for (int d = 1; d < 8; ++d)
+          if (at + d >= col && resid) a[d] += load_one<YF32>(resid, t * sld + at + d);
+#pragma unroll
+        for (int d = 1; d < 8; ++d)
+          if (at + d >= col) store_one<YF32>(y, t * yld + at + d, a[d]);
       }
-      store_row<YF32>(y, t * yld + col, a);
     } else {
       for (int j = 0; j < k; ++j) {
         const int64_t p = pos[t * k + j];
@@ -502,88 +510,96 @@ __global__ __launch_bounds__(256) void k_unpermute(const void *rows, int64_t rld
         const float f = w ? w[t * k + j] : 1.0f;
 #pragma unroll
         for (int d = 0; d < 7; ++d)
-          if (d < left) a[d] = fmaf(f, load_one<RF32>(rows, p * rld + col + d), a[d]);
+          if (d < left) a[d] = fmaf(f, load_one<RF32>(rows, p * rld + d), a[d]);
       }
 #pragma unroll
       for (int d = 0; d < 7; ++d)
         if (d < left)
-          store_one<YF32>(y, t * yld + col + d,
-                          resid ? a[d] + load_one<YF32>(resid, t * sld + col + d) : a[d]);
+          store_one<YF32>(y, t * yld + d,
+                          resid ? a[d] + load_one<YF32>(resid, t * sld + d) : a[d]);
     }
   }
 }
 
-// drows[pos[t][j]] = w[t][j] dy[t], dw[t][j] = <dy[t], rows[pos[t][j]]>: a workgroup takes a
-// token and two of its pairs at a time; its threads' partial sums are added in one order.
+// drows[pos[t][j]] = w[t][j] dy[t], dw[t][j] = <dy[t], rows[pos[t][j]]>: workgroup (t, y) takes
+// pairs 2 y and 2 y + 1 of token t; its threads' partial sums are added in one order.  (One
+// workgroup for all of a token's pairs: 219 tokens of 5 pairs, 5353 columns, 16.7 instead of
+// 9.8 us; 16 of 8, 2048, 6.8 instead of 3.3; 4096 of 8, 4096, 111 instead of 108.5.)
+// A lane takes eight columns; the last lane of a row that is no multiple of 8 takes the row's
+// last eight, of which it writes all (values that its neighbour writes too) and sums its own.
 template <bool YF32, bool RF32>
 __global__ __launch_bounds__(256) void k_unpermute_bwd(const void *dy, int64_t yld, const void *rows,
                                                        int64_t rld, int N, const int32_t *pos,
                                                        const float *w, int k, int H, void *drows,
                                                        int64_t dld, float *dw) {
   constexpr int J = 2;
-  __shared__ float part[32][4];
+  __shared__ float part[J][4];
   const int64_t t = blockIdx.x;
-  const int tid = threadIdx.x, wave = tid >> 6;
-  for (int j0 = 0; j0 < k; j0 += J) {
-    int64_t p[J];
-    float f[J], sum[J];
+  const int tid = threadIdx.x, wave = tid >> 6, j0 = J * blockIdx.y;
+  int64_t p[J];
+  float f[J], sum[J];
 #pragma unroll
-    for (int u = 0; u < J; ++u) {
-      p[u] = j0 + u < k ? pos[t * k + j0 + u] : -1;
-      if (p[u] >= N) p[u] = -1;
-      f[u] = w && j0 + u < k ? w[t * k + j0 + u] : 1.0f;
-      sum[u] = 0.0f;
-    }
-    for (int col = tid * 8; col < H; col += 256 * 8) {
-      if (H - col >= 8) {
-        Eight<RF32> v[J];
-        if (dw) {
-#pragma unroll
-          for (int u = 0; u < J; ++u)
-            if (p[u] >= 0) v[u].load(rows, p[u] * rld + col);
-        }
-        float g[8];
-        load_row<YF32>(dy, t * yld + col, g);
-        if (drows) {
-#pragma unroll
-          for (int u = 0; u < J; ++u)
-            if (p[u] >= 0) {
-              float o[8];
-#pragma unroll
-              for (int d = 0; d < 8; ++d) o[d] = g[d] * f[u];
-              store_row<RF32, 8, !RF32>(drows, p[u] * dld + col, o);
-            }
-        }
-        if (dw) {
-#pragma unroll
-          for (int u = 0; u < J; ++u)
-            if (p[u] >= 0) {
-#pragma unroll
-              for (int d = 0; d < 8; ++d) sum[u] = fmaf(g[d], v[u].get(d), sum[u]);
-            }
-        }
-      } else {
+  for (int u = 0; u < J; ++u) {
+    p[u] = j0 + u < k ? pos[t * k + j0 + u] : -1;
+    if (p[u] >= N) p[u] = -1;
+    f[u] = w && j0 + u < k ? w[t * k + j0 + u] : 1.0f;
+    sum[u] = 0.0f;
+  }
+  for (int own = tid * 8; own < H; own += 256 * 8) {
+    if (H >= 8) {
+      const int col = min(own, H - 8);
+      Eight<RF32> v[J];
+      if (dw) {
 #pragma unroll
         for (int u = 0; u < J; ++u)
-          if (p[u] >= 0)
-            for (int d = 0; d < H - col; ++d) {
-              const float o = load_one<YF32>(dy, t * yld + col + d);
-              if (dw) sum[u] = fmaf(o, load_one<RF32>(rows, p[u] * rld + col + d), sum[u]);
-              if (drows) store_one<RF32>(drows, p[u] * dld + col + d, o * f[u]);
-            }
+          if (p[u] >= 0) v[u].load(rows, p[u] * rld + col);
       }
-    }
-    if (dw) {
+      float g[8];
+      load_row<YF32>(dy, t * yld + col, g);
+      if (drows) {
 #pragma unroll
-      for (int u = 0; u < J; ++u) {
-        for (int o = 32; o; o >>= 1) sum[u] += __shfl_xor(sum[u], o, 64);
-        if ((tid & 63) == 0 && j0 + u < k) part[j0 + u][wave] = sum[u];
+        for (int u = 0; u < J; ++u)
+          if (p[u] >= 0) {
+            float o[8];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[d] = g[d] * f[u];
+            store_row<RF32, 8, !RF32>(drows, p[u] * dld + col, o);
+          }
       }
+      if (dw) {
+#pragma unroll
+        for (int u = 0; u < J; ++u) {
+          if (p[u] < 0) continue;
+          if (col == own) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) sum[u] = fmaf(g[d], v[u].get(d), sum[u]);
+          } else {
+#pragma unroll
+            for (int d = 1; d < 8; ++d)
+              if (col + d >= own) sum[u] = fmaf(g[d], v[u].get(d), sum[u]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < J; ++u)
+        if (p[u] >= 0)
+          for (int d = 0; d < H; ++d) {
+            const float o = load_one<YF32>(dy, t * yld + d);
+            if (dw) sum[u] = fmaf(o, load_one<RF32>(rows, p[u] * rld + d), sum[u]);
+            if (drows) store_one<RF32>(drows, p[u] * dld + d, o * f[u]);
+          }
     }
   }
   if (dw) {
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+      for (int o = 32; o; o >>= 1) sum[u] += __shfl_xor(sum[u], o, 64);
+      if ((tid & 63) == 0) part[u][wave] = sum[u];
+    }
     __syncthreads();
-    if (tid < k) dw[t * k + tid] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
+    if (tid < J && j0 + tid < k)
+      dw[t * k + j0 + tid] = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
   }
 }
 
@@ -662,7 +678,7 @@ hipError_t launch_unpermute_backward(const void *dy, int64_t yld, int y_dtype, c
                                      const float *w, int T, int k, int H, void *drows, int64_t dld,
                                      float *dw, hipStream_t s) {
   auto run = [&](auto kernel) {
-    kernel<<<T, 256, 0, s>>>(dy, yld, rows, rld, N, pos, w, k, H, drows, dld, dw);
+    kernel<<<dim3(T, (k + 1) / 2), 256, 0, s>>>(dy, yld, rows, rld, N, pos, w, k, H, drows, dld, dw);
   };
   const bool r32 = rows_dtype == AINFER_ACT_F32, y32 = y_dtype == AINFER_ACT_F32;
   if (y32) run(r32 ? k_unpermute_bwd<true, true> : k_unpermute_bwd<true, false>);

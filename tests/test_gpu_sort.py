@@ -62,7 +62,7 @@ def test_sort(torch, T, k, E, kind):
 
 
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
-@pytest.mark.parametrize("H", (1, 7, 8, 130, 515, 4096))
+@pytest.mark.parametrize("H", (1, 3, 5, 7, 8, 9, 15, 130, 515, 2047, 4096))
 def test_sort_row_lengths(torch, H, dtype):
     from ainfer_amd import moe
     dt = getattr(torch, dtype)
@@ -163,7 +163,7 @@ def back_state(torch, T, k, E, H, rows_dtype, y_dtype, pad=0, seed=0, kind="drop
 DTYPES = (("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float32", "bfloat16"),
           ("float32", "float32"))
 BACK = ((1, 1, 1, 1), (1, 8, 64, 4096), (3, 2, 5, 7), (16, 8, 256, 2048), (50, 10, 32, 515), (333, 32, 64, 64),
-        (1030, 3, 16, 1000))
+        (1030, 3, 16, 1000), (5, 3, 4, 9), (40, 6, 8, 2055))
 
 
 def half_step(torch, dtype):
@@ -194,10 +194,11 @@ def test_unpermute(torch, T, k, E, H, rd, yd):
                 assert (buf[:, 0] == 8).all() and (buf[:, -1] == 8).all()
 
 
-def test_unpermute_over_its_residual_and_bad_places(torch):
+@pytest.mark.parametrize("H", (136, 137, 143, 9, 5))
+def test_unpermute_over_its_residual_and_bad_places(torch, H):
     """resid as y; places outside the rows are left out, NaN weights of theirs too."""
     from ainfer_amd import moe
-    pos, rows, w, resid = back_state(torch, 40, 4, 8, 136, "float32", "float32", kind="any")
+    pos, rows, w, resid = back_state(torch, 40, 4, 8, H, "float32", "float32", kind="any")
     y = moe.unpermute(rows, pos, w, torch.empty_like(resid), resid=resid)
     z = resid.clone()
     moe.unpermute(rows, pos, w, z, resid=z)
