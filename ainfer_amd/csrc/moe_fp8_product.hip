@@ -10,9 +10,10 @@
 // Weights are laid out once (ainfer_moe_fp8_pack) as this instruction takes them: 64 rows x
 // 128 columns are four tiles of 16 rows, each 2 KB in the order of the lanes, so that a wave's
 // load is 1 KB of neighbouring bytes.  (Read from plain rows, 16 neighbouring lanes touch 16
-// rows, which the CU's address unit takes one by one: 8192^3 ran at 1394 TFLOP/s.)  Row r of tile i is row 16 (r / 4) +
-// 4 i + r % 4 of the 64, so that the lane that holds four results of each tile holds 16
-// neighbouring columns of a row of y.  Rows and columns behind the matrix are zeros.
+// rows, which the CU's address unit takes one by one: 8192^3 ran at 1394 TFLOP/s.)  Row r of tile i is row
+// 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the 64, so that the lane that holds four results
+// of each tile holds two times 8 neighbouring columns of a row of y, and the four lanes of a row
+// 32.  Rows and columns behind the matrix are zeros.
 #include <algorithm>
 
 #include "moe_common.h"
@@ -270,19 +271,20 @@ __global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
     }
     __syncthreads();
     if (wave == 0) {
-      const int m = mb * 64 + 16 * qd + 4 * i0;
+      const int m = mb * 64 + 8 * qd;
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         if (16 * j + col >= n) continue;
-        const int64_t at = (int64_t)(r0 + 16 * j + col) * a.y_ld + m;
+        const int64_t at = (int64_t)(r0 + 16 * j + col) * a.y_ld;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
+          const int c = m + 32 * ((i0 + i) >> 1) + 4 * ((i0 + i) & 1);
           f32x4 v = acc[j][i];
 #pragma unroll
           for (int w = 0; w < 3; ++w) v += sums[(w * NS * R + j * R + i) * 64 + lane];
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (m + 4 * i + r < a.M) store_one<F32>(a.y, at + 4 * i + r, v[r]);
+            if (c + r < a.M) store_one<F32>(a.y, at + c + r, v[r]);
         }
       }
     }
@@ -303,8 +305,6 @@ __global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
 // TFLOP/s).  8192^3 520 us, 2110 TFLOP/s (a library's bf16 product 1366); 4096 x 5120 -> 17408 378, 1930; 64 experts of 512 rows, 4096 -> 2048 345, 1590: there the
 // weights come from memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 274, 1000.
 //
-// Weight row r of a wave's tile i (four tiles of 16) is row 16 (r / 4) + 4 i + r % 4 of the
-// 64, so that a lane ends with 16 neighbouring columns of a row of y.
 constexpr int TILE_M = 256;
 
 template <int NS>
@@ -449,22 +449,48 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
     if (g < G) step(g, w0, s0, no(), w1, s1);
   }
 
-  // 16 neighbouring columns of row 16 j + col
-  const int m = mw + 16 * qd;
+  // Row 16 j + col, two times 32 columns: the row's four lanes write 64 neighbouring bytes at a
+  // time, bf16 as they hold them (8 columns each), fp32 after their two pieces of 4 columns
+  // became pieces qd and 4 + qd of the 32.  (16 columns a lane, written in pieces 64 bytes
+  // apart: 1024 x 1024 -> 16384 with fp32 outputs 53.7 instead of 44.5 us.)
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     const int row = 16 * j + col;
-    if (row < n) {
-      const int64_t at = (int64_t)(r0 + row) * a.y_ld + m;
-      float v[16];
+    const int64_t at = (int64_t)(r0 + row) * a.y_ld;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = acc[j][i >> 2][i & 3];
-      if (m + 16 <= a.M) {
-        store_row<F32>(a.y, at, v);
-      } else {
+    for (int h = 0; h < 2; ++h) {
+      f32x4 v[2] = {acc[j][2 * h], acc[j][2 * h + 1]};
+      if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < 15; ++i)
-          if (m + i < a.M) store_one<F32>(a.y, at + i, v[i]);
+        for (int d = 0; d < 4; ++d) {
+          const u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0][d]),
+                                                           __float_as_uint(v[1][d]), false, false);
+          const u32x2 t = __builtin_amdgcn_permlane32_swap(s[0], s[1], false, false);
+          v[0][d] = __uint_as_float(t[0]);
+          v[1][d] = __uint_as_float(t[1]);
+        }
+        if (row >= n) continue;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int m = mw + 32 * h + 16 * b + 4 * qd;
+          if (m + 4 <= a.M) {
+            *(f32x4_any *)((float *)a.y + at + m) = v[b];
+          } else {
+#pragma unroll
+            for (int d = 0; d < 3; ++d)
+              if (m + d < a.M) ((float *)a.y)[at + m + d] = v[b][d];
+          }
+        }
+      } else if (row < n) {
+        const int m = mw + 32 * h + 8 * qd;
+        const float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+        if (m + 8 <= a.M) {
+          store_row<false>(a.y, at + m, x);
+        } else {
+#pragma unroll
+          for (int d = 0; d < 7; ++d)
+            if (m + d < a.M) store_one<false>(a.y, at + m + d, x[d]);
+        }
       }
     }
   }
@@ -585,7 +611,7 @@ __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t *w, int M, int K
     const int64_t t = c >> 9, em = t / G;
     const int g = (int)(t - em * G), mb = (int)(em % MB64);
     const int64_t e = em / MB64;
-    const int r = lane & 15, m = mb * 64 + 16 * (r >> 2) + 4 * i + (r & 3);
+    const int r = lane & 15, m = mb * 64 + 32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3);
     const int k = g * 128 + 64 * h + 16 * (lane >> 4);
     uint32_t v[4] = {0, 0, 0, 0};
     if (m < M && k < K) {

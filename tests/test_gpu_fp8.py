@@ -197,16 +197,17 @@ def test_weight_quant(torch, E, M, K, dtype):
 
 @pytest.mark.parametrize("E,M,K", ((1, 1, 16), (2, 64, 128), (3, 130, 144), (1, 65, 272), (2, 304, 400)))
 def test_pack(torch, E, M, K):
-    """Tiles of 64 x 128: tile i's row r is row 16 (r / 4) + 4 i + r % 4, two halves of 64
-    columns, 16 of each quarter to lane 16 quarter + r; zeros behind the matrix."""
+    """Tiles of 64 x 128: tile i's row r is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4, two
+    halves of 64 columns, 16 of each quarter to lane 16 quarter + r; zeros behind the matrix."""
     from ainfer_amd import _lib as L
     from ainfer_amd import moe
     w = torch.randint(0, 256, (E, M, K), device="cuda", dtype=torch.uint8)
     mb, G = -(-M // 64), R.groups(K)
     full = torch.zeros(E, mb * 64, G * 128, dtype=torch.uint8, device="cuda")
     full[:, :M, :K] = w
-    # [e][mb][r / 4][i][r % 4][g][half][quarter][16] -> [e][mb][g][i][half][quarter][r][16]
-    want = full.view(E, mb, 4, 4, 4, G, 2, 4, 16).permute(0, 1, 5, 3, 6, 7, 2, 4, 8).reshape(-1)
+    # [e][mb][i / 2][r / 4][i % 2][r % 4][g][half][quarter][16]
+    #   -> [e][mb][g][i][half][quarter][r][16]
+    want = full.view(E, mb, 2, 4, 2, 4, G, 2, 4, 16).permute(0, 1, 6, 2, 4, 7, 8, 3, 5, 9).reshape(-1)
     f = moe.Fp8Weights(w, torch.ones(E, R.groups(M), G, device="cuda"))
     assert f.packed.numel() == want.numel() == L.lib().ainfer_moe_fp8_packed_bytes(E, M, K)
     assert torch.equal(f.packed, want)
