@@ -295,16 +295,16 @@ __global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
 // ---- tiles ------------------------------------------------------------------------
 // 256 weight rows x NS * 16 rows of x in a workgroup of four waves, each 64 of the weight
 // rows: weights go from global memory into registers (no wave shares them); rows of x and
-// their scales go through AHEAD + 1 stages of LDS by DMA, shared by the waves; both are sent
-// for AHEAD groups before they are used.  Two workgroups fit a CU, so that one's waits run
-// under the other's products.  (One workgroup of eight waves with 256 x 192: 8192^3 637 instead
-// of 580 us.)
+// their scales go through three stages of LDS by DMA, shared by the waves, two groups ahead;
+// weights AHEAD groups and the time from their last use to the next step.  Two workgroups fit a
+// CU, so that one's waits run under the other's products.  (One workgroup of eight waves with
+// 256 x 192: 8192^3 637 instead of 580 us.)
 //
 // Bound by the loads' way through a CU's L1: a group of 256 x 128 is 48 KB for 128 products, and
-// 8192^3 brings 48 bytes a ns to each CU (without the loads the products alone run at 2622
-// TFLOP/s).  8192^3 520 us, 2110 TFLOP/s (a library's bf16 product 1366); 4096 x 5120 -> 17408 378, 1930; 64 experts of 512 rows, 4096 -> 2048 345, 1590: there the
-// weights come from memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 274, 1000.
-//
+// 8192^3 brings 50 bytes a ns to each CU (without the loads the products alone run at 2622
+// TFLOP/s).  8192^3 507 us, 2170 TFLOP/s (a library's bf16 product 1366); 4096 x 5120 -> 17408
+// 354, 2065; 64 experts of about 512 rows, 4096 -> 2048 338, 1626: there the weights come from
+// memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 263, 1047.
 constexpr int TILE_M = 256;
 
 template <int NS>
@@ -350,13 +350,21 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
     __builtin_amdgcn_sched_barrier(0);
   };
   const uint32_t wlane = (uint32_t)lane * 16u;
-  auto load_w = [&](int g, Codes (&w)[4], float &s) __attribute__((always_inline)) {
-    s = sw[g + zero];
+  auto load_s = [&](int g) __attribute__((always_inline)) { return sw[g + zero]; };
+  auto load_w = [&](int g, int i, Codes &w) __attribute__((always_inline)) {
     const uint8_t *p = wbase + (int64_t)g * 8192;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int h = 0; h < 2; ++h) w.v[h] = *(const u32x4 *)(p + wlane + ((i - 2) * 2048 + h * 1024));
+  };
+  struct Weights {
+    Codes w[4];
+    float s;
+  };
+  auto load_all = [&](int g, Weights &w) __attribute__((always_inline)) {
+    w.s = load_s(g);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) w[i].v[h] = *(const u32x4 *)(p + wlane + ((i - 2) * 2048 + h * 1024));
+    for (int i = 0; i < 4; ++i) load_w(g, i, w.w[i]);
+    __builtin_amdgcn_sched_barrier(0);
   };
   f32x4 acc[NS][4];
 #pragma unroll
@@ -366,27 +374,26 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
   const uint32_t xr0 = (uint32_t)(col * 128 + ((qd ^ (col & 7)) << 4));
   const uint32_t xs0 = (uint32_t)(St::X + col * NS * 4);
 
-  // Group g: its loads were issued AHEAD groups ago, and behind its DMA there are its own
-  // nine loads of weights and (AHEAD 2) all of the next group's.  The loop's last steps load
-  // the last group again, so that these counts are the same in every one of them.  (A load
-  // whose value nothing takes would not be there to be counted: the steps behind the loop
-  // issue none, and wait for what is left.)
-  constexpr int NEWER = 9 + (AHEAD > 1 ? St::DMA + 1 + 9 : 0);
-  uint32_t here = 0, fill = AHEAD * St::BYTES;  // the stages of groups g and g + AHEAD
-  auto step = [&](int g, Codes (&w)[4], float s, auto loads, Codes (&next)[4], float &snext)
-                  __attribute__((always_inline)) {
+  // Group g: its rows were sent for at the start of the step two before, its weights at the
+  // end of the one AHEAD + 1 before, as their registers came free.  (Rows, then weights, at the
+  // start of the step AHEAD before: 8192^3 543 instead of 507 us, 64 experts of 512 rows 375
+  // instead of 346, 1024 x 4096 -> 4096 37.6 instead of 32.9.)  Behind the copies of g there are the loads of one group's weights, the copies
+  // of g + 1 and another group's weights.  The loop's last steps load the last group again, so
+  // that this count is the same in every one of them.  (A load whose value nothing takes would not
+  // be there to be counted: the steps behind the loop issue none, and wait for what is left.)
+  constexpr int NEWER = 9 + St::DMA + 1 + 9;
+  uint32_t here = 0, fill = 2 * St::BYTES;  // the stages of groups g and g + 2
+  auto step = [&](int g, Weights &w, auto loads) __attribute__((always_inline)) {
     constexpr bool LOADS = decltype(loads)::value;
     if constexpr (LOADS) wait_vm<NEWER>();
     else wait_vm<0>();
     block_barrier();
-    if constexpr (LOADS) {
-      issue(min(g + AHEAD, G - 1), lds0 + fill);
-      load_w(min(g + AHEAD, G - 1), next, snext);
-    }
+    if constexpr (LOADS) issue(min(g + 2, G - 1), lds0 + fill);
+    const int next = min(g + AHEAD + 1, G - 1);
     __builtin_amdgcn_sched_barrier(0);
     const uint8_t *st = lds + here;
-    here = here == AHEAD * St::BYTES ? 0 : here + St::BYTES;
-    fill = fill == AHEAD * St::BYTES ? 0 : fill + St::BYTES;
+    here = here == 2 * St::BYTES ? 0 : here + St::BYTES;
+    fill = fill == 2 * St::BYTES ? 0 : fill + St::BYTES;
     // One product and the four fmas of the one two before it at a time: the fmas run under
     // the products.  The barriers keep the compiler from reading all rows first (spills).
     constexpr int XB = F32 ? 1 : 2;  // fp32: the registers are the conversions'
@@ -395,13 +402,13 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
     f32x4 d[3];
     auto read_row = [&](int j) {
       x[j % XB] = {{*(const u32x4 *)(st + xr0 + j * 2048), *(const u32x4 *)(st + (xr0 ^ 64) + j * 2048)}};
-      f[j & 1] = *(const float *)(st + xs0 + j * 4) * s;
+      f[j & 1] = *(const float *)(st + xs0 + j * 4) * w.s;
     };
     read_row(0);
 #pragma unroll
     for (int t = 0; t < 4 * NS + 2; ++t) {
       const int j = t >> 2, i = t & 3;
-      if (t < 4 * NS) d[t % 3] = group_dot<F32>(w[i], x[j % XB]);
+      if (t < 4 * NS) d[t % 3] = group_dot<F32>(w.w[i], x[j % XB]);
       if (t >= 2) {
         const int u = t - 2;
 #pragma unroll
@@ -413,40 +420,44 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
       // (f of row j - 1 has been used)
       if (i == (XB == 2 ? 1 : 3) && j + 1 < NS) read_row(j + 1);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (LOADS) {
+        if (j == NS - 1) {
+          if (i == 0) w.s = load_s(next);
+          load_w(next, i, w.w[i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
   };
   // (loops without breaks, for which the compiler would wait for every load)
   using yes = std::true_type;
   using no = std::false_type;
-  Codes w0[4], w1[4];
-  float s0, s1;
+  Weights w0, w1, w2;
   // the ring's last readers and copies, of the item before
   wait_vm<0>();
   block_barrier();
+  if constexpr (AHEAD > 1) load_all(0, w0);
   issue(0, lds0);
-  load_w(0, w0, s0);
-  __builtin_amdgcn_sched_barrier(0);
+  load_all(min(AHEAD - 1, G - 1), AHEAD > 1 ? w1 : w0);
+  issue(min(1, G - 1), lds0 + St::BYTES);
+  load_all(min(AHEAD, G - 1), AHEAD > 1 ? w2 : w1);
   int g = 0;
   if constexpr (AHEAD > 1) {
-    Codes w2[4];
-    float s2;
-    issue(min(1, G - 1), lds0 + St::BYTES);
-    load_w(min(1, G - 1), w1, s1);
     for (; g + 3 <= G; g += 3) {
-      step(g, w0, s0, yes(), w2, s2);
-      step(g + 1, w1, s1, yes(), w0, s0);
-      step(g + 2, w2, s2, yes(), w1, s1);
+      step(g, w0, yes());
+      step(g + 1, w1, yes());
+      step(g + 2, w2, yes());
     }
     if (g < G) {
-      step(g, w0, s0, no(), w2, s2);
-      if (g + 1 < G) step(g + 1, w1, s1, no(), w0, s0);
+      step(g, w0, no());
+      if (g + 1 < G) step(g + 1, w1, no());
     }
   } else {
     for (; g + 2 <= G; g += 2) {
-      step(g, w0, s0, yes(), w1, s1);
-      step(g + 1, w1, s1, yes(), w0, s0);
+      step(g, w0, yes());
+      step(g + 1, w1, yes());
     }
-    if (g < G) step(g, w0, s0, no(), w1, s1);
+    if (g < G) step(g, w0, no());
   }
 
   // Row 16 j + col, two times 32 columns: the row's four lanes write 64 neighbouring bytes at a
@@ -500,7 +511,7 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
 // the 64 workgroups of an XCD read few tiles and few weights at a time from its L2.
 template <bool F32, int NT, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[(AHEAD + 1) * Stage<NT / 16>::BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[3 * Stage<NT / 16>::BYTES];
   __shared__ TileMap map;
   const int mb = (a.M + TILE_M - 1) / TILE_M;
   const int64_t items = (int64_t)map_tiles(a, NT, map) * mb;
@@ -550,33 +561,37 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
   const int64_t used = std::min(a.E, a.N), each = a.N / used;
   const int64_t slabs = (a.M + 63) / 64, mb = (a.M + TILE_M - 1) / TILE_M;
   auto row_tiles = [&](int rows) { return std::max<int64_t>(used, (a.N + rows - 1) / rows); };
-  // Tiles or split, us (bf16; rows x K -> M).  A tile's workgroup takes its K groups one by one,
-  // 0.22 + 0.115 us for each 16 rows of x (latency) while its CU is not full, and a split
-  // item's four waves 7.5e-6 us a column, so few items of many rows are split:
-  //   256 x 4096 -> 4096 20.5 split, 32.7 tiles; 512 x 4096 -> 4096 36.0, 35.8;
-  //   256 x 5120 -> 17408 119, 47; 8 experts of 32 rows, 4096 -> 2048 17.2, 28.5;
-  //   64 experts of 32 rows, 4096 -> 2048 114, 98; 96 of 21, 2560 -> 1792 96, 89.
+  // Tiles or split.  A tile's workgroup takes its K groups one by one, 0.5 us and 0.06 for each
+  // 16 rows of x (latency) while its CU is not full; the split form's items take 1 / 1000 us for
+  // a group and 64 weight rows x 32 rows of x, and weights that are read for the first time as
+  // much and a third again.  So few items of many rows are split (us, bf16; rows x K -> M):
+  //   256 x 4096 -> 4096 21.8 split, 29.0 tiles; 384 x 4096 -> 4096 29.9, 29.4; 512 38.5, 29.5;
+  //   64 x 5120 -> 17408 44.0, 38.8; 4 experts of 32 rows, 4096 -> 4096 24.2, 20.2; 16 of 18, 2048 ->
+  //   2048 21.0, 14.8; 64 of 32, 4096 -> 2048 145, 102; fp32: 4 of 64, 4096 -> 4096 32.6, 37.6;
+  //   16 of 18, 2048 -> 2048 20.9, 18.4.
   // With few rows an expert both read weights at the speed of the memory, and the split form
-  // gets more of it where its waves have 8 groups or more: 16 experts of 4 rows, 4096 -> 2048
-  // 25, 31; 64 of 8 86, 95; but 256 of 1, 2048 -> 1024 47, 44, and 512 of 1, 1024 -> 2048 32, 28.
+  // gets more of it: 128 rows over 256 experts, 2048 -> 1024 37.6, 41.8; 512 over 512 112, 119; 16
+  // experts of 4, 4096 -> 2048 23.6, 29.6; 64 of 8 88.6, 96.3; but with short rows 256 of 7, 2048 ->
+  // 1024 108, 97; 64 of 6, 512 -> 4096 42, 31.
   const int64_t items2 = row_tiles(32) * slabs, tile_items = row_tiles(nt) * mb;
-  const int64_t ns = std::min<int64_t>(nt / 16, (each + 15) / 16);
-  const int64_t few = (226 + 120 * ns) * std::max<int64_t>(512, tile_items) / 512 * (f32 ? 13 : 10) / 10;
-  if (items2 > few && (each > 12 || G < 32)) {
+  const int64_t units = (each + 15) / 16, per = (units + nt / 16 - 1) / (nt / 16);
+  const int64_t ns = (units + per - 1) / per;
+  const int64_t few = (f32 ? 1030 + 30 * ns : 440 + 50 * ns) * std::max<int64_t>(512, tile_items) / 512;
+  if (items2 + used * slabs * 4 / 3 > few && (each > 12 || (each > 4 && G < 32))) {
     // Higher tiles bring fewer bytes for a product through the CU's L1, which bounds large
-    // calls, and leave registers for one group ahead instead of two, which costs calls that
-    // do not fill the CUs.  us, 96 rows with two groups ahead and 128 with one: 8192^3 626,
-    // 520; 64 experts of 512 rows, 4096 -> 2048 408, 345; of 256 218, 197; of 32 107, 107; 1024 x
-    // 4096 -> 4096 38.8, 47; 256 x 5120 -> 17408 49.3, 58.  fp32, 64 rows with two and one: 8192 x
-    // 4096 -> 4096 309, 274; 64 experts of 256 rows 341, 310; of 128 176, 181.
+    // calls, and leave registers for one group of weights ahead instead of two, which costs calls
+    // that do not fill the CUs or bring mostly weights.  us, 96 rows with two groups ahead and 128
+    // with one: 4096 x 4096 -> 4096 76, 68; 2048 46.5, 42.9; 1500 x 2048 -> 5000 28.2, 25.3; 64
+    // experts of 128 rows, 4096 -> 2048 148, 139; 1024 x 4096 -> 4096 30.9, 38.1; 256 x 5120 -> 17408
+    // 40.5, 50.9; 512 experts of 8 rows, 2048 -> 1024 246, 253.  (fp32, 64 rows: two ahead are never
+    // slower: 4096 x 4096 -> 4096 127.5, 132.)
     // (at most: full tiles, and one that is not full for each expert)
     auto tiles = [&](auto kernel, int rows) {
       const int64_t most = (a.N / rows + used) * mb;
       kernel<<<(int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, 0, s>>>(a);
     };
-    if (f32 && row_tiles(64) * mb >= 2048) tiles(k_fp8_tiles<true, 64, 1>, 64);
-    else if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
-    else if (row_tiles(128) * mb >= 512) tiles(k_fp8_tiles<false, 128, 1>, 128);
+    if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
+    else if (row_tiles(128) * mb >= 200 && each > 16) tiles(k_fp8_tiles<false, 128, 1>, 128);
     else tiles(k_fp8_tiles<false, 96, 2>, 96);
     return hipGetLastError();
   }

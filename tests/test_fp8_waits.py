@@ -1,5 +1,5 @@
 """The product's kernels count their loads: a wait for the copies of a group leaves exactly the
-loads behind them in flight (moe_fp8_product.hip).  The built library's own code has to hold what
+loads and copies behind them in flight (moe_fp8_product.hip).  The built library's own code has to hold what
 the counts assume; no GPU needed."""
 import re
 import subprocess
@@ -29,6 +29,39 @@ def kernels(tmp_path):
     return out
 
 
+def access(line):
+    if re.match(r"buffer_load_\w+ .*\blds\b", line):
+        return "copy"
+    if re.match(r"(global|buffer|flat)_load", line):
+        return "load"
+    if re.match(r"(global|buffer|flat)_(store|atomic)", line):
+        return "other"
+    return None
+
+
+def tile_steps(code):
+    """(count waited for in front of the barrier, accesses behind it up to the next barrier or
+    branch) of every step that sends for more, and what is in flight ahead of the loop."""
+    found, wait, last, ops, ahead = [], None, None, None, []
+    for line in code + ["s_endpgm"]:
+        m = re.match(r"s_waitcnt vmcnt\((\d+)\)", line)
+        if re.match(r"s_(barrier|c?branch|endpgm|setpc)", line):
+            if ops and wait:
+                found.append((wait, ops))
+            elif ops and ops.count("copy") and ops.count("load") > 9:
+                ahead.append(ops)
+            ops = [] if line.startswith("s_barrier") else None
+            wait = last if line.startswith("s_barrier") else None
+            last = None
+        elif m:
+            last = int(m.group(1)) if last is None else min(last, int(m.group(1)))
+        elif access(line):
+            last = None
+            if ops is not None:
+                ops.append(access(line))
+    return found, ahead
+
+
 def steps(code):
     """(count waited for, accesses) of every stretch from a wait that leaves loads in flight
     to the next wait or branch, where it holds copies into LDS."""
@@ -39,12 +72,8 @@ def steps(code):
             if wait and "copy" in ops:
                 found.append((wait, ops))
             wait, ops = int(m.group(1)) if m else 0, []
-        elif re.match(r"buffer_load_\w+ .*\blds\b", line):
-            ops.append("copy")
-        elif re.match(r"(global|buffer|flat)_load", line):
-            ops.append("load")
-        elif re.match(r"(global|buffer|flat)_(store|atomic)", line):
-            ops.append("other")
+        elif access(line):
+            ops.append(access(line))
     return found
 
 
@@ -54,19 +83,29 @@ def test_waits_match_the_loads(tmp_path):
     found = kernels(tmp_path)
     tiles = {k: v for k, v in found.items() if "tiles" in k}
     split = {k: v for k, v in found.items() if "split" in k}
-    assert len(tiles) == 4 and len(split) == 8
-    for name, code in found.items():
-        if name in tiles:
-            ahead, per = int(re.search(r"ELi\d+ELi(\d)E", name).group(1)), 9
-        else:
-            ahead, per = 2, 2 * int(re.search(r"splitILb\dELi(\d)E", name).group(1)) + 1
-        n = 0
+    assert len(tiles) == 3 and len(split) == 8
+    for name, code in tiles.items():
+        ahead = int(re.search(r"ELi\d+ELi(\d)E", name).group(1))
+        found, first = tile_steps(code)
+        for wait, ops in found:
+            copies = ops.count("copy")
+            # copies of the group two ahead, then its step's weights: behind the copies waited for
+            # are the weights of that step, the next step's copies and its weights
+            assert copies and ops == ["copy"] * copies + ["load"] * 9, (name, wait, ops)
+            assert wait == 9 + copies + 9, (name, wait, ops)
+        for ops in first:  # as many behind the first group's copies
+            copies = ops.count("copy") // 2
+            lead = ["load"] * 9 if ahead == 2 else []
+            assert ops == lead + (["copy"] * copies + ["load"] * 9) * 2, (name, ops)
+        assert len(found) >= 4 * (ahead + 1) and len(first) >= 4, (name, len(found), len(first))
+    for name, code in split.items():
+        per, n = 2 * int(re.search(r"splitILb\dELi(\d)E", name).group(1)) + 1, 0
         for wait, ops in steps(code):
             copies, loads = ops.count("copy"), ops.count("load")
             if loads == 2 * per:
                 continue  # the first two groups, ahead of the loop
             # copies first, then the weights' loads, nothing else
             assert ops == ["copy"] * copies + ["load"] * per, (name, wait, ops)
-            assert wait == (per if ahead == 1 else per + copies + per), (name, wait, ops)
+            assert wait == per + copies + per, (name, wait, ops)
             n += 1
-        assert n >= (8 if name in tiles else 3), (name, n)
+        assert n >= 3, (name, n)

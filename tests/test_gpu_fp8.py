@@ -335,13 +335,15 @@ def spread(seed, E, most):
 
 
 # (rows of each expert, M, K): large enough for the tiled forms.  128 rows a tile and one group
-# ahead from 512 tiles on, else 96 and two (bf16); 64 rows, one group ahead from 2048 tiles on
-# (fp32); K of one to six groups, whole and not
+# of weights ahead from 200 tiles on, else 96 and two (bf16); 64 rows and two (fp32); K of one to
+# six groups, whole and not
 TILED = tuple((spread(K, 64, 300), M, K) for M in (1030, 2100)
               for K in (16, 128, 144, 256, 400, 512, 640, 752)) + (
     ([5000], 7000, 272), ([5000], 7001, 128), ([1, 4000, 0, 1000], 7000, 400),
     ([64] * 40 + [0] * 30 + [200] * 30, 1030, 384), ([2000, 3], 4100, 2048), ([7] * 300, 1500, 272),
-    ([0] * 500 + [3000] + [0] * 523, 2049, 272), ([40] * 1024, 300, 144))
+    ([0] * 500 + [3000] + [0] * 523, 2049, 272), ([40] * 1024, 300, 144)) + tuple(
+    (spread(K + 1, E, total), M, K) for E, total, M in ((64, 3000, 1030), (20, 200, 700))
+    for K in (16, 128, 144, 256, 400, 512, 640, 752))
 
 
 @pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
