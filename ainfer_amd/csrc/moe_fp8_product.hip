@@ -583,14 +583,17 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
     // that do not fill the CUs or bring mostly weights.  us, 96 rows with two groups ahead and 128
     // with one: 4096 x 4096 -> 4096 76, 68; 2048 46.5, 42.9; 1500 x 2048 -> 5000 28.2, 25.3; 64
     // experts of 128 rows, 4096 -> 2048 148, 139; 1024 x 4096 -> 4096 30.9, 38.1; 256 x 5120 -> 17408
-    // 40.5, 50.9; 512 experts of 8 rows, 2048 -> 1024 246, 253.  (fp32, 64 rows: two ahead are never
-    // slower: 4096 x 4096 -> 4096 127.5, 132.)
+    // 40.5, 50.9; 512 experts of 8 rows, 2048 -> 1024 246, 253.  fp32, 64 rows and
+    // two ahead, 96 and one: 64 experts of 256 rows, 4096 -> 2048 324, 310; of 128 195, 190; 1119 x
+    // 976 -> 13696 45.6, 43.3; 8192 x 4096 -> 4096 271, 267; 2048 x 4096 -> 4096 66, 80; 32 experts of
+    // 156, 1024 -> 2048 39, 44; 96 of 62, 2560 -> 1792 103.8, 105.3.
     // (at most: full tiles, and one that is not full for each expert)
     auto tiles = [&](auto kernel, int rows) {
       const int64_t most = (a.N / rows + used) * mb;
       kernel<<<(int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, 0, s>>>(a);
     };
-    if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
+    if (f32 && row_tiles(96) * mb >= 600 && each > 64) tiles(k_fp8_tiles<true, 96, 1>, 96);
+    else if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
     else if (row_tiles(128) * mb >= 200 && each > 16) tiles(k_fp8_tiles<false, 128, 1>, 128);
     else tiles(k_fp8_tiles<false, 96, 2>, 96);
     return hipGetLastError();

@@ -83,7 +83,7 @@ def test_waits_match_the_loads(tmp_path):
     found = kernels(tmp_path)
     tiles = {k: v for k, v in found.items() if "tiles" in k}
     split = {k: v for k, v in found.items() if "split" in k}
-    assert len(tiles) == 3 and len(split) == 8
+    assert len(tiles) == 4 and len(split) == 8
     for name, code in tiles.items():
         ahead = int(re.search(r"ELi\d+ELi(\d)E", name).group(1))
         found, first = tile_steps(code)

@@ -335,8 +335,8 @@ def spread(seed, E, most):
 
 
 # (rows of each expert, M, K): large enough for the tiled forms.  128 rows a tile and one group
-# of weights ahead from 200 tiles on, else 96 and two (bf16); 64 rows and two (fp32); K of one to
-# six groups, whole and not
+# of weights ahead from 200 tiles on, else 96 and two (bf16); 96 rows and one from 600 tiles on,
+# else 64 and two (fp32); K of one to six groups, whole and not
 TILED = tuple((spread(K, 64, 300), M, K) for M in (1030, 2100)
               for K in (16, 128, 144, 256, 400, 512, 640, 752)) + (
     ([5000], 7000, 272), ([5000], 7001, 128), ([1, 4000, 0, 1000], 7000, 400),
