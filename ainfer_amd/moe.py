@@ -810,7 +810,8 @@ class Fp8Experts:
     def forward(self, x, idx, w, y=None, resid=None, stream=None, keep=False):
         """y[t] = sum_j w[t][j] expert_{idx[t][j]}(x[t]) (+ resid[t]), x and y [T][H] bf16 or
         fp32 rows: rows sorted and quantised, gate and up, gated activation quantised,
-        down, weighted sums.  keep: (y, what backward needs) instead of y."""
+        down, weighted sums.  y and resid may be x.  keep: (y, what backward needs) instead of
+        y."""
         T, k = idx.shape
         I, dev = self.inter, self.gate_up.dev
         with torch.cuda.device(dev), _on(stream):

@@ -162,3 +162,39 @@ def test_captured_step(torch):
             torch.cuda.synchronize()
             for a, b in zip(got, step()):
                 assert torch.equal(a, b)
+
+
+def test_over_its_input(torch):
+    """y and resid may be x itself: the rows are sorted before anything is written."""
+    ex, _ = experts(torch, 8, 256, 128)
+    for T in (1, 7, 900):
+        x, idx, w = routed(torch, T, 3, 8, 256, torch.bfloat16)
+        want = ex.forward(x, idx, w, resid=x)
+        z = x.clone()
+        assert ex.forward(z, idx, w, y=z, resid=z) is z
+        assert torch.equal(z, want)
+
+
+def test_two_calls_at_once(torch):
+    """Calls on two streams, of sizes that take each form of the sort and of the products, do not
+    meet in anything."""
+    ex, _ = experts(torch, 8, 256, 128)
+    state = [routed(torch, T, 4, 8, 256, torch.bfloat16, seed=T) for T in (3, 900, 6000, 11000)]
+    dys = [torch.randn_like(x) for x, _, _ in state]
+
+    def step(i, stream=None):
+        y, kept = ex.forward(*state[i], stream=stream, keep=True)
+        return (y, *ex.backward(dys[i], kept, stream=stream))
+
+    want = [step(i) for i in range(4)]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for p, q in ((2, 3), (1, 2), (0, 3), (3, 1), (2, 2)):
+        got = []
+        for _ in range(3):
+            got.append((p, step(p, a)))
+            got.append((q, step(q, b)))
+        torch.cuda.synchronize()
+        for i, out in got:
+            for x, y in zip(out, want[i]):
+                assert torch.equal(x, y)
