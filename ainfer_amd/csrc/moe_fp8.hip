@@ -101,11 +101,8 @@ hipError_t quant_rows(const void *x, int64_t xld, const void *up, int64_t uld, i
   const int64_t items = (int64_t)N * ((K + 127) / 128) * 8, blocks = (items + 255) / 256;
   const int grid = (int)(blocks < 4096 ? blocks : 4096);
   const int pow2 = scale_kind == AINFER_FP8_SCALE_POW2;
-  if (dtype == AINFER_ACT_F32)
-    k_quant_rows<true, SILU><<<grid, 256, 0, s>>>(x, xld, up, uld, live, N, K, pow2, q, qld, sq);
-  else
-    k_quant_rows<false, SILU><<<grid, 256, 0, s>>>(x, xld, up, uld, live, N, K, pow2, q, qld, sq);
-  return hipGetLastError();
+  return enqueue(dtype == AINFER_ACT_F32 ? k_quant_rows<true, SILU> : k_quant_rows<false, SILU>, grid,
+                 256, s, x, xld, up, uld, live, N, K, pow2, q, qld, sq);
 }
 
 }  // namespace
@@ -126,9 +123,6 @@ hipError_t launch_weight_quant_fp8(const void *w, int dtype, int E, int M, int K
                                    uint8_t *q, float *scales, hipStream_t s) {
   const unsigned blocks = (unsigned)((int64_t)E * ((M + 127) / 128) * ((K + 127) / 128));
   const int pow2 = scale_kind == AINFER_FP8_SCALE_POW2;
-  if (dtype == AINFER_ACT_F32)
-    k_quant_weights<true><<<blocks, 256, 0, s>>>(w, M, K, pow2, q, scales);
-  else
-    k_quant_weights<false><<<blocks, 256, 0, s>>>(w, M, K, pow2, q, scales);
-  return hipGetLastError();
+  return enqueue(dtype == AINFER_ACT_F32 ? k_quant_weights<true> : k_quant_weights<false>, blocks, 256,
+                 s, w, M, K, pow2, q, scales);
 }

@@ -590,20 +590,18 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
     // (at most: full tiles, and one that is not full for each expert)
     auto tiles = [&](auto kernel, int rows) {
       const int64_t most = (a.N / rows + used) * mb;
-      kernel<<<(int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, 0, s>>>(a);
+      return enqueue(kernel, (int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, s, a);
     };
-    if (f32 && row_tiles(96) * mb >= 600 && each > 64) tiles(k_fp8_tiles<true, 96, 1>, 96);
-    else if (f32) tiles(k_fp8_tiles<true, 64, 2>, 64);
-    else if (row_tiles(128) * mb >= 200 && each > 16) tiles(k_fp8_tiles<false, 128, 1>, 128);
-    else tiles(k_fp8_tiles<false, 96, 2>, 96);
-    return hipGetLastError();
+    if (f32 && row_tiles(96) * mb >= 600 && each > 64) return tiles(k_fp8_tiles<true, 96, 1>, 96);
+    if (f32) return tiles(k_fp8_tiles<true, 64, 2>, 64);
+    if (row_tiles(128) * mb >= 200 && each > 16) return tiles(k_fp8_tiles<false, 128, 1>, 128);
+    return tiles(k_fp8_tiles<false, 96, 2>, 96);
   }
   auto split = [&](auto r_c, auto ns_c) {
     constexpr int R = decltype(r_c)::value, NS = decltype(ns_c)::value;
     const int64_t items = (a.N / (16 * NS) + used) * slabs * (4 / R);
     const int grid = (int)std::min<int64_t>(items, R == 4 ? 512 : 1024);
-    if (f32) k_fp8_split<true, R, NS><<<grid, 256, 0, s>>>(a);
-    else k_fp8_split<false, R, NS><<<grid, 256, 0, s>>>(a);
+    return enqueue(f32 ? k_fp8_split<true, R, NS> : k_fp8_split<false, R, NS>, grid, 256, s, a);
   };
   using one = std::integral_constant<int, 1>;
   using two = std::integral_constant<int, 2>;
@@ -612,11 +610,10 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
   // (1 x 5120 -> 17408 17.5, 19.2 with 32); tiles of 32 rows from 128 items of them on
   // (32 x 4096 -> 4096 9.0 with 16, 10.5; 64 x 4096 -> 4096 12.2, 10.3), 64 weight rows
   // from 256 on (64 x 4096 -> 4096 10.3 with 32, 13.5; 128 x 4096 -> 4096 15.8, 13.2).
-  if (each > 16 && items2 >= 256) split(four(), two());
-  else if (each > 16 && items2 >= 128) split(two(), two());
-  else if (row_tiles(16) > 1) split(two(), one());
-  else split(one(), one());
-  return hipGetLastError();
+  if (each > 16 && items2 >= 256) return split(four(), two());
+  if (each > 16 && items2 >= 128) return split(two(), two());
+  if (row_tiles(16) > 1) return split(two(), one());
+  return split(one(), one());
 }
 
 // A thread writes 16 codes: of a row's neighbouring columns, or (TRANS) of 16 rows.
@@ -655,7 +652,5 @@ hipError_t launch_fp8_pack(const uint8_t *w, int E, int M, int K, int transpose,
                            hipStream_t s) {
   const int64_t chunks = (int64_t)(fp8_packed_bytes(E, M, K) / 16);
   const int grid = (int)std::min<int64_t>((chunks + 255) / 256, 1 << 20);
-  if (transpose) k_fp8_pack<true><<<grid, 256, 0, s>>>(w, M, K, chunks, packed);
-  else k_fp8_pack<false><<<grid, 256, 0, s>>>(w, M, K, chunks, packed);
-  return hipGetLastError();
+  return enqueue(transpose ? k_fp8_pack<true> : k_fp8_pack<false>, grid, 256, s, w, M, K, chunks, packed);
 }

@@ -158,11 +158,8 @@ hipError_t launch_silu_backward(const void *d, int64_t dld, const void *g, int64
                                 hipStream_t s) {
   const int64_t blocks = ((int64_t)N * ((I + 7) / 8) + 255) / 256;
   const int grid = (int)(blocks < 4096 ? blocks : 4096);
-  if (dtype == AINFER_ACT_F32)
-    k_silu_bwd<true><<<grid, 256, 0, s>>>(d, dld, g, gld, u, uld, live, N, I, dg, dgld, du, duld);
-  else
-    k_silu_bwd<false><<<grid, 256, 0, s>>>(d, dld, g, gld, u, uld, live, N, I, dg, dgld, du, duld);
-  return hipGetLastError();
+  return enqueue(dtype == AINFER_ACT_F32 ? k_silu_bwd<true> : k_silu_bwd<false>, grid, 256, s, d, dld,
+                 g, gld, u, uld, live, N, I, dg, dgld, du, duld);
 }
 
 hipError_t launch_silu_rows(const void *g, int64_t gld, const void *u, int64_t uld, int in_dtype,

@@ -624,38 +624,31 @@ hipError_t launch_sort_rows(const ainfer_moe_sorting &d, const void *x, int64_t 
     const int pieces = !rows ? 1 : d.fp8 ? (H + 15) / 16 : (H + (f32 ? 3 : 7)) / (f32 ? 4 : 8);
     const int parts = std::max(1, std::min((pieces + 255) / 256, 256 / std::max(T, 1)));
     auto few = [&](auto kernel) {
-      kernel<<<dim3(T + 1, parts), 256, 0, s>>>(idx, T, k, E, offsets, pos, x, xld, H, pow2,
-                                                (uint8_t *)rows, rld, row_scales);
+      return enqueue(kernel, dim3(T + 1, parts), 256, s, idx, T, k, E, offsets, pos, x, xld, H, pow2,
+                     (uint8_t *)rows, rld, row_scales);
     };
-    if (!rows) few(k_sort_few<0>);
-    else if (d.fp8) few(f32 ? k_sort_few<9> : k_sort_few<8>);
-    else few(f32 ? k_sort_few<4> : k_sort_few<2>);
-    return hipGetLastError();
+    if (!rows) return few(k_sort_few<0>);
+    if (d.fp8) return few(f32 ? k_sort_few<9> : k_sort_few<8>);
+    return few(f32 ? k_sort_few<4> : k_sort_few<2>);
   }
+  hipError_t rc;
   if (n <= SORT_OWN) {
-    k_sort_own<<<(int)((n + 255) / 256), 1024, 0, s>>>(idx, (int)n, E, offsets, pos);
+    rc = enqueue(k_sort_own, (int)((n + 255) / 256), 1024, s, idx, (int)n, E, offsets, pos);
   } else {
     int32_t *counts = (int32_t *)ws;
     const int Ep = (E + 3) & ~3;
-    k_sort_count<<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts);
-    k_sort_place<<<chunks, 256, 0, s>>>(idx, n, E, Ep, rounds, counts, chunks, offsets, pos);
+    rc = enqueue(k_sort_count, chunks, 256, s, idx, n, E, Ep, rounds, counts);
+    if (rc == hipSuccess)
+      rc = enqueue(k_sort_place, chunks, 256, s, idx, n, E, Ep, rounds, counts, chunks, offsets, pos);
   }
-  if (!rows) return hipGetLastError();
+  if (rc != hipSuccess || !rows) return rc;
   auto grid = [](int64_t items) { return (int)std::min<int64_t>((items + 255) / 256, 8192); };
-  if (d.fp8) {
-    const int g = grid((int64_t)T * ((H + 127) / 128) * 8);
-    if (f32)
-      k_move_quant<true><<<g, 256, 0, s>>>(x, xld, pos, T, k, H, pow2, (uint8_t *)rows, rld, row_scales);
-    else
-      k_move_quant<false><<<g, 256, 0, s>>>(x, xld, pos, T, k, H, pow2, (uint8_t *)rows, rld, row_scales);
-  } else if (f32) {
-    k_move_rows<4><<<grid((int64_t)T * ((H + 3) / 4)), 256, 0, s>>>((const uint8_t *)x, xld, pos, T, k, H,
-                                                                   (uint8_t *)rows, rld);
-  } else {
-    k_move_rows<2><<<grid((int64_t)T * ((H + 7) / 8)), 256, 0, s>>>((const uint8_t *)x, xld, pos, T, k, H,
-                                                                   (uint8_t *)rows, rld);
-  }
-  return hipGetLastError();
+  if (d.fp8)
+    return enqueue(f32 ? k_move_quant<true> : k_move_quant<false>,
+                   grid((int64_t)T * ((H + 127) / 128) * 8), 256, s, x, xld, pos, T, k, H, pow2,
+                   (uint8_t *)rows, rld, row_scales);
+  return enqueue(f32 ? k_move_rows<4> : k_move_rows<2>, grid((int64_t)T * (f32 ? (H + 3) / 4 : (H + 7) / 8)),
+                 256, s, (const uint8_t *)x, xld, pos, T, k, H, (uint8_t *)rows, rld);
 }
 
 hipError_t launch_unpermute(const void *rows, int64_t rld, int rows_dtype, int N,
@@ -665,12 +658,11 @@ hipError_t launch_unpermute(const void *rows, int64_t rld, int rows_dtype, int N
   const int64_t items = (int64_t)T * ((H + 7) / 8);
   const int grid = (int)std::min<int64_t>((items + 255) / 256, 8192);
   auto run = [&](auto kernel) {
-    kernel<<<grid, 256, 0, s>>>(rows, rld, N, pos, w, T, k, H, resid, sld, y, yld);
+    return enqueue(kernel, grid, 256, s, rows, rld, N, pos, w, T, k, H, resid, sld, y, yld);
   };
   const bool r32 = rows_dtype == AINFER_ACT_F32, y32 = y_dtype == AINFER_ACT_F32;
-  if (r32) run(y32 ? k_unpermute<true, true> : k_unpermute<true, false>);
-  else run(y32 ? k_unpermute<false, true> : k_unpermute<false, false>);
-  return hipGetLastError();
+  if (r32) return run(y32 ? k_unpermute<true, true> : k_unpermute<true, false>);
+  return run(y32 ? k_unpermute<false, true> : k_unpermute<false, false>);
 }
 
 hipError_t launch_unpermute_backward(const void *dy, int64_t yld, int y_dtype, const void *rows,
@@ -678,10 +670,10 @@ hipError_t launch_unpermute_backward(const void *dy, int64_t yld, int y_dtype, c
                                      const float *w, int T, int k, int H, void *drows, int64_t dld,
                                      float *dw, hipStream_t s) {
   auto run = [&](auto kernel) {
-    kernel<<<dim3(T, (k + 1) / 2), 256, 0, s>>>(dy, yld, rows, rld, N, pos, w, k, H, drows, dld, dw);
+    return enqueue(kernel, dim3(T, (k + 1) / 2), 256, s, dy, yld, rows, rld, N, pos, w, k, H, drows, dld,
+                   dw);
   };
   const bool r32 = rows_dtype == AINFER_ACT_F32, y32 = y_dtype == AINFER_ACT_F32;
-  if (y32) run(r32 ? k_unpermute_bwd<true, true> : k_unpermute_bwd<true, false>);
-  else run(r32 ? k_unpermute_bwd<false, true> : k_unpermute_bwd<false, false>);
-  return hipGetLastError();
+  if (y32) return run(r32 ? k_unpermute_bwd<true, true> : k_unpermute_bwd<true, false>);
+  return run(r32 ? k_unpermute_bwd<false, true> : k_unpermute_bwd<false, false>);
 }
