@@ -355,18 +355,17 @@ def _vector(t, name, dtype, n, dev):
         raise L.MoeError(f"{name}: {n} contiguous {dtype} values on the inputs' device")
 
 
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(fn, dev, stream, *args):
     """fn(*args, stream) on the device the tensors are on; its current stream
     when none is given."""
-    if dev != torch._C._cuda_getDevice():
+    if dev != _current_device():
         with torch.cuda.device(dev):
-            return _enqueue(fn, dev, stream, args)
-    return _enqueue(fn, dev, stream, args)
-
-
-def _enqueue(fn, dev, stream, args):
-    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-    rc = fn(*args, raw)
+            return _call(fn, dev, stream, *args)
+    rc = fn(*args, _raw_stream(dev) if stream is None else stream.cuda_stream)
     if rc:
         L.check(rc)
 
