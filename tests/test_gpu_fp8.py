@@ -376,6 +376,17 @@ def test_product_pitches(torch, dtype):
             assert (buf[:, :off] == 3).all() and (buf[:, off + M:] == 3).all()
 
 
+@pytest.mark.parametrize("dtype", ("float32", "bfloat16"))
+def test_product_largest_pitch(torch, dtype):
+    """Rows of codes 2^24 bytes apart: a tile's last one is 2^31 - 2^24 behind its first."""
+    for M in (200, 30000):
+        q, sq, w, scales, offsets = state(torch, [130], M, 272, M)
+        far = torch.empty((129 << 24) + 272, dtype=torch.uint8, device="cuda").view(R.E4M3)
+        far = far.as_strided((130, 272), (1 << 24, 1))
+        far.copy_(q)
+        check(torch, far, sq, w, scales, offsets, getattr(torch, dtype))
+
+
 def test_product_garbage_behind_the_row(torch):
     """NaN codes in the padding of pitched rows and in the next row's weights change nothing."""
     for counts in ([2, 1], [70, 60]):
