@@ -121,18 +121,19 @@ __device__ __forceinline__ void fp8_codes(const float (&v)[N], float s, uint32_t
   }
 }
 
-// g / (1 + exp(-g)) * u to 2^-21 of itself and 2^-119 of u: exp(-g) as 2^(h + l), h + l = -g log2 e with the rounding
-// of h in l, by the hardware's exp2 and a factor 1 + l ln 2 (3 2^-24 together), the sum
-// 2^-24, the hardware's reciprocal 2^-23 and two products 2^-24 each.  The exponent's g is
-// kept within +-200, where exp(-g) is 0 or infinite; from exp(-g) = 2^126 on the reciprocal may
-// be 0 (g 2^-126 is what is lost, g being -87 to -89 there, and less below).  (With silu_mul's expf and division, and
-// a division for each code, 32768 x 1024 bf16 took 56.8 us, now 40.4.)
+// g / (1 + exp(-g)) * u to 2^-21 of itself and 2^-119 of u: exp(-g) as 2^(h + l), h + l = -g
+// log2 e with the rounding of h in l, by the hardware's exp2 and a factor 1 + l ln 2 (3 2^-24
+// together), the sum 2^-24, the hardware's reciprocal 2^-23 and two products 2^-24 each.  The
+// exponent's g is kept within +-200, where exp(-g) is 0 or infinite; from exp(-g) = 2^126 on the
+// reciprocal may be 0 (g 2^-126 is what is lost, g being -87 to -89 there, and less below).
+// (With silu_mul's expf and division, and a division for each code, 32768 x 1024 bf16 took 56.8
+// us, now 40.4.)
 __device__ __forceinline__ float silu_mul_near(float g, float u) {
   const float c = fminf(fmaxf(g, -200.0f), 200.0f);
   const float h = c * -1.44269502162933349609f;             // -log2 e, rounded
   const float l = fmaf(c, -1.44269502162933349609f, -h) + c * -1.92596299112661746e-8f;
   float e = __builtin_amdgcn_exp2f(h);
-  e = fmaf(e, l * 0.69314718056f, e);
+  e = fminf(fmaf(e, l * 0.69314718056f, e), INFINITY);  // an infinite e stays one (no NaN)
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 

@@ -374,13 +374,14 @@ __device__ __forceinline__ void run_tile(const Fp8Args &a, uint32_t lds0, const 
   const uint32_t xr0 = (uint32_t)(col * 128 + ((qd ^ (col & 7)) << 4));
   const uint32_t xs0 = (uint32_t)(St::X + col * NS * 4);
 
-  // Group g: its rows were sent for at the start of the step two before, its weights at the
-  // end of the one AHEAD + 1 before, as their registers came free.  (Rows, then weights, at the
+  // Group g: its rows were sent for at the start of the step two before, its weights at the end
+  // of the one AHEAD + 1 before, as their registers came free.  (Rows, then weights, at the
   // start of the step AHEAD before: 8192^3 543 instead of 507 us, 64 experts of 512 rows 375
-  // instead of 346, 1024 x 4096 -> 4096 37.6 instead of 32.9.)  Behind the copies of g there are the loads of one group's weights, the copies
-  // of g + 1 and another group's weights.  The loop's last steps load the last group again, so
-  // that this count is the same in every one of them.  (A load whose value nothing takes would not
-  // be there to be counted: the steps behind the loop issue none, and wait for what is left.)
+  // instead of 346, 1024 x 4096 -> 4096 37.6 instead of 32.9.)  Behind the copies of g there are
+  // the loads of one group's weights, the copies of g + 1 and another group's weights.  The
+  // loop's last steps load the last group again, so that this count is the same in every one of
+  // them.  (A load whose value nothing takes would not be there to be counted: the steps behind
+  // the loop issue none, and wait for what is left.)
   constexpr int NEWER = 9 + St::DMA + 1 + 9;
   uint32_t here = 0, fill = 2 * St::BYTES;  // the stages of groups g and g + 2
   auto step = [&](int g, Weights &w, auto loads) __attribute__((always_inline)) {

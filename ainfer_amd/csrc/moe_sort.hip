@@ -367,8 +367,8 @@ __global__ __launch_bounds__(256) void k_sort_few(const int32_t *idx, int T, int
 }
 
 // Rows as they are: a lane takes 16 bytes of a token's row to its k places (SIZE: bytes of an
-// element; the last piece of a row is its last 16), past the caches (ordinary stores: 68 instead of 51 us for 8192 rows of 4096 bf16,
-// half of 8 places each; 268 MB written).
+// element; the last piece of a row is its last 16), past the caches (ordinary stores: 68 instead
+// of 51 us for 8192 rows of 4096 bf16, half of 8 places each; 268 MB written).
 template <int SIZE>
 __global__ __launch_bounds__(256) void k_move_rows(const uint8_t *x, int64_t xld,
                                                    const int32_t *pos, int T, int k, int H,

@@ -572,7 +572,7 @@ typedef struct ainfer_moe_fp8 {
 } ainfer_moe_fp8;
 /* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
  *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
- * sums in fp32, y rounded once.  With bf16 y the matrix instruction drops what is more than 13
+ * sums and the two scales' products in fp32, y rounded once.  With bf16 y the matrix instruction drops what is more than 13
  * bits below the largest of eight neighbouring products: at most 7 * 2^-13 of the sum of
  * magnitudes, 1.4e-5 of it for normal values; with fp32 y products are whole.  q: N rows of K
  * codes at q_ld elements (16-byte aligned, a multiple of 16, at most 2^24), sq

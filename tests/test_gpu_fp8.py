@@ -159,6 +159,29 @@ def test_silu_mul_fp8(torch, n, I, dtype, pow2):
     assert (off <= (2.0 ** -4 + 2.0 ** -20) * v.abs() + 2.0 ** -10 * sw * (1 + 2.0 ** -20)).all()
 
 
+def test_silu_mul_fp8_of_far_gates(torch):
+    """Gates whose exponential nears fp32's largest value or passes it: within 2^-119 of up
+    beside the codes' rounding, and no infinities."""
+    from ainfer_amd import moe
+    n, I = 64, 256
+    g = gen(torch, 3)
+    gate = torch.linspace(-130, -70, n * I, device="cuda").view(n, I)
+    for size in (1.0, 1e30, 1e-30):
+        up = torch.randn(n, I, generator=g, device="cuda") * size
+        q, s = moe.silu_mul_fp8(gate, up)
+        v = gate.double() * torch.sigmoid(gate.double()) * up.double()
+        sw = R.wide(s.double(), 1, I)
+        off = (q.double() * sw - v).abs()
+        bound = (2.0 ** -4 + 2.0 ** -20) * v.abs() + 2.0 ** -10 * sw * (1 + 2.0 ** -20)
+        assert s.isfinite().all() and (off <= bound + 2.0 ** -119 * up.double().abs()).all()
+    far = torch.tensor([-3e38, -1e4, -200.5, 3e38, 1e4, 0.0, -0.0, float("inf")] * 16, device="cuda")
+    q, s = moe.silu_mul_fp8(far[None], torch.full_like(far, 0.5)[None])
+    assert s.isinf().all()  # the infinite gate's
+    q, s = moe.silu_mul_fp8(far[None, :112].where(far[:112].isfinite(), torch.zeros(())), torch.ones(
+        1, 112, device="cuda"))
+    assert s.isfinite().all() and (q.float() * s[0, 0] <= 3.1e38).all() and q.float().max() == 448
+
+
 def test_live_rows(torch):
     """Rows behind the count, and columns behind the row, are left as they are."""
     from ainfer_amd import moe
