@@ -572,18 +572,18 @@ typedef struct ainfer_moe_fp8 {
 } ainfer_moe_fp8;
 /* y[n][m] = sum over the groups g of 128 columns of sq[n][g] * scales[e][m / 128][g] *
  *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
- * sums and the two scales' products in fp32, y rounded once.  With bf16 y the matrix instruction drops what is more than 13
- * bits below the largest of eight neighbouring products: at most 7 * 2^-13 of the sum of
- * magnitudes, 1.4e-5 of it for normal values; with fp32 y products are whole.  q: N rows of K
- * codes at q_ld elements (16-byte aligned, a multiple of 16, at most 2^24), sq
- * [N][ceil(K / 128)], offsets device [E + 1] ascending (NULL with one expert: all N rows), y: N
- * rows of M values at y_ld elements.  Rows of y outside
- * [offsets[0], offsets[E]) are left as they were; offsets outside [0, N] are taken as
- * its ends, and rows of experts that overlap are unspecified.  A NaN code or scale
- * reaches the values whose sums it is in.  y must not overlap anything that is read.
- * The gradient to x is the same call with the transposed weights (M a multiple of 16):
- * ainfer_moe_fp8_pack(w, E, K, M, 1, ...) and scales [E][ceil(K / 128)][ceil(M / 128)], as
- * blocks are square. */
+ * sums and the two scales' products in fp32, y rounded once.  With bf16 y the matrix
+ * instruction drops what is more than 13 bits below the largest of eight neighbouring
+ * products: at most 7 * 2^-13 of the sum of magnitudes, 1.4e-5 of it for normal values;
+ * with fp32 y products are whole.  q: N rows of K codes at q_ld elements (16-byte
+ * aligned, a multiple of 16, at most 2^24), sq [N][ceil(K / 128)], offsets device [E +
+ * 1] ascending (NULL with one expert: all N rows), y: N rows of M values at y_ld
+ * elements.  Rows of y outside [offsets[0], offsets[E]) are left as they were; offsets
+ * outside [0, N] are taken as its ends, and rows of experts that overlap are
+ * unspecified.  A NaN code or scale reaches the values whose sums it is in.  y must not
+ * overlap anything that is read. The gradient to x is the same call with the transposed
+ * weights (M a multiple of 16): ainfer_moe_fp8_pack(w, E, K, M, 1, ...) and scales
+ * [E][ceil(K / 128)][ceil(M / 128)], as blocks are square. */
 int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_ld,
                            const float *sq, const int32_t *offsets, int32_t N, void *y,
                            int64_t y_ld, void *stream);
