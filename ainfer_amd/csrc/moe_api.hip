@@ -3,6 +3,7 @@
 // down -> combine.  Host code; every device buffer comes from the caller.
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -729,22 +730,42 @@ bool is_scale_kind(int32_t kind) {
 }
 // a pitch that fits rows of `cols` elements
 bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > MAX_ROW_LD; }
-// Whether `rows` rows that are written meet n bytes at p: all of their bytes where
-// the rows are whole, their first address where a pitch leaves room between them.
+// `rows` rows of `cols` elements as bytes; rows without room between them are one row
+struct ByteRows {
+  intptr_t at;
+  int64_t n, pitch, bytes;
+};
+ByteRows byte_rows(const void *p, int64_t rows, int64_t ld, int64_t cols, int size) {
+  if (rows == 1 || ld == cols) return {(intptr_t)p, rows > 0, rows * cols * size, rows * cols * size};
+  return {(intptr_t)p, rows, ld * size, cols * size};
+}
+// whether a row of r meets [at, at + n): the first row that ends behind `at` starts ahead of its end
+bool rows_meet(const ByteRows &r, intptr_t at, int64_t n) {
+  if (r.n == 0 || n == 0) return false;
+  const intptr_t end = r.at + r.bytes;
+  const int64_t i = at < end ? 0 : (at - end) / r.pitch + 1;
+  return i < r.n && r.at + i * r.pitch < at + n;
+}
+// Whether rows that are written meet n bytes at p.
 bool over(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, const void *p,
           size_t n) {
-  if (!out || !p) return false;
-  if (rows == 1 || ld == cols) return meet(out, (size_t)(rows * cols * size), p, n);
-  return out == p;
+  return out && p && rows_meet(byte_rows(out, rows, ld, cols, size), (intptr_t)p, (int64_t)n);
 }
-// Whether rows that are written meet rows that are read: all bytes where both are whole, the
-// first addresses else.
+// Whether rows that are written meet other rows.  With rows of both pitched, and differently, each
+// one's first row is looked for among the other's.
 bool over_rows(const void *out, int64_t rows, int64_t ld, int64_t cols, int size, const void *in,
                int64_t in_rows, int64_t in_ld, int64_t in_cols, int in_size) {
   if (!out || !in) return false;
-  if (in_rows == 1 || in_ld == in_cols)
-    return over(out, rows, ld, cols, size, in, (size_t)(in_rows * in_cols * in_size));
-  return out == in;
+  const ByteRows a = byte_rows(out, rows, ld, cols, size),
+                 b = byte_rows(in, in_rows, in_ld, in_cols, in_size);
+  if (a.n > 1 && b.n > 1 && a.pitch == b.pitch) {
+    // row j of b is d + (j - i) pitch from row i of a: the least such distance above -b.bytes
+    const int64_t d = b.at - a.at, low = -b.bytes - d;
+    const int64_t below = low / a.pitch - (low % a.pitch < 0);
+    const int64_t m = std::max(below + 1, 1 - a.n);
+    return m < b.n && d + m * a.pitch < a.bytes;
+  }
+  return (b.n && rows_meet(a, b.at, b.bytes)) || (a.n && rows_meet(b, a.at, a.bytes));
 }
 int check_fp8_sizes(int32_t E, int32_t M, int32_t K) {
   if (E < 1 || E > 1024 || M < 1 || M > (1 << 20) || K < 16 || K > 65536 || K % 16 ||
@@ -1306,15 +1327,18 @@ int ainfer_moe_silu_mul_backward(const void *dact, int64_t dact_ld, const void *
   const int sz = act_size(dtype);
   if (bad_ld(dact_ld, I) || bad_ld(gate_ld, I) || bad_ld(up_ld, I) || bad_ld(dgate_ld, I) ||
       bad_ld(dup_ld, I) || mis(dact, sz) || mis(gate, sz) || mis(up, sz) || mis(dgate, sz) ||
-      mis(dup, sz) || mis(n_live, 4) || dgate == dup)
+      mis(dup, sz) || mis(n_live, 4))
     return AINFER_ERR_ARG;
   // in place only where every element lies on its own input
   const void *in[3] = {dact, gate, up};
   const int64_t in_ld[3] = {dact_ld, gate_ld, up_ld};
+  auto meets = [&](const void *out, int64_t ld, int i) {
+    if (out == in[i]) return N > 1 && ld != in_ld[i];
+    return over_rows(out, N, ld, I, sz, in[i], N, in_ld[i], I, sz);
+  };
   for (int i = 0; i < 3; ++i)
-    if ((in[i] == dgate && N > 1 && in_ld[i] != dgate_ld) ||
-        (in[i] == dup && N > 1 && in_ld[i] != dup_ld))
-      return AINFER_ERR_ARG;
+    if (meets(dgate, dgate_ld, i) || meets(dup, dup_ld, i)) return AINFER_ERR_ARG;
+  if (over_rows(dgate, N, dgate_ld, I, sz, dup, N, dup_ld, I, sz)) return AINFER_ERR_ARG;
   if (over(dgate, N, dgate_ld, I, sz, n_live, 4) || over(dup, N, dup_ld, I, sz, n_live, 4))
     return AINFER_ERR_ARG;
   HIP_TRY(launch_silu_backward(dact, dact_ld, gate, gate_ld, up, up_ld, dtype, n_live, N, I, dgate,
@@ -1359,7 +1383,8 @@ int ainfer_moe_silu_mul_fp8(const void *gate, int64_t gate_ld, const void *up, i
     return AINFER_ERR_ARG;
   const size_t scales = (size_t)N * ((I + 127) / 128) * 4;
   if (over_rows(q, N, q_ld, I, 1, gate, N, gate_ld, I, sz) ||
-      over_rows(q, N, q_ld, I, 1, up, N, up_ld, I, sz) || meet(sq, scales, n_live, 4) || over(gate, N, gate_ld, I, sz, sq, scales) ||
+      over_rows(q, N, q_ld, I, 1, up, N, up_ld, I, sz) || meet(sq, scales, n_live, 4) ||
+      over(gate, N, gate_ld, I, sz, sq, scales) ||
       over(up, N, up_ld, I, sz, sq, scales) || over(q, N, q_ld, I, 1, sq, scales) ||
       over(q, N, q_ld, I, 1, n_live, 4))
     return AINFER_ERR_ARG;
@@ -1467,7 +1492,8 @@ int ainfer_moe_sort_rows(const ainfer_moe_sorting *s, const void *x, int64_t x_l
       auto hit = [&](const void *p, size_t bytes) {
         return over(rows, P, rows_ld, H, rsz, p, bytes) || over(x, T, x_ld, H, xsz, p, bytes);
       };
-      if (over_rows(rows, P, rows_ld, H, rsz, x, T, x_ld, H, xsz) || hit(offsets, no) || hit(pos, n) || hit(ws, nw) || hit(sc, ns) ||
+      if (over_rows(rows, P, rows_ld, H, rsz, x, T, x_ld, H, xsz) || hit(offsets, no) ||
+          hit(pos, n) || hit(ws, nw) || hit(sc, ns) ||
           over(rows, P, rows_ld, H, rsz, topk_idx, n))
         return AINFER_ERR_ARG;
     }
@@ -1494,7 +1520,8 @@ int ainfer_moe_unpermute(const void *rows, int64_t rows_ld, int32_t rows_dtype, 
   const size_t n = (size_t)T * top_k * 4;
   if (over_rows(y, T, y_ld, H, ysz, rows, N, rows_ld, H, rsz) ||
       over(y, T, y_ld, H, ysz, pos, n) || over(y, T, y_ld, H, ysz, w, n) ||
-      (resid == y && T > 1 && resid_ld != y_ld))
+      (resid == y ? T > 1 && resid_ld != y_ld
+                  : over_rows(y, T, y_ld, H, ysz, resid, T, resid_ld, H, ysz)))
     return AINFER_ERR_ARG;
   HIP_TRY(launch_unpermute(rows, rows_ld, rows_dtype, N, pos, w, T, top_k, H, resid, resid_ld, y,
                            y_ld, y_dtype, (hipStream_t)stream));
