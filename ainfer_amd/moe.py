@@ -621,7 +621,9 @@ class Fp8Weights:
     """The weights of E experts' projection (or one matrix, E = 1), resident on one
     device: e4m3 codes w [E][M][K] (float8_e4m3fn or uint8) laid out for the product
     (w itself is not kept), and their fp32 scales [E][ceil(M / 128)][ceil(K / 128)] (kept).
-    transpose: the weights are W^T, [E][K][M], for the gradient to x (M a multiple of 16)."""
+    transpose: the weights are W^T, [E][K][M], for the gradient to x (M a multiple of 16).
+    stream: where they are laid out, behind what is on it; w may be dropped at once, products
+    on other streams have to wait for it."""
 
     def __init__(self, w, scales, y_dtype=torch.bfloat16, transpose=False, stream=None):
         dev = w.get_device()
@@ -643,6 +645,9 @@ class Fp8Weights:
             self.scales = scales.transpose(1, 2).contiguous() if transpose else scales
         _call(L.lib().ainfer_moe_fp8_pack, dev, stream, w.data_ptr(), E, M, K, int(transpose),
               self.packed.data_ptr(), n)
+        if stream is not None:  # their memory is not given out again before it has been read
+            w.record_stream(stream)
+            scales.record_stream(stream)
         self.shape, self.dev, self.y_dtype = (E, M, K), dev, y_dtype
         self.structs = {dt: L.Fp8(E, M, K, code, self.packed.data_ptr(), self.scales.data_ptr())
                         for dt, code in _ACT.items()}
