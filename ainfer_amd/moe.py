@@ -811,12 +811,30 @@ class Fp8Experts:
         self.gate_up, self.down, self.back, self.pow2 = gate_up, down, back, pow2
         self.n_experts, self.inter, self.hidden = E, I, H
 
+    def _check(self, x, idx, w, y, resid):
+        """(T, k); every tensor of a call, before the first kernel is enqueued."""
+        _, dev, T, _, _ = _rows(x, "x", self.hidden)
+        if dev != self.gate_up.dev:
+            raise L.MoeError("x: on the experts' device")
+        for t, name, dt in ((idx, "idx", torch.int32), (w, "w", torch.float32)):
+            if not (t.dtype == dt and t.dim() == 2 and t.shape[0] == T and t.shape == idx.shape
+                    and t.get_device() == dev and t.is_contiguous()):
+                raise L.MoeError(f"{name}: contiguous {dt} [T][k] on x's device")
+        for t, name in ((y, "y"), (resid, "resid")):
+            if t is not None:
+                _, tdev, n, _, _ = _rows(t, name, self.hidden)
+                if tdev != dev or n != T:
+                    raise L.MoeError(f"{name}: a row for each of x's, on its device")
+        if resid is not None and resid.dtype != (x if y is None else y).dtype:
+            raise L.MoeError("resid: y's type")
+        return idx.shape
+
     def forward(self, x, idx, w, y=None, resid=None, stream=None, keep=False):
         """y[t] = sum_j w[t][j] expert_{idx[t][j]}(x[t]) (+ resid[t]), x and y [T][H] bf16 or
         fp32 rows: rows sorted and quantised, gate and up, gated activation quantised,
         down, weighted sums.  y and resid may be x.  keep: (y, what backward needs) instead of
         y."""
-        T, k = idx.shape
+        T, k = self._check(x, idx, w, y, resid)
         I, dev = self.inter, self.gate_up.dev
         with torch.cuda.device(dev), _on(stream):
             ws = sort_workspace(T, k, self.n_experts, x.device)
