@@ -833,7 +833,7 @@ class Fp8Experts:
         """y[t] = sum_j w[t][j] expert_{idx[t][j]}(x[t]) (+ resid[t]), x and y [T][H] bf16 or
         fp32 rows: rows sorted and quantised, gate and up, gated activation quantised,
         down, weighted sums.  y and resid may be x.  keep: (y, what backward needs) instead of
-        y."""
+        y; backward is to run on the same stream, or behind it."""
         T, k = self._check(x, idx, w, y, resid)
         I, dev = self.inter, self.gate_up.dev
         with torch.cuda.device(dev), _on(stream):
@@ -847,13 +847,19 @@ class Fp8Experts:
             unpermute(o, pos, w, y, resid)
         return (y, (h, o, offsets, pos, w)) if keep else y
 
-    def backward(self, dy, kept, stream=None):
+    def backward(self, dy, kept, stream=None, resid=None):
         """(dx [T][H] of dy's type, dw [T][k] fp32) from dy [T][H] and forward's kept
-        tensors.  The weights are constants; the products' gradients are quantised to
+        tensors.  dx is the experts' share alone: the gradient of forward's resid is dy.  resid
+        [T][H] of dy's type is added to dx before it is rounded: dy itself where forward's
+        resid was x.  The weights are constants; the products' gradients are quantised to
         e4m3 as the activations are, and each rounding passes its gradient on."""
         if self.back is None:
             raise L.MoeError("experts with transposed weights (back)")
         h, o, offsets, pos, w = kept
+        if resid is not None:
+            _, rdev, n, _, _ = _rows(resid, "resid", self.hidden)
+            if not (resid.dtype == dy.dtype and rdev == dy.get_device() and n == dy.shape[0]):
+                raise L.MoeError("resid: dy's shape, type and device")
         I = self.inter
         with torch.cuda.device(self.gate_up.dev), _on(stream):
             do, dw = unpermute_backward(dy, o, pos, w, torch.empty_like(o), torch.empty_like(w))
@@ -864,5 +870,5 @@ class Fp8Experts:
             silu_mul_backward(dact, h[:, :I], h[:, I:], dh[:, :I], dh[:, I:], live=offsets)
             q, sq = act_quant_fp8(dh, pow2=self.pow2, live=offsets)
             drows = self.back[0].product(q, sq, offsets=offsets)
-            dx = unpermute(drows, pos, None, torch.empty_like(dy))
+            dx = unpermute(drows, pos, None, torch.empty_like(dy), resid)
         return dx, dw
