@@ -40,7 +40,7 @@ EXPORTS = (
     "ainfer_moe_route_scored", "ainfer_moe_lora_workspace_bytes", "ainfer_moe_lora_apply",
     "ainfer_moe_silu_mul",
     "ainfer_moe_act_quant_fp8", "ainfer_moe_weight_quant_fp8", "ainfer_moe_fp8_packed_bytes",
-    "ainfer_moe_fp8_pack", "ainfer_moe_fp8_product",
+    "ainfer_moe_fp8_pack", "ainfer_moe_fp8_product", "ainfer_moe_debug_fp8_form",
     "ainfer_moe_silu_mul_fp8", "ainfer_moe_silu_mul_backward",
     "ainfer_moe_sort_workspace_bytes", "ainfer_moe_sort_rows", "ainfer_moe_unpermute",
     "ainfer_moe_unpermute_backward",
@@ -149,6 +149,7 @@ def lib():
         L.ainfer_moe_fp8_packed_bytes.argtypes = [I32, I32, I32]
         L.ainfer_moe_fp8_pack.argtypes = [P, I32, I32, I32, I32, P, SZ, P]
         L.ainfer_moe_fp8_product.argtypes = [C.POINTER(Fp8), P, I64, P, P, I32, P, I64, P]
+        L.ainfer_moe_debug_fp8_form.argtypes = [I32, I32, I32, I32, I32, C.POINTER(I32), C.POINTER(I32)]
         L.ainfer_moe_silu_mul_fp8.argtypes = [P, I64, P, I64, I32, P, I32, I32, I32, P, I64, P, P]
         L.ainfer_moe_silu_mul_backward.argtypes = [P, I64, P, I64, P, I64, I32, P, I32, I32, P, I64,
                                                    P, I64, P]

@@ -1451,6 +1451,19 @@ int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_
   return AINFER_OK;
 }
 
+int ainfer_moe_debug_fp8_form(int32_t E, int32_t M, int32_t K, int32_t N, int32_t y_dtype,
+                              int32_t *weight_rows, int32_t *rows) {
+  int rc = check_fp8_sizes(E, M, K);
+  if (rc) return rc;
+  if (N < 1 || N > AINFER_MOE_MAX_ROWS) return AINFER_ERR_TOKENS;
+  if (!is_act(y_dtype)) return AINFER_ERR_ARG;
+  if (!weight_rows || !rows) return AINFER_ERR_NULL;
+  const Fp8Form form = fp8_form(E, M, K, N, y_dtype == AINFER_ACT_F32);
+  *weight_rows = form.m;
+  *rows = form.rows;
+  return AINFER_OK;
+}
+
 size_t ainfer_moe_sort_workspace_bytes(int32_t max_tokens, int32_t top_k, int32_t n_experts) {
   if (max_tokens < 0 || max_tokens > AINFER_MOE_MAX_TOKENS || top_k < 1 || top_k > 32 ||
       n_experts < 1 || n_experts > 1024)

@@ -555,13 +555,12 @@ __global__ __launch_bounds__(256, 2) void k_fp8_tiles(Fp8Args a) {
 
 }  // namespace
 
-hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
-  const bool f32 = y_dtype == AINFER_ACT_F32;
-  const int nt = f32 ? 64 : 96, G = (a.K + 127) / 128;
+Fp8Form fp8_form(int E, int M, int K, int N, bool f32) {
+  const int nt = f32 ? 64 : 96, G = (K + 127) / 128;
   // what the host knows: at most `used` experts with rows, `each` rows of one on average
-  const int64_t used = std::min(a.E, a.N), each = a.N / used;
-  const int64_t slabs = (a.M + 63) / 64, mb = (a.M + TILE_M - 1) / TILE_M;
-  auto row_tiles = [&](int rows) { return std::max<int64_t>(used, (a.N + rows - 1) / rows); };
+  const int64_t used = std::min(E, N), each = N / used;
+  const int64_t slabs = (M + 63) / 64, mb = (M + TILE_M - 1) / TILE_M;
+  auto row_tiles = [&](int rows) { return std::max<int64_t>(used, (N + rows - 1) / rows); };
   // Tiles or split.  A tile's workgroup takes its K groups one by one, 0.5 us and 0.06 for each
   // 16 rows of x (latency) while its CU is not full; the split form's items take 1 / 1000 us for
   // a group and 64 weight rows x 32 rows of x, and weights that are read for the first time as
@@ -588,33 +587,45 @@ hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
     // two ahead, 96 and one: 64 experts of 256 rows, 4096 -> 2048 324, 310; of 128 195, 190; 1119 x
     // 976 -> 13696 45.6, 43.3; 8192 x 4096 -> 4096 271, 267; 2048 x 4096 -> 4096 66, 80; 32 experts of
     // 156, 1024 -> 2048 39, 44; 96 of 62, 2560 -> 1792 103.8, 105.3.
-    // (at most: full tiles, and one that is not full for each expert)
-    auto tiles = [&](auto kernel, int rows) {
-      const int64_t most = (a.N / rows + used) * mb;
+    if (f32 && row_tiles(96) * mb >= 600 && each > 64) return {TILE_M, 96};
+    if (f32) return {TILE_M, 64};
+    if (row_tiles(128) * mb >= 200 && each > 16) return {TILE_M, 128};
+    return {TILE_M, 96};
+  }
+  // Larger items read less, smaller ones are more: 16 weight rows for a single tile of rows
+  // (1 x 5120 -> 17408 17.5, 19.2 with 32); tiles of 32 rows from 128 items of them on
+  // (32 x 4096 -> 4096 9.0 with 16, 10.5; 64 x 4096 -> 4096 12.2, 10.3), 64 weight rows
+  // from 256 on (64 x 4096 -> 4096 10.3 with 32, 13.5; 128 x 4096 -> 4096 15.8, 13.2).
+  if (each > 16 && items2 >= 256) return {64, 32};
+  if (each > 16 && items2 >= 128) return {32, 32};
+  if (row_tiles(16) > 1) return {32, 16};
+  return {16, 16};
+}
+
+hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s) {
+  const bool f32 = y_dtype == AINFER_ACT_F32;
+  const Fp8Form form = fp8_form(a.E, a.M, a.K, a.N, f32);
+  // (at most: full tiles, and one that is not full for each expert)
+  const int64_t tiles_of_rows = a.N / form.rows + std::min(a.E, a.N);
+  if (form.m == TILE_M) {
+    const int64_t most = tiles_of_rows * ((a.M + TILE_M - 1) / TILE_M);
+    auto tiles = [&](auto kernel) {
       return enqueue(kernel, (int)std::min<int64_t>(512, (most + N_XCD - 1) / N_XCD * N_XCD), 256, s, a);
     };
-    if (f32 && row_tiles(96) * mb >= 600 && each > 64) return tiles(k_fp8_tiles<true, 96, 1>, 96);
-    if (f32) return tiles(k_fp8_tiles<true, 64, 2>, 64);
-    if (row_tiles(128) * mb >= 200 && each > 16) return tiles(k_fp8_tiles<false, 128, 1>, 128);
-    return tiles(k_fp8_tiles<false, 96, 2>, 96);
+    if (f32) return form.rows == 96 ? tiles(k_fp8_tiles<true, 96, 1>) : tiles(k_fp8_tiles<true, 64, 2>);
+    return form.rows == 128 ? tiles(k_fp8_tiles<false, 128, 1>) : tiles(k_fp8_tiles<false, 96, 2>);
   }
   auto split = [&](auto r_c, auto ns_c) {
     constexpr int R = decltype(r_c)::value, NS = decltype(ns_c)::value;
-    const int64_t items = (a.N / (16 * NS) + used) * slabs * (4 / R);
+    const int64_t items = tiles_of_rows * ((a.M + 63) / 64) * (4 / R);
     const int grid = (int)std::min<int64_t>(items, R == 4 ? 512 : 1024);
     return enqueue(f32 ? k_fp8_split<true, R, NS> : k_fp8_split<false, R, NS>, grid, 256, s, a);
   };
   using one = std::integral_constant<int, 1>;
   using two = std::integral_constant<int, 2>;
   using four = std::integral_constant<int, 4>;
-  // Larger items read less, smaller ones are more: 16 weight rows for a single tile of rows
-  // (1 x 5120 -> 17408 17.5, 19.2 with 32); tiles of 32 rows from 128 items of them on
-  // (32 x 4096 -> 4096 9.0 with 16, 10.5; 64 x 4096 -> 4096 12.2, 10.3), 64 weight rows
-  // from 256 on (64 x 4096 -> 4096 10.3 with 32, 13.5; 128 x 4096 -> 4096 15.8, 13.2).
-  if (each > 16 && items2 >= 256) return split(four(), two());
-  if (each > 16 && items2 >= 128) return split(two(), two());
-  if (row_tiles(16) > 1) return split(two(), one());
-  return split(one(), one());
+  if (form.rows == 32) return form.m == 64 ? split(four(), two()) : split(two(), two());
+  return form.m == 32 ? split(two(), one()) : split(one(), one());
 }
 
 // A thread writes 16 codes: of a row's neighbouring columns, or (TRANS) of 16 rows.

@@ -453,6 +453,12 @@ struct Fp8Args {
 size_t fp8_packed_bytes(int E, int M, int K);
 hipError_t launch_fp8_pack(const uint8_t *w, int E, int M, int K, int transpose, uint8_t *packed,
                            hipStream_t s);
+// The form of a product: weight rows and rows of an item.  256 weight rows are the tiles, which
+// go through K one group after the other; fewer are the split form, four waves of which share K.
+struct Fp8Form {
+  int m, rows;
+};
+Fp8Form fp8_form(int E, int M, int K, int N, bool f32);
 hipError_t launch_fp8_product(const Fp8Args &a, int y_dtype, hipStream_t s);
 
 // ---- tokens sorted by expert and back (moe_sort.hip) ---------------------------

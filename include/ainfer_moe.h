@@ -588,6 +588,11 @@ int ainfer_moe_fp8_product(const ainfer_moe_fp8 *w, const uint8_t *q, int64_t q_
                            const float *sq, const int32_t *offsets, int32_t N, void *y,
                            int64_t y_ld, void *stream);
 
+/* Test hook: which form of the product a call of N rows takes, by the weight rows and
+ * the rows of its work items (256 weight rows: tiles; fewer: the split form).  Host only. */
+int ainfer_moe_debug_fp8_form(int32_t E, int32_t M, int32_t K, int32_t N, int32_t y_dtype,
+                              int32_t *weight_rows, int32_t *rows);
+
 /* Gradient of ainfer_moe_silu_mul, computed in fp32: with sig = 1 / (1 + exp(-gate)),
  *   dgate = dact * up * sig * (1 + gate * (1 - sig)),   dup = dact * gate * sig.
  * N rows of I values (I up to 65536) of one type; dgate and dup may be dact, gate or up
