@@ -574,8 +574,9 @@ typedef struct ainfer_moe_fp8 {
  *           (sum over the group of q[n][k] * w[e][m][k]),  offsets[e] <= n < offsets[e + 1];
  * sums and the two scales' products in fp32, y rounded once.  With bf16 y the matrix
  * instruction drops what is more than 13 bits below the largest of eight neighbouring
- * products: at most 7 * 2^-13 of the sum of magnitudes, 1.4e-5 of it for normal values;
- * with fp32 y products are whole.  q: N rows of K codes at q_ld elements (16-byte
+ * products, by their codes' exponents: at most 7 * 2^-13 of the sum of magnitudes, where
+ * codes below 2^-6 (subnormal ones) count as 2^-6, so that beside those it may be 8 times
+ * as much; 1.1e-5 of a group's sum for normal values.  With fp32 y products are whole.  q: N rows of K codes at q_ld elements (16-byte
  * aligned, a multiple of 16, at most 2^24), sq [N][ceil(K / 128)], offsets device [E +
  * 1] ascending (NULL with one expert: all N rows), y: N rows of M values at y_ld
  * elements.  Rows of y outside [offsets[0], offsets[E]) are left as they were; offsets
