@@ -188,10 +188,12 @@ __global__ __launch_bounds__(256) void k_sort_place(const int32_t *idx, int64_t 
 // of them in the low half of a word and those of earlier chunks in the high half, four words
 // an expert for neighbouring lanes (pairs that all name one expert would take 64 turns of
 // the LDS at one word).  Its chunk is 256 pairs, placed by four of its waves.  Counting takes
-// 0.1 us for 1000 pairs; us of this launch, and of two that share the counts: 2400 pairs of 64
-// experts 7.4, 9.3 (each with a launch of short rows); 16000 8.6, 11.1; 40960 of 512
-// 11.5, 14.2, by a power law 12.5, 14.4, all of one 16.8, 14.8; 65528 of 64 13.4, 11.6.
-constexpr int SORT_OWN = 40960;  // 16 bits hold it
+// 0.1 us for 1000 pairs, in rounds of 16384.  us of this launch, and of two that share the counts:
+// 2400 pairs of 64 experts 7.4, 9.3 (each with a launch of short rows); 16000 8.6, 11.1.  Three
+// rounds are the most: in a graph, ids spread evenly, 49152 pairs of 16 experts 7.9, 7.7, of 64 7.7,
+// 7.9, of 512 6.9, 9.8; 53248 8.9, 7.8; 8.6, 7.9; 7.8, 10.2.  Busy experts cost this launch more:
+// 49152 by a power law 10.2, 7.9; 8.8, 8.0; 7.7, 9.8; all of one 14.4, 9.0.
+constexpr int SORT_OWN = 3 * 16384;  // 16 bits hold it
 typedef int32_t i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 __global__ __launch_bounds__(1024) void k_sort_own(const int32_t *idx, int n, int E,
