@@ -741,8 +741,8 @@ ByteRows byte_rows(const void *p, int64_t rows, int64_t ld, int64_t cols, int si
 }
 // whether a row of r meets [at, at + n): the first row that ends behind `at` starts ahead of its end
 bool rows_meet(const ByteRows &r, intptr_t at, int64_t n) {
-  if (r.n == 0 || n == 0) return false;
   const intptr_t end = r.at + r.bytes;
+  if (r.n < 2 || n == 0) return r.n && n && at < end && r.at < at + n;
   const int64_t i = at < end ? 0 : (at - end) / r.pitch + 1;
   return i < r.n && r.at + i * r.pitch < at + n;
 }

@@ -10,10 +10,10 @@
 // Weights are laid out once (ainfer_moe_fp8_pack) as this instruction takes them: 64 rows x
 // 128 columns are four tiles of 16 rows, each 2 KB in the order of the lanes, so that a wave's
 // load is 1 KB of neighbouring bytes.  (Read from plain rows, 16 neighbouring lanes touch 16
-// rows, which the CU's address unit takes one by one: 8192^3 ran at 1394 TFLOP/s.)  Row r of tile i is row
-// 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the 64, so that the lane that holds four results
-// of each tile holds two times 8 neighbouring columns of a row of y, and the four lanes of a row
-// 32.  Rows and columns behind the matrix are zeros.
+// rows, which the CU's address unit takes one by one: 8192^3 ran at 1394 TFLOP/s.)  Row r of tile
+// i is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the 64, so that the lane that holds four
+// results of each tile holds two times 8 neighbouring columns of a row of y, and the four lanes of
+// a row 32.  Rows and columns behind the matrix are zeros.
 #include <algorithm>
 
 #include "moe_common.h"
@@ -306,8 +306,8 @@ __global__ __launch_bounds__(256) void k_fp8_split(Fp8Args a) {
 // Bound by the loads' way through a CU's L1: a group of 256 x 128 is 48 KB for 128 products, and
 // 8192^3 brings 50 bytes a ns to each CU (without the loads the products alone run at 2622
 // TFLOP/s).  8192^3 507 us, 2170 TFLOP/s (a library's bf16 product 1366); 4096 x 5120 -> 17408
-// 354, 2065; 64 experts of about 512 rows, 4096 -> 2048 338, 1626: there the weights come from
-// memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 263, 1047.
+// 354, 2065; 64 experts of about 512 rows, 4096 -> 2048 335 to 351, 1570 to 1640: there the weights
+// come from memory, not from a cache; with fp32 outputs 8192 x 4096 -> 4096 263, 1047.
 constexpr int TILE_M = 256;
 
 template <int NS>
@@ -576,6 +576,12 @@ Fp8Form fp8_form(int E, int M, int K, int N, bool f32) {
   // gets more of it: 128 rows over 256 experts, 2048 -> 1024 37.6, 41.8; 512 over 512 112, 119; 16
   // experts of 4, 4096 -> 2048 23.6, 29.6; 64 of 8 88.6, 96.3; but with short rows 256 of 7, 2048 ->
   // 1024 108, 97; 64 of 6, 512 -> 4096 42, 31.
+  // The average is all that the host knows.  Where N is more than the rows in use, `each` is too
+  // high (64 experts, 4096 -> 2048, 512 rows in use: 95 as of N = 4096, 87 split); a caller that
+  // knows a smaller bound passes that as N.  Where few experts have most of the rows, the split
+  // form reads their weights again for every 16: 90% of 4000 rows on 8 of 512 experts, 4096 ->
+  // 2048 799 instead of 580 with tiles (spread evenly 719, 717); of 8192 on 8 of 1024, 4096 ->
+  // 1024 785, 610 (706, 723).
   const int64_t items2 = row_tiles(32) * slabs, tile_items = row_tiles(nt) * mb;
   const int64_t units = (each + 15) / 16, per = (units + nt / 16 - 1) / (nt / 16);
   const int64_t ns = (units + per - 1) / per;
@@ -589,7 +595,10 @@ Fp8Form fp8_form(int E, int M, int K, int N, bool f32) {
     // 40.5, 50.9; 512 experts of 8 rows, 2048 -> 1024 246, 253.  fp32, 64 rows and
     // two ahead, 96 and one: 64 experts of 256 rows, 4096 -> 2048 324, 310; of 128 195, 190; 1119 x
     // 976 -> 13696 45.6, 43.3; 8192 x 4096 -> 4096 271, 267; 2048 x 4096 -> 4096 66, 80; 32 experts of
-    // 156, 1024 -> 2048 39, 44; 96 of 62, 2560 -> 1792 103.8, 105.3.
+    // 156, 1024 -> 2048 39, 44.  An expert of up to 64 rows is one tile of either, one of 65 to 96
+    // two of 64 or one of 96: experts of 48 rows on average 134, 140 (128 experts, 2048 -> 2048), 103,
+    // 108 (96, 2560 -> 1792); 62 114, 114 (96); 64 138, 139 (128), 119, 113 (96), 75, 76 (64, 1024 ->
+    // 4096); 72 147, 144 (128), 122, 117 (96), 79, 76 (64); 96 166, 162 (128), 143, 131 (96).
     if (f32 && row_tiles(96) * mb >= 600 && each > 64) return {TILE_M, 96};
     if (f32) return {TILE_M, 64};
     if (row_tiles(128) * mb >= 200 && each > 16) return {TILE_M, 128};

@@ -82,7 +82,7 @@ __device__ __forceinline__ void silu_grad(float d, float g, float u, float &dg, 
 }
 
 // eight values read and written past the caches where that is one piece of 16 bytes a lane
-// (32768 x 1024 bf16: 60.3 us, 66.0 with ordinary accesses; with fp32's two pieces a lane
+// (32768 x 1024 bf16: 57 us, 63 with ordinary accesses; with fp32's two pieces a lane
 // 177 instead of 155 us for 40000 x 1000)
 template <bool F32>
 __device__ __forceinline__ void load8_once(const void *p, int64_t at, float (&v)[8]) {

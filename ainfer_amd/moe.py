@@ -656,7 +656,7 @@ class Fp8Weights:
         """y [N][M] = x W^T for codes q [N][K] and scales sq of rows sorted by expert
         (offsets [E + 1] int32; may be left out with one expert), in fp32 or bf16
         (ainfer_moe_fp8_product).  Rows outside the offsets keep what y holds (a new y has
-    anything there)."""
+        anything there)."""
         E, M, K = self.shape
         dev, n, _, ld = _codes(q, "q", K)
         if dev != self.dev:

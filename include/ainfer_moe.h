@@ -581,7 +581,8 @@ typedef struct ainfer_moe_fp8 {
  * 1] ascending (NULL with one expert: all N rows), y: N rows of M values at y_ld
  * elements.  Rows of y outside [offsets[0], offsets[E]) are left as they were; offsets
  * outside [0, N] are taken as its ends, and rows of experts that overlap are
- * unspecified.  A NaN code or scale reaches the values whose sums it is in.  y must not
+ * unspecified.  How the work is divided goes by N: a caller that knows that fewer rows are in use
+ * (many pairs belong to experts of other GPUs) does well to pass that many.  A NaN code or scale reaches the values whose sums it is in.  y must not
  * overlap anything that is read. The gradient to x is the same call with the transposed
  * weights (M a multiple of 16): ainfer_moe_fp8_pack(w, E, K, M, 1, ...) and scales
  * [E][ceil(K / 128)][ceil(M / 128)], as blocks are square. */
