@@ -52,8 +52,8 @@ def test_pitched_rows_of_the_other_calls(L):  # noqa: F811
     # 4 rows of 512 codes, 512 fp32 values
     R.refused(lambda **kw: R.quant(L, **kw), (
         dict(q=A + 2032, x_ld=1024, q_ld=4096), dict(q=A + 12288 + 2032, x_ld=1024, q_ld=4096),
-        dict(sq=D + 3072, q_ld=1024), dict(live=D + 3072 + 508, q_ld=1024),
-        dict(q=E - 3072, q_ld=1024), dict(sq=A + 4096 + 2044, x_ld=1024)), L.ERR_ARG)
+        dict(sq=D + 3 * 1024, q_ld=1024), dict(live=D + 3 * 1024 + 508, q_ld=1024),
+        dict(q=E - 3 * 1024, q_ld=1024), dict(sq=A + 4096 + 2044, x_ld=1024)), L.ERR_ARG)
     R.refused(lambda **kw: R.silu(L, **kw), (
         dict(q=B + 4096, u_ld=1024, q_ld=4096), dict(sq=D + 1024, q_ld=1024),
         dict(sq=A + 4096, g_ld=1024), dict(live=D + 2048, q_ld=1024)), L.ERR_ARG)
